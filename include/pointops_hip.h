@@ -525,6 +525,55 @@ hipError_t pointops_edge_write(const int64_t *table, const int64_t *ends, int64_
                                int32_t skip_self, int64_t *queries, int64_t *references,
                                hipStream_t stream);
 
+/* ------------------------------------------------------------ attention */
+
+/* Element types of the attention entry points. */
+enum { POINTOPS_F32 = 0, POINTOPS_F16 = 1, POINTOPS_BF16 = 2 };
+
+/* One attention call, given by a HOST pointer.  q is (B, Q, H, D), k and v
+ * (B, N, G, D), each with strides of batch, token and head in elements and
+ * D <= 128 contiguous; query head h reads key head h / (H / G).  The queries
+ * stand at the last Q of N positions (with `lengths` in a step: of the cloud's
+ * length).  The query at position p sees key j when |p - j| < window or
+ * j < sinks, and p >= j where `causal`; of cloud b only positions below
+ * lengths[b] exist (NULL: all N; values outside [0, N] are clamped).  A query
+ * that does not exist or sees nothing has an output of zeros and no gradient.
+ *
+ * `bias` (may be NULL) is (buckets, H) contiguous, of the same type: a score
+ * takes bias[bucket(p - j)][h].  The bucket of an offset d >= 0 is the number
+ * of `edges` (HOST pointer; 1 .. 255 ascending values in [1, 1024]) at or
+ * below d.  buckets = n_edges + 1: d < 0 counts as 0; twice that: the bucket
+ * of d < 0 is n_edges + 1 plus that of -d. */
+typedef struct {
+    const void *q, *k, *v;
+    const void *bias;
+    const void *lengths; /* int32 or int64 (length_bits), B values, or NULL */
+    const int32_t *edges;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t B, Q, N, H, G, D;
+    int64_t window, sinks;
+    int32_t n_edges, buckets, length_bits, causal, type;
+    float scale;
+} pointops_attention;
+
+/* out (B, Q, H, D) contiguous; lse (B, H, Q) f32, the logarithm to base 2 of
+ * each row's sum (+inf for a row without keys), may be NULL. */
+hipError_t pointops_attention_forward(const pointops_attention *in, void *out, float *lse,
+                                      hipStream_t stream);
+
+/* Gradients of the forward with the same `in`, whose `out` and `lse` it takes.
+ * grad_out (B, Q, H, D) has the strides grad_stride (HOST, 3 values: batch,
+ * token, head; D contiguous).  dq (B, Q, H, D), dk and dv (B, N, G, D) and
+ * dbias (buckets, H) (NULL: not wanted) are contiguous, of in->type; all of
+ * each is written, in an order of additions that does not change from call to
+ * call.  `workspace` holds pointops_attention_backward_workspace_bytes(in)
+ * bytes, at a multiple of 16. */
+size_t pointops_attention_backward_workspace_bytes(const pointops_attention *in);
+hipError_t pointops_attention_backward(const pointops_attention *in, const void *out,
+                                       const float *lse, const void *grad_out,
+                                       const int64_t *grad_stride, void *dq, void *dk, void *dv,
+                                       void *dbias, void *workspace, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,337 @@
+// Shared pieces of the attention kernels (gfx950): matrix-core fragments of
+// the three types, tiles in LDS, which keys a query sees, and the bias by
+// offset.
+//
+// Every product takes its tile operand (A, from LDS) by rows and its other
+// operand (B) from registers, one column a lane: with keys as rows and queries
+// as columns a lane holds the scores of one query, so that the softmax is a
+// lane's own arithmetic, and the scores are, as they lie, the B operand of the
+// next product.  What a lane holds of a 32 x 32 result is column lane % 32 and
+// rows 8 g + 4 h + e (g, e = 0 .. 3, h = lane / 32) in register 4 g + e.
+#pragma once
+
+#include <type_traits>
+
+#include "pointops_common.hpp"
+#include "pointops_hip.h"
+
+namespace pointops {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff();
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kOuter = 128;      // rows of a block that stay in registers, 32 a wave
+constexpr int kMaxHead = 128;    // largest head width
+constexpr int kMaxReach = 1024;  // the bias is constant beyond this offset
+
+// A fragment is 16 bytes a lane: 8 values of 16 bits or 4 of 32.  As a row
+// operand it holds bytes 32 c + 16 h .. + 15 of the lane's row (chunk c).
+template <typename T>
+constexpr int kPerFrag = 16 / static_cast<int>(sizeof(T));
+
+// acc += A B over one chunk (16 values of 16 bits in one instruction, or 8
+// of 32 bits in four; values 4 u + e of the two half-waves meet in step e).
+template <typename T>
+__device__ __forceinline__ f32x16 mma(i32x4 a, i32x4 b, f32x16 acc) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], acc, 0, 0, 0);
+        return acc;
+    } else if constexpr (__is_same(T, bf16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+    }
+}
+
+// Registers p[0 .. kPerFrag - 1] of a result as a B fragment of T (rounded to
+// nearest even for the 16-bit types).
+template <typename T>
+__device__ __forceinline__ i32x4 as_fragment(const float* p) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(i32x4, f32x4{p[0], p[1], p[2], p[3]});
+    } else if constexpr (__is_same(T, bf16)) {
+        bf16x8 r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = static_cast<bf16>(p[e]);
+        return __builtin_bit_cast(i32x4, r);
+    } else {
+        f16x8 r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = static_cast<f16>(p[e]);
+        return __builtin_bit_cast(i32x4, r);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v) { return static_cast<T>(v); }
+
+// Element e of a fragment.
+template <typename T>
+__device__ __forceinline__ float element(i32x4 f, int e) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(f32x4, f)[e];
+    else if constexpr (__is_same(T, bf16)) return static_cast<float>(__builtin_bit_cast(bf16x8, f)[e]);
+    else return static_cast<float>(__builtin_bit_cast(f16x8, f)[e]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The sum and the maximum of a value over the two half-waves.
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2i(v), f2i(v), false, false);
+    return i2f(r[0]) + i2f(r[1]);
+}
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2i(v), f2i(v), false, false);
+    return fmaxf(i2f(r[0]), i2f(r[1]));
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+// ------------------------------------------------------------------ tiles
+// 16 bytes of a row of `width` elements from element `at` on, zeros behind its
+// end.  VEC: rows are 16-byte aligned and `width` is a multiple of kPerFrag.
+template <typename T, bool VEC>
+__device__ __forceinline__ i32x4 load_row(const T* row, int at, int width) {
+    i32x4 r = {0, 0, 0, 0};
+    if constexpr (VEC) {
+        if (at < width) r = *reinterpret_cast<const i32x4*>(row + at);
+    } else {
+        union { i32x4 v; T e[kPerFrag<T>]; } u;
+        u.v = r;
+#pragma unroll
+        for (int e = 0; e < kPerFrag<T>; ++e)
+            if (at + e < width) u.e[e] = row[at + e];
+        r = u.v;
+    }
+    return r;
+}
+
+// Rows of DP elements in LDS, 16 bytes apart more than they are long: the
+// 16-byte reads of 32 rows then fall on all banks in turn.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int kStride = DP * static_cast<int>(sizeof(T)) + 16;
+    static constexpr int kChunks = DP * static_cast<int>(sizeof(T)) / 32;  // of a row operand
+    static constexpr int kRowsPerFrag = 2 * kPerFrag<T>;  // rows that a transposed fragment spans
+
+    // Row operand: row `row0` + lane % 32, chunk c.
+    __device__ static __forceinline__ i32x4 rows(const char* tile, int row0, int c) {
+        const int lane = lane_id();
+        return *reinterpret_cast<const i32x4*>(tile + (row0 + lane % 32) * kStride + 32 * c + 16 * (lane / 32));
+    }
+
+    // Transposed operand: its row is column d0 + lane % 32 of the tile, its
+    // values the tile's rows row0 + 8 g + 4 h + e in the order of a result's
+    // registers.  16-bit types by the transposing read (16 lanes take a 4 x 16
+    // block, each one column), 32-bit ones value by value.
+    __device__ static __forceinline__ i32x4 columns(const char* tile, int row0, int d0) {
+        const int lane = lane_id(), h = lane / 32;
+        if constexpr (sizeof(T) == 4) {
+            const char* p = tile + (row0 + 4 * h) * kStride + 4 * (d0 + lane % 32);
+            i32x4 r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = *reinterpret_cast<const int*>(p + e * kStride);
+            return r;
+        } else {
+            const int i = lane % 16;
+            const char* p = tile + (row0 + 4 * h + i / 4) * kStride + 2 * (d0 + 16 * ((lane / 16) % 2) + 4 * (i % 4));
+            typedef __attribute__((address_space(3))) s16x4 lds4;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * kStride));
+            const i32x2 a = __builtin_bit_cast(i32x2, x), b = __builtin_bit_cast(i32x2, y);
+            return i32x4{a[0], a[1], b[0], b[1]};
+        }
+    }
+};
+
+// A tile's way from memory to LDS through a block's registers: requested
+// while the one before is used.
+template <typename T, int DP, int ROWS, bool VEC>
+struct Stage {
+    static constexpr int kPerRow = DP * static_cast<int>(sizeof(T)) / 16;
+    static constexpr int kPieces = ROWS * kPerRow / kThreads;
+    static_assert(ROWS * kPerRow % kThreads == 0);
+    i32x4 r[kPieces];
+
+    // Rows first .. first + ROWS - 1; those outside [low, high) are zeros.
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int low, int high, int width) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int at = i * kThreads + static_cast<int>(threadIdx.x);
+            const int row = first + at / kPerRow;
+            r[i] = i32x4{0, 0, 0, 0};
+            if (row >= low && row < high)
+                r[i] = load_row<T, VEC>(base + row * stride, at % kPerRow * kPerFrag<T>, width);
+        }
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int at = i * kThreads + static_cast<int>(threadIdx.x);
+            *reinterpret_cast<i32x4*>(tile + at / kPerRow * Tile<T, DP>::kStride + at % kPerRow * 16) = r[i];
+        }
+    }
+};
+
+// Rows of an inner tile: 64, or 32 where a value has 32 bits (the same LDS).
+template <typename T>
+constexpr int kInner = sizeof(T) == 4 ? 32 : 64;
+
+// Registers from .. from + 3 of a result to elements at .. at + 3 of a row
+// (VEC: the row's width is a multiple of 4 and its start aligned to as many).
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int at, int width, const f32x16& v, int from) {
+    T piece[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) piece[f] = from_float<T>(v[from + f]);
+    if constexpr (VEC) {
+        if (at < width) __builtin_memcpy(__builtin_assume_aligned(row + at, 4 * sizeof(T)), piece, sizeof piece);
+    } else {
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+            if (at + f < width) row[at + f] = piece[f];
+    }
+}
+
+// -------------------------------------------------------------- arguments
+struct Rows {
+    const void* p;
+    int64_t b, n, h;  // strides of batch, token and head, in elements
+    template <typename T>
+    __device__ __forceinline__ const T* at(int64_t batch, int64_t head) const {
+        return static_cast<const T*>(p) + batch * b + head * h;
+    }
+};
+
+struct Args {
+    Rows q, k, v;
+    const void* bias;  // (n_edges + 1, or twice that) x H, or null
+    const void* lengths;
+    int B, Q, N, H, G, D;
+    int window, sinks;  // window in [1, N + 1]
+    int reach;          // the last edge: the bias is constant from there on
+    int n_edges;
+    int buckets;
+    int length_bits;
+    bool causal;
+    float scale_log2;  // scale log2(e): scores are in units of log 2
+    float scale;
+    int edges[255];
+
+    __device__ __forceinline__ int length(int b) const {
+        if (lengths == nullptr) return N;
+        const int64_t l = length_bits == 64 ? static_cast<const int64_t*>(lengths)[b]
+                                            : static_cast<const int32_t*>(lengths)[b];
+        return static_cast<int>(l < 0 ? 0 : l > N ? N : l);
+    }
+};
+
+// Keys that the query at position p sees: low .. low + count - 1, and those
+// below `first`.
+struct Seen {
+    int low, count, first;
+    __device__ __forceinline__ bool operator()(int j) const {
+        return static_cast<uint32_t>(j - low) < static_cast<uint32_t>(count) || j < first;
+    }
+};
+
+__device__ __forceinline__ int seen_low(const Args& a, int p) { return max(0, p - a.window + 1); }
+__device__ __forceinline__ int seen_high(const Args& a, int p, int len) {
+    return a.causal ? p : min(len - 1, p + a.window - 1);
+}
+__device__ __forceinline__ int seen_first(const Args& a, int p, int len) {
+    return min(a.sinks, a.causal ? min(p + 1, len) : len);
+}
+__device__ __forceinline__ Seen seen_by(const Args& a, int p, int len) {
+    if (p < 0 || p >= len) return {0, 0, 0};
+    const int low = seen_low(a, p);
+    return {low, seen_high(a, p, len) - low + 1, seen_first(a, p, len)};
+}
+
+// ------------------------------------------------------------------- bias
+// A block's bias by offset (query's position less key's) in LDS, in units of
+// log 2: entry offset + reach + kMargin, the ends repeated over the margins,
+// so that a tile with any offset inside the reach indexes it without a clamp.
+constexpr int kMargin = kOuter + 64;
+__host__ __device__ inline int bias_entries(int reach) { return 2 * (reach + kMargin) + 1; }
+
+// Bucket of an offset: the number of edges at or below its distance; the
+// buckets of later keys, where there are any, follow those of earlier ones.
+__device__ __forceinline__ int bucket_of(const Args& a, const int* edges, int offset) {
+    const bool later = offset < 0;
+    const bool two_sided = a.buckets > a.n_edges + 1;
+    const int d = later ? (two_sided ? -offset : 0) : offset;
+    int low = 0, high = a.n_edges;  // edges below `low` are <= d, those from `high` on are not
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (edges[mid] <= d) low = mid + 1;
+        else high = mid;
+    }
+    return low + (later && two_sided ? a.n_edges + 1 : 0);
+}
+
+// v log2(e), kept finite where v is: a mask of the type's lowest value stays
+// one that all keys of a row can share.
+__device__ __forceinline__ float bias_log2(float v) {
+    const float w = v * kLog2e;
+    if (w - w != 0.f && v - v == 0.f) return v < 0.f ? -3e38f : 3e38f;
+    return w;
+}
+
+// Fills the table for head `head` (edges: LDS, n_edges ints).  The caller's
+// next barrier makes it visible; this one has a barrier of its own.
+template <typename T>
+__device__ __forceinline__ void fill_bias(const Args& a, int head, float* table, int* edges) {
+    for (int i = threadIdx.x; i < a.n_edges; i += kThreads) edges[i] = a.edges[i];
+    __syncthreads();
+    const T* bias = static_cast<const T*>(a.bias) + head;
+    for (int i = threadIdx.x; i < bias_entries(a.reach); i += kThreads) {
+        const int b = bucket_of(a, edges, i - a.reach - kMargin);
+        table[i] = bias_log2(to_float(bias[static_cast<int64_t>(b) * a.H]));
+    }
+}
+
+// ---------------------------------------------------------------- dispatch
+// Head widths are padded to a multiple of 32.
+template <typename F>
+hipError_t with_width(int64_t D, F f) {
+    if (D <= 32) return f(std::integral_constant<int, 32>{});
+    if (D <= 64) return f(std::integral_constant<int, 64>{});
+    if (D <= 96) return f(std::integral_constant<int, 96>{});
+    return f(std::integral_constant<int, 128>{});
+}
+
+// Whether 16-byte reads serve these rows.
+template <typename T>
+bool vector_rows(const Rows& r, int64_t D) {
+    const int64_t n = kPerFrag<T>;
+    return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.b % n == 0 && r.n % n == 0 && r.h % n == 0 && D % n == 0;
+}
+
+// The device arguments of a call, and whether it is one that the kernels take.
+bool read_args(const pointops_attention* in, Args* out);
+
+}  // namespace attn
+}  // namespace pointops

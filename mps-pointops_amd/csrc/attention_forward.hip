@@ -1,0 +1,317 @@
+// Attention within a window of the order, with first keys that stay visible:
+// the forward pass.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  s_ij = scale q_i k_j + bias(i - j)
+//
+// over the keys j that query i sees.  One pass: a block of 4 waves holds 128
+// queries (32 a wave, one a lane column) with their running maximum, sum and
+// output in registers and takes its keys 64 (32 bits: 32) at a time through
+// LDS; tiles that no query of the block sees are never read, and masks are
+// applied only where a tile's edge runs through the window.  Scores, maxima,
+// sums and outputs are 32-bit; the weights p are rounded to the values' type
+// for the second product, as its matrix instruction takes them.
+#include "attention.hpp"
+
+namespace pointops {
+namespace attn {
+
+bool read_args(const pointops_attention* in, Args* out) {
+    const int64_t limit = (int64_t(1) << 30) - 1024;  // sums of two positions fit an int
+    if (in == nullptr || out == nullptr) return false;
+    if (in->B < 0 || in->Q < 0 || in->N < 0 || in->H < 0 || in->G < 0 || in->D < 1 || in->D > kMaxHead) return false;
+    if (in->B > limit || in->Q > limit || in->N > limit || in->H > limit || in->G > limit) return false;
+    if (in->type < POINTOPS_F32 || in->type > POINTOPS_BF16) return false;
+    if (in->H > 0 && (in->G < 1 || in->H % in->G != 0)) return false;
+    if (in->window < 1 || in->sinks < 0) return false;
+    if (in->lengths != nullptr && in->length_bits != 32 && in->length_bits != 64) return false;
+    Args& a = *out;
+    a.q = {in->q, in->q_stride[0], in->q_stride[1], in->q_stride[2]};
+    a.k = {in->k, in->k_stride[0], in->k_stride[1], in->k_stride[2]};
+    a.v = {in->v, in->v_stride[0], in->v_stride[1], in->v_stride[2]};
+    a.bias = in->bias;
+    a.lengths = in->lengths;
+    a.length_bits = in->length_bits;
+    a.B = static_cast<int>(in->B);
+    a.Q = static_cast<int>(in->Q);
+    a.N = static_cast<int>(in->N);
+    a.H = static_cast<int>(in->H);
+    a.G = static_cast<int>(in->G);
+    a.D = static_cast<int>(in->D);
+    a.window = static_cast<int>(in->window > in->N + 1 ? in->N + 1 : in->window);
+    a.sinks = static_cast<int>(in->sinks > in->N ? in->N : in->sinks);
+    a.causal = in->causal != 0;
+    a.scale = in->scale;
+    a.scale_log2 = in->scale * kLog2e;
+    a.reach = 0;
+    a.n_edges = 0;
+    a.buckets = 0;
+    if (in->bias != nullptr) {
+        if (in->edges == nullptr || in->n_edges < 1 || in->n_edges > 255) return false;
+        if (in->buckets != in->n_edges + 1 && in->buckets != 2 * (in->n_edges + 1)) return false;
+        for (int i = 0; i < in->n_edges; ++i) {
+            a.edges[i] = in->edges[i];
+            if (a.edges[i] < 1 || a.edges[i] > kMaxReach || (i > 0 && a.edges[i] < a.edges[i - 1])) return false;
+        }
+        a.n_edges = in->n_edges;
+        a.buckets = in->buckets;
+        a.reach = a.edges[a.n_edges - 1];
+    }
+    return true;
+}
+
+namespace {
+
+// One query by a whole wave, key by key: for rows whose result is not finite,
+// where a product with a masked key's infinity or NaN may have spread.  Here
+// only the keys that the row sees take part (one whose score is -inf has no
+// weight and is left out).
+template <typename T>
+__device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, int len, const float* table,
+                                            T* out, float* lse) {
+    const int lane = lane_id(), g = h / (a.H / a.G), p = i + a.N - a.Q;
+    const T* q = a.q.at<T>(b, h) + i * a.q.n;
+    const T* k = a.k.at<T>(b, g);
+    const T* v = a.v.at<T>(b, g);
+    const Seen seen = seen_by(a, p, len);
+    float m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
+    const bool d0 = lane < a.D, d1 = lane + kWave < a.D;
+    const float q0 = d0 ? to_float(q[lane]) : 0.f, q1 = d1 ? to_float(q[lane + kWave]) : 0.f;
+    auto key = [&](int64_t j) {
+        const float k0 = d0 ? to_float(k[j * a.k.n + lane]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + lane + kWave]) : 0.f;
+        float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2;
+        if (a.bias != nullptr) {
+            const int64_t off = p - j;
+            s += table[(off > a.reach ? a.reach : off < -a.reach ? -a.reach : off) + a.reach + kMargin];
+        }
+        if (s == -kInf) return;
+        const float top = fmaxf(m, s), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
+        m = top;
+        l = l * keep + w;
+        o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n + lane]) : 0.f);
+        o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + lane + kWave]) : 0.f);
+    };
+    for (int j = 0; j < seen.first; ++j) key(j);
+    for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d0) out[lane] = from_float<T>(o0 * inv);
+    if (d1) out[lane + kWave] = from_float<T>(o1 * inv);
+    if (lane == 0 && lse != nullptr) *lse = l == 0.f ? kInf : m + log2f(l);
+}
+
+// The running maximum may lie this far (in units of log 2) below the true one:
+// weights up to 2^8 cost no precision, and outputs are rescaled seldom.
+constexpr float kSlack = 8.f;
+
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Args a, T* __restrict__ out,
+                                                                        float* __restrict__ lse_out) {
+    using TileT = Tile<T, DP>;
+    constexpr int TK = kInner<T>, kSub = TK / 32, kOut = DP / 32;
+    extern __shared__ char lds[];
+    char* const ktile = lds;
+    char* const vtile = lds + TK * TileT::kStride;
+    float* const table = reinterpret_cast<float*>(lds + 2 * TK * TileT::kStride);
+
+    const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
+    const uint32_t blocks = (a.Q + kOuter - 1) / kOuter;
+    const uint32_t blk = xcd_local_block(blockIdx.x, gridDim.x);
+    const int bh = static_cast<int>(blk / blocks), b = bh / a.H, h = bh % a.H, g = h / (a.H / a.G);
+    const int i0 = static_cast<int>(blocks - 1 - blk % blocks) * kOuter;  // the longest rows of a causal call first
+    const int len = a.length(b), shift = a.N - a.Q;
+    const bool biased = a.bias != nullptr;
+    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
+
+    // The block's rows that exist, by position, and the tiles that they see.
+    const int rows = min(kOuter, a.Q - i0);
+    const int p_first = max(i0 + shift, 0), p_last = min(i0 + shift + rows, len) - 1;
+    int t = 0, t_first_end = 0, t_low = 0, t_high = -1;
+    if (p_first <= p_last) {
+        t_first_end = (seen_first(a, p_last, len) + TK - 1) / TK;
+        t_low = max(t_first_end, seen_low(a, p_first) / TK);
+        t_high = seen_high(a, p_last, len) / TK;
+        t = t_first_end > 0 ? 0 : t_low;
+    }
+    const int t_end = max(t_first_end, t_high + 1);  // one past the last tile
+
+    // This wave's rows.
+    const int w0 = i0 + 32 * wave + shift;  // position of its first row
+    const int w_count = min(32, i0 + rows - (i0 + 32 * wave));
+    const int w_first = max(w0, 0), w_last = min(w0 + w_count, len) - 1;
+    const bool w_any = w_first <= w_last, w_whole = w_any && w0 >= 0 && w0 + w_count <= len;
+    const int row = i0 + 32 * wave + lane % 32, p = row + shift;
+    const Seen seen = seen_by(a, p, len);
+
+    i32x4 q[TileT::kChunks];
+    {
+        const T* src = a.q.at<T>(b, h) + row * a.q.n;
+#pragma unroll
+        for (int c = 0; c < TileT::kChunks; ++c) {
+            q[c] = i32x4{0, 0, 0, 0};
+            if (row < a.Q) q[c] = load_row<T, VEC>(src, (2 * c + half) * kPerFrag<T>, a.D);
+        }
+    }
+    const T* const k = a.k.at<T>(b, g);
+    const T* const v = a.v.at<T>(b, g);
+    f32x16 o[kOut] = {};
+    float m = -kInf, l = 0.f;  // the maximum so far (see kSlack) and this half-wave's sum
+
+    Stage<T, DP, TK, VEC> ks, vs;
+    if (t < t_end) {
+        ks.load(k, a.k.n, t * TK, 0, len, a.D);
+        vs.load(v, a.v.n, t * TK, 0, len, a.D);
+    }
+    while (t < t_end) {
+        __syncthreads();
+        ks.store(ktile);
+        vs.store(vtile);
+        __syncthreads();
+        const int j0 = t * TK;
+        ++t;
+        if (t >= t_first_end && t < t_low) t = t_low;
+        if (t < t_end) {
+            ks.load(k, a.k.n, t * TK, 0, len, a.D);
+            vs.load(v, a.v.n, t * TK, 0, len, a.D);
+        }
+        if (!w_any) continue;
+        const bool meets = (j0 <= seen_high(a, w_last, len) && j0 + TK > seen_low(a, w_first)) ||
+                           j0 < seen_first(a, w_last, len);
+        if (!meets) continue;
+        const bool whole = w_whole && ((j0 + TK - 1 <= seen_high(a, w_first, len) && j0 >= seen_low(a, w_last)) ||
+                                       j0 + TK <= seen_first(a, w_first, len));
+
+        float s[kSub][16];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            f32x16 acc = {};
+#pragma unroll
+            for (int c = 0; c < TileT::kChunks; ++c) acc = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], acc);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = acc[r] * a.scale_log2;
+        }
+        if (biased) {
+            const int near = w0 - j0;  // offset of the wave's first row and the tile's first key
+            if (near - (TK - 1) >= a.reach || near + 31 <= -a.reach) {
+                const float far = table[near > 0 ? bias_entries(a.reach) - 1 : 0];
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[u][r] += far;
+            } else {
+                const float* at = table + near + lane % 32 - 4 * half + a.reach + kMargin;
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[u][r] += at[-(32 * u + 8 * (r / 4) + r % 4)];
+            }
+        }
+        if (!whole) {
+            const int j = j0 + 4 * half;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!seen(j + 32 * u + 8 * (r / 4) + r % 4)) s[u][r] = -kInf;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        top = halves_max(top);
+        if (ballot(top > m + kSlack) != 0) {
+            const float next = fmaxf(m, top);
+            const float keep = m == next ? 1.f : exp2_fast(m - next);
+            m = next;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < kOut; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+        }
+        const float base = m == -kInf ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = exp2_fast(s[u][r] - base);
+                l += s[u][r];
+            }
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
+                const i32x4 w = as_fragment<T>(&s[u][c * kPerFrag<T>]);
+#pragma unroll
+                for (int d = 0; d < kOut; ++d)
+                    o[d] = mma<T>(TileT::columns(vtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), w, o[d]);
+            }
+    }
+
+    l = halves_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float lse = l == 0.f ? kInf : m + log2f(l);
+    float odd = lse == kInf ? 0.f : lse * 0.f;  // NaN where anything is not finite
+#pragma unroll
+    for (int d = 0; d < kOut; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[d][r] *= inv;
+            odd += o[d][r] * 0.f;
+        }
+    uint64_t bad = ballot(row < a.Q && odd != 0.f);
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    if (row < a.Q && (bad >> (lane % 32) & 1) == 0) {
+        T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store4<T, VEC>(dst, 32 * d + 8 * e + 4 * half, a.D, o[d], 4 * e);
+        if (half == 0 && lse_out != nullptr) lse_out[(static_cast<int64_t>(b) * a.H + h) * a.Q + row] = lse;
+    }
+    while (bad != 0) {
+        const int r = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const int i = i0 + 32 * wave + r;
+        careful_row<T>(a, b, h, i, len, table, out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D,
+                       lse_out == nullptr ? nullptr : lse_out + (static_cast<int64_t>(b) * a.H + h) * a.Q + i);
+    }
+}
+
+template <typename T>
+hipError_t forward(const pointops_attention* in, const Args& a, void* out, float* lse, hipStream_t stream) {
+    const int64_t blocks = (in->Q + kOuter - 1) / kOuter * in->B * in->H;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    return with_width(in->D, [&](auto width) {
+        constexpr int DP = decltype(width)::value;
+        size_t lds = 2 * kInner<T> * Tile<T, DP>::kStride;
+        if (a.bias != nullptr) lds += 4 * (bias_entries(a.reach) + a.n_edges);
+        const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
+        const dim3 grid(static_cast<uint32_t>(blocks));
+        if (vec)
+            hipLaunchKernelGGL((attention_forward_kernel<T, DP, true>), grid, dim3(kThreads), lds, stream, a,
+                               static_cast<T*>(out), lse);
+        else
+            hipLaunchKernelGGL((attention_forward_kernel<T, DP, false>), grid, dim3(kThreads), lds, stream, a,
+                               static_cast<T*>(out), lse);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace pointops
+
+extern "C" hipError_t pointops_attention_forward(const pointops_attention* in, void* out, float* lse,
+                                                 hipStream_t stream) {
+    using namespace pointops::attn;
+    Args a;
+    if (!read_args(in, &a)) return hipErrorInvalidValue;
+    if (in->B == 0 || in->H == 0 || in->Q == 0) return hipSuccess;
+    if (in->q == nullptr || out == nullptr || (in->N > 0 && (in->k == nullptr || in->v == nullptr)))
+        return hipErrorInvalidValue;
+    switch (in->type) {
+        case POINTOPS_F32: return forward<float>(in, a, out, lse, stream);
+        case POINTOPS_F16: return forward<f16>(in, a, out, lse, stream);
+        default: return forward<bf16>(in, a, out, lse, stream);
+    }
+}

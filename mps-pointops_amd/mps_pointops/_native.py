@@ -74,6 +74,8 @@ _SIGNATURES: dict[str, list] = {
     "pointops_knn_finish": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f32, _vp],
     "pointops_group_rows": [_vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp],
     "pointops_group_rows_backward": [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "pointops_attention_forward": [_vp, _vp, _vp, _vp],
+    "pointops_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "pointops_chamfer_nearest_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "pointops_chamfer_nearest_f64": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "pointops_chamfer_backward_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
@@ -96,6 +98,7 @@ _SIZE_QUERIES: dict[str, list] = {
     "pointops_ball_query_backward_workspace_bytes": [_i64, _i64],
     "pointops_ball_query_auto_workspace_bytes": [_i64, _i64, _i64],
     "pointops_group_points_backward_workspace_bytes": [_i64, _i64, _i64, _i64],
+    "pointops_attention_backward_workspace_bytes": [_vp],
 }
 
 

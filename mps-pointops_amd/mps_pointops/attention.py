@@ -1,0 +1,241 @@
+"""Attention for networks over ordered points.
+
+A cloud whose points are ordered along a curve, or one that is written point
+by point, is a sequence of tokens.  These operators are what a transformer
+layer over such sequences asks for beside its matrix products:
+
+* ``window_attention``: attention within a window of the order, with a few
+  first tokens that every query sees and a bias learned by buckets of the
+  offset, with its gradients;
+
+Tensors are (batch, tokens, heads, width) in float32, float16 or bfloat16 on
+``device='cuda'``, with any strides; fewer key heads than query heads are
+shared by consecutive query heads.  Scores, softmax statistics, norms and sums
+are float32 throughout, and no result depends on the order in which the GPU
+happens to add.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import struct
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_MAX_HEAD = 128
+_MAX_TOKENS = (1 << 30) - 1024
+_MAX_REACH = 1024
+_MAX_SIDE = 256
+# pointops_attention of pointops_hip.h.
+_ARGS = struct.Struct("@6Q9q6q2q5if")
+
+
+# ------------------------------------------------------------------- buckets
+def _root_above(n: int, m: int) -> int:
+    """The smallest d with d ** m >= n."""
+    d = max(1, int(round(n ** (1.0 / m)))) if n < 1 << 1000 else 1 << -(-n.bit_length() // m)
+    while d ** m >= n:
+        d -= 1
+    while d ** m < n:
+        d += 1
+    return d
+
+
+@functools.lru_cache(maxsize=256)
+def bucket_edges(buckets: int, max_distance: int) -> tuple[int, ...]:
+    """The smallest distance of each bucket but the first.
+
+    Half of the ``buckets`` hold one distance each (0, 1, 2, ...), the others
+    share the distances from there to ``max_distance`` in even steps of the
+    logarithm, and all that lie farther are in the last one: with
+    ``e = buckets // 2``, distance d >= e is in bucket
+    ``min(buckets - 1, e + floor(log(d / e) / log(max_distance / e) * (buckets - e)))``,
+    computed in whole numbers.
+    """
+    if buckets < 2:
+        raise ValueError("at least 2 buckets are needed for each side")
+    single = buckets // 2
+    if max_distance <= single:
+        raise ValueError(f"max_distance must be more than {single}, the distances that have a bucket of their own")
+    steps = buckets - single
+    return tuple(range(1, single + 1)) + tuple(
+        _root_above(max_distance ** t * single ** (steps - t), steps) for t in range(1, steps))
+
+
+@functools.lru_cache(maxsize=256)
+def _edge_array(buckets: int, max_distance: int):
+    edges = bucket_edges(buckets, max_distance)
+    return (ctypes.c_int32 * len(edges))(*edges)
+
+
+def _check_table(table: Tensor, heads: int | None, max_distance: int | None, causal: bool, limit: int, name: str):
+    """The edges of a (buckets, heads) table's side."""
+    if table.ndim != 2 or (heads is not None and table.shape[1] != heads):
+        raise ValueError(f"{name} must have shape (buckets, heads)")
+    if max_distance is None:
+        raise ValueError(f"{name} needs max_distance")
+    count = table.shape[0]
+    if not causal and count % 2:
+        raise ValueError(f"{name} must have an even number of buckets where both sides are seen")
+    side = count if causal else count // 2
+    if side > _MAX_SIDE:
+        raise ValueError(f"{name} must have at most {_MAX_SIDE} buckets for each side")
+    if max_distance > limit:
+        raise ValueError(f"max_distance must be at most {limit}")
+    return _edge_array(side, int(max_distance))
+
+
+# ----------------------------------------------------------------- arguments
+def _rows(t: Tensor) -> Tensor:
+    """The tensor with its last dimension contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _check_heads(tensors: dict[str, Tensor]) -> None:
+    first = next(iter(tensors.values()))
+    if not all(isinstance(t, Tensor) for t in tensors.values()):
+        raise TypeError(f"{', '.join(tensors)} must be tensors")
+    for name, t in tensors.items():
+        if t.ndim != 4:
+            raise ValueError(f"{name} must have shape (batch, tokens, heads, width)")
+        if t.device != first.device:
+            raise ValueError(f"{', '.join(tensors)} must be on the same device")
+        if t.dtype not in _TYPES:
+            raise TypeError(f"{name} must be float32, float16 or bfloat16")
+        if t.dtype != first.dtype:
+            raise TypeError(f"{', '.join(tensors)} must have the same type")
+
+
+def _check_attention(q: Tensor, k: Tensor, v: Tensor, window, sinks, causal, bias, max_distance, lengths):
+    _check_heads({"q": q, "k": k, "v": v})
+    batch, queries, heads, width = q.shape
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    if k.shape[0] != batch or k.shape[3] != width:
+        raise ValueError("k and v must have q's batch size and head width")
+    key_heads = k.shape[2]
+    if heads and (key_heads == 0 or heads % key_heads):
+        raise ValueError("the number of query heads must be a multiple of the number of key heads")
+    if not 1 <= width <= _MAX_HEAD:
+        raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
+    if max(batch, queries, k.shape[1], heads) > _MAX_TOKENS:
+        raise ValueError(f"sizes must be at most {_MAX_TOKENS}")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1")
+    if sinks < 0:
+        raise ValueError("sinks must be non-negative")
+    edges = None
+    if bias is not None:
+        if not isinstance(bias, Tensor):
+            raise TypeError("bias must be a tensor")
+        if bias.dtype != q.dtype:
+            raise TypeError("bias must have q's type")
+        if bias.device != q.device:
+            raise ValueError("bias must be on q's device")
+        edges = _check_table(bias, heads, max_distance, causal, _MAX_REACH, "bias")
+    if lengths is not None:
+        if not isinstance(lengths, Tensor):
+            raise TypeError("lengths must be a tensor")
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError("lengths must be int32 or int64")
+        if lengths.shape != (batch,):
+            raise ValueError("lengths must have shape (batch,)")
+        if lengths.device != q.device:
+            raise ValueError("lengths must be on q's device")
+    return edges
+
+
+def _pack(q: Tensor, k: Tensor, v: Tensor, window, sinks, causal, bias, edges, lengths, scale) -> bytes:
+    """The call as a pointops_attention."""
+    batch, queries, heads, width = q.shape
+    keys, key_heads = k.shape[1], k.shape[2]
+    return _ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if lengths is None else lengths.data_ptr(), 0 if edges is None else ctypes.addressof(edges),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        batch, queries, keys, heads, key_heads, width,
+        keys + 1 if window is None else min(int(window), keys + 1), min(int(sinks), keys),
+        0 if edges is None else len(edges), 0 if bias is None else bias.shape[0],
+        0 if lengths is None else 8 * lengths.element_size(), bool(causal), _TYPES[q.dtype], scale)
+
+
+# ------------------------------------------------------------------ attention
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, lengths, edges, window, sinks, causal, scale):
+        batch, queries, heads, _ = q.shape
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        needed = any(ctx.needs_input_grad[:4])
+        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device) if needed else None
+        if out.numel():
+            args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
+            _native.call("pointops_attention_forward", args, out.data_ptr(), _native.ptr(lse),
+                         _native.stream(q.device))
+        if needed:
+            ctx.save_for_backward(q, k, v, bias, lengths, out, lse)
+            ctx.rest = edges, window, sinks, causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad: Tensor):
+        q, k, v, bias, lengths, out, lse = ctx.saved_tensors
+        edges, window, sinks, causal, scale = ctx.rest
+        grad = _rows(grad)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dbias = None
+        if bias is not None and ctx.needs_input_grad[3]:
+            dbias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
+        if q.shape[0] and q.shape[2]:
+            args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
+            size = _native.size_query("pointops_attention_backward_workspace_bytes", args)
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            strides = (ctypes.c_int64 * 3)(*grad.stride()[:3])
+            _native.call("pointops_attention_backward", args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(),
+                         strides, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _native.ptr(dbias),
+                         workspace.data_ptr(), _native.stream(q.device))
+        else:
+            for t in (dk, dv) if dbias is None else (dk, dv, dbias):
+                t.zero_()
+        return dq, dk, dv, dbias, None, None, None, None, None, None
+
+
+def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = None, sinks: int = 0,
+                     causal: bool = False, bias: Tensor | None = None, max_distance: int | None = None,
+                     lengths: Tensor | None = None, scale: float | None = None) -> Tensor:
+    """Attention of ``q (B, Q, H, D)`` over ``k, v (B, N, G, D)`` within a
+    window of the order; H is a multiple of G, and D at most 128.
+
+    The queries stand at the last Q of the N positions.  The query at position
+    p sees the key at j when ``|p - j| < window`` (``None``: any) or
+    ``j < sinks``, and only ``j <= p`` if ``causal``.  ``lengths (B,)`` (int32 or
+    int64; values are clamped to [0, N]): positions from a cloud's length on do
+    not exist.  A query that does not exist or sees no key yields zeros and has
+    no gradient; what lies in keys and values that no query sees (infinities and
+    NaN too) reaches no output.
+
+    Scores are ``scale * q . k`` (``D ** -0.5`` by default), plus
+    ``bias[bucket(p - j), h]`` if a table ``bias (buckets, H)`` of q's type is
+    given.  Its buckets are those of ``bucket_edges`` with ``max_distance`` (at
+    most 1024): of ``p - j`` if ``causal``, else one half of them for
+    ``p - j >= 0`` and the other, in the same way, for ``j - p``.  An entry of
+    -inf masks its offsets.
+
+    Returns ``(B, Q, H, D)`` of q's type, differentiable in q, k, v and bias.
+    """
+    edges = _check_attention(q, k, v, window, sinks, causal, bias, max_distance, lengths)
+    _native.require_device(q.device)
+    if scale is None:
+        scale = q.shape[3] ** -0.5
+    return _WindowAttention.apply(
+        _rows(q), _rows(k), _rows(v), None if bias is None else bias.contiguous(),
+        None if lengths is None else lengths.contiguous(), edges, window, sinks, causal, float(scale))
+
+
+__all__ = ["bucket_edges", "window_attention"]
