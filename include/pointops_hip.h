@@ -574,6 +574,62 @@ hipError_t pointops_attention_backward(const pointops_attention *in, const void 
                                        const int64_t *grad_stride, void *dq, void *dk, void *dv,
                                        void *dbias, void *workspace, hipStream_t stream);
 
+/* The forward of a few new queries over a cache, bound by reading what they
+ * see of it: the queries stand at the last Q positions of each cloud's
+ * lengths[b] keys (N where NULL).  `in->causal` must be set.  out (B, Q, H, D)
+ * contiguous; `workspace` holds pointops_attention_step_workspace_bytes(in)
+ * bytes (NULL where that is 0). */
+size_t pointops_attention_step_workspace_bytes(const pointops_attention *in);
+hipError_t pointops_attention_step(const pointops_attention *in, void *out, void *workspace,
+                                   hipStream_t stream);
+
+/* The bias as a dense tensor: out[h][i][j] = table[bucket(N - Q + i - j)][h],
+ * (H, Q, N) contiguous; table (buckets, H) contiguous, edges and buckets as in
+ * pointops_attention, but edges up to 2^30.  Q, N < 2^22. */
+hipError_t pointops_relative_bias(const void *table, const int32_t *edges, int32_t n_edges,
+                                  int32_t buckets, int32_t type, void *out, int64_t H, int64_t Q,
+                                  int64_t N, hipStream_t stream);
+
+/* grad_table (buckets, H) from grad (H, Q, N) with strides of head and row (the
+ * last dimension contiguous), in a fixed order of additions.  `workspace` holds
+ * pointops_relative_bias_backward_workspace_bytes(H, Q, N) bytes. */
+size_t pointops_relative_bias_backward_workspace_bytes(int64_t H, int64_t Q, int64_t N);
+hipError_t pointops_relative_bias_backward(const void *grad, int64_t stride_h, int64_t stride_i,
+                                           const int32_t *edges, int32_t n_edges, int32_t buckets,
+                                           int32_t type, void *grad_table, void *workspace,
+                                           int64_t H, int64_t Q, int64_t N, hipStream_t stream);
+
+/* Norm and rotation of queries and keys, given by a HOST pointer: q (B, N, H, D)
+ * and k (B, N, G, D) with strides of batch, token and head in elements, D <= 128
+ * contiguous; weights of D values each (NULL: ones) of `type` or f32
+ * (weight_type); cos and sin (B, N, R / 2) f32 with strides of batch (0: shared)
+ * and token, R <= D even. */
+typedef struct {
+    const void *q, *k;
+    const void *q_weight, *k_weight;
+    const float *cos, *sin;
+    int64_t q_stride[3], k_stride[3], angle_stride[2];
+    int64_t B, N, H, G, D, R;
+    int32_t type, weight_type;
+    float eps;
+} pointops_qk_norm;
+
+/* y = x / sqrt(mean(x^2) + eps) * weight of every row, its values i and
+ * i + R / 2 (i < R / 2) rotated by the token's angle i; q_out and k_out
+ * contiguous. */
+hipError_t pointops_qk_norm_rotate(const pointops_qk_norm *in, void *q_out, void *k_out,
+                                   hipStream_t stream);
+
+/* Its gradients: dq, dk contiguous, of `type`; dq_weight, dk_weight (NULL: not
+ * wanted) of weight_type.  `workspace` (NULL where no weight's gradient is
+ * wanted) holds pointops_qk_norm_rotate_backward_workspace_bytes(in) bytes. */
+size_t pointops_qk_norm_rotate_backward_workspace_bytes(const pointops_qk_norm *in);
+hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm *in, const void *q_grad,
+                                            const int64_t *q_grad_stride, const void *k_grad,
+                                            const int64_t *k_grad_stride, void *dq, void *dk,
+                                            void *dq_weight, void *dk_weight, void *workspace,
+                                            hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -195,6 +195,10 @@ struct Stage {
     }
 };
 
+// The running maximum may lie this far (in units of log 2) below the true one:
+// weights up to 2^8 cost no precision, and outputs are rescaled seldom.
+constexpr float kSlack = 8.f;
+
 // Rows of an inner tile: 64, or 32 where a value has 32 bits (the same LDS).
 template <typename T>
 constexpr int kInner = sizeof(T) == 4 ? 32 : 64;
@@ -225,20 +229,25 @@ struct Rows {
     }
 };
 
+// Buckets of an offset: edge[0 .. n - 1] ascending; count = n + 1, or twice
+// that where later keys have buckets of their own.
+struct Buckets {
+    int n, count;
+    int edge[255];
+};
+
 struct Args {
     Rows q, k, v;
-    const void* bias;  // (n_edges + 1, or twice that) x H, or null
+    const void* bias;  // (bk.count, H), or null
     const void* lengths;
     int B, Q, N, H, G, D;
     int window, sinks;  // window in [1, N + 1]
     int reach;          // the last edge: the bias is constant from there on
-    int n_edges;
-    int buckets;
     int length_bits;
     bool causal;
     float scale_log2;  // scale log2(e): scores are in units of log 2
     float scale;
-    int edges[255];
+    Buckets bk;
 
     __device__ __forceinline__ int length(int b) const {
         if (lengths == nullptr) return N;
@@ -279,17 +288,17 @@ __host__ __device__ inline int bias_entries(int reach) { return 2 * (reach + kMa
 
 // Bucket of an offset: the number of edges at or below its distance; the
 // buckets of later keys, where there are any, follow those of earlier ones.
-__device__ __forceinline__ int bucket_of(const Args& a, const int* edges, int offset) {
+__device__ __forceinline__ int bucket_of(const Buckets& bk, const int* edges, int offset) {
     const bool later = offset < 0;
-    const bool two_sided = a.buckets > a.n_edges + 1;
+    const bool two_sided = bk.count > bk.n + 1;
     const int d = later ? (two_sided ? -offset : 0) : offset;
-    int low = 0, high = a.n_edges;  // edges below `low` are <= d, those from `high` on are not
+    int low = 0, high = bk.n;  // edges below `low` are <= d, those from `high` on are not
     while (low < high) {
         const int mid = (low + high) >> 1;
         if (edges[mid] <= d) low = mid + 1;
         else high = mid;
     }
-    return low + (later && two_sided ? a.n_edges + 1 : 0);
+    return low + (later && two_sided ? bk.n + 1 : 0);
 }
 
 // v log2(e), kept finite where v is: a mask of the type's lowest value stays
@@ -300,18 +309,51 @@ __device__ __forceinline__ float bias_log2(float v) {
     return w;
 }
 
-// Fills the table for head `head` (edges: LDS, n_edges ints).  The caller's
+// Fills the table for head `head` (edges: LDS, bk.n ints).  The caller's
 // next barrier makes it visible; this one has a barrier of its own.
 template <typename T>
 __device__ __forceinline__ void fill_bias(const Args& a, int head, float* table, int* edges) {
-    for (int i = threadIdx.x; i < a.n_edges; i += kThreads) edges[i] = a.edges[i];
+    for (int i = threadIdx.x; i < a.bk.n; i += kThreads) edges[i] = a.bk.edge[i];
     __syncthreads();
     const T* bias = static_cast<const T*>(a.bias) + head;
     for (int i = threadIdx.x; i < bias_entries(a.reach); i += kThreads) {
-        const int b = bucket_of(a, edges, i - a.reach - kMargin);
+        const int b = bucket_of(a.bk, edges, i - a.reach - kMargin);
         table[i] = bias_log2(to_float(bias[static_cast<int64_t>(b) * a.H]));
     }
 }
+
+// ------------------------------------------------------------ careful rows
+// One query by a whole wave, key by key, for rows whose result is not finite:
+// there a product with a masked key's infinity or NaN may have spread.  Only
+// keys that the row sees are added (one whose score is -inf has no weight and
+// is left out).  Lane l holds elements l and l + 64.
+template <typename T>
+struct CarefulRow {
+    const Args& a;
+    const T *k, *v;
+    float q0, q1, m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
+    bool d0, d1;
+
+    __device__ __forceinline__ CarefulRow(const Args& args, int b, int g, const T* q) : a(args) {
+        const int lane = lane_id();
+        k = a.k.at<T>(b, g) + lane;
+        v = a.v.at<T>(b, g) + lane;
+        d0 = lane < a.D;
+        d1 = lane + kWave < a.D;
+        q0 = d0 ? to_float(q[lane]) : 0.f;
+        q1 = d1 ? to_float(q[lane + kWave]) : 0.f;
+    }
+    __device__ __forceinline__ void add(int64_t j, float bias) {
+        const float k0 = d0 ? to_float(k[j * a.k.n]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + kWave]) : 0.f;
+        const float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2 + bias;
+        if (s == -kInf) return;
+        const float top = fmaxf(m, s), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
+        m = top;
+        l = l * keep + w;
+        o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n]) : 0.f);
+        o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + kWave]) : 0.f);
+    }
+};
 
 // ---------------------------------------------------------------- dispatch
 // Head widths are padded to a multiple of 32.
@@ -329,6 +371,15 @@ bool vector_rows(const Rows& r, int64_t D) {
     const int64_t n = kPerFrag<T>;
     return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.b % n == 0 && r.n % n == 0 && r.h % n == 0 && D % n == 0;
 }
+
+// relative_bias.hip: reads the host's edges; false if they are none.
+bool read_buckets(const int32_t* edges, int n, int count, int64_t most, Buckets* out);
+
+// relative_bias.hip: grad[bucket][h] (type T: POINTOPS_*) from sums by offset,
+// part (B, H, blocks, entries) with offset o at entry o + zero; the first and
+// the last bucket of a side take what lies beyond it.
+hipError_t bucket_sums(const Buckets& bk, const float* part, int B, int H, int blocks, int entries, int zero, int type,
+                       void* grad, hipStream_t stream);
 
 // The device arguments of a call, and whether it is one that the kernels take.
 bool read_args(const pointops_attention* in, Args* out);

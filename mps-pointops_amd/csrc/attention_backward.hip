@@ -432,45 +432,6 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Args a, 
     (which == 0 ? dk : dv)[((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D + d] = from_float<T>(all);
 }
 
-// dbias[bucket][h]: the parts' sums over the bucket's offsets.  One block each.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_grad_bias_kernel(const Args a, const float* __restrict__ part,
-                                                                       int blocks, T* __restrict__ dbias) {
-    __shared__ float waves[kWaves];
-    const int h = blockIdx.x, bucket = blockIdx.y, entries = bias_entries(a.reach);
-    const int side = a.n_edges + 1, e = bucket % side, zero = a.reach + kMargin;
-    const bool two_sided = a.buckets > side, later = bucket >= side;
-    // Distances of the bucket, then entries of the table; the last one of a
-    // side has no end, and the first also takes later keys where they have no
-    // buckets of their own.
-    const int d_low = e == 0 ? 0 : a.edges[e - 1], d_high = e == a.n_edges ? zero : a.edges[e] - 1;
-    int low, high;
-    if (later) {
-        low = zero - d_high;
-        high = zero - max(d_low, 1);
-    } else {
-        low = e == 0 && !two_sided ? 0 : zero + d_low;
-        high = zero + d_high;
-    }
-    float all = 0.f;
-    const int count = high - low + 1;
-    if (count > 0) {
-        for (int b = 0; b < a.B; ++b) {
-            const float* const src = part + (static_cast<int64_t>(b) * a.H + h) * blocks * entries + low;
-            const int64_t total = static_cast<int64_t>(blocks) * count;
-            for (int64_t i = threadIdx.x; i < total; i += kThreads) all += src[i / count * entries + i % count];
-        }
-    }
-    all = wave_sum(all);
-    if (lane_id() == 0) waves[threadIdx.x / kWave] = all;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int w = 0; w < kWaves; ++w) sum += waves[w];
-        dbias[static_cast<int64_t>(bucket) * a.H + h] = from_float<T>(sum);
-    }
-}
-
 // The first keys' blocks take all later rows, the others window + 128 of them
 // (two windows where later keys are seen too): pieces of about that length.
 Pieces pieces_of(const Args& a) {
@@ -543,7 +504,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     constexpr size_t tiles = 2 * kInner<T> * TileT::kStride;
     const size_t entries = bias_entries(a.reach);
     size_t lds = tiles;
-    if (a.bias != nullptr) lds += 4 * (entries * (x.dbias != nullptr ? 1 + kSums : 1) + a.n_edges);
+    if (a.bias != nullptr) lds += 4 * (entries * (x.dbias != nullptr ? 1 + kSums : 1) + a.bk.n);
     auto* const by_query = attention_grad_query_kernel<T, DP, VEC>;
     if (lds > kLdsFree) {
         static std::atomic<uint64_t> allowed{0};
@@ -557,7 +518,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
-        lds = tiles + 8 * kInner<T> + (a.bias != nullptr ? 4 * (entries + a.n_edges) : 0);
+        lds = tiles + 8 * kInner<T> + (a.bias != nullptr ? 4 * (entries + a.bk.n) : 0);
         hipLaunchKernelGGL((attention_grad_key_kernel<T, DP, VEC>), dim3(static_cast<uint32_t>(grid_k)), dim3(kThreads),
                            lds, stream, a, x.lse, delta, x.grad, static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, cut);
         hipError_t err = hipGetLastError();
@@ -572,9 +533,9 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         }
     }
     if (x.dbias != nullptr) {
-        hipLaunchKernelGGL(attention_grad_bias_kernel<T>, dim3(a.H, a.buckets), dim3(kThreads), 0, stream, a, dbias_part,
-                           static_cast<int>(query_blocks), static_cast<T*>(x.dbias));
-        return hipGetLastError();
+        constexpr int type = sizeof(T) == 4 ? POINTOPS_F32 : __is_same(T, f16) ? POINTOPS_F16 : POINTOPS_BF16;
+        return bucket_sums(a.bk, dbias_part, a.B, a.H, static_cast<int>(query_blocks), bias_entries(a.reach),
+                           a.reach + kMargin, type, x.dbias, stream);
     }
     return hipSuccess;
 }

@@ -43,64 +43,33 @@ bool read_args(const pointops_attention* in, Args* out) {
     a.scale = in->scale;
     a.scale_log2 = in->scale * kLog2e;
     a.reach = 0;
-    a.n_edges = 0;
-    a.buckets = 0;
+    a.bk.n = a.bk.count = 0;
     if (in->bias != nullptr) {
-        if (in->edges == nullptr || in->n_edges < 1 || in->n_edges > 255) return false;
-        if (in->buckets != in->n_edges + 1 && in->buckets != 2 * (in->n_edges + 1)) return false;
-        for (int i = 0; i < in->n_edges; ++i) {
-            a.edges[i] = in->edges[i];
-            if (a.edges[i] < 1 || a.edges[i] > kMaxReach || (i > 0 && a.edges[i] < a.edges[i - 1])) return false;
-        }
-        a.n_edges = in->n_edges;
-        a.buckets = in->buckets;
-        a.reach = a.edges[a.n_edges - 1];
+        if (!read_buckets(in->edges, in->n_edges, in->buckets, kMaxReach, &a.bk)) return false;
+        a.reach = a.bk.edge[a.bk.n - 1];
     }
     return true;
 }
 
 namespace {
 
-// One query by a whole wave, key by key: for rows whose result is not finite,
-// where a product with a masked key's infinity or NaN may have spread.  Here
-// only the keys that the row sees take part (one whose score is -inf has no
-// weight and is left out).
 template <typename T>
 __device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, int len, const float* table,
                                             T* out, float* lse) {
-    const int lane = lane_id(), g = h / (a.H / a.G), p = i + a.N - a.Q;
-    const T* q = a.q.at<T>(b, h) + i * a.q.n;
-    const T* k = a.k.at<T>(b, g);
-    const T* v = a.v.at<T>(b, g);
+    const int lane = lane_id(), p = i + a.N - a.Q;
     const Seen seen = seen_by(a, p, len);
-    float m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
-    const bool d0 = lane < a.D, d1 = lane + kWave < a.D;
-    const float q0 = d0 ? to_float(q[lane]) : 0.f, q1 = d1 ? to_float(q[lane + kWave]) : 0.f;
-    auto key = [&](int64_t j) {
-        const float k0 = d0 ? to_float(k[j * a.k.n + lane]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + lane + kWave]) : 0.f;
-        float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2;
-        if (a.bias != nullptr) {
-            const int64_t off = p - j;
-            s += table[(off > a.reach ? a.reach : off < -a.reach ? -a.reach : off) + a.reach + kMargin];
-        }
-        if (s == -kInf) return;
-        const float top = fmaxf(m, s), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
-        m = top;
-        l = l * keep + w;
-        o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n + lane]) : 0.f);
-        o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + lane + kWave]) : 0.f);
+    CarefulRow<T> row(a, b, h / (a.H / a.G), a.q.at<T>(b, h) + i * a.q.n);
+    auto key = [&](int j) {
+        const int off = min(max(p - j, -a.reach), a.reach);
+        row.add(j, a.bias != nullptr ? table[off + a.reach + kMargin] : 0.f);
     };
     for (int j = 0; j < seen.first; ++j) key(j);
     for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d0) out[lane] = from_float<T>(o0 * inv);
-    if (d1) out[lane + kWave] = from_float<T>(o1 * inv);
-    if (lane == 0 && lse != nullptr) *lse = l == 0.f ? kInf : m + log2f(l);
+    const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
+    if (row.d0) out[lane] = from_float<T>(row.o0 * inv);
+    if (row.d1) out[lane + kWave] = from_float<T>(row.o1 * inv);
+    if (lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
 }
-
-// The running maximum may lie this far (in units of log 2) below the true one:
-// weights up to 2^8 cost no precision, and outputs are rescaled seldom.
-constexpr float kSlack = 8.f;
 
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Args a, T* __restrict__ out,
@@ -284,7 +253,7 @@ hipError_t forward(const pointops_attention* in, const Args& a, void* out, float
     return with_width(in->D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
         size_t lds = 2 * kInner<T> * Tile<T, DP>::kStride;
-        if (a.bias != nullptr) lds += 4 * (bias_entries(a.reach) + a.n_edges);
+        if (a.bias != nullptr) lds += 4 * (bias_entries(a.reach) + a.bk.n);
         const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
         const dim3 grid(static_cast<uint32_t>(blocks));
         if (vec)

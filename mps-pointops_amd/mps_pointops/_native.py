@@ -76,6 +76,12 @@ _SIGNATURES: dict[str, list] = {
     "pointops_group_rows_backward": [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "pointops_attention_forward": [_vp, _vp, _vp, _vp],
     "pointops_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "pointops_attention_step": [_vp, _vp, _vp, _vp],
+    "pointops_relative_bias": [_vp, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp],
+    "pointops_relative_bias_backward": [_vp, _i64, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i64, _i64,
+                                        _i64, _vp],
+    "pointops_qk_norm_rotate": [_vp, _vp, _vp, _vp],
+    "pointops_qk_norm_rotate_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "pointops_chamfer_nearest_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "pointops_chamfer_nearest_f64": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "pointops_chamfer_backward_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
@@ -99,6 +105,9 @@ _SIZE_QUERIES: dict[str, list] = {
     "pointops_ball_query_auto_workspace_bytes": [_i64, _i64, _i64],
     "pointops_group_points_backward_workspace_bytes": [_i64, _i64, _i64, _i64],
     "pointops_attention_backward_workspace_bytes": [_vp],
+    "pointops_attention_step_workspace_bytes": [_vp],
+    "pointops_relative_bias_backward_workspace_bytes": [_i64, _i64, _i64],
+    "pointops_qk_norm_rotate_backward_workspace_bytes": [_vp],
 }
 
 

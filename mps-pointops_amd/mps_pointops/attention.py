@@ -7,6 +7,10 @@ layer over such sequences asks for beside its matrix products:
 * ``window_attention``: attention within a window of the order, with a few
   first tokens that every query sees and a bias learned by buckets of the
   offset, with its gradients;
+* ``window_attention_step``: the same for one or a few new tokens over a cache;
+* ``qk_norm_rotate``: the norm of each head's query and key and their rotation
+  by the token's position in one pass, with its gradients;
+* ``relative_bias``: the learned bias as a dense tensor, with its gradient.
 
 Tensors are (batch, tokens, heads, width) in float32, float16 or bfloat16 on
 ``device='cuda'``, with any strides; fewer key heads than query heads are
@@ -238,4 +242,197 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = No
         None if lengths is None else lengths.contiguous(), edges, window, sinks, causal, float(scale))
 
 
-__all__ = ["bucket_edges", "window_attention"]
+def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor | None = None, *,
+                          window: int | None = None, sinks: int = 0, bias: Tensor | None = None,
+                          max_distance: int | None = None, scale: float | None = None) -> Tensor:
+    """``window_attention(..., causal=True)`` of one or a few new tokens a cloud
+    over its cache, without gradients.
+
+    ``k_cache, v_cache (B, N, G, D)`` hold the keys and values of the first
+    ``lengths (B,)`` positions (int32 or int64, clamped to [0, N]; None: all N),
+    the new tokens' own among them: ``q (B, Q, H, D)`` stands at the last Q of
+    those.  What lies behind a length is not read.  A query before the first
+    position yields zeros.
+    """
+    edges = _check_attention(q, k_cache, v_cache, window, sinks, True, bias, max_distance, lengths)
+    _native.require_device(q.device)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_cache, v_cache, bias)):
+        raise ValueError("window_attention_step has no gradients: call it under torch.no_grad(), "
+                         "or use window_attention")
+    q, k_cache, v_cache = _rows(q), _rows(k_cache), _rows(v_cache)
+    bias = None if bias is None else bias.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.numel():
+        args = _pack(q, k_cache, v_cache, window, sinks, True, bias, edges, lengths,
+                     q.shape[3] ** -0.5 if scale is None else float(scale))
+        size = _native.size_query("pointops_attention_step_workspace_bytes", args)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _native.call("pointops_attention_step", args, out.data_ptr(), _native.ptr(workspace),
+                     _native.stream(q.device))
+    return out
+
+
+# ------------------------------------------------------------- relative bias
+_MAX_BIAS_TOKENS = (1 << 22) - 1
+
+
+class _RelativeBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, edges, queries, keys):
+        buckets, heads = table.shape
+        out = torch.empty((heads, queries, keys), dtype=table.dtype, device=table.device)
+        if out.numel():
+            _native.call("pointops_relative_bias", table.data_ptr(), edges, len(edges), buckets, _TYPES[table.dtype],
+                         out.data_ptr(), heads, queries, keys, _native.stream(table.device))
+        ctx.rest = edges, buckets
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad: Tensor):
+        edges, buckets = ctx.rest
+        heads, queries, keys = grad.shape
+        grad = _rows(grad)
+        grad_table = torch.empty((buckets, heads), dtype=grad.dtype, device=grad.device)
+        size = _native.size_query("pointops_relative_bias_backward_workspace_bytes", heads, queries, keys)
+        workspace = torch.empty(size, dtype=torch.uint8, device=grad.device)
+        _native.call("pointops_relative_bias_backward", grad.data_ptr(), grad.stride(0), grad.stride(1), edges,
+                     len(edges), buckets, _TYPES[grad.dtype], grad_table.data_ptr(), workspace.data_ptr(),
+                     heads, queries, keys, _native.stream(grad.device))
+        return grad_table, None, None, None
+
+
+def relative_bias(table: Tensor, queries: int, keys: int, *, max_distance: int, causal: bool = False) -> Tensor:
+    """The bias that ``window_attention`` takes from ``table (buckets, H)``, as a
+    tensor ``(H, queries, keys)``: entry (h, i, j) is ``table[b, h]`` with b the
+    bucket of ``keys - queries + i - j`` (the queries stand at the last
+    positions).  ``max_distance`` may be up to 2**30 here.  Differentiable in the
+    table.
+    """
+    if not isinstance(table, Tensor):
+        raise TypeError("table must be a tensor")
+    if table.dtype not in _TYPES:
+        raise TypeError("table must be float32, float16 or bfloat16")
+    edges = _check_table(table, None, max_distance, causal, 1 << 30, "table")
+    if queries < 0 or keys < 0:
+        raise ValueError("queries and keys must be non-negative")
+    if max(queries, keys) > _MAX_BIAS_TOKENS or table.shape[1] > 65535:
+        raise ValueError(f"relative_bias supports at most {_MAX_BIAS_TOKENS} queries and keys and 65535 heads")
+    _native.require_device(table.device)
+    return _RelativeBias.apply(table.contiguous(), edges, int(queries), int(keys))
+
+
+# --------------------------------------------------------- norm and rotation
+# pointops_qk_norm of pointops_hip.h.
+_NORM_ARGS = struct.Struct("@6Q8q6q2if")
+
+
+def _pack_norm(q, k, q_weight, k_weight, cos, sin, eps) -> bytes:
+    batch, tokens, heads, width = q.shape
+    weight = q_weight if q_weight is not None else k_weight
+    return _NORM_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        *q.stride()[:3], *k.stride()[:3], 0 if cos.ndim == 2 else cos.stride(0), cos.stride(-2),
+        batch, tokens, heads, k.shape[2], width, 2 * cos.shape[-1],
+        _TYPES[q.dtype], _TYPES[q.dtype if weight is None else weight.dtype], eps)
+
+
+class _QkNormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        if q_out.numel() + k_out.numel():
+            _native.call("pointops_qk_norm_rotate", _pack_norm(q, k, q_weight, k_weight, cos, sin, eps),
+                         q_out.data_ptr(), k_out.data_ptr(), _native.stream(q.device))
+        if any(ctx.needs_input_grad[:4]):
+            ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
+            ctx.eps = eps
+        return q_out, k_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, q_grad: Tensor, k_grad: Tensor):
+        q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
+        q_grad, k_grad = _rows(q_grad), _rows(k_grad)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        weights = [w if need else None for w, need in zip((q_weight, k_weight), ctx.needs_input_grad[2:4])]
+        # A weight without a row to sum over has a gradient of zeros.
+        make = torch.empty_like if q.numel() + k.numel() else torch.zeros_like
+        dwq, dwk = (None if w is None else make(w) for w in weights)
+        if q.numel() + k.numel():
+            args = _pack_norm(q, k, q_weight, k_weight, cos, sin, ctx.eps)
+            workspace = None
+            if dwq is not None or dwk is not None:
+                size = _native.size_query("pointops_qk_norm_rotate_backward_workspace_bytes", args)
+                workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            three = ctypes.c_int64 * 3
+            _native.call("pointops_qk_norm_rotate_backward", args, q_grad.data_ptr(), three(*q_grad.stride()[:3]),
+                         k_grad.data_ptr(), three(*k_grad.stride()[:3]), dq.data_ptr(), dk.data_ptr(),
+                         _native.ptr(dwq), _native.ptr(dwk), _native.ptr(workspace), _native.stream(q.device))
+        return dq, dk, dwq, dwk, None, None, None
+
+
+def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tensor | None, cos: Tensor, sin: Tensor, *,
+                   eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """Norm and rotation of queries ``q (B, N, H, D)`` and keys ``k (B, N, G, D)``.
+
+    Each head's row x becomes ``y = x / sqrt(mean(x ** 2) + eps) * weight``
+    (weights ``(D,)`` of q's type or float32; None: ones), and of the first
+    ``R = 2 * cos.shape[-1] <= D`` values, y[i] and y[i + R / 2] turn by the
+    token's angle i::
+
+        out[i] = y[i] * cos[i] - y[i + R/2] * sin[i]
+        out[i + R/2] = y[i + R/2] * cos[i] + y[i] * sin[i]
+
+    ``cos, sin`` are float32, ``(N, R / 2)`` or ``(B, N, R / 2)``: angles of a
+    place in the order, or of a point's coordinates (a share of the R / 2 for each
+    axis).  They have no gradient.  Returns both in q's type, differentiable in
+    q, k and the weights.
+    """
+    _check_heads({"q": q, "k": k})
+    batch, tokens, heads, width = q.shape
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != width:
+        raise ValueError("k must have q's batch size, tokens and head width")
+    if not 1 <= width <= _MAX_HEAD:
+        raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
+    if max(batch, tokens, heads, k.shape[2]) > _MAX_TOKENS:
+        raise ValueError(f"sizes must be at most {_MAX_TOKENS}")
+    if not isinstance(cos, Tensor) or not isinstance(sin, Tensor):
+        raise TypeError("cos and sin must be tensors")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must be float32")
+    if cos.shape != sin.shape or cos.ndim not in (2, 3) or cos.shape[:-1] not in ((tokens,), (batch, tokens)):
+        raise ValueError("cos and sin must have shape (tokens, R / 2) or (batch, tokens, R / 2)")
+    if 2 * cos.shape[-1] > width:
+        raise ValueError("cos and sin must have at most half as many values as the head width")
+    if cos.device != q.device or sin.device != q.device:
+        raise ValueError("cos and sin must be on q's device")
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("cos and sin have no gradients here: detach them")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if not isinstance(w, Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if w.shape != (width,):
+            raise ValueError(f"{name} must have shape (width,)")
+        if w.dtype not in (q.dtype, torch.float32):
+            raise TypeError(f"{name} must have q's type or be float32")
+        if w.device != q.device:
+            raise ValueError(f"{name} must be on q's device")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError("q_weight and k_weight must have the same type")
+    _native.require_device(q.device)
+    cos, sin = _rows(cos), _rows(sin)
+    if cos.stride() != sin.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    return _QkNormRotate.apply(
+        _rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),
+        None if k_weight is None else k_weight.contiguous(), cos, sin, float(eps))
+
+
+__all__ = ["bucket_edges", "qk_norm_rotate", "relative_bias", "window_attention", "window_attention_step"]
