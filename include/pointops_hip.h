@@ -592,8 +592,9 @@ hipError_t pointops_relative_bias(const void *table, const int32_t *edges, int32
 
 /* grad_table (buckets, H) from grad (H, Q, N) with strides of head and row (the
  * last dimension contiguous), in a fixed order of additions.  `workspace` holds
- * pointops_relative_bias_backward_workspace_bytes(H, Q, N) bytes. */
-size_t pointops_relative_bias_backward_workspace_bytes(int64_t H, int64_t Q, int64_t N);
+ * pointops_relative_bias_backward_workspace_bytes(H, Q, N, buckets) bytes. */
+size_t pointops_relative_bias_backward_workspace_bytes(int64_t H, int64_t Q, int64_t N,
+                                                       int32_t buckets);
 hipError_t pointops_relative_bias_backward(const void *grad, int64_t stride_h, int64_t stride_i,
                                            const int32_t *edges, int32_t n_edges, int32_t buckets,
                                            int32_t type, void *grad_table, void *workspace,

@@ -103,11 +103,19 @@ __device__ __forceinline__ float halves_max(float v) {
     return fmaxf(i2f(r[0]), i2f(r[1]));
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) v += __shfl_xor(v, m);
+// The sum over aligned groups of L lanes, in every lane.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+    if constexpr (L >= 2) v += i2f(dpp<kDppQuadXor1>(f2i(v)));
+    if constexpr (L >= 4) v += i2f(dpp<kDppQuadXor2>(f2i(v)));
+    if constexpr (L >= 8) v += i2f(dpp<kDppRowHalfMirror>(f2i(v)));
+    if constexpr (L >= 16) v += i2f(dpp<kDppRowMirror>(f2i(v)));
+    if constexpr (L >= 32) v += __shfl_xor(v, 16);
+    if constexpr (L >= 64) v += __shfl_xor(v, 32);
     return v;
 }
+
+__device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v); }
 
 // ------------------------------------------------------------------ tiles
 // 16 bytes of a row of `width` elements from element `at` on, zeros behind its
@@ -375,11 +383,36 @@ bool vector_rows(const Rows& r, int64_t D) {
 // relative_bias.hip: reads the host's edges; false if they are none.
 bool read_buckets(const int32_t* edges, int n, int count, int64_t most, Buckets* out);
 
-// relative_bias.hip: grad[bucket][h] (type T: POINTOPS_*) from sums by offset,
-// part (B, H, blocks, entries) with offset o at entry o + zero; the first and
-// the last bucket of a side take what lies beyond it.
-hipError_t bucket_sums(const Buckets& bk, const float* part, int B, int H, int blocks, int entries, int zero, int type,
-                       void* grad, hipStream_t stream);
+// Adds a block's sums by offset (LDS, `entries` of them, offset o at entry o +
+// zero; the outermost buckets of a side take what lies beyond) by buckets:
+// dst[0 .. count - 1].  Eight lanes a bucket.
+__device__ __forceinline__ void add_buckets(const Buckets& bk, const float* sums, int entries, int zero, float* dst) {
+    const int side = bk.n + 1;
+    const bool two_sided = bk.count > side;
+    for (int first = 0; first < bk.count; first += kThreads / 8) {
+        const int bucket = first + static_cast<int>(threadIdx.x) / 8, e = bucket % side;
+        float all = 0.f;
+        if (bucket < bk.count) {
+            const int d_low = e == 0 ? 0 : bk.edge[e - 1], d_high = e == bk.n ? INT32_MAX : bk.edge[e] - 1;
+            int64_t low = static_cast<int64_t>(zero) + d_low, high = static_cast<int64_t>(zero) + d_high;
+            if (bucket >= side) {
+                low = static_cast<int64_t>(zero) - d_high;
+                high = static_cast<int64_t>(zero) - max(d_low, 1);
+            } else if (e == 0 && !two_sided) {
+                low = 0;  // later keys have no buckets of their own
+            }
+            const int from = static_cast<int>(max(low, int64_t(0))), to = static_cast<int>(min(high, int64_t(entries - 1)));
+            for (int i = from + static_cast<int>(threadIdx.x) % 8; i <= to; i += 8) all += sums[i];
+        }
+        all = group_sum<8>(all);
+        if (bucket < bk.count && threadIdx.x % 8 == 0) dst[bucket] = all;
+    }
+}
+
+// relative_bias.hip: grad[bucket][h] (of type POINTOPS_*) from part (B, H,
+// blocks, count).
+hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, void* grad,
+                        hipStream_t stream);
 
 // The device arguments of a call, and whether it is one that the kernels take.
 bool read_args(const pointops_attention* in, Args* out);

@@ -7,12 +7,12 @@
 // The weights are formed again from the scores and the forward's logarithms of
 // the sums.  Two kernels, so that every sum has one owner and a fixed order
 // (no atomics: results do not change from run to run): one holds 128 queries
-// in registers and passes over their keys (delta, dq and the bias's sums by
-// offset), the other holds 128 keys and passes over the queries that see them,
-// all heads that share the key head in turn (dk, dv).  The first keys that
-// every query sees are read by all rows: their pass is cut into pieces whose
-// 32-bit sums a last kernel joins.  ds and p are rounded to the inputs' type
-// for the second products, as the forward's weights are.
+// in registers and passes over their keys (delta, dq), the other holds 128 keys
+// and passes over the queries that see them, all heads that share the key head
+// in turn (dk, dv and the bias's sums by offset).  Long passes (the first keys,
+// which every query sees) and few blocks are cut into pieces whose 32-bit sums
+// a last kernel joins.  ds and p are rounded to the inputs' type for the second
+// products, as the forward's weights are; the bias's sums take them unrounded.
 #include <algorithm>
 #include <atomic>
 
@@ -22,14 +22,10 @@ namespace pointops {
 namespace attn {
 namespace {
 
-// Sums of ds by offset: one table a wave and half-wave (no two lanes of an
-// addition share an entry, and one wave's additions keep their order).
-constexpr int kSums = 2 * kWaves;
-
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void attention_grad_query_kernel(
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
-    float* __restrict__ delta_out, T* __restrict__ dq_out, float* __restrict__ dbias_part) {
+    float* __restrict__ delta_out, T* __restrict__ dq_out, const bool refine) {
     using TileT = Tile<T, DP>;
     constexpr int TK = kInner<T>, kOut = DP / 32;
     extern __shared__ char lds[];
@@ -44,13 +40,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const int bh = static_cast<int>(blk / blocks), b = bh / a.H, h = bh % a.H, g = h / (a.H / a.G);
     const int iblock = static_cast<int>(blocks - 1 - blk % blocks), i0 = iblock * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
-    const bool biased = a.bias != nullptr, summed = dbias_part != nullptr;
-    float* const sums = table + entries;  // kSums tables of `entries`, behind them the edges
-    if (biased) {
-        fill_bias<T>(a, h, table, reinterpret_cast<int*>(sums + (summed ? kSums * entries : 0)));
-        if (summed)
-            for (int i = threadIdx.x; i < kSums * entries; i += kThreads) sums[i] = 0.f;
-    }
+    const bool biased = a.bias != nullptr;
+    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
 
     const int rows = min(kOuter, a.Q - i0);
     const int p_first = max(i0 + shift, 0), p_last = min(i0 + shift + rows, len) - 1;
@@ -72,7 +63,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const Seen seen = seen_by(a, p, len);
 
     i32x4 q[TileT::kChunks], go[TileT::kChunks];
-    float delta = 0.f, lse = kInf;
+    float delta = 0.f, lse = kInf, rest = 0.f;
+    const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Q + row;
     {
         const T* const qrow = a.q.at<T>(b, h) + row * a.q.n;
         const T* const grow = grad.at<T>(b, h) + row * grad.n;
@@ -91,14 +83,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
             }
         }
         delta = halves_sum(delta);
-        const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Q + row;
         if (exists) lse = lse_in[stat];
-        if (row < a.Q && half == 0) delta_out[stat] = delta;
     }
     const T* const k = a.k.at<T>(b, g);
     const T* const v = a.v.at<T>(b, g);
     f32x16 dq[kOut] = {};
-    float far_early = 0.f, far_late = 0.f;  // ds of offsets beyond the reach
 
     Stage<T, DP, TK, VEC> ks, vs;
     if (t < t_end) {
@@ -158,20 +147,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                 ds[r] = w * (dp[r] - delta);
                 if (!whole && w == 0.f) ds[r] = 0.f;  // a masked key's infinity or NaN stays out
             }
-            if (summed) {
-                if (far) {
-                    float all = 0.f;
+            if (refine) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) all += ds[r];
-                    if (near > 0) far_early += all;
-                    else far_late += all;
-                } else {
-                    float* const mine = sums + (2 * wave + half) * entries + at;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(mine - (8 * (r / 4) + r % 4), ds[r], __ATOMIC_RELAXED,
-                                               __HIP_MEMORY_SCOPE_WORKGROUP);
-                }
+                for (int r = 0; r < 16; ++r) rest += ds[r];
             }
 #pragma unroll
             for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
@@ -192,37 +170,44 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
             for (int e = 0; e < 4; ++e) store4<T, VEC>(dst, 32 * d + 8 * e + 4 * half, a.D, dq[d], 4 * e);
         }
     }
-    if (summed) {
-        __syncthreads();
-        far_early = wave_sum(far_early);
-        far_late = wave_sum(far_late);
-        if (lane == 0) {
-            float* const mine = sums + 2 * wave * entries;
-            mine[entries - 1] += far_early;
-            mine[0] += far_late;
-        }
-        __syncthreads();
-        float* const dst = dbias_part + (static_cast<int64_t>(bh) * blocks + iblock) * entries;
-        for (int i = threadIdx.x; i < entries; i += kThreads) {
-            float all = 0.f;
-#pragma unroll
-            for (int w = 0; w < kSums; ++w) all += sums[w * entries + i];
-            dst[i] = all;
-        }
-    }
+    // The weights of a row sum to 1, so that what is left of its ds is what the
+    // rounded output took from delta.
+    if (refine) delta += halves_sum(rest);
+    if (row < a.Q && half == 0) delta_out[stat] = delta;
 }
 
-// A key block's share of the queries: pieces of the blocks that hold the first
-// keys, which all later rows see, and the whole range of the others.
+// How the passes of the key blocks are cut: the blocks that hold the first
+// keys, which all later rows see, into `of_first` pieces, the others into
+// `of_rest`.  Blocks in one piece write their results, the others 32-bit parts.
 struct Pieces {
-    int first_blocks;  // key blocks that are cut
-    int pieces;        // into so many
+    int first_blocks, key_blocks;
+    int of_first, of_rest;
+
+    __host__ __device__ int64_t units() const {
+        return static_cast<int64_t>(first_blocks) * of_first + static_cast<int64_t>(key_blocks - first_blocks) * of_rest;
+    }
+    __host__ __device__ int of(int block) const { return block < first_blocks ? of_first : of_rest; }
+    // The first unit of a key block.
+    __host__ __device__ int64_t unit(int block) const {
+        const int first = block < first_blocks ? block : first_blocks;
+        return static_cast<int64_t>(first) * of_first + static_cast<int64_t>(block - first) * of_rest;
+    }
+    __host__ __device__ bool joined() const { return (first_blocks > 0 && of_first > 1) || (key_blocks > first_blocks && of_rest > 1); }
 };
 
+// Sums of ds along the diagonals of a wave's 32 x 32 piece: rows (keys) are
+// written with zeros between them, so that lane x reads diagonal x - 32 of
+// every row without a test; the zeros stay for the whole kernel.  (As LDS
+// atomics, one an element, the sums took 125 us of 215 at 4 x 4096 queries, 8
+// heads, window 512, reach 121.)
+constexpr int kSkewRow = 68;
+constexpr int kSkewFloats = 32 + 32 * kSkewRow;
+
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
     const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const Rows grad,
-    T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, const Pieces cut) {
+    T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
+    const Pieces cut) {
     using TileT = Tile<T, DP>;
     constexpr int TQ = kInner<T>, kOut = DP / 32;
     extern __shared__ char lds[];
@@ -231,18 +216,20 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
     float* const stat = reinterpret_cast<float*>(lds + 2 * TQ * TileT::kStride);  // lse, then delta
     float* const table = stat + 2 * TQ;
     const int entries = bias_entries(a.reach);
+    const bool biased = a.bias != nullptr, summed = dbias_part != nullptr;
+    float* const skews = table + (entries + 3) / 4 * 4;  // one a wave, then the waves' sums by offset, the edges
+    float* const sums = skews + kWaves * kSkewFloats;
+    int* const edges = reinterpret_cast<int*>(summed ? sums + kWaves * entries : skews);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const int key_blocks = (a.N + kOuter - 1) / kOuter;
-    const uint32_t blocks = key_blocks + cut.first_blocks * (cut.pieces - 1);
+    const uint32_t units = static_cast<uint32_t>(cut.units());
     const uint32_t blk = xcd_local_block(blockIdx.x, gridDim.x);
-    const int bg = static_cast<int>(blk / blocks), b = bg / a.G, g = bg % a.G;
-    const int index = static_cast<int>(blk % blocks);
-    const bool pieced = index < cut.first_blocks * cut.pieces;
-    const int piece = pieced ? index % cut.pieces : 0;
-    const int jblock = pieced ? index / cut.pieces : index - cut.first_blocks * (cut.pieces - 1);
+    const int bg = static_cast<int>(blk / units), b = bg / a.G, g = bg % a.G;
+    const int unit = static_cast<int>(blk % units), first_units = cut.first_blocks * cut.of_first;
+    const int pieces = unit < first_units ? cut.of_first : cut.of_rest;
+    const int piece = (unit < first_units ? unit : unit - first_units) % pieces;
+    const int jblock = unit < first_units ? unit / pieces : cut.first_blocks + (unit - first_units) / pieces;
     const int j0 = jblock * kOuter, len = a.length(b), shift = a.N - a.Q;
-    const bool biased = a.bias != nullptr;
     const int group = a.H / a.G;
 
     // Queries that see any of the block's keys, by row.
@@ -257,12 +244,10 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
         i_first = max(p_low - shift, 0);
         i_last = min(p_high - shift, a.Q - 1);
     }
-    int t_first = i_first / TQ, t_end = i_last < i_first ? t_first : i_last / TQ + 1;
-    if (pieced) {
-        const int each = (t_end - t_first + cut.pieces - 1) / cut.pieces;
-        t_first = min(t_first + piece * each, t_end);
-        t_end = min(t_first + each, t_end);
-    }
+    // Their tiles, for every head in turn; this piece's share of them all.
+    const int t_first = i_first / TQ, tiles = i_last < i_first ? 0 : i_last / TQ + 1 - t_first;
+    const int64_t all_tiles = static_cast<int64_t>(tiles) * group;
+    const int64_t share_low = all_tiles * piece / pieces, share_high = all_tiles * (piece + 1) / pieces;
     const int i_low = max(-shift, 0), i_high = min(a.Q, len - shift);  // rows that exist
 
     // This wave's keys: one a lane column.
@@ -270,11 +255,16 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
     const int w_last = min(w0 + 32, len) - 1;
     const bool w_any = w0 <= w_last;
     const int j = w0 + lane % 32;
-    // The lane's key is seen from positions low .. low + count - 1.
+    // The lane's key is seen from positions low .. low + count - 1; all or any
+    // of the wave's from these.
     const bool first_key = j < a.sinks;
     const int see_low = a.causal ? j : first_key ? 0 : j - a.window + 1;
     const int see_high = first_key || j > len - a.window ? len - 1 : j + a.window - 1;
     const uint32_t see_count = static_cast<uint32_t>(max(see_high - see_low + 1, 0));
+    const int all_low = a.causal ? w_last : w_last < a.sinks ? 0 : w_last - a.window + 1;
+    const int all_high = w_last < a.sinks || w0 > len - a.window ? len - 1 : w0 + a.window - 1;
+    const int any_low = a.causal ? w0 : w0 < a.sinks ? 0 : w0 - a.window + 1;
+    const int any_high = w0 < a.sinks || w_last > len - a.window ? len - 1 : w_last + a.window - 1;
 
     i32x4 k[TileT::kChunks], v[TileT::kChunks];
     {
@@ -291,11 +281,21 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
         }
     }
     f32x16 dk[kOut] = {}, dv[kOut] = {};
+    float* const skew = skews + wave * kSkewFloats + 32;
+    float* const mine = sums + wave * entries;
+    if (summed)
+        for (int i = threadIdx.x; i < kWaves * kSkewFloats; i += kThreads) skews[i] = 0.f;
 
     for (int hh = 0; hh < group; ++hh) {
         const int h = g * group + hh;
+        const int from = t_first + static_cast<int>(max(share_low - static_cast<int64_t>(hh) * tiles, int64_t(0)));
+        const int to = t_first + static_cast<int>(min(share_high - static_cast<int64_t>(hh) * tiles, int64_t(tiles)));
+        if (from >= to && !summed) continue;
         __syncthreads();
-        if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
+        if (biased) fill_bias<T>(a, h, table, edges);
+        if (summed)
+            for (int i = threadIdx.x; i < kWaves * entries; i += kThreads) sums[i] = 0.f;
+        float far_early = 0.f, far_late = 0.f;  // ds of offsets beyond the reach
         const T* const q = a.q.at<T>(b, h);
         const T* const go = grad.at<T>(b, h);
         const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
@@ -312,21 +312,16 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
                 if (there) st = (is_lse ? lse_in : delta_in)[stats + i];
             }
         };
-        if (t_first < t_end) fetch(t_first);
-        for (int t = t_first; t < t_end; ++t) {
+        if (from < to) fetch(from);
+        for (int t = from; t < to; ++t) {
             __syncthreads();
             qs.store(qtile);
             gs.store(gtile);
             if (threadIdx.x < 2 * TQ) stat[threadIdx.x] = st;
             __syncthreads();
-            if (t + 1 < t_end) fetch(t + 1);
+            if (t + 1 < to) fetch(t + 1);
             if (!w_any) continue;
             const int p0 = t * TQ + shift;  // position of the tile's first row
-            // Positions that all, or any, of the wave's keys are seen from.
-            const int all_low = a.causal ? w_last : w_last < a.sinks ? 0 : w_last - a.window + 1;
-            const int all_high = w_last < a.sinks ? len - 1 : w0 > len - a.window ? len - 1 : w0 + a.window - 1;
-            const int any_low = a.causal ? w0 : w0 < a.sinks ? 0 : w0 - a.window + 1;
-            const int any_high = w0 < a.sinks || w_last > len - a.window ? len - 1 : w_last + a.window - 1;
             if (p0 > any_high || p0 + TQ <= any_low) continue;
             const bool whole = p0 >= all_low && p0 + TQ - 1 <= all_high;
             const int near = p0 - w0;
@@ -367,7 +362,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
                         const int r = 4 * e + f;
                         w[r] = exp2_fast(s[r] - lse[f]);
                         ds[r] = w[r] * (dp[r] - delta[f]);
-                        if (!whole && w[r] == 0.f) ds[r] = 0.f;
+                        if (!whole && w[r] == 0.f) ds[r] = 0.f;  // a masked row's infinity or NaN stays out
                     }
                 }
 #pragma unroll
@@ -379,24 +374,61 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
                         dk[d] = mma<T>(TileT::columns(qtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), y, dk[d]);
                     }
                 }
+                if (!summed) continue;
+                if (j >= len) {  // keys of zeros with scores of their own
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] = 0.f;
+                }
+                if (far) {
+                    float all = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) all += ds[r];
+                    if (near > 0) far_early += all;
+                    else far_late += all;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<f32x4*>(skew + lane % 32 * kSkewRow + 8 * e + 4 * half) =
+                            f32x4{ds[4 * e], ds[4 * e + 1], ds[4 * e + 2], ds[4 * e + 3]};
+                    float all[4] = {};
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) all[r % 4] += skew[r * (kSkewRow + 1) + lane - 32];
+                    mine[near + 32 * u + lane - 32 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
+                }
             }
+        }
+        if (summed) {
+            far_early = wave_sum(far_early);
+            far_late = wave_sum(far_late);
+            __syncthreads();  // the zeros of waves that had no tile
+            if (lane == 0) {
+                mine[entries - 1] += far_early;
+                mine[0] += far_late;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < entries; i += kThreads) {
+                float all = sums[i];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) all += sums[w * entries + i];
+                sums[i] = all;
+            }
+            __syncthreads();
+            add_buckets(a.bk, sums, entries, a.reach + kMargin,
+                        dbias_part + ((static_cast<int64_t>(b) * a.H + h) * units + unit) * a.bk.count);
         }
     }
 
-    // Keys behind the cloud's length were zeros with scores of their own: they
-    // have no gradient.
-    const float there = j < len ? 1.f : 0.f;
+    // Keys behind the cloud's length have no gradient.
 #pragma unroll
     for (int d = 0; d < kOut; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            dk[d][r] = there != 0.f ? dk[d][r] * a.scale : 0.f;
-            dv[d][r] = there != 0.f ? dv[d][r] : 0.f;
+            dk[d][r] = j < len ? dk[d][r] * a.scale : 0.f;
+            dv[d][r] = j < len ? dv[d][r] : 0.f;
         }
-    if (pieced) {
-        // (b g, first block, piece, dk or dv, key of the block, D)
-        float* const dst = part + (((static_cast<int64_t>(bg) * cut.first_blocks + jblock) * cut.pieces + piece) * 2 * kOuter +
-                                   (j - j0)) * DP;
+    if (pieces > 1) {
+        // (b g, unit, dk or dv, key of the block, DP)
+        float* const dst = part + ((static_cast<int64_t>(bg) * units + unit) * 2 * kOuter + (j - j0)) * DP;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
@@ -416,49 +448,67 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_key_kernel(
     }
 }
 
-// The pieces' sums, in their order: one thread an element.
+// The pieces' sums, in their order: a thread four values of a key.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Args a, const float* __restrict__ part, int DP,
                                                                   T* __restrict__ dk, T* __restrict__ dv,
                                                                   const Pieces cut) {
-    const int block = blockIdx.x, bg = block / cut.first_blocks, jblock = block % cut.first_blocks;
-    const int b = bg / a.G, g = bg % a.G;
-    const float* const src = part + static_cast<int64_t>(block) * cut.pieces * 2 * kOuter * DP;
-    const int at = blockIdx.y * kThreads + threadIdx.x;  // of 2 x kOuter x DP
+    const int bg = blockIdx.x / cut.key_blocks, jblock = blockIdx.x % cut.key_blocks;
+    const int b = bg / a.G, g = bg % a.G, pieces = cut.of(jblock);
+    if (pieces == 1) return;
+    const int64_t each = static_cast<int64_t>(2) * kOuter * DP;
+    const float* const src = part + (bg * cut.units() + cut.unit(jblock)) * each;
+    const int at = 4 * static_cast<int>(blockIdx.y * kThreads + threadIdx.x);  // of 2 x kOuter x DP
     const int which = at / (kOuter * DP), key = at / DP % kOuter, d = at % DP, j = jblock * kOuter + key;
     if (which > 1 || d >= a.D || j >= a.N) return;
-    float all = 0.f;
-    for (int i = 0; i < cut.pieces; ++i) all += src[static_cast<int64_t>(i) * 2 * kOuter * DP + at];
-    (which == 0 ? dk : dv)[((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D + d] = from_float<T>(all);
+    f32x4 all = {};
+    for (int i = 0; i < pieces; ++i) all += *reinterpret_cast<const f32x4*>(src + i * each + at);
+    T* const dst = (which == 0 ? dk : dv) + ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+        if (d + f < a.D) dst[d + f] = from_float<T>(all[f]);
 }
 
-// The first keys' blocks take all later rows, the others window + 128 of them
-// (two windows where later keys are seen too): pieces of about that length.
-Pieces pieces_of(const Args& a) {
-    if (a.sinks == 0 || a.N == 0) return {0, 1};
-    const int64_t rows = static_cast<int64_t>(a.causal ? 1 : 2) * a.window + kOuter;
-    const int64_t pieces = std::min<int64_t>(64, a.Q / std::max<int64_t>(rows, 512));
-    if (pieces < 2) return {0, 1};
-    return {(a.sinks + kOuter - 1) / kOuter, static_cast<int>(pieces)};
+// Blocks enough to give every compute unit two (a block's wave is alone on its
+// SIMD for the wider heads and waits for its tiles), with 4 tiles or more each;
+// the first keys' blocks in pieces about as long as the others.  At 4 x 4096
+// queries, 8 heads over 2, window 512, D 64 (256 blocks): 1 piece 127 us, 2
+// with their join 84.
+Pieces pieces_of(const Args& a, int inner) {
+    Pieces cut{0, (a.N + kOuter - 1) / kOuter, 1, 1};
+    const int64_t units = static_cast<int64_t>(cut.key_blocks) * a.B * a.G;
+    if (units == 0 || a.H == 0 || a.Q == 0) return cut;
+    const int64_t seen = std::min<int64_t>(a.Q, static_cast<int64_t>(a.causal ? 1 : 2) * a.window + kOuter);
+    const int64_t tiles = (seen + inner - 1) / inner * (a.H / a.G);
+    cut.of_rest = static_cast<int>(std::max<int64_t>(1, std::min((512 + units - 1) / units, tiles / 4)));
+    cut.of_first = cut.of_rest;
+    if (a.sinks > 0) {
+        cut.first_blocks = (a.sinks + kOuter - 1) / kOuter;
+        const int64_t first_tiles = (static_cast<int64_t>(a.Q) + inner - 1) / inner * (a.H / a.G);
+        const int64_t each = std::max<int64_t>(8, tiles / cut.of_rest);
+        cut.of_first = static_cast<int>(std::max<int64_t>(cut.of_rest, std::min<int64_t>(64, first_tiles / each)));
+    }
+    return cut;
 }
 
 int padded(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 
 struct Workspace {
+    Pieces cut;
     size_t delta, bias, part, bytes;
 };
 
-Workspace workspace_of(const Args& a) {
+Workspace workspace_of(const Args& a, int type) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t rows = static_cast<size_t>(a.B) * a.H, blocks = (static_cast<size_t>(a.Q) + kOuter - 1) / kOuter;
-    const Pieces cut = pieces_of(a);
+    const size_t rows = static_cast<size_t>(a.B) * a.H;
     Workspace w{};
+    w.cut = pieces_of(a, type == POINTOPS_F32 ? kInner<float> : kInner<f16>);
+    const size_t units = static_cast<size_t>(w.cut.units());
     w.delta = 0;
     w.bias = up(rows * a.Q * sizeof(float));
-    w.part = w.bias + (a.bias != nullptr ? up(rows * blocks * bias_entries(a.reach) * sizeof(float)) : 0);
-    w.bytes = w.part + (cut.pieces > 1 ? static_cast<size_t>(a.B) * a.G * cut.first_blocks * cut.pieces * 2 * kOuter *
-                                             padded(a.D) * sizeof(float)
-                                       : 0);
+    w.part = w.bias + (a.bias != nullptr ? up(rows * units * a.bk.count * sizeof(float)) : 0);
+    w.bytes = w.part;
+    if (w.cut.joined()) w.bytes += static_cast<size_t>(a.B) * a.G * units * 2 * kOuter * padded(a.D) * sizeof(float);
     return w;
 }
 
@@ -487,57 +537,58 @@ struct Grads {
     char* workspace;
 };
 
+template <typename T>
+constexpr int kType = sizeof(T) == 4 ? POINTOPS_F32 : __is_same(T, f16) ? POINTOPS_F16 : POINTOPS_BF16;
+
 template <typename T, int DP, bool VEC>
 hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     using TileT = Tile<T, DP>;
-    const Workspace w = workspace_of(a);
+    const Workspace w = workspace_of(a, kType<T>);
+    const Pieces cut = w.cut;
     float* const delta = reinterpret_cast<float*>(x.workspace + w.delta);
     float* const dbias_part = x.dbias != nullptr ? reinterpret_cast<float*>(x.workspace + w.bias) : nullptr;
     float* const part = reinterpret_cast<float*>(x.workspace + w.part);
-    const int64_t query_blocks = (static_cast<int64_t>(a.Q) + kOuter - 1) / kOuter;
-    const int64_t key_blocks = (static_cast<int64_t>(a.N) + kOuter - 1) / kOuter;
-    const Pieces cut = pieces_of(a);
-    const int64_t grid_q = query_blocks * a.B * a.H;
-    const int64_t grid_k = (key_blocks + static_cast<int64_t>(cut.first_blocks) * (cut.pieces - 1)) * a.B * a.G;
+    const int64_t grid_q = (static_cast<int64_t>(a.Q) + kOuter - 1) / kOuter * a.B * a.H;
+    const int64_t grid_k = cut.units() * a.B * a.G;
     if (grid_q > INT32_MAX || grid_k > INT32_MAX) return hipErrorInvalidValue;
 
     constexpr size_t tiles = 2 * kInner<T> * TileT::kStride;
-    const size_t entries = bias_entries(a.reach);
-    size_t lds = tiles;
-    if (a.bias != nullptr) lds += 4 * (entries * (x.dbias != nullptr ? 1 + kSums : 1) + a.bk.n);
-    auto* const by_query = attention_grad_query_kernel<T, DP, VEC>;
-    if (lds > kLdsFree) {
-        static std::atomic<uint64_t> allowed{0};
-        const hipError_t err = allow_lds(by_query, allowed, tiles + 4 * ((1 + kSums) * bias_entries(kMaxReach) + 255));
-        if (err != hipSuccess) return err;
-    }
+    const size_t entries = bias_entries(a.reach), table = a.bias != nullptr ? 4 * (entries + a.bk.n) : 0;
     if (grid_q > 0) {
-        hipLaunchKernelGGL(by_query, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), lds, stream, a,
-                           static_cast<const T*>(x.out), x.lse, x.grad, delta, static_cast<T*>(x.dq), dbias_part);
+        hipLaunchKernelGGL((attention_grad_query_kernel<T, DP, VEC>), dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads),
+                           tiles + table, stream, a, static_cast<const T*>(x.out), x.lse, x.grad, delta,
+                           static_cast<T*>(x.dq), dbias_part != nullptr);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
-        lds = tiles + 8 * kInner<T> + (a.bias != nullptr ? 4 * (entries + a.bk.n) : 0);
-        hipLaunchKernelGGL((attention_grad_key_kernel<T, DP, VEC>), dim3(static_cast<uint32_t>(grid_k)), dim3(kThreads),
-                           lds, stream, a, x.lse, delta, x.grad, static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, cut);
+        auto* const by_key = attention_grad_key_kernel<T, DP, VEC>;
+        // Tiles, the rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
+        auto lds_for = [&](size_t n, size_t edges) {
+            return tiles + 8 * kInner<T> + 4 * ((n + 3) / 4 * 4 + edges) +
+                   (dbias_part != nullptr ? 4 * kWaves * (kSkewFloats + n) : 0);
+        };
+        const size_t lds = a.bias != nullptr ? lds_for(entries, a.bk.n) : tiles + 8 * kInner<T>;
+        if (lds > kLdsFree) {
+            static std::atomic<uint64_t> allowed{0};
+            const hipError_t err = allow_lds(by_key, allowed, lds_for(bias_entries(kMaxReach), 255));
+            if (err != hipSuccess) return err;
+        }
+        hipLaunchKernelGGL(by_key, dim3(static_cast<uint32_t>(grid_k)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,
+                           static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, dbias_part, cut);
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
-        if (cut.pieces > 1) {
-            const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.G * cut.first_blocks),
-                            2 * kOuter * DP / kThreads);
+        if (cut.joined()) {
+            const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.G * cut.key_blocks),
+                            2 * kOuter * DP / (4 * kThreads));
             hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(kThreads), 0, stream, a, part, DP,
                                static_cast<T*>(x.dk), static_cast<T*>(x.dv), cut);
             err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
     }
-    if (x.dbias != nullptr) {
-        constexpr int type = sizeof(T) == 4 ? POINTOPS_F32 : __is_same(T, f16) ? POINTOPS_F16 : POINTOPS_BF16;
-        return bucket_sums(a.bk, dbias_part, a.B, a.H, static_cast<int>(query_blocks), bias_entries(a.reach),
-                           a.reach + kMargin, type, x.dbias, stream);
-    }
-    return hipSuccess;
+    if (dbias_part == nullptr) return hipSuccess;
+    return join_buckets(dbias_part, a.B, a.H, cut.units(), a.bk.count, kType<T>, x.dbias, stream);
 }
 
 template <typename T>
@@ -559,7 +610,7 @@ extern "C" {
 size_t pointops_attention_backward_workspace_bytes(const pointops_attention* in) {
     using namespace pointops::attn;
     Args a;
-    return read_args(in, &a) ? workspace_of(a).bytes : 0;
+    return read_args(in, &a) ? workspace_of(a, in->type).bytes : 0;
 }
 
 hipError_t pointops_attention_backward(const pointops_attention* in, const void* out, const float* lse,

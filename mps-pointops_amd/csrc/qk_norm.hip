@@ -32,18 +32,6 @@ struct NormArgs {
     float eps, inv_d;
 };
 
-// The sum over aligned groups of L lanes, in every lane.
-template <int L>
-__device__ __forceinline__ float group_sum(float v) {
-    if constexpr (L >= 2) v += i2f(dpp<kDppQuadXor1>(f2i(v)));
-    if constexpr (L >= 4) v += i2f(dpp<kDppQuadXor2>(f2i(v)));
-    if constexpr (L >= 8) v += i2f(dpp<kDppRowHalfMirror>(f2i(v)));
-    if constexpr (L >= 16) v += i2f(dpp<kDppRowMirror>(f2i(v)));
-    if constexpr (L >= 32) v += __shfl_xor(v, 16);
-    if constexpr (L >= 64) v += __shfl_xor(v, 32);
-    return v;
-}
-
 template <typename T, int VEC>
 struct Piece {
     static constexpr int kAlign = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16;

@@ -5,8 +5,8 @@
 // reads them, each once.  The forward's blocks work out the few offsets of
 // their rows once, in LDS, and copy from there.  In the backward a thread
 // walks down a few neighbouring diagonals, whose offset does not change, so
-// that the sums stay in registers and have a fixed order; a second kernel adds
-// the diagonals of each bucket.
+// that the sums stay in registers and have a fixed order; each block adds its
+// diagonals by bucket, and a second kernel the blocks.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -60,18 +60,20 @@ __global__ __launch_bounds__(kThreads) void relative_bias_kernel(const Buckets b
 }
 
 constexpr int kDiagonals = 4;   // neighbouring ones of a thread
-constexpr int kDiagRows = 128;  // rows of a block
+constexpr int kDiagRows = 64;   // rows of a block
+constexpr int kDiagSpan = kThreads * kDiagonals;
 
-// part[h][row block][offset + Q - 1]: a thread's diagonals hold key less row
-// = c .. c + 3.
+// A thread's diagonals hold key less row = c .. c + 3, down the block's rows;
+// part[h][block][bucket].
 template <typename T>
-__global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const T* __restrict__ grad, int64_t stride_h,
-                                                                      int64_t stride_i, float* __restrict__ part, int Q,
-                                                                      int N) {
+__global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buckets bk, const T* __restrict__ grad,
+                                                                      int64_t stride_h, int64_t stride_i,
+                                                                      float* __restrict__ part, int Q, int N) {
+    __shared__ float sums[kDiagSpan];  // by falling diagonal, so rising offset
     const int h = blockIdx.z, i0 = blockIdx.y * kDiagRows, i_end = min(Q, i0 + kDiagRows);
-    const int entries = Q + N - 1;
-    const int c = static_cast<int>(blockIdx.x * kThreads + threadIdx.x) * kDiagonals - (Q - 1);
-    if (c >= N) return;
+    // The block's diagonals: those that meet its rows are -(i_end - 1) .. N - 1 - i0.
+    const int c0 = static_cast<int>(blockIdx.x) * kDiagSpan - (i_end - 1);
+    const int c = c0 + static_cast<int>(threadIdx.x) * kDiagonals;
     float sum[kDiagonals] = {};
     const T* const src = grad + h * stride_h + c;
     // Rows where some, and where all, of the diagonals lie inside.
@@ -92,59 +94,37 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const T* _
         for (int e = 0; e < kDiagonals; ++e) sum[e] += to_float(v[e]);
     }
     edge(all_end, some_end);
-    float* const dst = part + (static_cast<int64_t>(h) * gridDim.y + blockIdx.y) * entries;
 #pragma unroll
-    for (int e = 0; e < kDiagonals; ++e)
-        if (c + e < N) dst[N - 1 - (c + e)] = sum[e];  // offset N - Q - c
+    for (int e = 0; e < kDiagonals; ++e) sums[kDiagSpan - 1 - (threadIdx.x * kDiagonals + e)] = sum[e];
+    __syncthreads();
+    // Diagonal c has offset N - Q - c: entry 0 is diagonal c0 + kDiagSpan - 1.
+    const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+    float* const dst = part + (h * static_cast<int64_t>(gridDim.x) * gridDim.y + block) * bk.count;
+    add_buckets(bk, sums, kDiagSpan, c0 + kDiagSpan - 1 - (N - Q), dst);
 }
 
-// One block a bucket and head.
+// Eight lanes of parts for each of 32 buckets of a head.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void bucket_sums_kernel(const Buckets bk, const float* __restrict__ part, int B,
-                                                               int blocks, int entries, int zero,
-                                                               T* __restrict__ grad) {
-    __shared__ float waves[kWaves];
-    const int H = gridDim.x, h = blockIdx.x, bucket = blockIdx.y, side = bk.n + 1, e = bucket % side;
-    const bool two_sided = bk.count > side, later = bucket >= side;
-    // The bucket's distances, then its entries.  The last one of a side has no
-    // end; the first also takes later keys that have no buckets of their own.
-    const int d_low = e == 0 ? 0 : bk.edge[e - 1];
-    int64_t low, high;
-    if (later) {
-        low = e == bk.n ? 0 : static_cast<int64_t>(zero) - (bk.edge[e] - 1);
-        high = static_cast<int64_t>(zero) - max(d_low, 1);
-    } else {
-        low = e == 0 && !two_sided ? 0 : static_cast<int64_t>(zero) + d_low;
-        high = e == bk.n ? entries - 1 : static_cast<int64_t>(zero) + bk.edge[e] - 1;
-    }
-    low = max(low, int64_t(0));
-    high = min(high, static_cast<int64_t>(entries) - 1);
+__global__ __launch_bounds__(kThreads) void join_buckets_kernel(const float* __restrict__ part, int B, int64_t blocks,
+                                                                int count, T* __restrict__ grad) {
+    constexpr int kLanes = 8, kBuckets = kThreads / kLanes;
+    __shared__ float sums[kLanes][kBuckets];
+    const int H = gridDim.x, h = blockIdx.x, x = threadIdx.x % kBuckets, y = threadIdx.x / kBuckets;
+    const int bucket = blockIdx.y * kBuckets + x;
     float all = 0.f;
-    if (low <= high) {
-        const int64_t count = high - low + 1, total = count * blocks;
+    if (bucket < count)
         for (int b = 0; b < B; ++b) {
-            const float* const src = part + (static_cast<int64_t>(b) * H + h) * blocks * entries + low;
-            int64_t at = threadIdx.x;
-            int64_t block = at / count, rest = at % count;
-            const int64_t step = kThreads / count, left = kThreads % count;
-            for (; at < total; at += kThreads) {
-                all += src[block * entries + rest];
-                block += step;
-                rest += left;
-                if (rest >= count) {
-                    rest -= count;
-                    ++block;
-                }
-            }
+            const float* const src = part + (static_cast<int64_t>(b) * H + h) * blocks * count + bucket;
+#pragma unroll 8
+            for (int64_t i = y; i < blocks; i += kLanes) all += src[i * count];
         }
-    }
-    all = wave_sum(all);
-    if (lane_id() == 0) waves[threadIdx.x / kWave] = all;
+    sums[y][x] = all;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int w = 0; w < kWaves; ++w) sum += waves[w];
-        grad[static_cast<int64_t>(bucket) * H + h] = from_float<T>(sum);
+    if (y == 0 && bucket < count) {
+        all = sums[0][x];
+#pragma unroll
+        for (int i = 1; i < kLanes; ++i) all += sums[i][x];
+        grad[static_cast<int64_t>(bucket) * H + h] = from_float<T>(all);
     }
 }
 
@@ -164,19 +144,13 @@ hipError_t launch_bias(const Buckets& bk, const void* table, void* out, int H, i
     return hipGetLastError();
 }
 
-template <typename T>
-hipError_t launch_diagonals(const void* grad, int64_t stride_h, int64_t stride_i, float* part, int H, int Q, int N,
-                            hipStream_t stream) {
-    const int per = kThreads * kDiagonals;
-    const dim3 grid(static_cast<uint32_t>((static_cast<int64_t>(Q) + N - 1 + per - 1) / per),
-                    static_cast<uint32_t>((Q + kDiagRows - 1) / kDiagRows), static_cast<uint32_t>(H));
-    hipLaunchKernelGGL(relative_bias_grad_kernel<T>, grid, dim3(kThreads), 0, stream, static_cast<const T*>(grad), stride_h,
-                       stride_i, part, Q, N);
-    return hipGetLastError();
+dim3 diagonal_grid(int64_t H, int64_t Q, int64_t N) {
+    return dim3(static_cast<uint32_t>((N + kDiagRows - 1 + kDiagSpan - 1) / kDiagSpan),
+                static_cast<uint32_t>((Q + kDiagRows - 1) / kDiagRows), static_cast<uint32_t>(H));
 }
 
 // Sizes that the kernels' launches hold.
-constexpr int64_t kBiasLimit = int64_t(1) << 22;
+constexpr int64_t kBiasLimit = int64_t(1) << 22;  // rows of 64 in a grid's second dimension
 bool bias_sizes(int64_t Q, int64_t N, int64_t H, int32_t type) {
     return Q >= 0 && N >= 0 && H >= 0 && Q < kBiasLimit && N < kBiasLimit && H <= 65535 && type >= POINTOPS_F32 &&
            type <= POINTOPS_BF16;
@@ -184,20 +158,20 @@ bool bias_sizes(int64_t Q, int64_t N, int64_t H, int32_t type) {
 
 }  // namespace
 
-hipError_t bucket_sums(const Buckets& bk, const float* part, int B, int H, int blocks, int entries, int zero, int type,
-                       void* grad, hipStream_t stream) {
-    const dim3 grid(H, bk.count);
+hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, void* grad,
+                        hipStream_t stream) {
+    const dim3 grid(H, (count + kThreads / 8 - 1) / (kThreads / 8));
     switch (type) {
         case POINTOPS_F32:
-            hipLaunchKernelGGL(bucket_sums_kernel<float>, grid, dim3(kThreads), 0, stream, bk, part, B, blocks, entries, zero,
+            hipLaunchKernelGGL(join_buckets_kernel<float>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
                                static_cast<float*>(grad));
             break;
         case POINTOPS_F16:
-            hipLaunchKernelGGL(bucket_sums_kernel<f16>, grid, dim3(kThreads), 0, stream, bk, part, B, blocks, entries, zero,
+            hipLaunchKernelGGL(join_buckets_kernel<f16>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
                                static_cast<f16*>(grad));
             break;
         default:
-            hipLaunchKernelGGL(bucket_sums_kernel<bf16>, grid, dim3(kThreads), 0, stream, bk, part, B, blocks, entries, zero,
+            hipLaunchKernelGGL(join_buckets_kernel<bf16>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
                                static_cast<bf16*>(grad));
     }
     return hipGetLastError();
@@ -224,10 +198,11 @@ hipError_t pointops_relative_bias(const void* table, const int32_t* edges, int32
     }
 }
 
-size_t pointops_relative_bias_backward_workspace_bytes(int64_t H, int64_t Q, int64_t N) {
+size_t pointops_relative_bias_backward_workspace_bytes(int64_t H, int64_t Q, int64_t N, int32_t buckets) {
     using namespace pointops::attn;
-    if (!bias_sizes(Q, N, H, POINTOPS_F32) || Q == 0 || N == 0) return 0;
-    return static_cast<size_t>(H) * ((Q + kDiagRows - 1) / kDiagRows) * (Q + N - 1) * sizeof(float);
+    if (!bias_sizes(Q, N, H, POINTOPS_F32) || Q == 0 || N == 0 || buckets < 0) return 0;
+    const dim3 grid = diagonal_grid(H, Q, N);
+    return static_cast<size_t>(H) * grid.x * grid.y * buckets * sizeof(float);
 }
 
 hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, int64_t stride_i, const int32_t* edges,
@@ -241,15 +216,18 @@ hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, i
     if (grad_table == nullptr || (Q > 0 && N > 0 && (grad == nullptr || workspace == nullptr))) return hipErrorInvalidValue;
     const int h = static_cast<int>(H), q = static_cast<int>(Q), n = static_cast<int>(N);
     float* const part = static_cast<float*>(workspace);
-    if (Q == 0 || N == 0) return bucket_sums(bk, nullptr, 0, h, 0, 0, 0, type, grad_table, stream);
-    hipError_t err;
-    switch (type) {
-        case POINTOPS_F32: err = launch_diagonals<float>(grad, stride_h, stride_i, part, h, q, n, stream); break;
-        case POINTOPS_F16: err = launch_diagonals<f16>(grad, stride_h, stride_i, part, h, q, n, stream); break;
-        default: err = launch_diagonals<bf16>(grad, stride_h, stride_i, part, h, q, n, stream);
-    }
+    if (Q == 0 || N == 0) return join_buckets(nullptr, 0, h, 0, bk.count, type, grad_table, stream);
+    const dim3 grid = diagonal_grid(H, Q, N);
+    if (grid.y > 65535) return hipErrorInvalidValue;
+    auto sums = [&](auto zero) {
+        using T = decltype(zero);
+        hipLaunchKernelGGL(relative_bias_grad_kernel<T>, grid, dim3(kThreads), 0, stream, bk, static_cast<const T*>(grad),
+                           stride_h, stride_i, part, q, n);
+        return hipGetLastError();
+    };
+    const hipError_t err = type == POINTOPS_F32 ? sums(float{}) : type == POINTOPS_F16 ? sums(f16{}) : sums(bf16{});
     if (err != hipSuccess) return err;
-    return bucket_sums(bk, part, 1, h, (q + kDiagRows - 1) / kDiagRows, q + n - 1, q - 1, type, grad_table, stream);
+    return join_buckets(part, 1, h, static_cast<int64_t>(grid.x) * grid.y, bk.count, type, grad_table, stream);
 }
 
 }  // extern "C"

@@ -106,7 +106,7 @@ _SIZE_QUERIES: dict[str, list] = {
     "pointops_group_points_backward_workspace_bytes": [_i64, _i64, _i64, _i64],
     "pointops_attention_backward_workspace_bytes": [_vp],
     "pointops_attention_step_workspace_bytes": [_vp],
-    "pointops_relative_bias_backward_workspace_bytes": [_i64, _i64, _i64],
+    "pointops_relative_bias_backward_workspace_bytes": [_i64, _i64, _i64, _i32],
     "pointops_qk_norm_rotate_backward_workspace_bytes": [_vp],
 }
 

@@ -295,7 +295,8 @@ class _RelativeBias(torch.autograd.Function):
         heads, queries, keys = grad.shape
         grad = _rows(grad)
         grad_table = torch.empty((buckets, heads), dtype=grad.dtype, device=grad.device)
-        size = _native.size_query("pointops_relative_bias_backward_workspace_bytes", heads, queries, keys)
+        size = _native.size_query("pointops_relative_bias_backward_workspace_bytes", heads, queries, keys,
+                                  buckets)
         workspace = torch.empty(size, dtype=torch.uint8, device=grad.device)
         _native.call("pointops_relative_bias_backward", grad.data_ptr(), grad.stride(0), grad.stride(1), edges,
                      len(edges), buckets, _TYPES[grad.dtype], grad_table.data_ptr(), workspace.data_ptr(),
