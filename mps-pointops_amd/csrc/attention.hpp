@@ -10,6 +10,7 @@
 // rows 8 g + 4 h + e (g, e = 0 .. 3, h = lane / 32) in register 4 g + e.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "pointops_common.hpp"
@@ -118,6 +119,8 @@ __device__ __forceinline__ float group_sum(float v) {
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v); }
 
 // ------------------------------------------------------------------ tiles
+constexpr int kRawBuffer = 0x00027000;  // word 3 of a buffer descriptor for plain bytes
+
 // 16 bytes of a row of `width` elements from element `at` on, zeros behind its
 // end.  VEC: rows are 16-byte aligned and `width` is a multiple of kPerFrag.
 template <typename T, bool VEC>
@@ -136,11 +139,14 @@ __device__ __forceinline__ i32x4 load_row(const T* row, int at, int width) {
     return r;
 }
 
-// Rows of DP elements in LDS, 16 bytes apart more than they are long: the
-// 16-byte reads of 32 rows then fall on all banks in turn.
+// Rows of DP elements in LDS, an odd number of 16-byte units apart: the row
+// operands' reads of 16 rows fall on all banks.  Rows of 256 bytes are 3 units
+// longer, as with one the transposing reads of four neighbouring rows would
+// meet in the same banks.
 template <typename T, int DP>
 struct Tile {
-    static constexpr int kStride = DP * static_cast<int>(sizeof(T)) + 16;
+    static constexpr int kBytes = DP * static_cast<int>(sizeof(T));
+    static constexpr int kStride = kBytes + (kBytes == 256 ? 48 : 16);
     static constexpr int kChunks = DP * static_cast<int>(sizeof(T)) / 32;  // of a row operand
     static constexpr int kRowsPerFrag = 2 * kPerFrag<T>;  // rows that a transposed fragment spans
 
@@ -175,7 +181,10 @@ struct Tile {
 };
 
 // A tile's way from memory to LDS through a block's registers: requested
-// while the one before is used.
+// before the one ahead of it is used.  Rows outside [first, high) and columns
+// behind the row's width are zeros: where rows allow 16-byte reads, by a buffer
+// descriptor that ends with the last row (a read behind its end returns zeros
+// and touches nothing), so that a thread's offsets are the same for all tiles.
 template <typename T, int DP, int ROWS, bool VEC>
 struct Stage {
     static constexpr int kPerRow = DP * static_cast<int>(sizeof(T)) / 16;
@@ -183,15 +192,28 @@ struct Stage {
     static_assert(ROWS * kPerRow % kThreads == 0);
     i32x4 r[kPieces];
 
-    // Rows first .. first + ROWS - 1; those outside [low, high) are zeros.
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int low, int high, int width) {
+    // Rows first .. first + ROWS - 1 of [0, high); all arguments are uniform.
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int high, int width) {
+        if constexpr (VEC) {
+            const int64_t bytes = (static_cast<int64_t>(high - 1 - first) * stride + width) * static_cast<int64_t>(sizeof(T));
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(base + first * stride), 0,
+                first < high ? static_cast<int>(min(bytes, int64_t(INT32_MAX))) : 0, kRawBuffer);
+            const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int at = i * kThreads + static_cast<int>(threadIdx.x);
-            const int row = first + at / kPerRow;
-            r[i] = i32x4{0, 0, 0, 0};
-            if (row >= low && row < high)
-                r[i] = load_row<T, VEC>(base + row * stride, at % kPerRow * kPerFrag<T>, width);
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t at = i * kThreads + threadIdx.x, col = at % kPerRow;
+                const uint32_t offset = static_cast<int>(col) * kPerFrag<T> < width ? at / kPerRow * step + col * 16 : 0x80000000u;
+                r[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int at = i * kThreads + static_cast<int>(threadIdx.x);
+                const int row = first + at / kPerRow;
+                r[i] = i32x4{0, 0, 0, 0};
+                if (row < high) r[i] = load_row<T, false>(base + row * stride, at % kPerRow * kPerFrag<T>, width);
+            }
         }
     }
     __device__ __forceinline__ void store(char* tile) const {
@@ -257,11 +279,12 @@ struct Args {
     float scale;
     Buckets bk;
 
+    // Uniform, as b is.
     __device__ __forceinline__ int length(int b) const {
         if (lengths == nullptr) return N;
         const int64_t l = length_bits == 64 ? static_cast<const int64_t*>(lengths)[b]
                                             : static_cast<const int32_t*>(lengths)[b];
-        return static_cast<int>(l < 0 ? 0 : l > N ? N : l);
+        return uniform(static_cast<int>(l < 0 ? 0 : l > N ? N : l));
     }
 };
 
@@ -285,6 +308,43 @@ __device__ __forceinline__ Seen seen_by(const Args& a, int p, int len) {
     if (p < 0 || p >= len) return {0, 0, 0};
     const int low = seen_low(a, p);
     return {low, seen_high(a, p, len) - low + 1, seen_first(a, p, len)};
+}
+
+// The tiles of `inner` keys that a block of rows sees: 0 .. first_end - 1 (the
+// first keys'), then low .. end - 1 (the window's).
+struct Walk {
+    int first_end = 0, low = 0, end = 0;
+    __device__ __forceinline__ Walk(const Args& a, int p_first, int p_last, int len, int inner) {
+        if (p_first > p_last) return;
+        first_end = (seen_first(a, p_last, len) + inner - 1) / inner;
+        low = max(first_end, seen_low(a, p_first) / inner);
+        end = max(first_end, seen_high(a, p_last, len) / inner + 1);
+    }
+    __device__ __forceinline__ int begin() const { return first_end > 0 ? 0 : low; }
+    __device__ __forceinline__ int after(int t) const { return t + 1 >= first_end && t + 1 < low ? low : t + 1; }
+};
+
+// A block's place among `outer` heads (or key heads) of `inner` blocks each.
+// The hardware deals blocks to the 8 XCDs in turn: where the heads are a
+// multiple of 8, each XCD takes an eighth of them (whose keys and values then
+// share its L2), their first blocks before their second ones.
+struct Place {
+    int outer, inner;
+};
+__device__ __forceinline__ Place place(int outer, int inner) {
+    const uint32_t id = blockIdx.x, n = static_cast<uint32_t>(outer);
+    if (n % 8 != 0) return {static_cast<int>(id % n), static_cast<int>(id / n)};
+    const uint32_t xcd = id % 8, rank = id / 8, each = n / 8;
+    return {static_cast<int>(xcd * each + rank % each), static_cast<int>(rank / each)};
+}
+
+// Block `rank` of a head's `blocks`, in the order in which they are handed out:
+// the later half from the last one down, then the earlier half from the first
+// one up.  A causal call's rows grow with their position, and blocks that meet
+// on a compute unit are then a long and a short one.
+__device__ __forceinline__ int folded(int rank, int blocks) {
+    const int late = (blocks + 1) / 2;
+    return rank < late ? blocks - 1 - rank : rank - late;
 }
 
 // ------------------------------------------------------------------- bias
@@ -373,12 +433,29 @@ hipError_t with_width(int64_t D, F f) {
     return f(std::integral_constant<int, 128>{});
 }
 
-// Whether 16-byte reads serve these rows.
+// Whether 16-byte reads through a buffer descriptor serve these rows: aligned,
+// one behind the other, and a tile of them within 2 GiB.
 template <typename T>
 bool vector_rows(const Rows& r, int64_t D) {
     const int64_t n = kPerFrag<T>;
-    return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.b % n == 0 && r.n % n == 0 && r.h % n == 0 && D % n == 0;
+    return r.n >= D && r.n < (int64_t(1) << 22) && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.b % n == 0 && r.n % n == 0 && r.h % n == 0 && D % n == 0;
 }
+
+// Allows a kernel `most` bytes of dynamic LDS, once per device (the limit belongs
+// to the process: each kernel asks for the most that any call of it needs).
+template <typename K>
+inline hipError_t allow_lds(K kernel, std::atomic<uint64_t>& allowed, size_t most) {
+    int dev = 0;
+    const hipError_t err = hipGetDevice(&dev);
+    if (err != hipSuccess) return err;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if ((allowed.load(std::memory_order_acquire) & bit) != 0) return hipSuccess;
+    const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+    if (set == hipSuccess) allowed.fetch_or(bit, std::memory_order_release);
+    return set;
+}
+constexpr size_t kLdsFree = 64 * 1024;  // what a launch may take without asking
 
 // relative_bias.hip: reads the host's edges; false if they are none.
 bool read_buckets(const int32_t* edges, int n, int count, int64_t most, Buckets* out);

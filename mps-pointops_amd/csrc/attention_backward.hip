@@ -27,32 +27,22 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
     float* __restrict__ delta_out, T* __restrict__ dq_out, const bool refine) {
     using TileT = Tile<T, DP>;
-    constexpr int TK = kInner<T>, kOut = DP / 32;
-    extern __shared__ char lds[];
-    char* const ktile = lds;
-    char* const vtile = lds + TK * TileT::kStride;
-    float* const table = reinterpret_cast<float*>(lds + 2 * TK * TileT::kStride);
+    constexpr int TK = kInner<T>, kOut = DP / 32, kTileBytes = TK * TileT::kStride;
+    extern __shared__ char lds[];  // two pairs of a key and a value tile, the bias's table
+    float* const table = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int entries = bias_entries(a.reach);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const uint32_t blocks = (a.Q + kOuter - 1) / kOuter;
-    const uint32_t blk = xcd_local_block(blockIdx.x, gridDim.x);
-    const int bh = static_cast<int>(blk / blocks), b = bh / a.H, h = bh % a.H, g = h / (a.H / a.G);
-    const int iblock = static_cast<int>(blocks - 1 - blk % blocks), i0 = iblock * kOuter;
+    const int blocks = (a.Q + kOuter - 1) / kOuter;
+    const Place at = place(a.B * a.H, blocks);
+    const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
+    const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
     const bool biased = a.bias != nullptr;
     if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
 
     const int rows = min(kOuter, a.Q - i0);
-    const int p_first = max(i0 + shift, 0), p_last = min(i0 + shift + rows, len) - 1;
-    int t = 0, t_first_end = 0, t_low = 0, t_high = -1;
-    if (p_first <= p_last) {
-        t_first_end = (seen_first(a, p_last, len) + TK - 1) / TK;
-        t_low = max(t_first_end, seen_low(a, p_first) / TK);
-        t_high = seen_high(a, p_last, len) / TK;
-        t = t_first_end > 0 ? 0 : t_low;
-    }
-    const int t_end = max(t_first_end, t_high + 1);
+    const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
 
     const int w0 = i0 + 32 * wave + shift;
     const int w_count = min(32, i0 + rows - (i0 + 32 * wave));
@@ -62,14 +52,21 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const bool exists = row < a.Q && p >= 0 && p < len;
     const Seen seen = seen_by(a, p, len);
 
+    const T* const k = a.k.at<T>(b, g);
+    const T* const v = a.v.at<T>(b, g);
+    Stage<T, DP, TK, VEC> ks, vs;
+    int t = walk.begin();
+    if (t < walk.end) {
+        ks.load(k, a.k.n, t * TK, len, a.D);
+        vs.load(v, a.v.n, t * TK, len, a.D);
+    }
     i32x4 q[TileT::kChunks], go[TileT::kChunks];
     float delta = 0.f, lse = kInf, rest = 0.f;
     const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Q + row;
     {
         const T* const qrow = a.q.at<T>(b, h) + row * a.q.n;
         const T* const grow = grad.at<T>(b, h) + row * grad.n;
-        const int64_t at = (static_cast<int64_t>(b) * a.Q + row) * a.H + h;
-        const T* const orow = out + at * a.D;
+        const T* const orow = out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
 #pragma unroll
         for (int c = 0; c < TileT::kChunks; ++c) {
             const int d = (2 * c + half) * kPerFrag<T>;
@@ -85,80 +82,78 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         delta = halves_sum(delta);
         if (exists) lse = lse_in[stat];
     }
-    const T* const k = a.k.at<T>(b, g);
-    const T* const v = a.v.at<T>(b, g);
-    f32x16 dq[kOut] = {};
-
-    Stage<T, DP, TK, VEC> ks, vs;
-    if (t < t_end) {
-        ks.load(k, a.k.n, t * TK, 0, len, a.D);
-        vs.load(v, a.v.n, t * TK, 0, len, a.D);
+    if (t < walk.end) {
+        ks.store(lds);
+        vs.store(lds + kTileBytes);
     }
-    while (t < t_end) {
-        __syncthreads();
-        ks.store(ktile);
-        vs.store(vtile);
-        __syncthreads();
+    __syncthreads();
+
+    const float factor = biased ? 1.f : a.scale_log2;
+    f32x16 dq[kOut] = {};
+    char* ktile = lds;
+    while (t < walk.end) {
+        char* const vtile = ktile + kTileBytes;
         const int j0 = t * TK;
-        ++t;
-        if (t >= t_first_end && t < t_low) t = t_low;
-        if (t < t_end) {
-            ks.load(k, a.k.n, t * TK, 0, len, a.D);
-            vs.load(v, a.v.n, t * TK, 0, len, a.D);
+        t = walk.after(t);
+        if (t < walk.end) {
+            ks.load(k, a.k.n, t * TK, len, a.D);
+            vs.load(v, a.v.n, t * TK, len, a.D);
         }
-        if (!w_any) continue;
-        const bool meets = (j0 <= seen_high(a, w_last, len) && j0 + TK > seen_low(a, w_first)) ||
-                           j0 < seen_first(a, w_last, len);
-        if (!meets) continue;
-        const bool whole = w_whole && ((j0 + TK - 1 <= seen_high(a, w_first, len) && j0 >= seen_low(a, w_last)) ||
-                                       j0 + TK <= seen_first(a, w_first, len));
-        const int near = w0 - j0;
-        const bool far = near - (TK - 1) >= a.reach || near + 31 <= -a.reach;
+        const bool meets = w_any && ((j0 <= seen_high(a, w_last, len) && j0 + TK > seen_low(a, w_first)) ||
+                                     j0 < seen_first(a, w_last, len));
+        if (meets) {
+            const bool whole = w_whole && ((j0 + TK - 1 <= seen_high(a, w_first, len) && j0 >= seen_low(a, w_last)) ||
+                                           j0 + TK <= seen_first(a, w_first, len));
+            const int near = w0 - j0;
+            const bool far = near - (TK - 1) >= a.reach || near + 31 <= -a.reach;
 #pragma unroll
-        for (int u = 0; u < TK / 32; ++u) {
-            f32x16 s = {}, dp = {};
+            for (int u = 0; u < TK / 32; ++u) {
+                f32x16 s = {}, dp = {};
 #pragma unroll
-            for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], s);
+                for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], s);
 #pragma unroll
-            for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(vtile, 32 * u, c), go[c], dp);
+                for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(vtile, 32 * u, c), go[c], dp);
+                if (biased) {
+                    s *= a.scale_log2;
+                    if (far) {
+                        s += table[near > 0 ? entries - 1 : 0];
+                    } else {
+                        const float* const from = table + near + lane % 32 - 4 * half - 32 * u + a.reach + kMargin;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= a.scale_log2;
-            const int at = near + lane % 32 - 4 * half - 32 * u + a.reach + kMargin;
-            if (biased) {
-                if (far) {
-                    const float add = table[near > 0 ? entries - 1 : 0];
+                        for (int r = 0; r < 16; ++r) s[r] += from[-(8 * (r / 4) + r % 4)];
+                    }
+                }
+                float ds[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] += add;
-                } else {
+                for (int r = 0; r < 16; ++r) {
+                    float w = exp2_fast(__builtin_fmaf(s[r], factor, -lse));
+                    ds[r] = w * (dp[r] - delta);
+                }
+                if (!whole) {
+                    const int j = j0 + 32 * u + 4 * half;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] += table[at - (8 * (r / 4) + r % 4)];
+                    for (int r = 0; r < 16; ++r)
+                        if (!seen(j + 8 * (r / 4) + r % 4)) ds[r] = 0.f;
+                }
+                if (refine) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) rest += ds[r];
+                }
+#pragma unroll
+                for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
+                    const i32x4 x = as_fragment<T>(&ds[c * kPerFrag<T>]);
+#pragma unroll
+                    for (int d = 0; d < kOut; ++d)
+                        dq[d] = mma<T>(TileT::columns(ktile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, dq[d]);
                 }
             }
-            if (!whole) {
-                const int j = j0 + 32 * u + 4 * half;
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!seen(j + 8 * (r / 4) + r % 4)) s[r] = -kInf;
-            }
-            float ds[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float w = exp2_fast(s[r] - lse);
-                ds[r] = w * (dp[r] - delta);
-                if (!whole && w == 0.f) ds[r] = 0.f;  // a masked key's infinity or NaN stays out
-            }
-            if (refine) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) rest += ds[r];
-            }
-#pragma unroll
-            for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                const i32x4 w = as_fragment<T>(&ds[c * kPerFrag<T>]);
-#pragma unroll
-                for (int d = 0; d < kOut; ++d)
-                    dq[d] = mma<T>(TileT::columns(ktile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), w, dq[d]);
-            }
         }
+        ktile = ktile == lds ? lds + 2 * kTileBytes : lds;
+        if (t < walk.end) {
+            ks.store(ktile);
+            vs.store(ktile + kTileBytes);
+        }
+        __syncthreads();
     }
 
     if (row < a.Q) {
@@ -195,13 +190,13 @@ struct Pieces {
     __host__ __device__ bool joined() const { return (first_blocks > 0 && of_first > 1) || (key_blocks > first_blocks && of_rest > 1); }
 };
 
-// Sums of ds along the diagonals of a wave's 32 x 32 piece: rows (keys) are
-// written with zeros between them, so that lane x reads diagonal x - 32 of
+// Sums of ds along the diagonals of a wave's 16 x 32 piece: rows (keys) are
+// written with zeros between them, so that lane x reads diagonal x - 16 of
 // every row without a test; the zeros stay for the whole kernel.  (As LDS
 // atomics, one an element, the sums took 125 us of 215 at 4 x 4096 queries, 8
-// heads, window 512, reach 121.)
+// heads, window 512, reach 91.)
 constexpr int kSkewRow = 68;
-constexpr int kSkewFloats = 32 + 32 * kSkewRow;
+constexpr int kSkewFloats = 16 + 16 * kSkewRow;
 
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
@@ -209,12 +204,10 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
     const Pieces cut) {
     using TileT = Tile<T, DP>;
-    constexpr int TQ = kInner<T>, kOut = DP / 32;
-    extern __shared__ char lds[];
-    char* const qtile = lds;
-    char* const gtile = lds + TQ * TileT::kStride;
-    float* const stat = reinterpret_cast<float*>(lds + 2 * TQ * TileT::kStride);  // lse, then delta
-    float* const table = stat + 2 * TQ;
+    constexpr int TQ = kInner<T>, kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
+    constexpr int kSet = 2 * kTileBytes + 8 * TQ;  // a tile of queries, one of gradients, their lse and delta
+    extern __shared__ char lds[];                  // two sets, then the bias's tables
+    float* const table = reinterpret_cast<float*>(lds + 2 * kSet);
     const int entries = bias_entries(a.reach);
     const bool biased = a.bias != nullptr, summed = dbias_part != nullptr;
     float* const skews = table + (entries + 3) / 4 * 4;  // one a wave, then the waves' sums by offset, the edges
@@ -222,17 +215,21 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     int* const edges = reinterpret_cast<int*>(summed ? sums + kWaves * entries : skews);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const uint32_t units = static_cast<uint32_t>(cut.units());
-    const uint32_t blk = xcd_local_block(blockIdx.x, gridDim.x);
-    const int bg = static_cast<int>(blk / units), b = bg / a.G, g = bg % a.G;
-    const int unit = static_cast<int>(blk % units), first_units = cut.first_blocks * cut.of_first;
+    const int units = static_cast<int>(cut.units());
+    const Place at = place(a.B * a.G, units);
+    const int bg = at.outer, b = bg / a.G, g = bg % a.G;
+    // The first keys' pieces, then the others (a causal call's earlier keys are seen by more rows).
+    const int first_units = cut.first_blocks * cut.of_first;
+    const int unit = at.inner < first_units ? at.inner : units - 1 - folded(at.inner - first_units, units - first_units);
     const int pieces = unit < first_units ? cut.of_first : cut.of_rest;
     const int piece = (unit < first_units ? unit : unit - first_units) % pieces;
     const int jblock = unit < first_units ? unit / pieces : cut.first_blocks + (unit - first_units) / pieces;
     const int j0 = jblock * kOuter, len = a.length(b), shift = a.N - a.Q;
     const int group = a.H / a.G;
 
-    // Queries that see any of the block's keys, by row.
+    // Queries that see any of the block's keys, by row; tiles count from the
+    // first row that exists.
+    const int i_low = max(-shift, 0), i_high = min(a.Q, len - shift);
     const int j_last = min(j0 + kOuter, len) - 1;
     int i_first = 0, i_last = -1;
     if (j_last >= j0) {
@@ -241,14 +238,13 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         int p_high = first || j_last > len - a.window ? len - 1 : j_last + a.window - 1;
         p_low = max(p_low, 0);
         p_high = min(p_high, len - 1);
-        i_first = max(p_low - shift, 0);
-        i_last = min(p_high - shift, a.Q - 1);
+        i_first = max(p_low - shift, i_low);
+        i_last = min(p_high - shift, i_high - 1);
     }
     // Their tiles, for every head in turn; this piece's share of them all.
-    const int t_first = i_first / TQ, tiles = i_last < i_first ? 0 : i_last / TQ + 1 - t_first;
+    const int t_first = (i_first - i_low) / TQ, tiles = i_last < i_first ? 0 : (i_last - i_low) / TQ + 1 - t_first;
     const int64_t all_tiles = static_cast<int64_t>(tiles) * group;
     const int64_t share_low = all_tiles * piece / pieces, share_high = all_tiles * (piece + 1) / pieces;
-    const int i_low = max(-shift, 0), i_high = min(a.Q, len - shift);  // rows that exist
 
     // This wave's keys: one a lane column.
     const int w0 = j0 + 32 * wave;
@@ -281,7 +277,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         }
     }
     f32x16 dk[kOut] = {}, dv[kOut] = {};
-    float* const skew = skews + wave * kSkewFloats + 32;
+    float* const skew = skews + wave * kSkewFloats + 16;
+    const float factor = biased ? 1.f : a.scale_log2;
     float* const mine = sums + wave * entries;
     if (summed)
         for (int i = threadIdx.x; i < kWaves * kSkewFloats; i += kThreads) skews[i] = 0.f;
@@ -302,105 +299,116 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         Stage<T, DP, TQ, VEC> qs, gs;
         float st = 0.f;
         auto fetch = [&](int t) {
-            qs.load(q, a.q.n, t * TQ, i_low, i_high, a.D);
-            gs.load(go, grad.n, t * TQ, i_low, i_high, a.D);
+            const int i0 = i_low + t * TQ;
+            qs.load(q, a.q.n, i0, i_high, a.D);
+            gs.load(go, grad.n, i0, i_high, a.D);
             if (threadIdx.x < 2 * TQ) {
                 const bool is_lse = threadIdx.x < TQ;
-                const int i = t * TQ + threadIdx.x % TQ;
-                const bool there = i >= i_low && i < i_high;
+                const int i = i0 + threadIdx.x % TQ;
                 st = is_lse ? kInf : 0.f;
-                if (there) st = (is_lse ? lse_in : delta_in)[stats + i];
+                if (i < i_high) st = (is_lse ? lse_in : delta_in)[stats + i];
             }
         };
-        if (from < to) fetch(from);
+        char* set = lds;
+        auto put = [&] {
+            qs.store(set);
+            gs.store(set + kTileBytes);
+            if (threadIdx.x < 2 * TQ) reinterpret_cast<float*>(set + 2 * kTileBytes)[threadIdx.x] = st;
+        };
+        if (from < to) {
+            fetch(from);
+            put();
+        }
+        __syncthreads();
         for (int t = from; t < to; ++t) {
-            __syncthreads();
-            qs.store(qtile);
-            gs.store(gtile);
-            if (threadIdx.x < 2 * TQ) stat[threadIdx.x] = st;
-            __syncthreads();
             if (t + 1 < to) fetch(t + 1);
-            if (!w_any) continue;
-            const int p0 = t * TQ + shift;  // position of the tile's first row
-            if (p0 > any_high || p0 + TQ <= any_low) continue;
-            const bool whole = p0 >= all_low && p0 + TQ - 1 <= all_high;
-            const int near = p0 - w0;
-            const bool far = near - 31 >= a.reach || near + TQ - 1 <= -a.reach;
+            const char* const qtile = set;
+            const char* const gtile = set + kTileBytes;
+            const float* const stat = reinterpret_cast<const float*>(set + 2 * kTileBytes);
+            const int p0 = i_low + t * TQ + shift;  // position of the tile's first row
+            if (w_any && p0 <= any_high && p0 + TQ > any_low) {
+                const bool whole = p0 >= all_low && p0 + TQ - 1 <= all_high;
+                const int near = p0 - w0;
+                const bool far = near - 31 >= a.reach || near + TQ - 1 <= -a.reach;
 #pragma unroll
-            for (int u = 0; u < TQ / 32; ++u) {
-                f32x16 s = {}, dp = {};
+                for (int u = 0; u < TQ / 32; ++u) {
+                    f32x16 s = {}, dp = {};
 #pragma unroll
-                for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(qtile, 32 * u, c), k[c], s);
+                    for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(qtile, 32 * u, c), k[c], s);
 #pragma unroll
-                for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(gtile, 32 * u, c), v[c], dp);
+                    for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(gtile, 32 * u, c), v[c], dp);
+                    if (biased) {
+                        s *= a.scale_log2;
+                        if (far) {
+                            s += table[near > 0 ? entries - 1 : 0];
+                        } else {
+                            const float* const from = table + near - lane % 32 + 4 * half + 32 * u + a.reach + kMargin;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= a.scale_log2;
-                if (biased) {
+                            for (int r = 0; r < 16; ++r) s[r] += from[8 * (r / 4) + r % 4];
+                        }
+                    }
+                    float w[16], ds[16];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4 lse = *reinterpret_cast<const f32x4*>(stat + 32 * u + 8 * e + 4 * half);
+                        const f32x4 delta = *reinterpret_cast<const f32x4*>(stat + TQ + 32 * u + 8 * e + 4 * half);
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+                            const int r = 4 * e + f;
+                            w[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[f]));
+                            ds[r] = w[r] * (dp[r] - delta[f]);
+                        }
+                    }
+                    if (!whole) {
+                        const int p = p0 + 32 * u + 4 * half - see_low;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) w[r] = ds[r] = 0.f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
+                        const i32x4 x = as_fragment<T>(&w[c * kPerFrag<T>]), y = as_fragment<T>(&ds[c * kPerFrag<T>]);
+#pragma unroll
+                        for (int d = 0; d < kOut; ++d) {
+                            dv[d] = mma<T>(TileT::columns(gtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, dv[d]);
+                            dk[d] = mma<T>(TileT::columns(qtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), y, dk[d]);
+                        }
+                    }
+                    if (!summed) continue;
+                    if (j >= len) {  // keys of zeros with scores of their own
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) ds[r] = 0.f;
+                    }
                     if (far) {
-                        const float add = table[near > 0 ? entries - 1 : 0];
+                        float all = 0.f;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] += add;
+                        for (int r = 0; r < 16; ++r) all += ds[r];
+                        if (near > 0) far_early += all;
+                        else far_late += all;
                     } else {
-                        const float* const at = table + near - lane % 32 + 4 * half + 32 * u + a.reach + kMargin;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] += at[8 * (r / 4) + r % 4];
+                        for (int x = 0; x < 2; ++x) {
+                            if (lane % 32 / 16 == x) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    *reinterpret_cast<f32x4*>(skew + lane % 16 * kSkewRow + 8 * e + 4 * half) =
+                                        f32x4{ds[4 * e], ds[4 * e + 1], ds[4 * e + 2], ds[4 * e + 3]};
+                            }
+                            float all[4] = {};
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) all[r % 4] += skew[r * (kSkewRow + 1) + lane - 16];
+                            mine[near + 32 * u - 16 * x + lane - 16 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
+                        }
                     }
-                }
-                if (!whole) {
-                    const int p = p0 + 32 * u + 4 * half - see_low;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) s[r] = -kInf;
-                }
-                float w[16], ds[16];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f32x4 lse = *reinterpret_cast<const f32x4*>(stat + 32 * u + 8 * e + 4 * half);
-                    const f32x4 delta = *reinterpret_cast<const f32x4*>(stat + TQ + 32 * u + 8 * e + 4 * half);
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        const int r = 4 * e + f;
-                        w[r] = exp2_fast(s[r] - lse[f]);
-                        ds[r] = w[r] * (dp[r] - delta[f]);
-                        if (!whole && w[r] == 0.f) ds[r] = 0.f;  // a masked row's infinity or NaN stays out
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                    const i32x4 x = as_fragment<T>(&w[c * kPerFrag<T>]), y = as_fragment<T>(&ds[c * kPerFrag<T>]);
-#pragma unroll
-                    for (int d = 0; d < kOut; ++d) {
-                        dv[d] = mma<T>(TileT::columns(gtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, dv[d]);
-                        dk[d] = mma<T>(TileT::columns(qtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), y, dk[d]);
-                    }
-                }
-                if (!summed) continue;
-                if (j >= len) {  // keys of zeros with scores of their own
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ds[r] = 0.f;
-                }
-                if (far) {
-                    float all = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) all += ds[r];
-                    if (near > 0) far_early += all;
-                    else far_late += all;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<f32x4*>(skew + lane % 32 * kSkewRow + 8 * e + 4 * half) =
-                            f32x4{ds[4 * e], ds[4 * e + 1], ds[4 * e + 2], ds[4 * e + 3]};
-                    float all[4] = {};
-#pragma unroll
-                    for (int r = 0; r < 32; ++r) all[r % 4] += skew[r * (kSkewRow + 1) + lane - 32];
-                    mine[near + 32 * u + lane - 32 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
                 }
             }
+            set = set == lds ? lds + kSet : lds;
+            if (t + 1 < to) put();
+            __syncthreads();
         }
         if (summed) {
             far_early = wave_sum(far_early);
             far_late = wave_sum(far_late);
-            __syncthreads();  // the zeros of waves that had no tile
             if (lane == 0) {
                 mine[entries - 1] += far_early;
                 mine[0] += far_late;
@@ -512,23 +520,6 @@ Workspace workspace_of(const Args& a, int type) {
     return w;
 }
 
-// Allows a kernel the LDS that its largest bias tables need, once per device
-// (the limit belongs to the process).
-template <typename K>
-hipError_t allow_lds(K kernel, std::atomic<uint64_t>& allowed, size_t most) {
-    int dev = 0;
-    const hipError_t err = hipGetDevice(&dev);
-    if (err != hipSuccess) return err;
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if ((allowed.load(std::memory_order_acquire) & bit) != 0) return hipSuccess;
-    const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
-    if (set == hipSuccess) allowed.fetch_or(bit, std::memory_order_release);
-    return set;
-}
-
-constexpr size_t kLdsFree = 64 * 1024;  // what a launch may take without asking
-
 struct Grads {
     const void* out;
     const float* lse;
@@ -552,26 +543,31 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     const int64_t grid_k = cut.units() * a.B * a.G;
     if (grid_q > INT32_MAX || grid_k > INT32_MAX) return hipErrorInvalidValue;
 
-    constexpr size_t tiles = 2 * kInner<T> * TileT::kStride;
+    constexpr size_t tiles = 4 * kInner<T> * TileT::kStride, stats = 16 * kInner<T>;
     const size_t entries = bias_entries(a.reach), table = a.bias != nullptr ? 4 * (entries + a.bk.n) : 0;
     if (grid_q > 0) {
-        hipLaunchKernelGGL((attention_grad_query_kernel<T, DP, VEC>), dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads),
-                           tiles + table, stream, a, static_cast<const T*>(x.out), x.lse, x.grad, delta,
+        auto* const by_query = attention_grad_query_kernel<T, DP, VEC>;
+        if (tiles + table > kLdsFree) {
+            static std::atomic<uint64_t> allowed{0};
+            const hipError_t err = allow_lds(by_query, allowed, tiles + 4 * (bias_entries(kMaxReach) + 255));
+            if (err != hipSuccess) return err;
+        }
+        hipLaunchKernelGGL(by_query, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), tiles + table, stream, a,
+                           static_cast<const T*>(x.out), x.lse, x.grad, delta,
                            static_cast<T*>(x.dq), dbias_part != nullptr);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
         auto* const by_key = attention_grad_key_kernel<T, DP, VEC>;
-        // Tiles, the rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
-        auto lds_for = [&](size_t n, size_t edges) {
-            return tiles + 8 * kInner<T> + 4 * ((n + 3) / 4 * 4 + edges) +
-                   (dbias_part != nullptr ? 4 * kWaves * (kSkewFloats + n) : 0);
+        // The tiles, their rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
+        auto lds_for = [&](size_t n, size_t edges, bool sums) {
+            return tiles + stats + 4 * ((n + 3) / 4 * 4 + edges) + (sums ? 4 * kWaves * (kSkewFloats + n) : 0);
         };
-        const size_t lds = a.bias != nullptr ? lds_for(entries, a.bk.n) : tiles + 8 * kInner<T>;
+        const size_t lds = a.bias != nullptr ? lds_for(entries, a.bk.n, dbias_part != nullptr) : tiles + stats;
         if (lds > kLdsFree) {
             static std::atomic<uint64_t> allowed{0};
-            const hipError_t err = allow_lds(by_key, allowed, lds_for(bias_entries(kMaxReach), 255));
+            const hipError_t err = allow_lds(by_key, allowed, lds_for(bias_entries(kMaxReach), 255, true));
             if (err != hipSuccess) return err;
         }
         hipLaunchKernelGGL(by_key, dim3(static_cast<uint32_t>(grid_k)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,

@@ -76,31 +76,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
                                                                         float* __restrict__ lse_out) {
     using TileT = Tile<T, DP>;
     constexpr int TK = kInner<T>, kSub = TK / 32, kOut = DP / 32;
-    extern __shared__ char lds[];
-    char* const ktile = lds;
-    char* const vtile = lds + TK * TileT::kStride;
-    float* const table = reinterpret_cast<float*>(lds + 2 * TK * TileT::kStride);
+    constexpr int kTileBytes = TK * TileT::kStride;
+    extern __shared__ char lds[];  // two pairs of a key and a value tile, the bias's table
+    float* const table = reinterpret_cast<float*>(lds + 4 * kTileBytes);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const uint32_t blocks = (a.Q + kOuter - 1) / kOuter;
-    const uint32_t blk = xcd_local_block(blockIdx.x, gridDim.x);
-    const int bh = static_cast<int>(blk / blocks), b = bh / a.H, h = bh % a.H, g = h / (a.H / a.G);
-    const int i0 = static_cast<int>(blocks - 1 - blk % blocks) * kOuter;  // the longest rows of a causal call first
+    const int blocks = (a.Q + kOuter - 1) / kOuter;
+    const Place at = place(a.B * a.H, blocks);
+    const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
+    const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
     const bool biased = a.bias != nullptr;
     if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
 
     // The block's rows that exist, by position, and the tiles that they see.
     const int rows = min(kOuter, a.Q - i0);
-    const int p_first = max(i0 + shift, 0), p_last = min(i0 + shift + rows, len) - 1;
-    int t = 0, t_first_end = 0, t_low = 0, t_high = -1;
-    if (p_first <= p_last) {
-        t_first_end = (seen_first(a, p_last, len) + TK - 1) / TK;
-        t_low = max(t_first_end, seen_low(a, p_first) / TK);
-        t_high = seen_high(a, p_last, len) / TK;
-        t = t_first_end > 0 ? 0 : t_low;
-    }
-    const int t_end = max(t_first_end, t_high + 1);  // one past the last tile
+    const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
 
     // This wave's rows.
     const int w0 = i0 + 32 * wave + shift;  // position of its first row
@@ -110,6 +101,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
     const int row = i0 + 32 * wave + lane % 32, p = row + shift;
     const Seen seen = seen_by(a, p, len);
 
+    const T* const k = a.k.at<T>(b, g);
+    const T* const v = a.v.at<T>(b, g);
+    Stage<T, DP, TK, VEC> ks, vs;
+    int t = walk.begin();
+    if (t < walk.end) {
+        ks.load(k, a.k.n, t * TK, len, a.D);
+        vs.load(v, a.v.n, t * TK, len, a.D);
+    }
     i32x4 q[TileT::kChunks];
     {
         const T* src = a.q.at<T>(b, h) + row * a.q.n;
@@ -119,101 +118,104 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
             if (row < a.Q) q[c] = load_row<T, VEC>(src, (2 * c + half) * kPerFrag<T>, a.D);
         }
     }
-    const T* const k = a.k.at<T>(b, g);
-    const T* const v = a.v.at<T>(b, g);
-    f32x16 o[kOut] = {};
-    float m = -kInf, l = 0.f;  // the maximum so far (see kSlack) and this half-wave's sum
-
-    Stage<T, DP, TK, VEC> ks, vs;
-    if (t < t_end) {
-        ks.load(k, a.k.n, t * TK, 0, len, a.D);
-        vs.load(v, a.v.n, t * TK, 0, len, a.D);
+    if (t < walk.end) {
+        ks.store(lds);
+        vs.store(lds + kTileBytes);
     }
-    while (t < t_end) {
-        __syncthreads();
-        ks.store(ktile);
-        vs.store(vtile);
-        __syncthreads();
-        const int j0 = t * TK;
-        ++t;
-        if (t >= t_first_end && t < t_low) t = t_low;
-        if (t < t_end) {
-            ks.load(k, a.k.n, t * TK, 0, len, a.D);
-            vs.load(v, a.v.n, t * TK, 0, len, a.D);
-        }
-        if (!w_any) continue;
-        const bool meets = (j0 <= seen_high(a, w_last, len) && j0 + TK > seen_low(a, w_first)) ||
-                           j0 < seen_first(a, w_last, len);
-        if (!meets) continue;
-        const bool whole = w_whole && ((j0 + TK - 1 <= seen_high(a, w_first, len) && j0 >= seen_low(a, w_last)) ||
-                                       j0 + TK <= seen_first(a, w_first, len));
+    __syncthreads();
 
-        float s[kSub][16];
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-            f32x16 acc = {};
-#pragma unroll
-            for (int c = 0; c < TileT::kChunks; ++c) acc = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], acc);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = acc[r] * a.scale_log2;
+    // Scores as the products leave them, in units of 1 / factor: a bias needs
+    // them scaled, and a negative scale turns their order.
+    const bool scaled = biased || !(a.scale > 0.f);
+    const float factor = scaled ? 1.f : a.scale_log2;
+    f32x16 o[kOut] = {};
+    float m = -kInf, l = 0.f;  // the maximum so far (scaled; see kSlack) and this half-wave's sum
+    char* ktile = lds;
+    while (t < walk.end) {
+        char* const vtile = ktile + kTileBytes;
+        const int j0 = t * TK;
+        t = walk.after(t);
+        if (t < walk.end) {
+            ks.load(k, a.k.n, t * TK, len, a.D);
+            vs.load(v, a.v.n, t * TK, len, a.D);
         }
-        if (biased) {
-            const int near = w0 - j0;  // offset of the wave's first row and the tile's first key
-            if (near - (TK - 1) >= a.reach || near + 31 <= -a.reach) {
-                const float far = table[near > 0 ? bias_entries(a.reach) - 1 : 0];
+        const bool meets = w_any && ((j0 <= seen_high(a, w_last, len) && j0 + TK > seen_low(a, w_first)) ||
+                                     j0 < seen_first(a, w_last, len));
+        if (meets) {
+            const bool whole = w_whole && ((j0 + TK - 1 <= seen_high(a, w_first, len) && j0 >= seen_low(a, w_last)) ||
+                                           j0 + TK <= seen_first(a, w_first, len));
+            f32x16 s[kSub];
 #pragma unroll
-                for (int u = 0; u < kSub; ++u)
+            for (int u = 0; u < kSub; ++u) {
+                s[u] = f32x16{};
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] += far;
-            } else {
-                const float* at = table + near + lane % 32 - 4 * half + a.reach + kMargin;
-#pragma unroll
-                for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] += at[-(32 * u + 8 * (r / 4) + r % 4)];
+                for (int c = 0; c < TileT::kChunks; ++c) s[u] = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], s[u]);
             }
-        }
-        if (!whole) {
-            const int j = j0 + 4 * half;
+            if (scaled) {
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) s[u] *= a.scale_log2;
+            }
+            if (biased) {
+                const int near = w0 - j0;  // offset of the wave's first row and the tile's first key
+                if (near - (TK - 1) >= a.reach || near + 31 <= -a.reach) {
+                    const float far = table[near > 0 ? bias_entries(a.reach) - 1 : 0];
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u) s[u] += far;
+                } else {
+                    const float* from = table + near + lane % 32 - 4 * half + a.reach + kMargin;
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[u][r] += from[-(32 * u + 8 * (r / 4) + r % 4)];
+                }
+            }
+            if (!whole) {
+                const int j = j0 + 4 * half;
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!seen(j + 32 * u + 8 * (r / 4) + r % 4)) s[u][r] = -kInf;
+            }
+            float top = s[0][0];
 #pragma unroll
             for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!seen(j + 32 * u + 8 * (r / 4) + r % 4)) s[u][r] = -kInf;
-        }
-        float top = s[0][0];
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = halves_max(top) * factor;
+            if (ballot(top > m + kSlack) != 0) {
+                const float next = fmaxf(m, top);
+                const float keep = m == next ? 1.f : exp2_fast(m - next);
+                m = next;
+                l *= keep;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-        top = halves_max(top);
-        if (ballot(top > m + kSlack) != 0) {
-            const float next = fmaxf(m, top);
-            const float keep = m == next ? 1.f : exp2_fast(m - next);
-            m = next;
-            l *= keep;
-#pragma unroll
-            for (int d = 0; d < kOut; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= keep;
-        }
-        const float base = m == -kInf ? 0.f : m;
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[u][r] = exp2_fast(s[u][r] - base);
-                l += s[u][r];
+                for (int d = 0; d < kOut; ++d) o[d] *= keep;
             }
+            const float base = m == -kInf ? 0.f : m;
+            float w[kSub][16];
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+            for (int u = 0; u < kSub; ++u)
 #pragma unroll
-            for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                const i32x4 w = as_fragment<T>(&s[u][c * kPerFrag<T>]);
+                for (int r = 0; r < 16; ++r) {
+                    w[u][r] = exp2_fast(__builtin_fmaf(s[u][r], factor, -base));
+                    l += w[u][r];
+                }
 #pragma unroll
-                for (int d = 0; d < kOut; ++d)
-                    o[d] = mma<T>(TileT::columns(vtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), w, o[d]);
-            }
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
+                    const i32x4 x = as_fragment<T>(&w[u][c * kPerFrag<T>]);
+#pragma unroll
+                    for (int d = 0; d < kOut; ++d)
+                        o[d] = mma<T>(TileT::columns(vtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, o[d]);
+                }
+        }
+        ktile = ktile == lds ? lds + 2 * kTileBytes : lds;
+        if (t < walk.end) {
+            ks.store(ktile);
+            vs.store(ktile + kTileBytes);
+        }
+        __syncthreads();
     }
 
     l = halves_sum(l);
@@ -252,16 +254,17 @@ hipError_t forward(const pointops_attention* in, const Args& a, void* out, float
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     return with_width(in->D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        size_t lds = 2 * kInner<T> * Tile<T, DP>::kStride;
-        if (a.bias != nullptr) lds += 4 * (bias_entries(a.reach) + a.bk.n);
+        constexpr size_t tiles = 4 * kInner<T> * Tile<T, DP>::kStride;
+        const size_t lds = tiles + (a.bias != nullptr ? 4 * (bias_entries(a.reach) + a.bk.n) : 0);
         const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
         const dim3 grid(static_cast<uint32_t>(blocks));
-        if (vec)
-            hipLaunchKernelGGL((attention_forward_kernel<T, DP, true>), grid, dim3(kThreads), lds, stream, a,
-                               static_cast<T*>(out), lse);
-        else
-            hipLaunchKernelGGL((attention_forward_kernel<T, DP, false>), grid, dim3(kThreads), lds, stream, a,
-                               static_cast<T*>(out), lse);
+        auto* const kernel = vec ? attention_forward_kernel<T, DP, true> : attention_forward_kernel<T, DP, false>;
+        if (lds > kLdsFree) {
+            static std::atomic<uint64_t> allowed[2];
+            const hipError_t err = allow_lds(kernel, allowed[vec], tiles + 4 * (bias_entries(kMaxReach) + 255));
+            if (err != hipSuccess) return err;
+        }
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, a, static_cast<T*>(out), lse);
         return hipGetLastError();
     });
 }
