@@ -180,6 +180,43 @@ struct Tile {
     }
 };
 
+// The compiler's scheduler keeps what is before this before what is behind it.
+// The products below ask for their operands as a batch, a phase ahead of their
+// use: left to itself it reads each right before its product, which then waits
+// for LDS (at one wave a SIMD that was two thirds of the time).
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Row operands of a tile's rows row0 .. row0 + 31, all chunks.
+template <typename T, int DP>
+struct RowFrags {
+    static constexpr int kChunks = Tile<T, DP>::kChunks;
+    i32x4 f[kChunks];
+    __device__ __forceinline__ void load(const char* tile, int row0) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) f[c] = Tile<T, DP>::rows(tile, row0, c);
+    }
+    __device__ __forceinline__ f32x16 times(const i32x4 (&b)[kChunks]) const {
+        f32x16 acc = {};
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) acc = mma<T>(f[c], b[c], acc);
+        return acc;
+    }
+};
+
+// Transposed operands of all columns, of the rows that one fragment spans.
+template <typename T, int DP>
+struct ColumnFrags {
+    i32x4 f[DP / 32];
+    __device__ __forceinline__ void load(const char* tile, int row0) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) f[d] = Tile<T, DP>::columns(tile, row0, 32 * d);
+    }
+    __device__ __forceinline__ void add(i32x4 b, f32x16 (&acc)[DP / 32]) const {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = mma<T>(f[d], b, acc[d]);
+    }
+};
+
 // A tile's way from memory to LDS through a block's registers: requested
 // before the one ahead of it is used.  Rows outside [first, high) and columns
 // behind the row's width are zeros: where rows allow 16-byte reads, by a buffer

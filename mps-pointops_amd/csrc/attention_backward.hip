@@ -22,12 +22,13 @@ namespace pointops {
 namespace attn {
 namespace {
 
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, bool VEC, bool BIAS>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void attention_grad_query_kernel(
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
     float* __restrict__ delta_out, T* __restrict__ dq_out, const bool refine) {
     using TileT = Tile<T, DP>;
     constexpr int TK = kInner<T>, kOut = DP / 32, kTileBytes = TK * TileT::kStride;
+    constexpr bool kTight = sizeof(T) == 2 && DP == 128;  // no registers for both products' operands at once
     extern __shared__ char lds[];  // two pairs of a key and a value tile, the bias's table
     float* const table = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int entries = bias_entries(a.reach);
@@ -38,8 +39,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
     const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
-    const bool biased = a.bias != nullptr;
-    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
+    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
 
     const int rows = min(kOuter, a.Q - i0);
     const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     }
     __syncthreads();
 
-    const float factor = biased ? 1.f : a.scale_log2;
+    const float factor = BIAS ? 1.f : a.scale_log2;
     f32x16 dq[kOut] = {};
     char* ktile = lds;
     while (t < walk.end) {
@@ -108,12 +108,17 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
             const bool far = near - (TK - 1) >= a.reach || near + 31 <= -a.reach;
 #pragma unroll
             for (int u = 0; u < TK / 32; ++u) {
-                f32x16 s = {}, dp = {};
-#pragma unroll
-                for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], s);
-#pragma unroll
-                for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(vtile, 32 * u, c), go[c], dp);
-                if (biased) {
+                RowFrags<T, DP> kf, vf;
+                kf.load(ktile, 32 * u);
+                if (!kTight) vf.load(vtile, 32 * u);
+                keep_order();
+                f32x16 s = kf.times(q);
+                if (kTight) vf.load(vtile, 32 * u);
+                const f32x16 dp = vf.times(go);
+                ColumnFrags<T, DP> cf[2];  // of this chunk of keys and the next
+                cf[0].load(ktile, 32 * u);
+                keep_order();
+                if constexpr (BIAS) {
                     s *= a.scale_log2;
                     if (far) {
                         s += table[near > 0 ? entries - 1 : 0];
@@ -139,12 +144,12 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
 #pragma unroll
                     for (int r = 0; r < 16; ++r) rest += ds[r];
                 }
+                constexpr int kSteps = 16 / kPerFrag<T>;
 #pragma unroll
-                for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                    const i32x4 x = as_fragment<T>(&ds[c * kPerFrag<T>]);
-#pragma unroll
-                    for (int d = 0; d < kOut; ++d)
-                        dq[d] = mma<T>(TileT::columns(ktile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, dq[d]);
+                for (int c = 0; c < kSteps; ++c) {
+                    if (c + 1 < kSteps) cf[(c + 1) % 2].load(ktile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
+                    keep_order();
+                    cf[c % 2].add(as_fragment<T>(&ds[c * kPerFrag<T>]), dq);
                 }
             }
         }
@@ -198,18 +203,19 @@ struct Pieces {
 constexpr int kSkewRow = 68;
 constexpr int kSkewFloats = 16 + 16 * kSkewRow;
 
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, bool VEC, bool BIAS>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
     const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const Rows grad,
     T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
     const Pieces cut) {
     using TileT = Tile<T, DP>;
     constexpr int TQ = kInner<T>, kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
+    constexpr bool kTight = sizeof(T) == 4 ? DP == 128 : BIAS && DP == 64;  // as above
     constexpr int kSet = 2 * kTileBytes + 8 * TQ;  // a tile of queries, one of gradients, their lse and delta
     extern __shared__ char lds[];                  // two sets, then the bias's tables
     float* const table = reinterpret_cast<float*>(lds + 2 * kSet);
     const int entries = bias_entries(a.reach);
-    const bool biased = a.bias != nullptr, summed = dbias_part != nullptr;
+    const bool summed = BIAS && dbias_part != nullptr;
     float* const skews = table + (entries + 3) / 4 * 4;  // one a wave, then the waves' sums by offset, the edges
     float* const sums = skews + kWaves * kSkewFloats;
     int* const edges = reinterpret_cast<int*>(summed ? sums + kWaves * entries : skews);
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     }
     f32x16 dk[kOut] = {}, dv[kOut] = {};
     float* const skew = skews + wave * kSkewFloats + 16;
-    const float factor = biased ? 1.f : a.scale_log2;
+    const float factor = BIAS ? 1.f : a.scale_log2;
     float* const mine = sums + wave * entries;
     if (summed)
         for (int i = threadIdx.x; i < kWaves * kSkewFloats; i += kThreads) skews[i] = 0.f;
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         const int to = t_first + static_cast<int>(min(share_high - static_cast<int64_t>(hh) * tiles, int64_t(tiles)));
         if (from >= to && !summed) continue;
         __syncthreads();
-        if (biased) fill_bias<T>(a, h, table, edges);
+        if constexpr (BIAS) fill_bias<T>(a, h, table, edges);
         if (summed)
             for (int i = threadIdx.x; i < kWaves * entries; i += kThreads) sums[i] = 0.f;
         float far_early = 0.f, far_late = 0.f;  // ds of offsets beyond the reach
@@ -332,12 +338,24 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 const bool far = near - 31 >= a.reach || near + TQ - 1 <= -a.reach;
 #pragma unroll
                 for (int u = 0; u < TQ / 32; ++u) {
-                    f32x16 s = {}, dp = {};
+                    RowFrags<T, DP> qf, gf;
+                    qf.load(qtile, 32 * u);
+                    if (!kTight) gf.load(gtile, 32 * u);
+                    f32x4 lse[4], delta[4];
 #pragma unroll
-                    for (int c = 0; c < TileT::kChunks; ++c) s = mma<T>(TileT::rows(qtile, 32 * u, c), k[c], s);
-#pragma unroll
-                    for (int c = 0; c < TileT::kChunks; ++c) dp = mma<T>(TileT::rows(gtile, 32 * u, c), v[c], dp);
-                    if (biased) {
+                    for (int e = 0; e < 4; ++e) {
+                        lse[e] = *reinterpret_cast<const f32x4*>(stat + 32 * u + 8 * e + 4 * half);
+                        delta[e] = *reinterpret_cast<const f32x4*>(stat + TQ + 32 * u + 8 * e + 4 * half);
+                    }
+                    keep_order();
+                    f32x16 s = qf.times(k);
+                    if (kTight) gf.load(gtile, 32 * u);
+                    const f32x16 dp = gf.times(v);
+                    ColumnFrags<T, DP> qc[2], gc[2];  // of this chunk of queries and the next
+                    gc[0].load(gtile, 32 * u);
+                    qc[0].load(qtile, 32 * u);
+                    keep_order();
+                    if constexpr (BIAS) {
                         s *= a.scale_log2;
                         if (far) {
                             s += table[near > 0 ? entries - 1 : 0];
@@ -349,15 +367,9 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                     }
                     float w[16], ds[16];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const f32x4 lse = *reinterpret_cast<const f32x4*>(stat + 32 * u + 8 * e + 4 * half);
-                        const f32x4 delta = *reinterpret_cast<const f32x4*>(stat + TQ + 32 * u + 8 * e + 4 * half);
-#pragma unroll
-                        for (int f = 0; f < 4; ++f) {
-                            const int r = 4 * e + f;
-                            w[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[f]));
-                            ds[r] = w[r] * (dp[r] - delta[f]);
-                        }
+                    for (int r = 0; r < 16; ++r) {
+                        w[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[r / 4][r % 4]));
+                        ds[r] = w[r] * (dp[r] - delta[r / 4][r % 4]);
                     }
                     if (!whole) {
                         const int p = p0 + 32 * u + 4 * half - see_low;
@@ -365,14 +377,16 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                         for (int r = 0; r < 16; ++r)
                             if (static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) w[r] = ds[r] = 0.f;
                     }
+                    constexpr int kSteps = 16 / kPerFrag<T>;
 #pragma unroll
-                    for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                        const i32x4 x = as_fragment<T>(&w[c * kPerFrag<T>]), y = as_fragment<T>(&ds[c * kPerFrag<T>]);
-#pragma unroll
-                        for (int d = 0; d < kOut; ++d) {
-                            dv[d] = mma<T>(TileT::columns(gtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, dv[d]);
-                            dk[d] = mma<T>(TileT::columns(qtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), y, dk[d]);
+                    for (int c = 0; c < kSteps; ++c) {
+                        if (c + 1 < kSteps) {
+                            gc[(c + 1) % 2].load(gtile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
+                            qc[(c + 1) % 2].load(qtile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
                         }
+                        keep_order();
+                        gc[c % 2].add(as_fragment<T>(&w[c * kPerFrag<T>]), dv);
+                        qc[c % 2].add(as_fragment<T>(&ds[c * kPerFrag<T>]), dk);
                     }
                     if (!summed) continue;
                     if (j >= len) {  // keys of zeros with scores of their own
@@ -531,7 +545,7 @@ struct Grads {
 template <typename T>
 constexpr int kType = sizeof(T) == 4 ? POINTOPS_F32 : __is_same(T, f16) ? POINTOPS_F16 : POINTOPS_BF16;
 
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, bool VEC, bool BIAS>
 hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     using TileT = Tile<T, DP>;
     const Workspace w = workspace_of(a, kType<T>);
@@ -546,7 +560,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     constexpr size_t tiles = 4 * kInner<T> * TileT::kStride, stats = 16 * kInner<T>;
     const size_t entries = bias_entries(a.reach), table = a.bias != nullptr ? 4 * (entries + a.bk.n) : 0;
     if (grid_q > 0) {
-        auto* const by_query = attention_grad_query_kernel<T, DP, VEC>;
+        auto* const by_query = attention_grad_query_kernel<T, DP, VEC, BIAS>;
         if (tiles + table > kLdsFree) {
             static std::atomic<uint64_t> allowed{0};
             const hipError_t err = allow_lds(by_query, allowed, tiles + 4 * (bias_entries(kMaxReach) + 255));
@@ -559,7 +573,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
-        auto* const by_key = attention_grad_key_kernel<T, DP, VEC>;
+        auto* const by_key = attention_grad_key_kernel<T, DP, VEC, BIAS>;
         // The tiles, their rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
         auto lds_for = [&](size_t n, size_t edges, bool sums) {
             return tiles + stats + 4 * ((n + 3) / 4 * 4 + edges) + (sums ? 4 * kWaves * (kSkewFloats + n) : 0);
@@ -593,7 +607,9 @@ hipError_t backward(const Args& a, const Grads& x, hipStream_t stream) {
                      vector_rows<T>(x.grad, a.D) && reinterpret_cast<uintptr_t>(x.out) % 16 == 0;
     return with_width(a.D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        return vec ? launch_backward<T, DP, true>(a, x, stream) : launch_backward<T, DP, false>(a, x, stream);
+        if (a.bias != nullptr)
+            return vec ? launch_backward<T, DP, true, true>(a, x, stream) : launch_backward<T, DP, false, true>(a, x, stream);
+        return vec ? launch_backward<T, DP, true, false>(a, x, stream) : launch_backward<T, DP, false, false>(a, x, stream);
     });
 }
 

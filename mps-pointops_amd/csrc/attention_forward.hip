@@ -71,8 +71,8 @@ __device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, 
     if (lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
 }
 
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Args a, T* __restrict__ out,
+template <typename T, int DP, bool VEC, bool BIAS>
+__global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_forward_kernel(const Args a, T* __restrict__ out,
                                                                         float* __restrict__ lse_out) {
     using TileT = Tile<T, DP>;
     constexpr int TK = kInner<T>, kSub = TK / 32, kOut = DP / 32;
@@ -86,8 +86,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
     const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
-    const bool biased = a.bias != nullptr;
-    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
+    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
 
     // The block's rows that exist, by position, and the tiles that they see.
     const int rows = min(kOuter, a.Q - i0);
@@ -126,7 +125,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
 
     // Scores as the products leave them, in units of 1 / factor: a bias needs
     // them scaled, and a negative scale turns their order.
-    const bool scaled = biased || !(a.scale > 0.f);
+    const bool scaled = BIAS || !(a.scale > 0.f);
     const float factor = scaled ? 1.f : a.scale_log2;
     f32x16 o[kOut] = {};
     float m = -kInf, l = 0.f;  // the maximum so far (scaled; see kSlack) and this half-wave's sum
@@ -147,15 +146,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
             f32x16 s[kSub];
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
-                s[u] = f32x16{};
-#pragma unroll
-                for (int c = 0; c < TileT::kChunks; ++c) s[u] = mma<T>(TileT::rows(ktile, 32 * u, c), q[c], s[u]);
+                RowFrags<T, DP> f;
+                f.load(ktile, 32 * u);
+                keep_order();
+                s[u] = f.times(q);
             }
+            ColumnFrags<T, DP> vf[2];  // of this chunk of keys and the next
+            vf[0].load(vtile, 0);
+            keep_order();
             if (scaled) {
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) s[u] *= a.scale_log2;
             }
-            if (biased) {
+            if constexpr (BIAS) {
                 const int near = w0 - j0;  // offset of the wave's first row and the tile's first key
                 if (near - (TK - 1) >= a.reach || near + 31 <= -a.reach) {
                     const float far = table[near > 0 ? bias_entries(a.reach) - 1 : 0];
@@ -200,15 +203,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(const Ar
                     w[u][r] = exp2_fast(__builtin_fmaf(s[u][r], factor, -base));
                     l += w[u][r];
                 }
+            constexpr int kPer = 16 / kPerFrag<T>, kSteps = kSub * kPer;
 #pragma unroll
-            for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
-                    const i32x4 x = as_fragment<T>(&w[u][c * kPerFrag<T>]);
-#pragma unroll
-                    for (int d = 0; d < kOut; ++d)
-                        o[d] = mma<T>(TileT::columns(vtile, 32 * u + c * TileT::kRowsPerFrag, 32 * d), x, o[d]);
-                }
+            for (int c = 0; c < kSteps; ++c) {
+                if (c + 1 < kSteps) vf[(c + 1) % 2].load(vtile, (c + 1) * TileT::kRowsPerFrag);
+                keep_order();
+                vf[c % 2].add(as_fragment<T>(&w[c / kPer][c % kPer * kPerFrag<T>]), o);
+            }
         }
         ktile = ktile == lds ? lds + 2 * kTileBytes : lds;
         if (t < walk.end) {
@@ -258,10 +259,12 @@ hipError_t forward(const pointops_attention* in, const Args& a, void* out, float
         const size_t lds = tiles + (a.bias != nullptr ? 4 * (bias_entries(a.reach) + a.bk.n) : 0);
         const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
         const dim3 grid(static_cast<uint32_t>(blocks));
-        auto* const kernel = vec ? attention_forward_kernel<T, DP, true> : attention_forward_kernel<T, DP, false>;
+        const bool bias = a.bias != nullptr;
+        auto* const kernel = vec ? (bias ? attention_forward_kernel<T, DP, true, true> : attention_forward_kernel<T, DP, true, false>)
+                                 : (bias ? attention_forward_kernel<T, DP, false, true> : attention_forward_kernel<T, DP, false, false>);
         if (lds > kLdsFree) {
-            static std::atomic<uint64_t> allowed[2];
-            const hipError_t err = allow_lds(kernel, allowed[vec], tiles + 4 * (bias_entries(kMaxReach) + 255));
+            static std::atomic<uint64_t> allowed[2][2];
+            const hipError_t err = allow_lds(kernel, allowed[vec][bias], tiles + 4 * (bias_entries(kMaxReach) + 255));
             if (err != hipSuccess) return err;
         }
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, a, static_cast<T*>(out), lse);
