@@ -255,13 +255,35 @@ __global__ __launch_bounds__(kThreads) void attention_step_join_kernel(const Arg
     top = wave_max(top);
     const float base = top == -kInf ? 0.f : top;
     float sum = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float* const at = src + s * step;
-        const float by = exp2_fast(at[0] - base);
-        sum = __builtin_fmaf(at[1], by, sum);
-        if (lane < a.D) x0 = __builtin_fmaf(at[2 + lane], by, x0);
-        if (lane + kWave < a.D) x1 = __builtin_fmaf(at[2 + lane + kWave], by, x1);
+    const int c0 = min(lane, a.D - 1), c1 = min(lane + kWave, a.D - 1);
+    for (int first = 0; first < splits; first += kWave) {
+        // A lane's split: its factor; then the splits' rows one after another.
+        const int s = first + lane;
+        float by = 0.f;
+        if (s < splits) {
+            by = exp2_fast(src[s * step] - base);
+            sum = __builtin_fmaf(src[s * step + 1], by, sum);
+        }
+        const int count = min(kWave, splits - first);
+        const float* const rows = src + first * step + 2;
+        constexpr int kAtOnce = 8;
+        for (int i = 0; i < count; i += kAtOnce) {
+            float y0[kAtOnce], y1[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int64_t at = min(i + k, count - 1) * step;
+                y0[k] = rows[at + c0];
+                y1[k] = rows[at + c1];
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float f = i + k < count ? i2f(readlane(f2i(by), min(i + k, count - 1))) : 0.f;
+                x0 = __builtin_fmaf(y0[k], f, x0);
+                x1 = __builtin_fmaf(y1[k], f, x1);
+            }
+        }
     }
+    sum = wave_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row / group) * a.H + g * group + row % group) * a.D;
     if (lane < a.D) dst[lane] = from_float<T>(x0 * inv);

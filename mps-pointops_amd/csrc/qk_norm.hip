@@ -10,9 +10,12 @@
 // Bound by memory: every value is read once and written once.  A row (token
 // and head) is held by 1 to 64 neighbouring lanes, each with two pieces of up
 // to 16 bytes: values i and i + R/2 of rotated ones, so that no lane needs
-// another's, or two pieces of the others.  A lane keeps its head and columns
-// for all its tokens, and with them the weights and their gradient's sums, in
-// registers; the sums of a block, then of all, are added in a fixed order.
+// another's, or two pieces of the others.  Where a part is no multiple of the
+// piece, its last piece starts earlier: two lanes then hold the same values and
+// write the same results, and one of them leaves them out of the sums.  A group
+// of lanes keeps its columns for all its heads and tokens: the angles are read
+// once a token, the weights once, and the weights' gradients are summed in
+// registers, then over a block, then over all, in a fixed order.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -28,54 +31,69 @@ struct NormArgs {
     int64_t angle_b, angle_n;
     int64_t tokens;  // B N
     int64_t step;    // tokens that are in work at a time
+    int slices;      // groups of lanes that share a token's heads
     int N, H, G, D, R;
     float eps, inv_d;
 };
 
 template <typename T, int VEC>
 struct Piece {
-    static constexpr int kAlign = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16;
     float v[VEC];
     __device__ __forceinline__ void load(const T* p, bool there) {
-        if (there) {
-            T raw[VEC];
-            __builtin_memcpy(raw, __builtin_assume_aligned(p, kAlign), sizeof raw);
+        T raw[VEC] = {};
+        if (there) __builtin_memcpy(raw, p, sizeof raw);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = to_float(raw[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-        }
+        for (int e = 0; e < VEC; ++e) v[e] = to_float(raw[e]);
     }
     __device__ __forceinline__ void store(T* p, bool there) const {
         T raw[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) raw[e] = from_float<T>(v[e]);
-        if (there) __builtin_memcpy(__builtin_assume_aligned(p, kAlign), raw, sizeof raw);
+        if (there) __builtin_memcpy(p, raw, sizeof raw);
     }
 };
 
-// A lane's place: its head, its pieces' columns, its first token.
+// Columns of unit `unit`: its two pieces' first columns, and how many values at
+// their start are the piece's before.  A piece that does not exist is at D.
+template <int VEC>
+struct Columns {
+    int a, b, skip_a, skip_b;
+    bool turned;
+    __host__ __device__ Columns(int unit, int D, int R) {
+        const int half = R / 2, turning = (half + VEC - 1) / VEC;
+        turned = unit < turning;
+        if (turned) {
+            a = unit * VEC < half - VEC ? unit * VEC : half - VEC;
+            b = half + a;
+            skip_a = skip_b = unit * VEC - a;
+            return;
+        }
+        const int at = 2 * (unit - turning) * VEC, rest = D - R;
+        a = at >= rest ? rest : at < rest - VEC ? at : rest - VEC;
+        b = at + VEC >= rest ? rest : at + VEC < rest - VEC ? at + VEC : rest - VEC;
+        skip_a = at - a;
+        skip_b = at + VEC - b;
+        a += R;
+        b += R;
+    }
+};
+
+// A lane's place: its slice of the heads, its pieces' columns, its token.
 template <typename T, int VEC, int L>
 struct Place {
-    int head, col_a, col_b;  // head: q's, then k's
-    bool turned, has_a, has_b, is_q;
+    Columns<VEC> col;
+    int slice;
+    bool has_a, has_b;
     int b, n, step_b, step_n;
     int64_t token;
 
-    __device__ __forceinline__ explicit Place(const NormArgs& a) {
+    __device__ __forceinline__ explicit Place(const NormArgs& a) : col(threadIdx.x % L, a.D, a.R) {
         const int64_t group = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;
-        const int unit = threadIdx.x % L, heads = a.H + a.G;
-        head = static_cast<int>(group % heads);
-        token = group / heads;
-        is_q = head < a.H;
+        slice = static_cast<int>(group % a.slices);
+        token = group / a.slices;
         if (token >= a.step) token = a.tokens;  // groups behind the last whole set
-        const int half = a.R / 2, turning = half / VEC;
-        turned = unit < turning;
-        col_a = turned ? unit * VEC : a.R + 2 * (unit - turning) * VEC;
-        col_b = turned ? half + unit * VEC : col_a + VEC;
-        has_a = col_a < a.D;
-        has_b = col_b < a.D;
+        has_a = col.a < a.D;
+        has_b = col.b < a.D;
         b = static_cast<int>(token / a.N);
         n = static_cast<int>(token % a.N);
         step_b = static_cast<int>(a.step / a.N);
@@ -90,53 +108,89 @@ struct Place {
             ++b;
         }
     }
-    __device__ __forceinline__ const T* in(const Rows& q, const Rows& k, int H) const {
-        return is_q ? q.at<T>(b, head) + n * q.n : k.at<T>(b, head - H) + n * k.n;
+    // Head `head` of q's, then of k's, as it comes and as a row of the contiguous results.
+    __device__ __forceinline__ const T* in(const Rows& q, const Rows& k, int H, int head) const {
+        return head < H ? q.at<T>(b, head) + n * q.n : k.at<T>(b, head - H) + n * k.n;
     }
-    // Row of the contiguous output.
-    __device__ __forceinline__ T* out(T* q, T* k, const NormArgs& a) const {
-        return is_q ? q + (token * a.H + head) * a.D : k + (token * a.G + head - a.H) * a.D;
+    __device__ __forceinline__ T* out(T* q, T* k, const NormArgs& a, int head) const {
+        return head < a.H ? q + (token * a.H + head) * a.D : k + (token * a.G + head - a.H) * a.D;
     }
 };
 
 template <typename W, int VEC>
-__device__ __forceinline__ void load_weight(Piece<W, VEC>& p, const void* w, int col, bool there) {
-    if (w != nullptr) {
-        p.load(static_cast<const W*>(w) + col, there);
-    } else {
+struct Weights {
+    Piece<W, VEC> a, b;
+    __device__ __forceinline__ void load(const void* w, const Columns<VEC>& col, bool has_a, bool has_b) {
+        const bool given = w != nullptr;
+        a.load(static_cast<const W*>(w) + col.a, given && has_a);
+        b.load(static_cast<const W*>(w) + col.b, given && has_b);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) p.v[e] = there ? 1.f : 0.f;
+        for (int e = 0; e < VEC; ++e) {
+            a.v[e] = given ? a.v[e] : 1.f;
+            b.v[e] = given ? b.v[e] : 1.f;
+        }
     }
+};
+
+constexpr int kAhead = 2;  // heads whose values are asked for at once
+
+// By value: a conditional of two array elements would choose an address.
+__device__ __forceinline__ float pick(bool first, float x, float y) { return first ? x : y; }
+
+// The sum of x y over the row, each value once.
+template <int VEC>
+__device__ __forceinline__ float row_part(const float (&xa)[VEC], const float (&ya)[VEC], const float (&xb)[VEC],
+                                          const float (&yb)[VEC], const Columns<VEC>& col) {
+    const uint32_t keep_a = ~0u << col.skip_a, keep_b = ~0u << col.skip_b;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        sum = __builtin_fmaf((keep_a >> e & 1) != 0 ? xa[e] : 0.f, ya[e], sum);
+        sum = __builtin_fmaf((keep_b >> e & 1) != 0 ? xb[e] : 0.f, yb[e], sum);
+    }
+    return sum;
 }
 
 template <typename T, typename W, int VEC, int L>
 __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const NormArgs a, T* __restrict__ q_out, T* __restrict__ k_out) {
     Place<T, VEC, L> at(a);
-    Piece<W, VEC> wa, wb;
-    load_weight(wa, at.is_q ? a.wq : a.wk, at.col_a, at.has_a);
-    load_weight(wb, at.is_q ? a.wq : a.wk, at.col_b, at.has_b);
+    const Columns<VEC> col = at.col;
+    const int heads = a.H + a.G;
+    Weights<W, VEC> wq, wk;
+    wq.load(a.wq, col, at.has_a, at.has_b);
+    wk.load(a.wk, col, at.has_a, at.has_b);
     for (; at.token < a.tokens; at.next(a)) {
-        const T* const x = at.in(a.q, a.k, a.H);
-        Piece<T, VEC> xa, xb;
         Piece<float, VEC> c, s;
-        xa.load(x + at.col_a, at.has_a);
-        xb.load(x + at.col_b, at.has_b);
-        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + at.col_a;
-        c.load(a.cos + angle, at.turned);
-        s.load(a.sin + angle, at.turned);
-        float sum = 0.f;
+        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + col.a;
+        c.load(a.cos + angle, col.turned);
+        s.load(a.sin + angle, col.turned);
+        for (int first = at.slice; first < heads; first += kAhead * a.slices) {
+            Piece<T, VEC> xa[kAhead], xb[kAhead];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum = __builtin_fmaf(xa.v[e], xa.v[e], __builtin_fmaf(xb.v[e], xb.v[e], sum));
-        const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
+            for (int u = 0; u < kAhead; ++u) {
+                const int head = first + u * a.slices;
+                const T* const x = at.in(a.q, a.k, a.H, head);
+                xa[u].load(x + col.a, at.has_a && head < heads);
+                xb[u].load(x + col.b, at.has_b && head < heads);
+            }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float ya = xa.v[e] * r * wa.v[e], yb = xb.v[e] * r * wb.v[e];
-            xa.v[e] = at.turned ? ya * c.v[e] - yb * s.v[e] : ya;
-            xb.v[e] = at.turned ? yb * c.v[e] + ya * s.v[e] : yb;
+            for (int u = 0; u < kAhead; ++u) {
+                const int head = first + u * a.slices;
+                const float sum = row_part<VEC>(xa[u].v, xa[u].v, xb[u].v, xb[u].v, col);
+                const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
+                const bool is_q = head < a.H;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float ya = xa[u].v[e] * r * pick(is_q, wq.a.v[e], wk.a.v[e]);
+                    const float yb = xb[u].v[e] * r * pick(is_q, wq.b.v[e], wk.b.v[e]);
+                    xa[u].v[e] = col.turned ? ya * c.v[e] - yb * s.v[e] : ya;
+                    xb[u].v[e] = col.turned ? yb * c.v[e] + ya * s.v[e] : yb;
+                }
+                T* const out = at.out(q_out, k_out, a, head);
+                xa[u].store(out + col.a, at.has_a && head < heads);
+                xb[u].store(out + col.b, at.has_b && head < heads);
+            }
         }
-        T* const out = at.out(q_out, k_out, a);
-        xa.store(out + at.col_a, at.has_a);
-        xb.store(out + at.col_b, at.has_b);
     }
 }
 
@@ -145,113 +199,140 @@ __global__ __launch_bounds__(kThreads) void qk_norm_grad_kernel(const NormArgs a
                                                                 T* __restrict__ dq, T* __restrict__ dk,
                                                                 float* __restrict__ part) {
     __shared__ float sums[kThreads / L][2 * L * VEC];  // a group's columns: its first pieces, then its second
-    __shared__ bool of_q[kThreads / L];
     Place<T, VEC, L> at(a);
-    Piece<W, VEC> wa, wb;
-    load_weight(wa, at.is_q ? a.wq : a.wk, at.col_a, at.has_a);
-    load_weight(wb, at.is_q ? a.wq : a.wk, at.col_b, at.has_b);
-    float sa[VEC] = {}, sb[VEC] = {};
+    const Columns<VEC> col = at.col;
+    const int heads = a.H + a.G;
+    Weights<W, VEC> wq, wk;
+    wq.load(a.wq, col, at.has_a, at.has_b);
+    wk.load(a.wk, col, at.has_a, at.has_b);
+    float sa[2][VEC] = {}, sb[2][VEC] = {};  // q's and k's
     for (; at.token < a.tokens; at.next(a)) {
-        const T* const x = at.in(a.q, a.k, a.H);
-        const T* const g = at.in(gq, gk, a.H);
-        Piece<T, VEC> xa, xb, ga, gb;
         Piece<float, VEC> c, s;
-        xa.load(x + at.col_a, at.has_a);
-        xb.load(x + at.col_b, at.has_b);
-        ga.load(g + at.col_a, at.has_a);
-        gb.load(g + at.col_b, at.has_b);
-        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + at.col_a;
-        c.load(a.cos + angle, at.turned);
-        s.load(a.sin + angle, at.turned);
-        float sum = 0.f, along = 0.f;
+        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + col.a;
+        c.load(a.cos + angle, col.turned);
+        s.load(a.sin + angle, col.turned);
+        for (int first = at.slice; first < heads; first += kAhead * a.slices) {
+            Piece<T, VEC> xa[kAhead], xb[kAhead], ga[kAhead], gb[kAhead];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            sum = __builtin_fmaf(xa.v[e], xa.v[e], __builtin_fmaf(xb.v[e], xb.v[e], sum));
-            const float da = at.turned ? ga.v[e] * c.v[e] + gb.v[e] * s.v[e] : ga.v[e];
-            const float db = at.turned ? gb.v[e] * c.v[e] - ga.v[e] * s.v[e] : gb.v[e];
-            ga.v[e] = da;
-            gb.v[e] = db;
-            along = __builtin_fmaf(da * wa.v[e], xa.v[e], __builtin_fmaf(db * wb.v[e], xb.v[e], along));
-        }
-        const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
-        const float mean = group_sum<L>(along) * r * a.inv_d;
+            for (int u = 0; u < kAhead; ++u) {
+                const int head = first + u * a.slices;
+                const T* const x = at.in(a.q, a.k, a.H, head);
+                const T* const g = at.in(gq, gk, a.H, head);
+                xa[u].load(x + col.a, at.has_a && head < heads);
+                xb[u].load(x + col.b, at.has_b && head < heads);
+                ga[u].load(g + col.a, at.has_a && head < heads);
+                gb[u].load(g + col.b, at.has_b && head < heads);
+            }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float ua = xa.v[e] * r, ub = xb.v[e] * r;
-            sa[e] = __builtin_fmaf(ga.v[e], ua, sa[e]);
-            sb[e] = __builtin_fmaf(gb.v[e], ub, sb[e]);
-            xa.v[e] = r * (ga.v[e] * wa.v[e] - ua * mean);
-            xb.v[e] = r * (gb.v[e] * wb.v[e] - ub * mean);
+            for (int u = 0; u < kAhead; ++u) {
+                const int head = first + u * a.slices;
+                const bool is_q = head < a.H;
+                float ua[VEC], ub[VEC];  // dy w
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float da = col.turned ? ga[u].v[e] * c.v[e] + gb[u].v[e] * s.v[e] : ga[u].v[e];
+                    const float db = col.turned ? gb[u].v[e] * c.v[e] - ga[u].v[e] * s.v[e] : gb[u].v[e];
+                    ga[u].v[e] = da;
+                    gb[u].v[e] = db;
+                    ua[e] = da * pick(is_q, wq.a.v[e], wk.a.v[e]);
+                    ub[e] = db * pick(is_q, wq.b.v[e], wk.b.v[e]);
+                }
+                const float sum = row_part<VEC>(xa[u].v, xa[u].v, xb[u].v, xb[u].v, col);
+                const float along = row_part<VEC>(xa[u].v, ua, xb[u].v, ub, col);
+                const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
+                const float mean = group_sum<L>(along) * r * a.inv_d;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float na = xa[u].v[e] * r, nb = xb[u].v[e] * r;
+                    const float ta = ga[u].v[e] * na, tb = gb[u].v[e] * nb;
+                    sa[0][e] += is_q ? ta : 0.f;
+                    sb[0][e] += is_q ? tb : 0.f;
+                    sa[1][e] += is_q ? 0.f : ta;
+                    sb[1][e] += is_q ? 0.f : tb;
+                    xa[u].v[e] = r * (ua[e] - na * mean);
+                    xb[u].v[e] = r * (ub[e] - nb * mean);
+                }
+                // Of a row of one value the difference leaves eps r^2 alone, which rounding would bury.
+                if constexpr (VEC == 1 && L == 1)
+                    if (a.D == 1) xa[u].v[0] = r * r * r * a.eps * ua[0];
+                T* const out = at.out(dq, dk, a, head);
+                xa[u].store(out + col.a, at.has_a && head < heads);
+                xb[u].store(out + col.b, at.has_b && head < heads);
+            }
         }
-        // Of a row of one value the difference leaves eps r^2 alone, which rounding would bury.
-        if constexpr (VEC == 1 && L == 1)
-            if (a.D == 1) xa.v[0] = r * r * r * a.eps * ga.v[0] * wa.v[0];
-        T* const out = at.out(dq, dk, a);
-        xa.store(out + at.col_a, at.has_a);
-        xb.store(out + at.col_b, at.has_b);
     }
     if (part == nullptr) return;
-    const int group = threadIdx.x / L, unit = threadIdx.x % L;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        sums[group][unit * VEC + e] = sa[e];
-        sums[group][(L + unit) * VEC + e] = sb[e];
-    }
-    if (unit == 0) of_q[group] = at.is_q;
-    __syncthreads();
     // part (blocks, q or k, columns in the lanes' order)
     constexpr int kColumns = 2 * L * VEC;
-    for (int i = threadIdx.x; i < 2 * kColumns; i += kThreads) {
-        const bool q = i < kColumns;
-        float all = 0.f;
-        for (int gr = 0; gr < kThreads / L; ++gr)
-            if (of_q[gr] == q) all += sums[gr][i % kColumns];
-        part[static_cast<int64_t>(blockIdx.x) * 2 * kColumns + i] = all;
+    const int group = threadIdx.x / L, unit = threadIdx.x % L;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            sums[group][unit * VEC + e] = sa[which][e];
+            sums[group][(L + unit) * VEC + e] = sb[which][e];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < kColumns; i += kThreads) {
+            float all = 0.f;
+#pragma unroll 8
+            for (int gr = 0; gr < kThreads / L; ++gr) all += sums[gr][i];
+            part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * kColumns + i] = all;
+        }
     }
 }
 
-// dw from the blocks' parts: one wave a column, the blocks over its lanes.
-template <typename W>
-__global__ __launch_bounds__(kThreads) void qk_norm_weight_kernel(const float* __restrict__ part, int blocks, int L, int VEC,
-                                                                  int D, int R, W* __restrict__ dwq, W* __restrict__ dwk) {
-    const int id = blockIdx.x * kWaves + threadIdx.x / kWave, columns = 2 * L * VEC;
-    if (id >= 2 * columns) return;
-    const int i = id % columns, piece = i / (L * VEC), unit = i / VEC % L, e = i % VEC;
-    const int half = R / 2, turning = half / VEC;
-    const int col = (unit < turning ? unit * VEC + piece * half : R + (2 * (unit - turning) + piece) * VEC) + e;
+// dw from the blocks' parts: a block for 16 columns, 16 lanes of blocks each.
+template <typename W, int VEC, int L>
+__global__ __launch_bounds__(kThreads) void qk_norm_weight_kernel(const float* __restrict__ part, int blocks, int D, int R,
+                                                                  W* __restrict__ dwq, W* __restrict__ dwk) {
+    constexpr int kColumns = 2 * L * VEC, kAcross = 16, kLanes = kThreads / kAcross;
+    __shared__ float sums[kLanes][kAcross];
+    const int x = threadIdx.x % kAcross, y = threadIdx.x / kAcross, id = blockIdx.x * kAcross + x;
     float all = 0.f;
-    for (int b = lane_id(); b < blocks; b += kWave) all += part[static_cast<int64_t>(b) * 2 * columns + id];
-    all = wave_sum(all);
-    W* const dst = id < columns ? dwq : dwk;
-    if (lane_id() == 0 && col < D && dst != nullptr) dst[col] = from_float<W>(all);
+    if (id < 2 * kColumns) {
+#pragma unroll 8
+        for (int b = y; b < blocks; b += kLanes) all += part[static_cast<int64_t>(b) * 2 * kColumns + id];
+    }
+    sums[y][x] = all;
+    __syncthreads();
+    if (y != 0 || id >= 2 * kColumns) return;
+    for (int i = 1; i < kLanes; ++i) all += sums[i][x];
+    const int i = id % kColumns, e = i % VEC, unit = i / VEC % L;
+    const Columns<VEC> col(unit, D, R);
+    const bool second = i >= L * VEC;
+    const int at = (second ? col.b : col.a) + e;
+    W* const dst = id < kColumns ? dwq : dwk;
+    // A value that two pieces hold is the first one's.
+    if (dst != nullptr && (second ? col.b : col.a) < D && e >= (second ? col.skip_b : col.skip_a)) dst[at] = from_float<W>(all);
 }
 
 constexpr int64_t kBlocks = 2048;
 
 struct Shape {
-    int vec, lanes;
+    int vec, lanes, slices;
     int64_t blocks, step;
 };
 
-// The widest pieces that all rows, the rotated half and the rest allow, and
-// blocks enough to fill the card (each keeps its sums until its end).
-Shape shape_of(const pointops_qk_norm& in, int64_t extra_alignment) {
-    const int size = in.type == POINTOPS_F32 ? 4 : 2;
-    int64_t bits = static_cast<int64_t>(16 / size) | (in.R / 2) | (in.D - in.R) | extra_alignment;
-    for (int i = 0; i < 3; ++i) bits |= in.q_stride[i] | in.k_stride[i];
-    bits |= reinterpret_cast<uintptr_t>(in.q) / size | reinterpret_cast<uintptr_t>(in.k) / size;
-    if (in.R > 0)
-        bits |= in.angle_stride[0] | in.angle_stride[1] | reinterpret_cast<uintptr_t>(in.cos) / 4 |
-                reinterpret_cast<uintptr_t>(in.sin) / 4;
+// The widest pieces that the rotated half and the rest hold, and blocks enough
+// to fill the card (each keeps its sums until its end).  A wave takes
+// neighbouring heads of a token, or all of its heads at once where the whole
+// call is small and its latency counts.
+Shape shape_of(const pointops_qk_norm& in) {
+    const int half = static_cast<int>(in.R / 2), rest = static_cast<int>(in.D - in.R);
     Shape s;
-    s.vec = static_cast<int>(bits & -bits);
-    const int64_t rest = (in.D - in.R) / s.vec, units = in.R / 2 / s.vec + (rest + 1) / 2;
+    s.vec = in.type == POINTOPS_F32 ? 4 : 8;
+    while ((half > 0 && s.vec > half) || (rest > 0 && s.vec > rest)) s.vec /= 2;
+    const int units = (half + s.vec - 1) / s.vec + ((rest + s.vec - 1) / s.vec + 1) / 2;
     s.lanes = 1;
     while (s.lanes < units) s.lanes *= 2;
     const int64_t tokens = in.B * in.N, heads = in.H + in.G, groups = kThreads / s.lanes;
-    s.blocks = std::min(kBlocks, (tokens * heads + groups - 1) / groups);
-    s.blocks = std::max(s.blocks, (heads + groups - 1) / groups);
-    s.step = std::min(tokens, s.blocks * groups / heads);
+    const bool small = tokens * heads * s.lanes <= (1 << 18);
+    s.slices = static_cast<int>(small ? heads : std::min<int64_t>(heads, kWave / s.lanes));
+    s.blocks = std::min(kBlocks, (tokens * s.slices + groups - 1) / groups);
+    s.blocks = std::max(s.blocks, (s.slices + groups - 1) / groups);
+    s.step = std::min(tokens, s.blocks * groups / s.slices);
     return s;
 }
 
@@ -275,6 +356,7 @@ NormArgs args_of(const pointops_qk_norm& in, const Shape& s) {
     a.angle_n = in.angle_stride[1];
     a.tokens = in.B * in.N;
     a.step = s.step;
+    a.slices = s.slices;
     a.N = static_cast<int>(in.N);
     a.H = static_cast<int>(in.H);
     a.G = static_cast<int>(in.G);
@@ -295,9 +377,9 @@ hipError_t with_shape(const pointops_qk_norm& in, const Shape& s, F f) {
             case 2: return f(t, w, vec, std::integral_constant<int, 2>{});
             case 4: return f(t, w, vec, std::integral_constant<int, 4>{});
             case 8: return f(t, w, vec, std::integral_constant<int, 8>{});
-            case 16: if constexpr (VEC <= 4) return f(t, w, vec, std::integral_constant<int, 16>{}); break;
-            case 32: if constexpr (VEC <= 2) return f(t, w, vec, std::integral_constant<int, 32>{}); break;
-            case 64: if constexpr (VEC <= 1) return f(t, w, vec, std::integral_constant<int, 64>{}); break;
+            case 16: return f(t, w, vec, std::integral_constant<int, 16>{});
+            case 32: if constexpr (VEC <= 4) return f(t, w, vec, std::integral_constant<int, 32>{}); break;
+            case 64: if constexpr (VEC <= 2) return f(t, w, vec, std::integral_constant<int, 64>{}); break;
         }
         return hipErrorInvalidValue;
     };
@@ -318,10 +400,6 @@ hipError_t with_shape(const pointops_qk_norm& in, const Shape& s, F f) {
     }
 }
 
-bool weights_aligned(const pointops_qk_norm& in) {
-    return reinterpret_cast<uintptr_t>(in.q_weight) % 16 == 0 && reinterpret_cast<uintptr_t>(in.k_weight) % 16 == 0;
-}
-
 }  // namespace
 }  // namespace attn
 }  // namespace pointops
@@ -336,7 +414,7 @@ hipError_t pointops_qk_norm_rotate(const pointops_qk_norm* in, void* q_out, void
     if ((in->H > 0 && (in->q == nullptr || q_out == nullptr)) || (in->G > 0 && (in->k == nullptr || k_out == nullptr)) ||
         (in->R > 0 && (in->cos == nullptr || in->sin == nullptr)))
         return hipErrorInvalidValue;
-    const Shape s = shape_of(*in, weights_aligned(*in) ? 0 : 1);
+    const Shape s = shape_of(*in);
     if (s.blocks > INT32_MAX) return hipErrorInvalidValue;
     const NormArgs a = args_of(*in, s);
     return with_shape(*in, s, [&](auto t, auto w, auto vec, auto lanes) {
@@ -352,8 +430,8 @@ hipError_t pointops_qk_norm_rotate(const pointops_qk_norm* in, void* q_out, void
 size_t pointops_qk_norm_rotate_backward_workspace_bytes(const pointops_qk_norm* in) {
     using namespace pointops::attn;
     if (!valid(in) || in->B == 0 || in->N == 0 || in->H + in->G == 0) return 0;
-    // For each block, q's and k's columns: at most 128 each, whatever the pieces' width.
-    return static_cast<size_t>(std::max(kBlocks, in->H + in->G)) * 2 * 128 * sizeof(float);
+    // For each block, q's and k's columns: at most 256 each.
+    return static_cast<size_t>(std::max(kBlocks, in->H + in->G)) * 2 * 256 * sizeof(float);
 }
 
 hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const void* q_grad, const int64_t* q_grad_stride,
@@ -371,18 +449,10 @@ hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const vo
         return hipErrorInvalidValue;
     const bool sums = dq_weight != nullptr || dk_weight != nullptr;
     if (sums && workspace == nullptr) return hipErrorInvalidValue;
-    const int size = in->type == POINTOPS_F32 ? 4 : 2;
     Rows gq{}, gk{};
-    int64_t bits = weights_aligned(*in) ? 0 : 1;
-    if (q_grad_stride != nullptr) {
-        gq = {q_grad, q_grad_stride[0], q_grad_stride[1], q_grad_stride[2]};
-        bits |= gq.b | gq.n | gq.h | static_cast<int64_t>(reinterpret_cast<uintptr_t>(q_grad) / size);
-    }
-    if (k_grad_stride != nullptr) {
-        gk = {k_grad, k_grad_stride[0], k_grad_stride[1], k_grad_stride[2]};
-        bits |= gk.b | gk.n | gk.h | static_cast<int64_t>(reinterpret_cast<uintptr_t>(k_grad) / size);
-    }
-    const Shape s = shape_of(*in, bits);
+    if (q_grad_stride != nullptr) gq = {q_grad, q_grad_stride[0], q_grad_stride[1], q_grad_stride[2]};
+    if (k_grad_stride != nullptr) gk = {k_grad, k_grad_stride[0], k_grad_stride[1], k_grad_stride[2]};
+    const Shape s = shape_of(*in);
     if (s.blocks > INT32_MAX) return hipErrorInvalidValue;
     const NormArgs a = args_of(*in, s);
     float* const part = sums ? static_cast<float*>(workspace) : nullptr;
@@ -394,9 +464,8 @@ hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const vo
                            stream, a, gq, gk, static_cast<T*>(dq), static_cast<T*>(dk), part);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess || !sums) return err;
-        hipLaunchKernelGGL(qk_norm_weight_kernel<W>, dim3((4 * L * VEC + kWaves - 1) / kWaves), dim3(kThreads), 0, stream,
-                           part, static_cast<int>(s.blocks), L, VEC, a.D, a.R, static_cast<W*>(dq_weight),
-                           static_cast<W*>(dk_weight));
+        hipLaunchKernelGGL((qk_norm_weight_kernel<W, VEC, L>), dim3((4 * L * VEC + 15) / 16), dim3(kThreads), 0, stream, part,
+                           static_cast<int>(s.blocks), a.D, a.R, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
         return hipGetLastError();
     });
 }

@@ -173,7 +173,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle (without building a Stream object: 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def call(name: str, *args) -> None:

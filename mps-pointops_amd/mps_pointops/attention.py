@@ -169,21 +169,28 @@ def _pack(q: Tensor, k: Tensor, v: Tensor, window, sinks, causal, bias, edges, l
         0 if lengths is None else 8 * lengths.element_size(), bool(causal), _TYPES[q.dtype], scale)
 
 
+def _tracked(*tensors: Tensor | None) -> bool:
+    """Whether the call's graph is recorded."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 # ------------------------------------------------------------------ attention
+def _attend(q, k, v, bias, lengths, edges, window, sinks, causal, scale, lse):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.numel():
+        args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
+        _native.call("pointops_attention_forward", args, out.data_ptr(), _native.ptr(lse), _native.stream(q.device))
+    return out
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, lengths, edges, window, sinks, causal, scale):
         batch, queries, heads, _ = q.shape
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        needed = any(ctx.needs_input_grad[:4])
-        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device) if needed else None
-        if out.numel():
-            args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
-            _native.call("pointops_attention_forward", args, out.data_ptr(), _native.ptr(lse),
-                         _native.stream(q.device))
-        if needed:
-            ctx.save_for_backward(q, k, v, bias, lengths, out, lse)
-            ctx.rest = edges, window, sinks, causal, scale
+        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device)
+        out = _attend(q, k, v, bias, lengths, edges, window, sinks, causal, scale, lse)
+        ctx.save_for_backward(q, k, v, bias, lengths, out, lse)
+        ctx.rest = edges, window, sinks, causal, scale
         return out
 
     @staticmethod
@@ -237,9 +244,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = No
     _native.require_device(q.device)
     if scale is None:
         scale = q.shape[3] ** -0.5
-    return _WindowAttention.apply(
-        _rows(q), _rows(k), _rows(v), None if bias is None else bias.contiguous(),
-        None if lengths is None else lengths.contiguous(), edges, window, sinks, causal, float(scale))
+    args = (_rows(q), _rows(k), _rows(v), None if bias is None else bias.contiguous(),
+            None if lengths is None else lengths.contiguous(), edges, window, sinks, causal, float(scale))
+    return _WindowAttention.apply(*args) if _tracked(q, k, v, bias) else _attend(*args, None)
 
 
 def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor | None = None, *,
@@ -256,7 +263,7 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     """
     edges = _check_attention(q, k_cache, v_cache, window, sinks, True, bias, max_distance, lengths)
     _native.require_device(q.device)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_cache, v_cache, bias)):
+    if _tracked(q, k_cache, v_cache, bias):
         raise ValueError("window_attention_step has no gradients: call it under torch.no_grad(), "
                          "or use window_attention")
     q, k_cache, v_cache = _rows(q), _rows(k_cache), _rows(v_cache)
@@ -277,16 +284,20 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
 _MAX_BIAS_TOKENS = (1 << 22) - 1
 
 
+def _dense_bias(table, edges, queries, keys):
+    buckets, heads = table.shape
+    out = torch.empty((heads, queries, keys), dtype=table.dtype, device=table.device)
+    if out.numel():
+        _native.call("pointops_relative_bias", table.data_ptr(), edges, len(edges), buckets, _TYPES[table.dtype],
+                     out.data_ptr(), heads, queries, keys, _native.stream(table.device))
+    return out
+
+
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, edges, queries, keys):
-        buckets, heads = table.shape
-        out = torch.empty((heads, queries, keys), dtype=table.dtype, device=table.device)
-        if out.numel():
-            _native.call("pointops_relative_bias", table.data_ptr(), edges, len(edges), buckets, _TYPES[table.dtype],
-                         out.data_ptr(), heads, queries, keys, _native.stream(table.device))
-        ctx.rest = edges, buckets
-        return out
+        ctx.rest = edges, table.shape[0]
+        return _dense_bias(table, edges, queries, keys)
 
     @staticmethod
     @once_differentiable
@@ -321,7 +332,8 @@ def relative_bias(table: Tensor, queries: int, keys: int, *, max_distance: int, 
     if max(queries, keys) > _MAX_BIAS_TOKENS or table.shape[1] > 65535:
         raise ValueError(f"relative_bias supports at most {_MAX_BIAS_TOKENS} queries and keys and 65535 heads")
     _native.require_device(table.device)
-    return _RelativeBias.apply(table.contiguous(), edges, int(queries), int(keys))
+    args = table.contiguous(), edges, int(queries), int(keys)
+    return _RelativeBias.apply(*args) if _tracked(table) else _dense_bias(*args)
 
 
 # --------------------------------------------------------- norm and rotation
@@ -340,18 +352,21 @@ def _pack_norm(q, k, q_weight, k_weight, cos, sin, eps) -> bytes:
         _TYPES[q.dtype], _TYPES[q.dtype if weight is None else weight.dtype], eps)
 
 
+def _norm(q, k, q_weight, k_weight, cos, sin, eps):
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q_out.numel() + k_out.numel():
+        _native.call("pointops_qk_norm_rotate", _pack_norm(q, k, q_weight, k_weight, cos, sin, eps),
+                     q_out.data_ptr(), k_out.data_ptr(), _native.stream(q.device))
+    return q_out, k_out
+
+
 class _QkNormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        if q_out.numel() + k_out.numel():
-            _native.call("pointops_qk_norm_rotate", _pack_norm(q, k, q_weight, k_weight, cos, sin, eps),
-                         q_out.data_ptr(), k_out.data_ptr(), _native.stream(q.device))
-        if any(ctx.needs_input_grad[:4]):
-            ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
-            ctx.eps = eps
-        return q_out, k_out
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
+        ctx.eps = eps
+        return _norm(q, k, q_weight, k_weight, cos, sin, eps)
 
     @staticmethod
     @once_differentiable
@@ -431,9 +446,9 @@ def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     cos, sin = _rows(cos), _rows(sin)
     if cos.stride() != sin.stride():
         cos, sin = cos.contiguous(), sin.contiguous()
-    return _QkNormRotate.apply(
-        _rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),
-        None if k_weight is None else k_weight.contiguous(), cos, sin, float(eps))
+    args = (_rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),
+            None if k_weight is None else k_weight.contiguous(), cos, sin, float(eps))
+    return _QkNormRotate.apply(*args) if _tracked(q, k, q_weight, k_weight) else _norm(*args)
 
 
 __all__ = ["bucket_edges", "qk_norm_rotate", "relative_bias", "window_attention", "window_attention_step"]
