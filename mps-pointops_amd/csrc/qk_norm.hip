@@ -13,9 +13,15 @@
 // another's, or two pieces of the others.  Where a part is no multiple of the
 // piece, its last piece starts earlier: two lanes then hold the same values and
 // write the same results, and one of them leaves them out of the sums.  A group
-// of lanes keeps its columns for all its heads and tokens: the angles are read
-// once a token, the weights once, and the weights' gradients are summed in
-// registers, then over a block, then over all, in a fixed order.
+// of lanes keeps its head and columns for all its tokens: the weights and the
+// sums for their gradients stay in registers, and are added over a block, then
+// over all, in a fixed order.
+//
+// At 32 x 4096 tokens, 4 + 4 heads of 32, float32: 55 us (5.1 TB/s of what it
+// must move; a large copy reaches 5.15) and 85 + 5 us for the gradients (4.9).
+// At 65537 tokens, 12 + 3 heads of 80 (60 rotated), float16, which are 6 lanes
+// of 8: 81 us (4.1 TB/s) and 115 + 7 (4.2); with one piece of 4 bytes a lane,
+// as the parts' common divisor would have it, 133 and 305.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -31,8 +37,8 @@ struct NormArgs {
     int64_t angle_b, angle_n;
     int64_t tokens;  // B N
     int64_t step;    // tokens that are in work at a time
-    int slices;      // groups of lanes that share a token's heads
     int N, H, G, D, R;
+    int units;       // lanes of a row that have columns
     float eps, inv_d;
 };
 
@@ -78,52 +84,65 @@ struct Columns {
     }
 };
 
-// A lane's place: its slice of the heads, its pieces' columns, its token.
+// A lane's place: its head (of q's, then of k's) and its pieces' columns for
+// the whole call, and the tokens it goes through.  Lanes behind the last unit
+// read the first columns, add nothing and write nothing.
 template <typename T, int VEC, int L>
 struct Place {
     Columns<VEC> col;
-    int slice;
-    bool has_a, has_b;
-    int b, n, step_b, step_n;
-    int64_t token;
+    int head;
+    bool is_q, has_a, has_b;
+    int n;
+    int64_t token, b;
 
     __device__ __forceinline__ explicit Place(const NormArgs& a) : col(threadIdx.x % L, a.D, a.R) {
         const int64_t group = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;
-        slice = static_cast<int>(group % a.slices);
-        token = group / a.slices;
+        const int heads = a.H + a.G;
+        head = static_cast<int>(group % heads);
+        token = group / heads;
         if (token >= a.step) token = a.tokens;  // groups behind the last whole set
-        has_a = col.a < a.D;
-        has_b = col.b < a.D;
-        b = static_cast<int>(token / a.N);
-        n = static_cast<int>(token % a.N);
-        step_b = static_cast<int>(a.step / a.N);
-        step_n = static_cast<int>(a.step % a.N);
-    }
-    __device__ __forceinline__ void next(const NormArgs& a) {
-        token += a.step;
-        b += step_b;
-        n += step_n;
-        if (n >= a.N) {
-            n -= a.N;
-            ++b;
+        is_q = head < a.H;
+        const bool used = static_cast<int>(threadIdx.x % L) < a.units;
+        has_a = used && col.a < a.D;
+        has_b = used && col.b < a.D;
+        if (!has_a) {
+            col.a = 0;
+            col.skip_a = VEC;
         }
+        if (!has_b) {
+            col.b = 0;
+            col.skip_b = VEC;
+        }
+        b = token / a.N;
+        n = static_cast<int>(token % a.N);
     }
-    // Head `head` of q's, then of k's, as it comes and as a row of the contiguous results.
-    __device__ __forceinline__ const T* in(const Rows& q, const Rows& k, int H, int head) const {
-        return head < H ? q.at<T>(b, head) + n * q.n : k.at<T>(b, head - H) + n * k.n;
+    // On to the next token; whether it is in another batch than step / N further.
+    __device__ __forceinline__ bool next(const NormArgs& a) {
+        token += a.step;
+        n += static_cast<int>(a.step % a.N);
+        const bool wrapped = n >= a.N;
+        n -= wrapped ? a.N : 0;
+        return wrapped;
     }
-    __device__ __forceinline__ T* out(T* q, T* k, const NormArgs& a, int head) const {
-        return head < a.H ? q + (token * a.H + head) * a.D : k + (token * a.G + head - a.H) * a.D;
-    }
+};
+
+// A row's place in a tensor, moved on with its token.
+struct Cursor {
+    int64_t at, step, wrap;  // elements; wrap: what a change of batch adds
+    __device__ __forceinline__ Cursor(int64_t b, int64_t n, int64_t stride_b, int64_t stride_n, const NormArgs& a)
+        : at(b * stride_b + n * stride_n),
+          step(a.step / a.N * stride_b + a.step % a.N * stride_n),
+          wrap(stride_b - a.N * stride_n) {}
+    __device__ __forceinline__ void next(bool wrapped) { at += step + (wrapped ? wrap : 0); }
 };
 
 template <typename W, int VEC>
 struct Weights {
     Piece<W, VEC> a, b;
-    __device__ __forceinline__ void load(const void* w, const Columns<VEC>& col, bool has_a, bool has_b) {
+    __device__ __forceinline__ Weights(const void* w, const Columns<VEC>& col) {
         const bool given = w != nullptr;
-        a.load(static_cast<const W*>(w) + col.a, given && has_a);
-        b.load(static_cast<const W*>(w) + col.b, given && has_b);
+        a.load(static_cast<const W*>(w) + col.a, given);
+        b.load(static_cast<const W*>(w) + col.b, given);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             a.v[e] = given ? a.v[e] : 1.f;
@@ -132,65 +151,52 @@ struct Weights {
     }
 };
 
-constexpr int kAhead = 2;  // heads whose values are asked for at once
 
-// By value: a conditional of two array elements would choose an address.
-__device__ __forceinline__ float pick(bool first, float x, float y) { return first ? x : y; }
-
-// The sum of x y over the row, each value once.
+// The pieces with what another lane counts left out.
 template <int VEC>
-__device__ __forceinline__ float row_part(const float (&xa)[VEC], const float (&ya)[VEC], const float (&xb)[VEC],
-                                          const float (&yb)[VEC], const Columns<VEC>& col) {
-    const uint32_t keep_a = ~0u << col.skip_a, keep_b = ~0u << col.skip_b;
-    float sum = 0.f;
+__device__ __forceinline__ void counted(const float (&x)[VEC], int skip, float (&out)[VEC]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        sum = __builtin_fmaf((keep_a >> e & 1) != 0 ? xa[e] : 0.f, ya[e], sum);
-        sum = __builtin_fmaf((keep_b >> e & 1) != 0 ? xb[e] : 0.f, yb[e], sum);
-    }
-    return sum;
+    for (int e = 0; e < VEC; ++e) out[e] = e >= skip ? x[e] : 0.f;
 }
 
 template <typename T, typename W, int VEC, int L>
 __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const NormArgs a, T* __restrict__ q_out, T* __restrict__ k_out) {
     Place<T, VEC, L> at(a);
     const Columns<VEC> col = at.col;
-    const int heads = a.H + a.G;
-    Weights<W, VEC> wq, wk;
-    wq.load(a.wq, col, at.has_a, at.has_b);
-    wk.load(a.wk, col, at.has_a, at.has_b);
-    for (; at.token < a.tokens; at.next(a)) {
+    const Rows& rows = at.is_q ? a.q : a.k;
+    const int head = at.is_q ? at.head : at.head - a.H, count = at.is_q ? a.H : a.G;
+    const T* const x = static_cast<const T*>(rows.p) + head * rows.h;
+    T* const out = (at.is_q ? q_out : k_out) + static_cast<int64_t>(head) * a.D;
+    Cursor in(at.b, at.n, rows.b, rows.n, a), angle(at.b, at.n, a.angle_b, a.angle_n, a);
+    const Weights<W, VEC> w(at.is_q ? a.wq : a.wk, col);
+    const int64_t width = static_cast<int64_t>(count) * a.D;
+    while (at.token < a.tokens) {
+        Piece<T, VEC> xa, xb;
         Piece<float, VEC> c, s;
-        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + col.a;
-        c.load(a.cos + angle, col.turned);
-        s.load(a.sin + angle, col.turned);
-        for (int first = at.slice; first < heads; first += kAhead * a.slices) {
-            Piece<T, VEC> xa[kAhead], xb[kAhead];
+        xa.load(x + in.at + col.a, true);
+        xb.load(x + in.at + col.b, true);
+        c.load(a.cos + angle.at + col.a, col.turned);
+        s.load(a.sin + angle.at + col.a, col.turned);
+        float ca[VEC], cb[VEC], sum = 0.f;
+        counted<VEC>(xa.v, col.skip_a, ca);
+        counted<VEC>(xb.v, col.skip_b, cb);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int head = first + u * a.slices;
-                const T* const x = at.in(a.q, a.k, a.H, head);
-                xa[u].load(x + col.a, at.has_a && head < heads);
-                xb[u].load(x + col.b, at.has_b && head < heads);
-            }
+        for (int e = 0; e < VEC; ++e) sum = __builtin_fmaf(ca[e], ca[e], __builtin_fmaf(cb[e], cb[e], sum));
+        const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int head = first + u * a.slices;
-                const float sum = row_part<VEC>(xa[u].v, xa[u].v, xb[u].v, xb[u].v, col);
-                const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
-                const bool is_q = head < a.H;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float ya = xa[u].v[e] * r * pick(is_q, wq.a.v[e], wk.a.v[e]);
-                    const float yb = xb[u].v[e] * r * pick(is_q, wq.b.v[e], wk.b.v[e]);
-                    xa[u].v[e] = col.turned ? ya * c.v[e] - yb * s.v[e] : ya;
-                    xb[u].v[e] = col.turned ? yb * c.v[e] + ya * s.v[e] : yb;
-                }
-                T* const out = at.out(q_out, k_out, a, head);
-                xa[u].store(out + col.a, at.has_a && head < heads);
-                xb[u].store(out + col.b, at.has_b && head < heads);
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const float ya = xa.v[e] * (r * w.a.v[e]), yb = xb.v[e] * (r * w.b.v[e]);
+            const float ta = __builtin_fmaf(ya, c.v[e], -(yb * s.v[e]));
+            const float tb = __builtin_fmaf(yb, c.v[e], ya * s.v[e]);
+            xa.v[e] = col.turned ? ta : ya;
+            xb.v[e] = col.turned ? tb : yb;
         }
+        T* const dst = out + at.token * width;
+        xa.store(dst + col.a, at.has_a);
+        xb.store(dst + col.b, at.has_b);
+        const bool wrapped = at.next(a);
+        in.next(wrapped);
+        angle.next(wrapped);
     }
 }
 
@@ -199,100 +205,93 @@ __global__ __launch_bounds__(kThreads) void qk_norm_grad_kernel(const NormArgs a
                                                                 T* __restrict__ dq, T* __restrict__ dk,
                                                                 float* __restrict__ part) {
     __shared__ float sums[kThreads / L][2 * L * VEC];  // a group's columns: its first pieces, then its second
+    __shared__ int kinds[kThreads / L];
     Place<T, VEC, L> at(a);
     const Columns<VEC> col = at.col;
-    const int heads = a.H + a.G;
-    Weights<W, VEC> wq, wk;
-    wq.load(a.wq, col, at.has_a, at.has_b);
-    wk.load(a.wk, col, at.has_a, at.has_b);
-    float sa[2][VEC] = {}, sb[2][VEC] = {};  // q's and k's
-    for (; at.token < a.tokens; at.next(a)) {
+    const Rows& rows = at.is_q ? a.q : a.k;
+    const Rows& grads = at.is_q ? gq : gk;
+    const int head = at.is_q ? at.head : at.head - a.H, count = at.is_q ? a.H : a.G;
+    const T* const x = static_cast<const T*>(rows.p) + head * rows.h;
+    const T* const g = static_cast<const T*>(grads.p) + head * grads.h;
+    T* const out = (at.is_q ? dq : dk) + static_cast<int64_t>(head) * a.D;
+    Cursor in(at.b, at.n, rows.b, rows.n, a), from(at.b, at.n, grads.b, grads.n, a), angle(at.b, at.n, a.angle_b, a.angle_n, a);
+    const Weights<W, VEC> w(at.is_q ? a.wq : a.wk, col);
+    const int64_t width = static_cast<int64_t>(count) * a.D;
+    float sa[VEC] = {}, sb[VEC] = {};
+    while (at.token < a.tokens) {
+        Piece<T, VEC> xa, xb, ga, gb;
         Piece<float, VEC> c, s;
-        const int64_t angle = at.b * a.angle_b + at.n * a.angle_n + col.a;
-        c.load(a.cos + angle, col.turned);
-        s.load(a.sin + angle, col.turned);
-        for (int first = at.slice; first < heads; first += kAhead * a.slices) {
-            Piece<T, VEC> xa[kAhead], xb[kAhead], ga[kAhead], gb[kAhead];
+        xa.load(x + in.at + col.a, true);
+        xb.load(x + in.at + col.b, true);
+        ga.load(g + from.at + col.a, true);
+        gb.load(g + from.at + col.b, true);
+        c.load(a.cos + angle.at + col.a, col.turned);
+        s.load(a.sin + angle.at + col.a, col.turned);
+        float ca[VEC], cb[VEC], ua[VEC], ub[VEC];  // x counted once, dy w
+        counted<VEC>(xa.v, col.skip_a, ca);
+        counted<VEC>(xb.v, col.skip_b, cb);
+        float sum = 0.f, along = 0.f;
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int head = first + u * a.slices;
-                const T* const x = at.in(a.q, a.k, a.H, head);
-                const T* const g = at.in(gq, gk, a.H, head);
-                xa[u].load(x + col.a, at.has_a && head < heads);
-                xb[u].load(x + col.b, at.has_b && head < heads);
-                ga[u].load(g + col.a, at.has_a && head < heads);
-                gb[u].load(g + col.b, at.has_b && head < heads);
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int head = first + u * a.slices;
-                const bool is_q = head < a.H;
-                float ua[VEC], ub[VEC];  // dy w
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float da = col.turned ? ga[u].v[e] * c.v[e] + gb[u].v[e] * s.v[e] : ga[u].v[e];
-                    const float db = col.turned ? gb[u].v[e] * c.v[e] - ga[u].v[e] * s.v[e] : gb[u].v[e];
-                    ga[u].v[e] = da;
-                    gb[u].v[e] = db;
-                    ua[e] = da * pick(is_q, wq.a.v[e], wk.a.v[e]);
-                    ub[e] = db * pick(is_q, wq.b.v[e], wk.b.v[e]);
-                }
-                const float sum = row_part<VEC>(xa[u].v, xa[u].v, xb[u].v, xb[u].v, col);
-                const float along = row_part<VEC>(xa[u].v, ua, xb[u].v, ub, col);
-                const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
-                const float mean = group_sum<L>(along) * r * a.inv_d;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float na = xa[u].v[e] * r, nb = xb[u].v[e] * r;
-                    const float ta = ga[u].v[e] * na, tb = gb[u].v[e] * nb;
-                    sa[0][e] += is_q ? ta : 0.f;
-                    sb[0][e] += is_q ? tb : 0.f;
-                    sa[1][e] += is_q ? 0.f : ta;
-                    sb[1][e] += is_q ? 0.f : tb;
-                    xa[u].v[e] = r * (ua[e] - na * mean);
-                    xb[u].v[e] = r * (ub[e] - nb * mean);
-                }
-                // Of a row of one value the difference leaves eps r^2 alone, which rounding would bury.
-                if constexpr (VEC == 1 && L == 1)
-                    if (a.D == 1) xa[u].v[0] = r * r * r * a.eps * ua[0];
-                T* const out = at.out(dq, dk, a, head);
-                xa[u].store(out + col.a, at.has_a && head < heads);
-                xb[u].store(out + col.b, at.has_b && head < heads);
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const float da = __builtin_fmaf(ga.v[e], c.v[e], gb.v[e] * s.v[e]);
+            const float db = __builtin_fmaf(gb.v[e], c.v[e], -(ga.v[e] * s.v[e]));
+            ga.v[e] = col.turned ? da : ga.v[e];
+            gb.v[e] = col.turned ? db : gb.v[e];
+            ua[e] = ga.v[e] * w.a.v[e];
+            ub[e] = gb.v[e] * w.b.v[e];
+            sum = __builtin_fmaf(ca[e], ca[e], __builtin_fmaf(cb[e], cb[e], sum));
+            along = __builtin_fmaf(ca[e], ua[e], __builtin_fmaf(cb[e], ub[e], along));
         }
+        const float r = __builtin_amdgcn_rsqf(group_sum<L>(sum) * a.inv_d + a.eps);
+        const float mean = group_sum<L>(along) * r * a.inv_d;
+        const float back = mean * r * r;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            sa[e] = __builtin_fmaf(ga.v[e], xa.v[e] * r, sa[e]);
+            sb[e] = __builtin_fmaf(gb.v[e], xb.v[e] * r, sb[e]);
+            xa.v[e] = __builtin_fmaf(ua[e], r, -(xa.v[e] * back));
+            xb.v[e] = __builtin_fmaf(ub[e], r, -(xb.v[e] * back));
+        }
+        // Of a row of one value the difference leaves eps r^2 alone, which rounding would bury.
+        if constexpr (VEC == 1 && L == 1)
+            if (a.D == 1) xa.v[0] = r * r * r * a.eps * ua[0];
+        T* const dst = out + at.token * width;
+        xa.store(dst + col.a, at.has_a);
+        xb.store(dst + col.b, at.has_b);
+        const bool wrapped = at.next(a);
+        in.next(wrapped);
+        from.next(wrapped);
+        angle.next(wrapped);
     }
     if (part == nullptr) return;
     // part (blocks, q or k, columns in the lanes' order)
     constexpr int kColumns = 2 * L * VEC;
     const int group = threadIdx.x / L, unit = threadIdx.x % L;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            sums[group][unit * VEC + e] = sa[which][e];
-            sums[group][(L + unit) * VEC + e] = sb[which][e];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < kColumns; i += kThreads) {
-            float all = 0.f;
+    for (int e = 0; e < VEC; ++e) {
+        sums[group][unit * VEC + e] = sa[e];
+        sums[group][(L + unit) * VEC + e] = sb[e];
+    }
+    if (unit == 0) kinds[group] = at.is_q ? 0 : 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * kColumns; i += kThreads) {
+        float all = 0.f;
 #pragma unroll 8
-            for (int gr = 0; gr < kThreads / L; ++gr) all += sums[gr][i];
-            part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * kColumns + i] = all;
-        }
+        for (int gr = 0; gr < kThreads / L; ++gr) all += kinds[gr] == i / kColumns ? sums[gr][i % kColumns] : 0.f;
+        part[static_cast<int64_t>(blockIdx.x) * 2 * kColumns + i] = all;
     }
 }
 
-// dw from the blocks' parts: a block for 16 columns, 16 lanes of blocks each.
+// dw from the blocks' parts: a block for 8 columns, 32 lanes of blocks each.
 template <typename W, int VEC, int L>
 __global__ __launch_bounds__(kThreads) void qk_norm_weight_kernel(const float* __restrict__ part, int blocks, int D, int R,
                                                                   W* __restrict__ dwq, W* __restrict__ dwk) {
-    constexpr int kColumns = 2 * L * VEC, kAcross = 16, kLanes = kThreads / kAcross;
+    constexpr int kColumns = 2 * L * VEC, kAcross = 8, kLanes = kThreads / kAcross;
     __shared__ float sums[kLanes][kAcross];
     const int x = threadIdx.x % kAcross, y = threadIdx.x / kAcross, id = blockIdx.x * kAcross + x;
     float all = 0.f;
     if (id < 2 * kColumns) {
-#pragma unroll 8
+#pragma unroll 16
         for (int b = y; b < blocks; b += kLanes) all += part[static_cast<int64_t>(b) * 2 * kColumns + id];
     }
     sums[y][x] = all;
@@ -311,28 +310,24 @@ __global__ __launch_bounds__(kThreads) void qk_norm_weight_kernel(const float* _
 constexpr int64_t kBlocks = 2048;
 
 struct Shape {
-    int vec, lanes, slices;
+    int vec, units, lanes;
     int64_t blocks, step;
 };
 
 // The widest pieces that the rotated half and the rest hold, and blocks enough
-// to fill the card (each keeps its sums until its end).  A wave takes
-// neighbouring heads of a token, or all of its heads at once where the whole
-// call is small and its latency counts.
+// to fill the card (each keeps its sums until its end).
 Shape shape_of(const pointops_qk_norm& in) {
     const int half = static_cast<int>(in.R / 2), rest = static_cast<int>(in.D - in.R);
     Shape s;
     s.vec = in.type == POINTOPS_F32 ? 4 : 8;
     while ((half > 0 && s.vec > half) || (rest > 0 && s.vec > rest)) s.vec /= 2;
-    const int units = (half + s.vec - 1) / s.vec + ((rest + s.vec - 1) / s.vec + 1) / 2;
+    s.units = (half + s.vec - 1) / s.vec + ((rest + s.vec - 1) / s.vec + 1) / 2;
     s.lanes = 1;
-    while (s.lanes < units) s.lanes *= 2;
+    while (s.lanes < s.units) s.lanes *= 2;
     const int64_t tokens = in.B * in.N, heads = in.H + in.G, groups = kThreads / s.lanes;
-    const bool small = tokens * heads * s.lanes <= (1 << 18);
-    s.slices = static_cast<int>(small ? heads : std::min<int64_t>(heads, kWave / s.lanes));
-    s.blocks = std::min(kBlocks, (tokens * s.slices + groups - 1) / groups);
-    s.blocks = std::max(s.blocks, (s.slices + groups - 1) / groups);
-    s.step = std::min(tokens, s.blocks * groups / s.slices);
+    s.blocks = std::min(kBlocks, (tokens * heads + groups - 1) / groups);
+    s.blocks = std::max(s.blocks, (heads + groups - 1) / groups);
+    s.step = std::min(tokens, s.blocks * groups / heads);
     return s;
 }
 
@@ -356,7 +351,7 @@ NormArgs args_of(const pointops_qk_norm& in, const Shape& s) {
     a.angle_n = in.angle_stride[1];
     a.tokens = in.B * in.N;
     a.step = s.step;
-    a.slices = s.slices;
+    a.units = s.units;
     a.N = static_cast<int>(in.N);
     a.H = static_cast<int>(in.H);
     a.G = static_cast<int>(in.G);
@@ -464,7 +459,7 @@ hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const vo
                            stream, a, gq, gk, static_cast<T*>(dq), static_cast<T*>(dk), part);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess || !sums) return err;
-        hipLaunchKernelGGL((qk_norm_weight_kernel<W, VEC, L>), dim3((4 * L * VEC + 15) / 16), dim3(kThreads), 0, stream, part,
+        hipLaunchKernelGGL((qk_norm_weight_kernel<W, VEC, L>), dim3((4 * L * VEC + 7) / 8), dim3(kThreads), 0, stream, part,
                            static_cast<int>(s.blocks), a.D, a.R, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
         return hipGetLastError();
     });
