@@ -39,7 +39,6 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
     const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
-    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
 
     const int rows = min(kOuter, a.Q - i0);
     const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
@@ -60,6 +59,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         ks.load(k, a.k.n, t * TK, len, a.D);
         vs.load(v, a.v.n, t * TK, len, a.D);
     }
+    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
     i32x4 q[TileT::kChunks], go[TileT::kChunks];
     float delta = 0.f, lse = kInf, rest = 0.f;
     const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Q + row;

@@ -86,7 +86,6 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
     const int i0 = folded(at.inner, blocks) * kOuter;
     const int len = a.length(b), shift = a.N - a.Q;
-    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
 
     // The block's rows that exist, by position, and the tiles that they see.
     const int rows = min(kOuter, a.Q - i0);
@@ -108,6 +107,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         ks.load(k, a.k.n, t * TK, len, a.D);
         vs.load(v, a.v.n, t * TK, len, a.D);
     }
+    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
     i32x4 q[TileT::kChunks];
     {
         const T* src = a.q.at<T>(b, h) + row * a.q.n;

@@ -17,7 +17,13 @@ namespace pointops {
 namespace attn {
 namespace {
 
-constexpr int kTile = 32;  // keys at a time; queries of a block
+constexpr int kTile = 32;  // keys of a wave at a time; queries of a block
+
+// Waves of a block: 8 where all that is seen is 32 tiles or fewer, which are
+// then one block's work and need no join, 4 otherwise (4 x 65536 keys, 32 heads
+// over 8 of 128, bfloat16: 171 us by 4 waves, 183 by 8) and for 32-bit values,
+// whose tiles take twice the LDS.
+constexpr int kShortTiles = 32;
 
 // The tiles that a block of rows sees: the first keys', then the window's.
 struct Tiles {
@@ -27,10 +33,11 @@ struct Tiles {
     }
 };
 
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void attention_step_kernel(
+template <typename T, int DP, bool VEC, int WAVES>
+__global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attention_step_kernel(
     const Args a, T* __restrict__ out, float* __restrict__ part, int row_blocks, int splits) {
     using TileT = Tile<T, DP>;
+    constexpr int kWaves = WAVES, kThreads = kWave * kWaves;
     constexpr int kOut = DP / 32, kPerRow = DP * static_cast<int>(sizeof(T)) / 16, kPieces = kTile * kPerRow / kWave;
     constexpr int kSumStride = DP + 4;
     constexpr int kTileBytes = kTile * TileT::kStride;
@@ -291,28 +298,30 @@ __global__ __launch_bounds__(kThreads) void attention_step_join_kernel(const Arg
 }
 
 struct Plan {
-    int row_blocks, splits;
+    int row_blocks, waves, splits;
 };
 
-// Enough blocks to fill the card, each wave with two tiles or more.
-Plan plan_of(const Args& a) {
+// Splits of the keys that give every compute unit four blocks, with at least
+// two tiles a wave.
+Plan plan_of(const Args& a, int type) {
     const int64_t rows = static_cast<int64_t>(a.Q) * (a.H / a.G), row_blocks = (rows + kTile - 1) / kTile;
     const int64_t all = (static_cast<int64_t>(a.N) + kTile - 1) / kTile;
     const int64_t window = (static_cast<int64_t>(a.window) + a.Q - 1) / kTile + 2 + (a.sinks + kTile - 1) / kTile;
     const int64_t tiles = std::min(all, window), units = std::max<int64_t>(1, row_blocks * a.B * a.G);
-    const int64_t splits = std::min((1024 + units - 1) / units, tiles / (2 * kWaves));
-    return {static_cast<int>(row_blocks), static_cast<int>(std::max<int64_t>(1, splits))};
+    if (type != POINTOPS_F32 && tiles <= kShortTiles) return {static_cast<int>(row_blocks), 8, 1};
+    const int64_t splits = std::min((1024 + units - 1) / units, tiles / 8);
+    return {static_cast<int>(row_blocks), 4, static_cast<int>(std::max<int64_t>(1, splits))};
 }
 
-size_t workspace_of(const Args& a) {
-    const Plan p = plan_of(a);
+size_t workspace_of(const Args& a, int type) {
+    const Plan p = plan_of(a, type);
     if (p.splits == 1) return 0;
     return static_cast<size_t>(a.B) * a.G * p.row_blocks * p.splits * kTile * (a.D + 2) * sizeof(float);
 }
 
 template <typename T>
-hipError_t step(const Args& a, void* out, void* workspace, hipStream_t stream) {
-    const Plan plan = plan_of(a);
+hipError_t step(const Args& a, int type, void* out, void* workspace, hipStream_t stream) {
+    const Plan plan = plan_of(a, type);
     const int64_t blocks = static_cast<int64_t>(a.B) * a.G * plan.row_blocks * plan.splits;
     const int64_t rows = static_cast<int64_t>(a.B) * a.H * a.Q;
     if (blocks > INT32_MAX || (rows + kWaves - 1) / kWaves > INT32_MAX) return hipErrorInvalidValue;
@@ -321,13 +330,17 @@ hipError_t step(const Args& a, void* out, void* workspace, hipStream_t stream) {
     float* const part = static_cast<float*>(workspace);
     const hipError_t err = with_width(a.D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        const dim3 grid(static_cast<uint32_t>(blocks));
-        if (vec)
-            hipLaunchKernelGGL((attention_step_kernel<T, DP, true>), grid, dim3(kThreads), lds, stream, a,
+        auto launch = [&](auto* kernel, int waves) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kWave * waves), lds, stream, a,
                                static_cast<T*>(out), part, plan.row_blocks, plan.splits);
-        else
-            hipLaunchKernelGGL((attention_step_kernel<T, DP, false>), grid, dim3(kThreads), lds, stream, a,
-                               static_cast<T*>(out), part, plan.row_blocks, plan.splits);
+        };
+        if constexpr (sizeof(T) == 2) {
+            if (plan.waves == 8) {
+                launch(vec ? attention_step_kernel<T, DP, true, 8> : attention_step_kernel<T, DP, false, 8>, 8);
+                return hipGetLastError();
+            }
+        }
+        launch(vec ? attention_step_kernel<T, DP, true, 4> : attention_step_kernel<T, DP, false, 4>, 4);
         return hipGetLastError();
     });
     if (err != hipSuccess || plan.splits == 1) return err;
@@ -345,7 +358,7 @@ extern "C" {
 size_t pointops_attention_step_workspace_bytes(const pointops_attention* in) {
     using namespace pointops::attn;
     Args a;
-    return read_args(in, &a) && a.H > 0 ? workspace_of(a) : 0;
+    return read_args(in, &a) && a.H > 0 ? workspace_of(a, in->type) : 0;
 }
 
 hipError_t pointops_attention_step(const pointops_attention* in, void* out, void* workspace, hipStream_t stream) {
@@ -357,11 +370,11 @@ hipError_t pointops_attention_step(const pointops_attention* in, void* out, void
     if (static_cast<int64_t>(a.Q) * (a.H / a.G) > (int64_t(1) << 30)) return hipErrorInvalidValue;
     if (in->q == nullptr || out == nullptr || (in->N > 0 && (in->k == nullptr || in->v == nullptr)))
         return hipErrorInvalidValue;
-    if (workspace == nullptr && workspace_of(a) != 0) return hipErrorInvalidValue;
+    if (workspace == nullptr && workspace_of(a, in->type) != 0) return hipErrorInvalidValue;
     switch (in->type) {
-        case POINTOPS_F32: return step<float>(a, out, workspace, stream);
-        case POINTOPS_F16: return step<f16>(a, out, workspace, stream);
-        default: return step<bf16>(a, out, workspace, stream);
+        case POINTOPS_F32: return step<float>(a, in->type, out, workspace, stream);
+        case POINTOPS_F16: return step<f16>(a, in->type, out, workspace, stream);
+        default: return step<bf16>(a, in->type, out, workspace, stream);
     }
 }
 

@@ -27,50 +27,71 @@ bool read_buckets(const int32_t* edges, int n, int count, int64_t most, Buckets*
 
 namespace {
 
-constexpr int kBiasRows = 64;    // of a block
+constexpr int kBiasRows = 64;    // of a block, or fewer where there are few blocks
 constexpr int kBiasCols = 1024;  // of a block
 
-// VEC values a store (rows are a multiple of that).
-template <typename T, int VEC>
+// Threads write 16 bytes each along a row, at any alignment, and its last
+// values one by one.
+template <typename T>
 __global__ __launch_bounds__(kThreads) void relative_bias_kernel(const Buckets bk, const T* __restrict__ table,
                                                                  T* __restrict__ out, int H, int Q, int N,
-                                                                 int col_blocks) {
+                                                                 int col_blocks, int block_rows) {
+    constexpr int VEC = kPerFrag<T>, kWide = kBiasCols / VEC, kStep = kThreads / kWide;
     __shared__ int edges[255];
-    __shared__ T values[kBiasRows + kBiasCols];  // of offset base + kBiasRows - 1 - x
+    __shared__ T values[kBiasRows + kBiasCols + VEC];  // entry x: offset base + rows - 1 - x
     const int h = blockIdx.x / col_blocks, j0 = static_cast<int>(blockIdx.x % col_blocks) * kBiasCols;
-    const int i0 = blockIdx.y * kBiasRows, rows = min(kBiasRows, Q - i0), cols = min(kBiasCols, N - j0);
+    const int i0 = blockIdx.y * block_rows, rows = min(block_rows, Q - i0), cols = min(kBiasCols, N - j0);
     const int base = N - Q + i0 - j0;  // offset of the first row and column
     for (int x = threadIdx.x; x < bk.n; x += kThreads) edges[x] = bk.edge[x];
     __syncthreads();
     for (int x = threadIdx.x; x < rows + cols - 1; x += kThreads)
         values[x] = table[static_cast<int64_t>(bucket_of(bk, edges, base + rows - 1 - x)) * H + h];
     __syncthreads();
-    T* const dst = out + (static_cast<int64_t>(h) * Q + i0) * N + j0;
-    const int per = cols / VEC;
-    // Threads along a row, then down the rows.
-    const int wide = kBiasCols / VEC, step = max(1, kThreads / wide);
-    for (int row = threadIdx.x / wide; row < rows; row += step)
-        for (int c = threadIdx.x % wide; c < per; c += kThreads) {
-            T v[VEC];
+    const int c = static_cast<int>(threadIdx.x) % kWide * VEC;
+    if (c >= cols) return;
+    for (int row = threadIdx.x / kWide; row < rows; row += kStep) {
+        T* const dst = out + (static_cast<int64_t>(h) * Q + i0 + row) * N + j0 + c;
+        T v[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = values[rows - 1 - row + c * VEC + e];
-            __builtin_memcpy(__builtin_assume_aligned(dst + static_cast<int64_t>(row) * N + c * VEC, VEC * sizeof(T)), v,
-                             sizeof v);
+        for (int e = 0; e < VEC; ++e) v[e] = values[rows - 1 - row + c + e];
+        if (c + VEC <= cols) {
+            typedef int words __attribute__((ext_vector_type(4), aligned(2)));
+            words w;
+            __builtin_memcpy(&w, v, sizeof w);
+            *reinterpret_cast<words*>(dst) = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (c + e < cols) dst[e] = v[e];
         }
+    }
 }
 
 constexpr int kDiagonals = 4;   // neighbouring ones of a thread
-constexpr int kDiagRows = 64;   // rows of a block
+constexpr int kDiagRows = 64;   // rows of a block, or fewer where there are few blocks
 constexpr int kDiagSpan = kThreads * kDiagonals;
+
+// kDiagonals values at any address, read past the caches' order of use: what
+// the forward has just written fills them, and the gradient is read once (16 x
+// 2048 x 2048, float32, aligned rows: 87 us with ordinary loads, 52 = 5.2 TB/s).
+template <typename T>
+struct Values {
+    T e[kDiagonals];
+};
+template <typename T>
+__device__ __forceinline__ Values<T> read_once(const T* p) {
+    typedef int words __attribute__((ext_vector_type(kDiagonals * sizeof(T) / 4), aligned(alignof(T))));
+    return __builtin_bit_cast(Values<T>, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+}
 
 // A thread's diagonals hold key less row = c .. c + 3, down the block's rows;
 // part[h][block][bucket].
 template <typename T>
 __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buckets bk, const T* __restrict__ grad,
                                                                       int64_t stride_h, int64_t stride_i,
-                                                                      float* __restrict__ part, int Q, int N) {
+                                                                      float* __restrict__ part, int Q, int N, int block_rows) {
     __shared__ float sums[kDiagSpan];  // by falling diagonal, so rising offset
-    const int h = blockIdx.z, i0 = blockIdx.y * kDiagRows, i_end = min(Q, i0 + kDiagRows);
+    const int h = blockIdx.z, i0 = blockIdx.y * block_rows, i_end = min(Q, i0 + block_rows);
     // The block's diagonals: those that meet its rows are -(i_end - 1) .. N - 1 - i0.
     const int c0 = static_cast<int>(blockIdx.x) * kDiagSpan - (i_end - 1);
     const int c = c0 + static_cast<int>(threadIdx.x) * kDiagonals;
@@ -88,10 +109,9 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buck
     edge(some, all);
 #pragma unroll 8
     for (int i = all; i < all_end; ++i) {
-        T v[kDiagonals];
-        __builtin_memcpy(v, src + i * stride_i + i, sizeof v);
+        const auto v = read_once<T>(src + i * stride_i + i);
 #pragma unroll
-        for (int e = 0; e < kDiagonals; ++e) sum[e] += to_float(v[e]);
+        for (int e = 0; e < kDiagonals; ++e) sum[e] += to_float(v.e[e]);
     }
     edge(all_end, some_end);
 #pragma unroll
@@ -106,28 +126,29 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buck
 // The same where every row starts at a multiple of 16 bytes: a thread reads
 // aligned pieces of V values, the same columns for V rows and V columns further
 // for the next V, so that 2 V - 1 diagonals stay in its registers; its
-// neighbour's share of them is added at the end.  16 x 2048 x 2048, float32: 92
-// us by the kernel above, KERNEL_US by this one.
+// neighbour's share of them is added at the end.  16 x 2048 x 2048, float32: 60 us
+// by the kernel above, by this one 52.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void relative_bias_grad_aligned_kernel(const Buckets bk, const T* __restrict__ grad,
                                                                               int64_t stride_h, int64_t stride_i,
-                                                                              float* __restrict__ part, int Q, int N) {
+                                                                              float* __restrict__ part, int Q, int N,
+                                                                              int block_rows) {
     constexpr int V = kPerFrag<T>, kSpan = kThreads * V + V - 1;
     __shared__ float sums[kSpan];  // by falling diagonal, so rising offset
-    const int h = blockIdx.z, i0 = blockIdx.y * kDiagRows, rows = min(kDiagRows, Q - i0);
-    // Columns at the block's first row: from -kDiagRows on.
-    const int first = static_cast<int>(blockIdx.x) * kThreads * V - kDiagRows;
+    const int h = blockIdx.z, i0 = blockIdx.y * block_rows, rows = min(block_rows, Q - i0);
+    // Columns at the block's first row: from -block_rows on.
+    const int first = static_cast<int>(blockIdx.x) * kThreads * V - block_rows;
     const int c0 = first + static_cast<int>(threadIdx.x) * V;
     float sum[2 * V - 1] = {};
     const T* const src = grad + h * stride_h + i0 * stride_i;
 #pragma unroll 2
-    for (int r = 0; r < kDiagRows; r += V) {
+    for (int r = 0; r < block_rows; r += V) {
         const int col = c0 + r;
         i32x4 v[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             v[i] = i32x4{0, 0, 0, 0};
-            if (col >= 0 && col < N && r + i < rows) v[i] = *reinterpret_cast<const i32x4*>(src + (r + i) * stride_i + col);
+            if (col >= 0 && col < N && r + i < rows) v[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(src + (r + i) * stride_i + col));
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -180,23 +201,24 @@ __global__ __launch_bounds__(kThreads) void join_buckets_kernel(const float* __r
 
 template <typename T>
 hipError_t launch_bias(const Buckets& bk, const void* table, void* out, int H, int Q, int N, hipStream_t stream) {
-    constexpr int VEC = 16 / static_cast<int>(sizeof(T));
     const int col_blocks = (N + kBiasCols - 1) / kBiasCols;
-    const int64_t x = static_cast<int64_t>(col_blocks) * H, y = (static_cast<int64_t>(Q) + kBiasRows - 1) / kBiasRows;
+    const int64_t x = static_cast<int64_t>(col_blocks) * H;
+    const int rows = x * ((Q + kBiasRows - 1) / kBiasRows) >= 512 ? kBiasRows : kBiasRows / 8;
+    const int64_t y = (static_cast<int64_t>(Q) + rows - 1) / rows;
     if (x > INT32_MAX || y > 65535) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<uint32_t>(x), static_cast<uint32_t>(y));
-    const T* const src = static_cast<const T*>(table);
-    T* const dst = static_cast<T*>(out);
-    if (N % VEC == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0)
-        hipLaunchKernelGGL((relative_bias_kernel<T, VEC>), grid, dim3(kThreads), 0, stream, bk, src, dst, H, Q, N, col_blocks);
-    else
-        hipLaunchKernelGGL((relative_bias_kernel<T, 1>), grid, dim3(kThreads), 0, stream, bk, src, dst, H, Q, N, col_blocks);
+    hipLaunchKernelGGL(relative_bias_kernel<T>, dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(y)), dim3(kThreads), 0,
+                       stream, bk, static_cast<const T*>(table), static_cast<T*>(out), H, Q, N, col_blocks, rows);
     return hipGetLastError();
 }
 
+// Rows of a block, and the blocks of `span` columns and those rows.
+int diagonal_rows(int64_t H, int64_t Q, int64_t N) {
+    return H * ((Q + kDiagRows - 1) / kDiagRows) * ((N + kDiagSpan - 1) / kDiagSpan) >= 512 ? kDiagRows : kDiagRows / 4;
+}
 dim3 diagonal_grid(int64_t H, int64_t Q, int64_t N, int64_t span) {
-    return dim3(static_cast<uint32_t>((N + kDiagRows + span - 1) / span),
-                static_cast<uint32_t>((Q + kDiagRows - 1) / kDiagRows), static_cast<uint32_t>(H));
+    const int64_t rows = diagonal_rows(H, Q, N);
+    return dim3(static_cast<uint32_t>((N + rows + span - 1) / span), static_cast<uint32_t>((Q + rows - 1) / rows),
+                static_cast<uint32_t>(H));
 }
 
 // Sizes that the kernels' launches hold.
@@ -275,7 +297,7 @@ hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, i
         using T = decltype(zero);
         auto* const kernel = aligned ? relative_bias_grad_aligned_kernel<T> : relative_bias_grad_kernel<T>;
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, bk, static_cast<const T*>(grad), stride_h, stride_i, part,
-                           q, n);
+                           q, n, diagonal_rows(H, Q, N));
         return hipGetLastError();
     };
     const hipError_t err = type == POINTOPS_F32 ? sums(float{}) : type == POINTOPS_F16 ? sums(f16{}) : sums(bf16{});
