@@ -9,9 +9,9 @@
 // (no atomics: results do not change from run to run): one holds 128 queries
 // in registers and passes over their keys (delta, dq), the other holds 128 keys
 // and passes over the queries that see them, all heads that share the key head
-// in turn (dk, dv and the bias's sums by offset).  Long passes (the first keys,
-// which every query sees) and few blocks are cut into pieces whose 32-bit sums
-// a last kernel joins.  ds and p are rounded to the inputs' type for the second
+// in turn (dk, dv and the bias's sums by offset).  The first keys, which every
+// query sees, have passes of their own for the queries beyond their window; they
+// and few blocks are cut into pieces whose 32-bit sums a last kernel joins.  ds and p are rounded to the inputs' type for the second
 // products, as the forward's weights are; the bias's sums take them unrounded.
 #include <algorithm>
 #include <atomic>
@@ -59,7 +59,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         ks.load(k, a.k.n, t * TK, len, a.D);
         vs.load(v, a.v.n, t * TK, len, a.D);
     }
-    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
+    const bool biased = BIAS && (VEC || a.bias != nullptr);  // rows that are not aligned have one kernel for both
+    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + entries));
     i32x4 q[TileT::kChunks], go[TileT::kChunks];
     float delta = 0.f, lse = kInf, rest = 0.f;
     const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Q + row;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     }
     __syncthreads();
 
-    const float factor = BIAS ? 1.f : a.scale_log2;
+    const float factor = biased ? 1.f : a.scale_log2;
     f32x16 dq[kOut] = {};
     char* ktile = lds;
     while (t < walk.end) {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                 ColumnFrags<T, DP> cf[2];  // of this chunk of keys and the next
                 cf[0].load(ktile, 32 * u);
                 keep_order();
-                if constexpr (BIAS) {
+                if (biased) {
                     s *= a.scale_log2;
                     if (far) {
                         s += table[near > 0 ? entries - 1 : 0];
@@ -176,23 +177,24 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     if (row < a.Q && half == 0) delta_out[stat] = delta;
 }
 
-// How the passes of the key blocks are cut: the blocks that hold the first
-// keys, which all later rows see, into `of_first` pieces, the others into
-// `of_rest`.  Blocks in one piece write their results, the others 32-bit parts.
+// How the passes of the keys are cut.  A key block passes over the queries
+// within its window, in `of_rest` pieces; the queries beyond the window, which
+// see the first keys alone, are passed over by groups of 32 of those, each in
+// `of_first` pieces.  A key block whose sums are in more than one place writes
+// 32-bit parts.
 struct Pieces {
-    int first_blocks, key_blocks;
-    int of_first, of_rest;
+    int key_blocks, of_rest;
+    int groups, of_first;
 
-    __host__ __device__ int64_t units() const {
-        return static_cast<int64_t>(first_blocks) * of_first + static_cast<int64_t>(key_blocks - first_blocks) * of_rest;
+    __host__ __device__ int units() const { return key_blocks * of_rest; }
+    __host__ __device__ int first_units() const { return groups * of_first; }
+    __host__ __device__ int first_blocks() const { return (32 * groups + kOuter - 1) / kOuter; }
+    __host__ __device__ bool parted(int block) const { return of_rest > 1 || block < first_blocks(); }
+    // Units whose parts are kept, and their floats with the groups', of one key head.
+    __host__ __device__ int kept() const { return of_rest > 1 ? units() : first_blocks(); }
+    __host__ __device__ int64_t floats(int DP) const {
+        return (static_cast<int64_t>(kept()) * kOuter + static_cast<int64_t>(first_units()) * 32) * 2 * DP;
     }
-    __host__ __device__ int of(int block) const { return block < first_blocks ? of_first : of_rest; }
-    // The first unit of a key block.
-    __host__ __device__ int64_t unit(int block) const {
-        const int first = block < first_blocks ? block : first_blocks;
-        return static_cast<int64_t>(first) * of_first + static_cast<int64_t>(block - first) * of_rest;
-    }
-    __host__ __device__ bool joined() const { return (first_blocks > 0 && of_first > 1) || (key_blocks > first_blocks && of_rest > 1); }
 };
 
 // Sums of ds along the diagonals of a wave's 16 x 32 piece: rows (keys) are
@@ -203,13 +205,15 @@ struct Pieces {
 constexpr int kSkewRow = 68;
 constexpr int kSkewFloats = 16 + 16 * kSkewRow;
 
-template <typename T, int DP, bool VEC, bool BIAS>
+// FIRST: the passes beyond the window.  All waves hold the same 32 keys there
+// and take 32 queries each in turn; their sums are added at the end.
+template <typename T, int DP, bool VEC, bool BIAS, bool FIRST>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
     const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const Rows grad,
     T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
     const Pieces cut) {
     using TileT = Tile<T, DP>;
-    constexpr int TQ = kInner<T>, kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
+    constexpr int TQ = kInner<T>, kSub = TQ / 32, kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
     constexpr bool kTight = sizeof(T) == 4 ? DP == 128 : BIAS && DP == 64;  // as above
     constexpr int kSet = 2 * kTileBytes + 8 * TQ;  // a tile of queries, one of gradients, their lse and delta
     extern __shared__ char lds[];                  // two sets, then the bias's tables
@@ -221,52 +225,64 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     int* const edges = reinterpret_cast<int*>(summed ? sums + kWaves * entries : skews);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const int units = static_cast<int>(cut.units());
+    const int units = FIRST ? cut.first_units() : cut.units(), pieces = FIRST ? cut.of_first : cut.of_rest;
     const Place at = place(a.B * a.G, units);
     const int bg = at.outer, b = bg / a.G, g = bg % a.G;
-    // The first keys' pieces, then the others (a causal call's earlier keys are seen by more rows).
-    const int first_units = cut.first_blocks * cut.of_first;
-    const int unit = at.inner < first_units ? at.inner : units - 1 - folded(at.inner - first_units, units - first_units);
-    const int pieces = unit < first_units ? cut.of_first : cut.of_rest;
-    const int piece = (unit < first_units ? unit : unit - first_units) % pieces;
-    const int jblock = unit < first_units ? unit / pieces : cut.first_blocks + (unit - first_units) / pieces;
-    const int j0 = jblock * kOuter, len = a.length(b), shift = a.N - a.Q;
-    const int group = a.H / a.G;
+    // A causal call's earlier keys are seen by more rows: long and short passes meet.
+    const int unit = FIRST ? at.inner : units - 1 - folded(at.inner, units);
+    const int piece = unit % pieces, block = unit / pieces;
+    const int len = a.length(b), shift = a.N - a.Q, group = a.H / a.G;
+
+    // This wave's keys, one a lane column; the block's.
+    const int j0 = FIRST ? 32 * block : kOuter * block, w0 = FIRST ? j0 : j0 + 32 * wave;
+    const int exist = FIRST ? min(len, a.sinks) : len;
+    const int w_last = min(w0 + 32, exist) - 1, j_last = FIRST ? w_last : min(j0 + kOuter, exist) - 1;
+    const bool w_any = w0 <= w_last;
+    const int j = w0 + lane % 32;
+
+    // Positions from which the lane's key is seen, see_low .. see_low +
+    // see_count - 1, or (beyond a window on both sides) all but those.
+    const bool other = FIRST && !a.causal;
+    auto window_end = [&](int key) { return key > len - a.window ? len - 1 : key + a.window - 1; };  // of the keys' own
+    int see_low = a.causal ? j : j - a.window + 1;
+    uint32_t see_count = static_cast<uint32_t>(max(window_end(j) - see_low + 1, 0));
+    if constexpr (FIRST) {
+        if (a.causal) {
+            see_low = window_end(j) + 1;
+            see_count = j < exist ? static_cast<uint32_t>(max(len - see_low, 0)) : 0u;
+        } else if (j >= exist) {
+            see_low = -1;
+            see_count = 0xffffffffu;
+        }
+    }
+    // Whether any, and whether all, of the wave's keys are seen from any (all)
+    // of the positions p .. p + TQ - 1.
+    auto meets = [&](int p) {
+        if constexpr (FIRST) return p + TQ - 1 > window_end(w0) || (other && p <= w_last - a.window);
+        return p <= window_end(w_last) && p + TQ > (a.causal ? w0 : w0 - a.window + 1);
+    };
+    auto wholly = [&](int p) {
+        if constexpr (FIRST) return w_last == w0 + 31 && (p > window_end(w_last) || (other && p + TQ - 1 <= w0 - a.window));
+        return p >= (a.causal ? w_last : w_last - a.window + 1) && p + TQ - 1 <= window_end(w0);
+    };
 
     // Queries that see any of the block's keys, by row; tiles count from the
     // first row that exists.
     const int i_low = max(-shift, 0), i_high = min(a.Q, len - shift);
-    const int j_last = min(j0 + kOuter, len) - 1;
     int i_first = 0, i_last = -1;
-    if (j_last >= j0) {
-        const bool first = j0 < a.sinks;
-        int p_low = a.causal ? j0 : first ? 0 : j0 - a.window + 1;
-        int p_high = first || j_last > len - a.window ? len - 1 : j_last + a.window - 1;
-        p_low = max(p_low, 0);
-        p_high = min(p_high, len - 1);
-        i_first = max(p_low - shift, i_low);
-        i_last = min(p_high - shift, i_high - 1);
+    if (j0 <= j_last) {
+        int p_low = a.causal ? j0 : j0 - a.window + 1, p_high = window_end(j_last);
+        if constexpr (FIRST) {
+            p_low = a.causal ? window_end(j0) + 1 : 0;
+            p_high = len - 1;
+        }
+        i_first = max(max(p_low, 0) - shift, i_low);
+        i_last = min(min(p_high, len - 1) - shift, i_high - 1);
     }
     // Their tiles, for every head in turn; this piece's share of them all.
     const int t_first = (i_first - i_low) / TQ, tiles = i_last < i_first ? 0 : (i_last - i_low) / TQ + 1 - t_first;
     const int64_t all_tiles = static_cast<int64_t>(tiles) * group;
     const int64_t share_low = all_tiles * piece / pieces, share_high = all_tiles * (piece + 1) / pieces;
-
-    // This wave's keys: one a lane column.
-    const int w0 = j0 + 32 * wave;
-    const int w_last = min(w0 + 32, len) - 1;
-    const bool w_any = w0 <= w_last;
-    const int j = w0 + lane % 32;
-    // The lane's key is seen from positions low .. low + count - 1; all or any
-    // of the wave's from these.
-    const bool first_key = j < a.sinks;
-    const int see_low = a.causal ? j : first_key ? 0 : j - a.window + 1;
-    const int see_high = first_key || j > len - a.window ? len - 1 : j + a.window - 1;
-    const uint32_t see_count = static_cast<uint32_t>(max(see_high - see_low + 1, 0));
-    const int all_low = a.causal ? w_last : w_last < a.sinks ? 0 : w_last - a.window + 1;
-    const int all_high = w_last < a.sinks || w0 > len - a.window ? len - 1 : w0 + a.window - 1;
-    const int any_low = a.causal ? w0 : w0 < a.sinks ? 0 : w0 - a.window + 1;
-    const int any_high = w0 < a.sinks || w_last > len - a.window ? len - 1 : w_last + a.window - 1;
 
     i32x4 k[TileT::kChunks], v[TileT::kChunks];
     {
@@ -284,7 +300,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     }
     f32x16 dk[kOut] = {}, dv[kOut] = {};
     float* const skew = skews + wave * kSkewFloats + 16;
-    const float factor = BIAS ? 1.f : a.scale_log2;
+    const bool biased = BIAS && (VEC || a.bias != nullptr);
+    const float factor = biased ? 1.f : a.scale_log2;
     float* const mine = sums + wave * entries;
     if (summed)
         for (int i = threadIdx.x; i < kWaves * kSkewFloats; i += kThreads) skews[i] = 0.f;
@@ -293,10 +310,23 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         const int h = g * group + hh;
         const int from = t_first + static_cast<int>(max(share_low - static_cast<int64_t>(hh) * tiles, int64_t(0)));
         const int to = t_first + static_cast<int>(min(share_high - static_cast<int64_t>(hh) * tiles, int64_t(tiles)));
-        if (from >= to && !summed) continue;
+        float* const bucket_part =
+            summed ? dbias_part + ((static_cast<int64_t>(b) * a.H + h) * (cut.units() + cut.first_units()) +
+                                   (FIRST ? cut.units() : 0) + unit) * a.bk.count : nullptr;
+        if (from >= to) {
+            if (summed)
+                for (int i = threadIdx.x; i < a.bk.count; i += kThreads) bucket_part[i] = 0.f;
+            continue;
+        }
+        // Where all offsets are beyond the reach, one value serves all and one bucket takes all.
+        const bool all_far = i_low + from * TQ + shift - (j0 + (FIRST ? 31 : kOuter - 1)) >= a.reach;
         __syncthreads();
-        if constexpr (BIAS) fill_bias<T>(a, h, table, edges);
-        if (summed)
+        if (biased) {
+            if (!all_far) fill_bias<T>(a, h, table, edges);
+            else if (threadIdx.x == 0)
+                table[entries - 1] = bias_log2(to_float(static_cast<const T*>(a.bias)[static_cast<int64_t>(a.bk.n) * a.H + h]));
+        }
+        if (summed && !all_far)
             for (int i = threadIdx.x; i < kWaves * entries; i += kThreads) sums[i] = 0.f;
         float far_early = 0.f, far_late = 0.f;  // ds of offsets beyond the reach
         const T* const q = a.q.at<T>(b, h);
@@ -321,10 +351,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             gs.store(set + kTileBytes);
             if (threadIdx.x < 2 * TQ) reinterpret_cast<float*>(set + 2 * kTileBytes)[threadIdx.x] = st;
         };
-        if (from < to) {
-            fetch(from);
-            put();
-        }
+        fetch(from);
+        put();
         __syncthreads();
         for (int t = from; t < to; ++t) {
             if (t + 1 < to) fetch(t + 1);
@@ -332,12 +360,13 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             const char* const gtile = set + kTileBytes;
             const float* const stat = reinterpret_cast<const float*>(set + 2 * kTileBytes);
             const int p0 = i_low + t * TQ + shift;  // position of the tile's first row
-            if (w_any && p0 <= any_high && p0 + TQ > any_low) {
-                const bool whole = p0 >= all_low && p0 + TQ - 1 <= all_high;
+            if (w_any && meets(p0)) {
+                const bool whole = wholly(p0);
                 const int near = p0 - w0;
                 const bool far = near - 31 >= a.reach || near + TQ - 1 <= -a.reach;
 #pragma unroll
-                for (int u = 0; u < TQ / 32; ++u) {
+                for (int u = 0; u < kSub; ++u) {
+                    if (FIRST && (t * kSub + u) % kWaves != wave) continue;
                     RowFrags<T, DP> qf, gf;
                     qf.load(qtile, 32 * u);
                     if (!kTight) gf.load(gtile, 32 * u);
@@ -355,7 +384,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                     gc[0].load(gtile, 32 * u);
                     qc[0].load(qtile, 32 * u);
                     keep_order();
-                    if constexpr (BIAS) {
+                    if (biased) {
                         s *= a.scale_log2;
                         if (far) {
                             s += table[near > 0 ? entries - 1 : 0];
@@ -375,7 +404,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                         const int p = p0 + 32 * u + 4 * half - see_low;
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if (static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) w[r] = ds[r] = 0.f;
+                            if ((static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) != other) w[r] = ds[r] = 0.f;
                     }
                     constexpr int kSteps = 16 / kPerFrag<T>;
 #pragma unroll
@@ -389,7 +418,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                         qc[c % 2].add(as_fragment<T>(&ds[c * kPerFrag<T>]), dk);
                     }
                     if (!summed) continue;
-                    if (j >= len) {  // keys of zeros with scores of their own
+                    if (!FIRST && j >= len) {  // keys of zeros with scores of their own
 #pragma unroll
                         for (int r = 0; r < 16; ++r) ds[r] = 0.f;
                     }
@@ -423,6 +452,13 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         if (summed) {
             far_early = wave_sum(far_early);
             far_late = wave_sum(far_late);
+            if (all_far) {
+                if (lane == 0) sums[wave] = far_early;
+                __syncthreads();
+                for (int i = threadIdx.x; i < a.bk.count; i += kThreads)
+                    bucket_part[i] = i == a.bk.n ? (sums[0] + sums[1]) + (sums[2] + sums[3]) : 0.f;
+                continue;
+            }
             if (lane == 0) {
                 mine[entries - 1] += far_early;
                 mine[0] += far_late;
@@ -435,8 +471,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 sums[i] = all;
             }
             __syncthreads();
-            add_buckets(a.bk, sums, entries, a.reach + kMargin,
-                        dbias_part + ((static_cast<int64_t>(b) * a.H + h) * units + unit) * a.bk.count);
+            add_buckets(a.bk, sums, entries, a.reach + kMargin, bucket_part);
         }
     }
 
@@ -448,9 +483,33 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             dk[d][r] = j < len ? dk[d][r] * a.scale : 0.f;
             dv[d][r] = j < len ? dv[d][r] : 0.f;
         }
-    if (pieces > 1) {
-        // (b g, unit, dk or dv, key of the block, DP)
-        float* const dst = part + ((static_cast<int64_t>(bg) * units + unit) * 2 * kOuter + (j - j0)) * DP;
+    float* const parts = part + bg * cut.floats(DP);
+    if constexpr (FIRST) {
+        // The waves' sums, added in order; then the part: (unit, dk or dv, key, DP).
+        constexpr int kRow = DP + 4;
+        float* const all = reinterpret_cast<float*>(lds);
+        for (int w = 0; w < kWaves; ++w) {
+            __syncthreads();
+            if (w != wave) continue;
+#pragma unroll
+            for (int d = 0; d < kOut; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f32x4* const x = reinterpret_cast<f32x4*>(all + lane % 32 * kRow + 32 * d + 8 * e + 4 * half);
+                    f32x4* const y = reinterpret_cast<f32x4*>(all + (32 + lane % 32) * kRow + 32 * d + 8 * e + 4 * half);
+                    const f32x4 zero = {};
+                    const f32x4 xk = {dk[d][4 * e], dk[d][4 * e + 1], dk[d][4 * e + 2], dk[d][4 * e + 3]};
+                    const f32x4 xv = {dv[d][4 * e], dv[d][4 * e + 1], dv[d][4 * e + 2], dv[d][4 * e + 3]};
+                    *x = (w == 0 ? zero : *x) + xk;
+                    *y = (w == 0 ? zero : *y) + xv;
+                }
+        }
+        __syncthreads();
+        float* const dst = parts + static_cast<int64_t>(cut.kept()) * 2 * kOuter * DP + static_cast<int64_t>(unit) * 2 * 32 * DP;
+        for (int i = threadIdx.x; i < 2 * 32 * DP; i += kThreads) dst[i] = all[i / DP * kRow + i % DP];
+    } else if (cut.parted(block)) {
+        // (unit, dk or dv, key of the block, DP)
+        float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kOuter + (j - j0)) * DP;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
@@ -459,32 +518,40 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 store4<float, true>(dst + kOuter * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
             }
     } else if (j < a.N) {
-        const int64_t at = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
+        const int64_t to = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                store4<T, VEC>(dk_out + at, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
-                store4<T, VEC>(dv_out + at, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
+                store4<T, VEC>(dk_out + to, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
+                store4<T, VEC>(dv_out + to, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
             }
     }
 }
 
-// The pieces' sums, in their order: a thread four values of a key.
+// The parts' sums, in their order: a thread four values of a key.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Args a, const float* __restrict__ part, int DP,
                                                                   T* __restrict__ dk, T* __restrict__ dv,
                                                                   const Pieces cut) {
-    const int bg = blockIdx.x / cut.key_blocks, jblock = blockIdx.x % cut.key_blocks;
-    const int b = bg / a.G, g = bg % a.G, pieces = cut.of(jblock);
-    if (pieces == 1) return;
+    const int bg = blockIdx.x / cut.key_blocks, block = blockIdx.x % cut.key_blocks;
+    const int b = bg / a.G, g = bg % a.G;
+    if (!cut.parted(block)) return;
     const int64_t each = static_cast<int64_t>(2) * kOuter * DP;
-    const float* const src = part + (bg * cut.units() + cut.unit(jblock)) * each;
+    const float* const parts = part + bg * cut.floats(DP);
     const int at = 4 * static_cast<int>(blockIdx.y * kThreads + threadIdx.x);  // of 2 x kOuter x DP
-    const int which = at / (kOuter * DP), key = at / DP % kOuter, d = at % DP, j = jblock * kOuter + key;
+    const int which = at / (kOuter * DP), key = at / DP % kOuter, d = at % DP, j = block * kOuter + key;
     if (which > 1 || d >= a.D || j >= a.N) return;
     f32x4 all = {};
-    for (int i = 0; i < pieces; ++i) all += *reinterpret_cast<const f32x4*>(src + i * each + at);
+    for (int i = 0; i < cut.of_rest; ++i)
+        all += *reinterpret_cast<const f32x4*>(parts + (static_cast<int64_t>(block) * cut.of_rest + i) * each + at);
+    if (j / 32 < cut.groups) {
+        const float* const first = parts + cut.kept() * each + static_cast<int64_t>(j / 32) * cut.of_first * 2 * 32 * DP;
+        const int own = (which * 32 + j % 32) * DP + d;
+#pragma unroll 4
+        for (int i = 0; i < cut.of_first; ++i)
+            all += *reinterpret_cast<const f32x4*>(first + static_cast<int64_t>(i) * 2 * 32 * DP + own);
+    }
     T* const dst = (which == 0 ? dk : dv) + ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
 #pragma unroll
     for (int f = 0; f < 4; ++f)
@@ -492,23 +559,19 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Args a, 
 }
 
 // Blocks enough to give every compute unit two (a block's wave is alone on its
-// SIMD for the wider heads and waits for its tiles), with 4 tiles or more each;
-// the first keys' blocks in pieces about as long as the others.  At 4 x 4096
-// queries, 8 heads over 2, window 512, D 64 (256 blocks): 1 piece 127 us, 2
-// with their join 84.
+// SIMD for the wider heads and waits for its tiles), with 4 tiles or more each.
 Pieces pieces_of(const Args& a, int inner) {
-    Pieces cut{0, (a.N + kOuter - 1) / kOuter, 1, 1};
-    const int64_t units = static_cast<int64_t>(cut.key_blocks) * a.B * a.G;
+    Pieces cut{(a.N + kOuter - 1) / kOuter, 1, 0, 1};
+    const int64_t heads = static_cast<int64_t>(a.B) * a.G, units = cut.key_blocks * heads;
     if (units == 0 || a.H == 0 || a.Q == 0) return cut;
-    const int64_t seen = std::min<int64_t>(a.Q, static_cast<int64_t>(a.causal ? 1 : 2) * a.window + kOuter);
-    const int64_t tiles = (seen + inner - 1) / inner * (a.H / a.G);
-    cut.of_rest = static_cast<int>(std::max<int64_t>(1, std::min((512 + units - 1) / units, tiles / 4)));
-    cut.of_first = cut.of_rest;
-    if (a.sinks > 0) {
-        cut.first_blocks = (a.sinks + kOuter - 1) / kOuter;
-        const int64_t first_tiles = (static_cast<int64_t>(a.Q) + inner - 1) / inner * (a.H / a.G);
-        const int64_t each = std::max<int64_t>(8, tiles / cut.of_rest);
-        cut.of_first = static_cast<int>(std::max<int64_t>(cut.of_rest, std::min<int64_t>(64, first_tiles / each)));
+    auto pieces = [&](int64_t rows, int64_t blocks, int64_t least) {
+        const int64_t tiles = (rows + inner - 1) / inner * (a.H / a.G);
+        return static_cast<int>(std::max<int64_t>(1, std::min((512 + blocks - 1) / blocks, tiles / least)));
+    };
+    cut.of_rest = pieces(std::min<int64_t>(a.Q, static_cast<int64_t>(a.causal ? 1 : 2) * a.window + kOuter), units, 4);
+    if (a.sinks > 0 && a.window < a.N) {
+        cut.groups = (a.sinks + 31) / 32;
+        cut.of_first = pieces(a.Q, cut.groups * heads, 2);
     }
     return cut;
 }
@@ -525,12 +588,11 @@ Workspace workspace_of(const Args& a, int type) {
     const size_t rows = static_cast<size_t>(a.B) * a.H;
     Workspace w{};
     w.cut = pieces_of(a, type == POINTOPS_F32 ? kInner<float> : kInner<f16>);
-    const size_t units = static_cast<size_t>(w.cut.units());
+    const size_t units = static_cast<size_t>(w.cut.units()) + w.cut.first_units();
     w.delta = 0;
     w.bias = up(rows * a.Q * sizeof(float));
     w.part = w.bias + (a.bias != nullptr ? up(rows * units * a.bk.count * sizeof(float)) : 0);
-    w.bytes = w.part;
-    if (w.cut.joined()) w.bytes += static_cast<size_t>(a.B) * a.G * units * 2 * kOuter * padded(a.D) * sizeof(float);
+    w.bytes = w.part + static_cast<size_t>(a.B) * a.G * w.cut.floats(padded(a.D)) * sizeof(float);
     return w;
 }
 
@@ -554,8 +616,8 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     float* const dbias_part = x.dbias != nullptr ? reinterpret_cast<float*>(x.workspace + w.bias) : nullptr;
     float* const part = reinterpret_cast<float*>(x.workspace + w.part);
     const int64_t grid_q = (static_cast<int64_t>(a.Q) + kOuter - 1) / kOuter * a.B * a.H;
-    const int64_t grid_k = cut.units() * a.B * a.G;
-    if (grid_q > INT32_MAX || grid_k > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t heads = static_cast<int64_t>(a.B) * a.G, grid_k = cut.units() * heads, grid_first = cut.first_units() * heads;
+    if (grid_q > INT32_MAX || grid_k > INT32_MAX || grid_first > INT32_MAX) return hipErrorInvalidValue;
 
     constexpr size_t tiles = 4 * kInner<T> * TileT::kStride, stats = 16 * kInner<T>;
     const size_t entries = bias_entries(a.reach), table = a.bias != nullptr ? 4 * (entries + a.bk.n) : 0;
@@ -573,24 +635,27 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
-        auto* const by_key = attention_grad_key_kernel<T, DP, VEC, BIAS>;
         // The tiles, their rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
         auto lds_for = [&](size_t n, size_t edges, bool sums) {
             return tiles + stats + 4 * ((n + 3) / 4 * 4 + edges) + (sums ? 4 * kWaves * (kSkewFloats + n) : 0);
         };
         const size_t lds = a.bias != nullptr ? lds_for(entries, a.bk.n, dbias_part != nullptr) : tiles + stats;
-        if (lds > kLdsFree) {
-            static std::atomic<uint64_t> allowed{0};
-            const hipError_t err = allow_lds(by_key, allowed, lds_for(bias_entries(kMaxReach), 255, true));
-            if (err != hipSuccess) return err;
-        }
-        hipLaunchKernelGGL(by_key, dim3(static_cast<uint32_t>(grid_k)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,
-                           static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, dbias_part, cut);
-        hipError_t err = hipGetLastError();
+        auto launch = [&](auto* kernel, int64_t grid, std::atomic<uint64_t>& allowed) {
+            if (lds > kLdsFree) {
+                const hipError_t err = allow_lds(kernel, allowed, lds_for(bias_entries(kMaxReach), 255, true));
+                if (err != hipSuccess) return err;
+            }
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,
+                               static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, dbias_part, cut);
+            return hipGetLastError();
+        };
+        static std::atomic<uint64_t> allowed[2];
+        hipError_t err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, false>, grid_k, allowed[0]);
+        if (err == hipSuccess && grid_first > 0)
+            err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, true>, grid_first, allowed[1]);
         if (err != hipSuccess) return err;
-        if (cut.joined()) {
-            const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.G * cut.key_blocks),
-                            2 * kOuter * DP / (4 * kThreads));
+        if (cut.kept() > 0) {
+            const dim3 grid(static_cast<uint32_t>(heads * cut.key_blocks), 2 * kOuter * DP / (4 * kThreads));
             hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(kThreads), 0, stream, a, part, DP,
                                static_cast<T*>(x.dk), static_cast<T*>(x.dv), cut);
             err = hipGetLastError();
@@ -598,7 +663,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         }
     }
     if (dbias_part == nullptr) return hipSuccess;
-    return join_buckets(dbias_part, a.B, a.H, cut.units(), a.bk.count, kType<T>, x.dbias, stream);
+    return join_buckets(dbias_part, a.B, a.H, cut.units() + cut.first_units(), a.bk.count, kType<T>, x.dbias, stream);
 }
 
 template <typename T>
@@ -607,9 +672,8 @@ hipError_t backward(const Args& a, const Grads& x, hipStream_t stream) {
                      vector_rows<T>(x.grad, a.D) && reinterpret_cast<uintptr_t>(x.out) % 16 == 0;
     return with_width(a.D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        if (a.bias != nullptr)
-            return vec ? launch_backward<T, DP, true, true>(a, x, stream) : launch_backward<T, DP, false, true>(a, x, stream);
-        return vec ? launch_backward<T, DP, true, false>(a, x, stream) : launch_backward<T, DP, false, false>(a, x, stream);
+        if (!vec) return launch_backward<T, DP, false, true>(a, x, stream);
+        return a.bias != nullptr ? launch_backward<T, DP, true, true>(a, x, stream) : launch_backward<T, DP, true, false>(a, x, stream);
     });
 }
 

@@ -107,7 +107,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         ks.load(k, a.k.n, t * TK, len, a.D);
         vs.load(v, a.v.n, t * TK, len, a.D);
     }
-    if constexpr (BIAS) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
+    const bool biased = BIAS && (VEC || a.bias != nullptr);  // rows that are not aligned have one kernel for both
+    if (biased) fill_bias<T>(a, h, table, reinterpret_cast<int*>(table + bias_entries(a.reach)));
     i32x4 q[TileT::kChunks];
     {
         const T* src = a.q.at<T>(b, h) + row * a.q.n;
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
 
     // Scores as the products leave them, in units of 1 / factor: a bias needs
     // them scaled, and a negative scale turns their order.
-    const bool scaled = BIAS || !(a.scale > 0.f);
+    const bool scaled = biased || !(a.scale > 0.f);
     const float factor = scaled ? 1.f : a.scale_log2;
     f32x16 o[kOut] = {};
     float m = -kInf, l = 0.f;  // the maximum so far (scaled; see kSlack) and this half-wave's sum
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) s[u] *= a.scale_log2;
             }
-            if constexpr (BIAS) {
+            if (biased) {
                 const int near = w0 - j0;  // offset of the wave's first row and the tile's first key
                 if (near - (TK - 1) >= a.reach || near + 31 <= -a.reach) {
                     const float far = table[near > 0 ? bias_entries(a.reach) - 1 : 0];
@@ -260,11 +261,13 @@ hipError_t forward(const pointops_attention* in, const Args& a, void* out, float
         const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
         const dim3 grid(static_cast<uint32_t>(blocks));
         const bool bias = a.bias != nullptr;
-        auto* const kernel = vec ? (bias ? attention_forward_kernel<T, DP, true, true> : attention_forward_kernel<T, DP, true, false>)
-                                 : (bias ? attention_forward_kernel<T, DP, false, true> : attention_forward_kernel<T, DP, false, false>);
+        const int which = !vec ? 0 : bias ? 1 : 2;
+        auto* const kernel = which == 0   ? attention_forward_kernel<T, DP, false, true>
+                             : which == 1 ? attention_forward_kernel<T, DP, true, true>
+                                          : attention_forward_kernel<T, DP, true, false>;
         if (lds > kLdsFree) {
-            static std::atomic<uint64_t> allowed[2][2];
-            const hipError_t err = allow_lds(kernel, allowed[vec][bias], tiles + 4 * (bias_entries(kMaxReach) + 255));
+            static std::atomic<uint64_t> allowed[3];
+            const hipError_t err = allow_lds(kernel, allowed[which], tiles + 4 * (bias_entries(kMaxReach) + 255));
             if (err != hipSuccess) return err;
         }
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, a, static_cast<T*>(out), lse);
