@@ -270,6 +270,36 @@ constexpr float kSlack = 8.f;
 template <typename T>
 constexpr int kInner = sizeof(T) == 4 ? 32 : 64;
 
+// Where 128 rows a block would leave compute units with one block or none, a
+// block takes 64: two waves share each 32 of them and take half of every inner
+// tile (of 64 rows) each, and their sums are joined in LDS at the end.
+template <typename T, int SPLIT>
+struct Cut {
+    static constexpr int kRows = kOuter / SPLIT;  // of a block
+    static constexpr int kInnerRows = SPLIT == 2 ? 64 : kInner<T>;
+    static constexpr int kSub = kInnerRows / 32 / SPLIT;  // 32-row pieces of an inner tile that a wave takes
+};
+inline bool few_blocks(int64_t blocks) { return blocks < 512; }
+// Rows of up to 256 bytes: the wider ones' tiles of 64 would leave no LDS for a bias.
+template <typename T, int DP>
+constexpr bool kSplits = DP * sizeof(T) <= 256;
+
+// A wave's registers to its partner, lane by lane.
+template <int N>
+__device__ __forceinline__ void put_sums(float* lds, const f32x16 (&v)[N]) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) lds[(d * 16 + r) * kWave + lane_id()] = v[d][r];
+}
+template <int N>
+__device__ __forceinline__ void get_sums(const float* lds, f32x16 (&v)[N], float keep, float by) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[d][r] = __builtin_fmaf(lds[(d * 16 + r) * kWave + lane_id()], by, v[d][r] * keep);
+}
+
 // Registers from .. from + 3 of a result to elements at .. at + 3 of a row
 // (VEC: the row's width is a multiple of 4 and its start aligned to as many).
 template <typename T, bool VEC>

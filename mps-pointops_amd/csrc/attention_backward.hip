@@ -22,32 +22,34 @@ namespace pointops {
 namespace attn {
 namespace {
 
-template <typename T, int DP, bool VEC, bool BIAS>
+template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void attention_grad_query_kernel(
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
     float* __restrict__ delta_out, T* __restrict__ dq_out, const bool refine) {
     using TileT = Tile<T, DP>;
-    constexpr int TK = kInner<T>, kOut = DP / 32, kTileBytes = TK * TileT::kStride;
+    constexpr int TK = Cut<T, SPLIT>::kInnerRows, kSub = Cut<T, SPLIT>::kSub, kRows = Cut<T, SPLIT>::kRows;
+    constexpr int kOut = DP / 32, kTileBytes = TK * TileT::kStride;
     constexpr bool kTight = sizeof(T) == 2 && DP == 128;  // no registers for both products' operands at once
     extern __shared__ char lds[];  // two pairs of a key and a value tile, the bias's table
     float* const table = reinterpret_cast<float*>(lds + 4 * kTileBytes);
     const int entries = bias_entries(a.reach);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const int blocks = (a.Q + kOuter - 1) / kOuter;
+    const int wave_row = 32 * (wave % (kWaves / SPLIT)), sub = wave / (kWaves / SPLIT) * kSub;  // its rows, its pieces
+    const int blocks = (a.Q + kRows - 1) / kRows;
     const Place at = place(a.B * a.H, blocks);
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
-    const int i0 = folded(at.inner, blocks) * kOuter;
+    const int i0 = folded(at.inner, blocks) * kRows;
     const int len = a.length(b), shift = a.N - a.Q;
 
-    const int rows = min(kOuter, a.Q - i0);
+    const int rows = min(kRows, a.Q - i0);
     const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
 
-    const int w0 = i0 + 32 * wave + shift;
-    const int w_count = min(32, i0 + rows - (i0 + 32 * wave));
+    const int w0 = i0 + wave_row + shift;
+    const int w_count = min(32, i0 + rows - (i0 + wave_row));
     const int w_first = max(w0, 0), w_last = min(w0 + w_count, len) - 1;
     const bool w_any = w_first <= w_last, w_whole = w_any && w0 >= 0 && w0 + w_count <= len;
-    const int row = i0 + 32 * wave + lane % 32, p = row + shift;
+    const int row = i0 + wave_row + lane % 32, p = row + shift;
     const bool exists = row < a.Q && p >= 0 && p < len;
     const Seen seen = seen_by(a, p, len);
 
@@ -108,23 +110,24 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
             const int near = w0 - j0;
             const bool far = near - (TK - 1) >= a.reach || near + 31 <= -a.reach;
 #pragma unroll
-            for (int u = 0; u < TK / 32; ++u) {
+            for (int u = 0; u < kSub; ++u) {
+                const int own = 32 * (sub + u);  // first row of the piece
                 RowFrags<T, DP> kf, vf;
-                kf.load(ktile, 32 * u);
-                if (!kTight) vf.load(vtile, 32 * u);
+                kf.load(ktile, own);
+                if (!kTight) vf.load(vtile, own);
                 keep_order();
                 f32x16 s = kf.times(q);
-                if (kTight) vf.load(vtile, 32 * u);
+                if (kTight) vf.load(vtile, own);
                 const f32x16 dp = vf.times(go);
                 ColumnFrags<T, DP> cf[2];  // of this chunk of keys and the next
-                cf[0].load(ktile, 32 * u);
+                cf[0].load(ktile, own);
                 keep_order();
                 if (biased) {
                     s *= a.scale_log2;
                     if (far) {
                         s += table[near > 0 ? entries - 1 : 0];
                     } else {
-                        const float* const from = table + near + lane % 32 - 4 * half - 32 * u + a.reach + kMargin;
+                        const float* const from = table + near + lane % 32 - 4 * half - own + a.reach + kMargin;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[r] += from[-(8 * (r / 4) + r % 4)];
                     }
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                     ds[r] = w * (dp[r] - delta);
                 }
                 if (!whole) {
-                    const int j = j0 + 32 * u + 4 * half;
+                    const int j = j0 + own + 4 * half;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (!seen(j + 8 * (r / 4) + r % 4)) ds[r] = 0.f;
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                 constexpr int kSteps = 16 / kPerFrag<T>;
 #pragma unroll
                 for (int c = 0; c < kSteps; ++c) {
-                    if (c + 1 < kSteps) cf[(c + 1) % 2].load(ktile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
+                    if (c + 1 < kSteps) cf[(c + 1) % 2].load(ktile, own + (c + 1) * TileT::kRowsPerFrag);
                     keep_order();
                     cf[c % 2].add(as_fragment<T>(&ds[c * kPerFrag<T>]), dq);
                 }
@@ -162,6 +165,17 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         __syncthreads();
     }
 
+    if constexpr (SPLIT == 2) {
+        float* const other = reinterpret_cast<float*>(lds) + wave % 2 * (16 * kOut + 1) * kWave;
+        if (wave >= 2) {
+            put_sums(other + kWave, dq);
+            other[lane] = rest;
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+        rest += other[lane];
+        get_sums(other + kWave, dq, 1.f, 1.f);
+    }
     if (row < a.Q) {
         T* const dst = dq_out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
 #pragma unroll
@@ -177,23 +191,25 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     if (row < a.Q && half == 0) delta_out[stat] = delta;
 }
 
-// How the passes of the keys are cut.  A key block passes over the queries
-// within its window, in `of_rest` pieces; the queries beyond the window, which
+// How the passes of the keys are cut.  A key block of `rows` keys passes over the
+// queries within its window, in `of_rest` pieces; the queries beyond the window, which
 // see the first keys alone, are passed over by groups of 32 of those, each in
 // `of_first` pieces.  A key block whose sums are in more than one place writes
 // 32-bit parts.
 struct Pieces {
-    int key_blocks, of_rest;
+    int rows, key_blocks, of_rest;
     int groups, of_first;
 
     __host__ __device__ int units() const { return key_blocks * of_rest; }
     __host__ __device__ int first_units() const { return groups * of_first; }
-    __host__ __device__ int first_blocks() const { return (32 * groups + kOuter - 1) / kOuter; }
-    __host__ __device__ bool parted(int block) const { return of_rest > 1 || block < first_blocks(); }
+    __host__ __device__ int first_blocks() const { return (32 * groups + rows - 1) / rows; }
+    // The blocks with parts come first.
+    __host__ __device__ int joined_blocks() const { return of_rest > 1 ? key_blocks : first_blocks(); }
+    __host__ __device__ bool parted(int block) const { return block < joined_blocks(); }
     // Units whose parts are kept, and their floats with the groups', of one key head.
-    __host__ __device__ int kept() const { return of_rest > 1 ? units() : first_blocks(); }
+    __host__ __device__ int kept() const { return joined_blocks() * of_rest; }
     __host__ __device__ int64_t floats(int DP) const {
-        return (static_cast<int64_t>(kept()) * kOuter + static_cast<int64_t>(first_units()) * 32) * 2 * DP;
+        return (static_cast<int64_t>(kept()) * rows + static_cast<int64_t>(first_units()) * 32) * 2 * DP;
     }
 };
 
@@ -207,13 +223,14 @@ constexpr int kSkewFloats = 16 + 16 * kSkewRow;
 
 // FIRST: the passes beyond the window.  All waves hold the same 32 keys there
 // and take 32 queries each in turn; their sums are added at the end.
-template <typename T, int DP, bool VEC, bool BIAS, bool FIRST>
+template <typename T, int DP, bool VEC, bool BIAS, bool FIRST, int SPLIT>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
     const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const Rows grad,
     T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
     const Pieces cut) {
     using TileT = Tile<T, DP>;
-    constexpr int TQ = kInner<T>, kSub = TQ / 32, kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
+    constexpr int TQ = Cut<T, SPLIT>::kInnerRows, kSub = Cut<T, SPLIT>::kSub, kRows = Cut<T, SPLIT>::kRows;
+    constexpr int kOut = DP / 32, kTileBytes = TQ * TileT::kStride;
     constexpr bool kTight = sizeof(T) == 4 ? DP == 128 : BIAS && DP == 64;  // as above
     constexpr int kSet = 2 * kTileBytes + 8 * TQ;  // a tile of queries, one of gradients, their lse and delta
     extern __shared__ char lds[];                  // two sets, then the bias's tables
@@ -234,9 +251,10 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     const int len = a.length(b), shift = a.N - a.Q, group = a.H / a.G;
 
     // This wave's keys, one a lane column; the block's.
-    const int j0 = FIRST ? 32 * block : kOuter * block, w0 = FIRST ? j0 : j0 + 32 * wave;
+    const int sub = wave / (kWaves / SPLIT) * kSub;  // its pieces of a tile
+    const int j0 = FIRST ? 32 * block : kRows * block, w0 = FIRST ? j0 : j0 + 32 * (wave % (kWaves / SPLIT));
     const int exist = FIRST ? min(len, a.sinks) : len;
-    const int w_last = min(w0 + 32, exist) - 1, j_last = FIRST ? w_last : min(j0 + kOuter, exist) - 1;
+    const int w_last = min(w0 + 32, exist) - 1, j_last = FIRST ? w_last : min(j0 + kRows, exist) - 1;
     const bool w_any = w0 <= w_last;
     const int j = w0 + lane % 32;
 
@@ -319,7 +337,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             continue;
         }
         // Where all offsets are beyond the reach, one value serves all and one bucket takes all.
-        const bool all_far = i_low + from * TQ + shift - (j0 + (FIRST ? 31 : kOuter - 1)) >= a.reach;
+        const bool all_far = i_low + from * TQ + shift - (j0 + (FIRST ? 31 : kRows - 1)) >= a.reach;
         __syncthreads();
         if (biased) {
             if (!all_far) fill_bias<T>(a, h, table, edges);
@@ -367,29 +385,30 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) {
                     if (FIRST && (t * kSub + u) % kWaves != wave) continue;
+                    const int own = 32 * (sub + u);  // first row of the piece
                     RowFrags<T, DP> qf, gf;
-                    qf.load(qtile, 32 * u);
-                    if (!kTight) gf.load(gtile, 32 * u);
+                    qf.load(qtile, own);
+                    if (!kTight) gf.load(gtile, own);
                     f32x4 lse[4], delta[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        lse[e] = *reinterpret_cast<const f32x4*>(stat + 32 * u + 8 * e + 4 * half);
-                        delta[e] = *reinterpret_cast<const f32x4*>(stat + TQ + 32 * u + 8 * e + 4 * half);
+                        lse[e] = *reinterpret_cast<const f32x4*>(stat + own + 8 * e + 4 * half);
+                        delta[e] = *reinterpret_cast<const f32x4*>(stat + TQ + own + 8 * e + 4 * half);
                     }
                     keep_order();
                     f32x16 s = qf.times(k);
-                    if (kTight) gf.load(gtile, 32 * u);
+                    if (kTight) gf.load(gtile, own);
                     const f32x16 dp = gf.times(v);
                     ColumnFrags<T, DP> qc[2], gc[2];  // of this chunk of queries and the next
-                    gc[0].load(gtile, 32 * u);
-                    qc[0].load(qtile, 32 * u);
+                    gc[0].load(gtile, own);
+                    qc[0].load(qtile, own);
                     keep_order();
                     if (biased) {
                         s *= a.scale_log2;
                         if (far) {
                             s += table[near > 0 ? entries - 1 : 0];
                         } else {
-                            const float* const from = table + near - lane % 32 + 4 * half + 32 * u + a.reach + kMargin;
+                            const float* const from = table + near - lane % 32 + 4 * half + own + a.reach + kMargin;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) s[r] += from[8 * (r / 4) + r % 4];
                         }
@@ -401,7 +420,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                         ds[r] = w[r] * (dp[r] - delta[r / 4][r % 4]);
                     }
                     if (!whole) {
-                        const int p = p0 + 32 * u + 4 * half - see_low;
+                        const int p = p0 + own + 4 * half - see_low;
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             if ((static_cast<uint32_t>(p + 8 * (r / 4) + r % 4) >= see_count) != other) w[r] = ds[r] = 0.f;
@@ -410,8 +429,8 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
 #pragma unroll
                     for (int c = 0; c < kSteps; ++c) {
                         if (c + 1 < kSteps) {
-                            gc[(c + 1) % 2].load(gtile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
-                            qc[(c + 1) % 2].load(qtile, 32 * u + (c + 1) * TileT::kRowsPerFrag);
+                            gc[(c + 1) % 2].load(gtile, own + (c + 1) * TileT::kRowsPerFrag);
+                            qc[(c + 1) % 2].load(qtile, own + (c + 1) * TileT::kRowsPerFrag);
                         }
                         keep_order();
                         gc[c % 2].add(as_fragment<T>(&w[c * kPerFrag<T>]), dv);
@@ -440,7 +459,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                             float all[4] = {};
 #pragma unroll
                             for (int r = 0; r < 16; ++r) all[r % 4] += skew[r * (kSkewRow + 1) + lane - 16];
-                            mine[near + 32 * u - 16 * x + lane - 16 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
+                            mine[near + own - 16 * x + lane - 16 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
                         }
                     }
                 }
@@ -475,6 +494,18 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         }
     }
 
+    if constexpr (SPLIT == 2) {
+        float* const other = reinterpret_cast<float*>(lds) + wave % 2 * 32 * kOut * kWave;
+        __syncthreads();
+        if (wave >= 2) {
+            put_sums(other, dk);
+            put_sums(other + 16 * kOut * kWave, dv);
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+        get_sums(other, dk, 1.f, 1.f);
+        get_sums(other + 16 * kOut * kWave, dv, 1.f, 1.f);
+    }
     // Keys behind the cloud's length have no gradient.
 #pragma unroll
     for (int d = 0; d < kOut; ++d)
@@ -505,17 +536,17 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 }
         }
         __syncthreads();
-        float* const dst = parts + static_cast<int64_t>(cut.kept()) * 2 * kOuter * DP + static_cast<int64_t>(unit) * 2 * 32 * DP;
+        float* const dst = parts + static_cast<int64_t>(cut.kept()) * 2 * cut.rows * DP + static_cast<int64_t>(unit) * 2 * 32 * DP;
         for (int i = threadIdx.x; i < 2 * 32 * DP; i += kThreads) dst[i] = all[i / DP * kRow + i % DP];
     } else if (cut.parted(block)) {
         // (unit, dk or dv, key of the block, DP)
-        float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kOuter + (j - j0)) * DP;
+        float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kRows + (j - j0)) * DP;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 store4<float, true>(dst, 32 * d + 8 * e + 4 * half, DP, dk[d], 4 * e);
-                store4<float, true>(dst + kOuter * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
+                store4<float, true>(dst + kRows * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
             }
     } else if (j < a.N) {
         const int64_t to = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
@@ -534,44 +565,57 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Args a, const float* __restrict__ part, int DP,
                                                                   T* __restrict__ dk, T* __restrict__ dv,
                                                                   const Pieces cut) {
-    const int bg = blockIdx.x / cut.key_blocks, block = blockIdx.x % cut.key_blocks;
+    const int blocks = cut.joined_blocks(), bg = blockIdx.x / blocks, block = blockIdx.x % blocks;
     const int b = bg / a.G, g = bg % a.G;
-    if (!cut.parted(block)) return;
-    const int64_t each = static_cast<int64_t>(2) * kOuter * DP;
+    const int64_t each = static_cast<int64_t>(2) * cut.rows * DP;
     const float* const parts = part + bg * cut.floats(DP);
-    const int at = 4 * static_cast<int>(blockIdx.y * kThreads + threadIdx.x);  // of 2 x kOuter x DP
-    const int which = at / (kOuter * DP), key = at / DP % kOuter, d = at % DP, j = block * kOuter + key;
+    const int at = 4 * static_cast<int>(blockIdx.y * kThreads + threadIdx.x);  // of 2 x rows x DP
+    const int which = at / (cut.rows * DP), key = at / DP % cut.rows, d = at % DP, j = block * cut.rows + key;
     if (which > 1 || d >= a.D || j >= a.N) return;
+    // Eight parts are asked for at once: each comes from memory.
     f32x4 all = {};
-    for (int i = 0; i < cut.of_rest; ++i)
-        all += *reinterpret_cast<const f32x4*>(parts + (static_cast<int64_t>(block) * cut.of_rest + i) * each + at);
-    if (j / 32 < cut.groups) {
-        const float* const first = parts + cut.kept() * each + static_cast<int64_t>(j / 32) * cut.of_first * 2 * 32 * DP;
-        const int own = (which * 32 + j % 32) * DP + d;
-#pragma unroll 4
-        for (int i = 0; i < cut.of_first; ++i)
-            all += *reinterpret_cast<const f32x4*>(first + static_cast<int64_t>(i) * 2 * 32 * DP + own);
-    }
+    auto add = [&](const float* from, int64_t step, int count) {
+        constexpr int kAtOnce = 8;
+        for (int i = 0; i < count; i += kAtOnce) {
+            f32x4 x[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) x[u] = *reinterpret_cast<const f32x4*>(from + min(i + u, count - 1) * step);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (i + u < count) all += x[u];
+        }
+    };
+    add(parts + static_cast<int64_t>(block) * cut.of_rest * each + at, each, cut.of_rest);
+    if (j / 32 < cut.groups)
+        add(parts + cut.kept() * each + static_cast<int64_t>(j / 32) * cut.of_first * 2 * 32 * DP + (which * 32 + j % 32) * DP + d,
+            2 * 32 * DP, cut.of_first);
     T* const dst = (which == 0 ? dk : dv) + ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
 #pragma unroll
     for (int f = 0; f < 4; ++f)
         if (d + f < a.D) dst[d + f] = from_float<T>(all[f]);
 }
 
-// Blocks enough to give every compute unit two (a block's wave is alone on its
-// SIMD for the wider heads and waits for its tiles), with 4 tiles or more each.
-Pieces pieces_of(const Args& a, int inner) {
-    Pieces cut{(a.N + kOuter - 1) / kOuter, 1, 0, 1};
-    const int64_t heads = static_cast<int64_t>(a.B) * a.G, units = cut.key_blocks * heads;
-    if (units == 0 || a.H == 0 || a.Q == 0) return cut;
+// Blocks of 64 keys where those of 128 are few, and pieces where these are: up
+// to two blocks a compute unit (512; a few more would be a round of their own),
+// of 4 tiles or more.
+Pieces pieces_of(const Args& a, int inner, bool may_split) {
+    Pieces cut{kOuter, (a.N + kOuter - 1) / kOuter, 1, 0, 1};
+    const int64_t heads = static_cast<int64_t>(a.B) * a.G;
+    if (heads == 0 || a.N == 0 || a.H == 0 || a.Q == 0) return cut;
+    if (may_split && few_blocks(cut.key_blocks * heads)) {
+        cut.rows = kOuter / 2;
+        cut.key_blocks = (a.N + cut.rows - 1) / cut.rows;
+        inner = Cut<float, 2>::kInnerRows;
+    }
     auto pieces = [&](int64_t rows, int64_t blocks, int64_t least) {
         const int64_t tiles = (rows + inner - 1) / inner * (a.H / a.G);
-        return static_cast<int>(std::max<int64_t>(1, std::min((512 + blocks - 1) / blocks, tiles / least)));
+        return static_cast<int>(std::max<int64_t>(1, std::min(512 / blocks, tiles / least)));
     };
-    cut.of_rest = pieces(std::min<int64_t>(a.Q, static_cast<int64_t>(a.causal ? 1 : 2) * a.window + kOuter), units, 4);
+    cut.of_rest = pieces(std::min<int64_t>(a.Q, static_cast<int64_t>(a.causal ? 1 : 2) * a.window + cut.rows),
+                         cut.key_blocks * heads, 4);
     if (a.sinks > 0 && a.window < a.N) {
         cut.groups = (a.sinks + 31) / 32;
-        cut.of_first = pieces(a.Q, cut.groups * heads, 2);
+        cut.of_first = std::min(32, pieces(a.Q, cut.groups * heads, 2));
     }
     return cut;
 }
@@ -583,11 +627,11 @@ struct Workspace {
     size_t delta, bias, part, bytes;
 };
 
-Workspace workspace_of(const Args& a, int type) {
+Workspace workspace_of(const Args& a, int type, bool may_split) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t rows = static_cast<size_t>(a.B) * a.H;
     Workspace w{};
-    w.cut = pieces_of(a, type == POINTOPS_F32 ? kInner<float> : kInner<f16>);
+    w.cut = pieces_of(a, type == POINTOPS_F32 ? kInner<float> : kInner<f16>, may_split);
     const size_t units = static_cast<size_t>(w.cut.units()) + w.cut.first_units();
     w.delta = 0;
     w.bias = up(rows * a.Q * sizeof(float));
@@ -610,52 +654,63 @@ constexpr int kType = sizeof(T) == 4 ? POINTOPS_F32 : __is_same(T, f16) ? POINTO
 template <typename T, int DP, bool VEC, bool BIAS>
 hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     using TileT = Tile<T, DP>;
-    const Workspace w = workspace_of(a, kType<T>);
+    constexpr bool kSplit = VEC && kSplits<T, DP>;
+    const Workspace w = workspace_of(a, kType<T>, kSplit);
     const Pieces cut = w.cut;
     float* const delta = reinterpret_cast<float*>(x.workspace + w.delta);
     float* const dbias_part = x.dbias != nullptr ? reinterpret_cast<float*>(x.workspace + w.bias) : nullptr;
     float* const part = reinterpret_cast<float*>(x.workspace + w.part);
-    const int64_t grid_q = (static_cast<int64_t>(a.Q) + kOuter - 1) / kOuter * a.B * a.H;
     const int64_t heads = static_cast<int64_t>(a.B) * a.G, grid_k = cut.units() * heads, grid_first = cut.first_units() * heads;
+    const bool split_q = kSplit && few_blocks((static_cast<int64_t>(a.Q) + kOuter - 1) / kOuter * a.B * a.H);
+    const bool split_k = kSplit && cut.rows < kOuter;
+    const int64_t rows_q = split_q ? kOuter / 2 : kOuter;
+    const int64_t grid_q = (static_cast<int64_t>(a.Q) + rows_q - 1) / rows_q * a.B * a.H;
     if (grid_q > INT32_MAX || grid_k > INT32_MAX || grid_first > INT32_MAX) return hipErrorInvalidValue;
 
-    constexpr size_t tiles = 4 * kInner<T> * TileT::kStride, stats = 16 * kInner<T>;
+    auto tiles = [](bool split) { return 4 * (split ? Cut<T, 2>::kInnerRows : kInner<T>) * static_cast<size_t>(TileT::kStride); };
     const size_t entries = bias_entries(a.reach), table = a.bias != nullptr ? 4 * (entries + a.bk.n) : 0;
     if (grid_q > 0) {
-        auto* const by_query = attention_grad_query_kernel<T, DP, VEC, BIAS>;
-        if (tiles + table > kLdsFree) {
-            static std::atomic<uint64_t> allowed{0};
-            const hipError_t err = allow_lds(by_query, allowed, tiles + 4 * (bias_entries(kMaxReach) + 255));
+        auto* kernel = attention_grad_query_kernel<T, DP, VEC, BIAS, 1>;
+        if constexpr (kSplit)
+            if (split_q) kernel = attention_grad_query_kernel<T, DP, VEC, BIAS, 2>;
+        const size_t lds = tiles(split_q) + table;
+        if (lds > kLdsFree) {
+            static std::atomic<uint64_t> allowed[2];
+            const hipError_t err = allow_lds(kernel, allowed[split_q], tiles(split_q) + 4 * (bias_entries(kMaxReach) + 255));
             if (err != hipSuccess) return err;
         }
-        hipLaunchKernelGGL(by_query, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), tiles + table, stream, a,
-                           static_cast<const T*>(x.out), x.lse, x.grad, delta,
-                           static_cast<T*>(x.dq), dbias_part != nullptr);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), lds, stream, a,
+                           static_cast<const T*>(x.out), x.lse, x.grad, delta, static_cast<T*>(x.dq), dbias_part != nullptr);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
     if (grid_k > 0) {
         // The tiles, their rows' statistics, the bias's table; with its sums also the skews and the waves' sums.
-        auto lds_for = [&](size_t n, size_t edges, bool sums) {
-            return tiles + stats + 4 * ((n + 3) / 4 * 4 + edges) + (sums ? 4 * kWaves * (kSkewFloats + n) : 0);
+        auto lds_for = [&](bool split, size_t n, size_t edges, bool sums) {
+            return tiles(split) + tiles(split) / TileT::kStride * 4 + 4 * ((n + 3) / 4 * 4 + edges) +
+                   (sums ? 4 * kWaves * (kSkewFloats + n) : 0);
         };
-        const size_t lds = a.bias != nullptr ? lds_for(entries, a.bk.n, dbias_part != nullptr) : tiles + stats;
-        auto launch = [&](auto* kernel, int64_t grid, std::atomic<uint64_t>& allowed) {
+        auto launch = [&](auto* kernel, bool split, int64_t grid, std::atomic<uint64_t>& allowed) {
+            const size_t lds = a.bias != nullptr ? lds_for(split, entries, a.bk.n, dbias_part != nullptr)
+                                                 : lds_for(split, 0, 0, false);
             if (lds > kLdsFree) {
-                const hipError_t err = allow_lds(kernel, allowed, lds_for(bias_entries(kMaxReach), 255, true));
+                const hipError_t err = allow_lds(kernel, allowed, lds_for(split, bias_entries(kMaxReach), 255, true));
                 if (err != hipSuccess) return err;
             }
             hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,
                                static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, dbias_part, cut);
             return hipGetLastError();
         };
-        static std::atomic<uint64_t> allowed[2];
-        hipError_t err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, false>, grid_k, allowed[0]);
+        static std::atomic<uint64_t> allowed[3];
+        hipError_t err = hipSuccess;
+        if constexpr (kSplit)
+            if (split_k) err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, false, 2>, true, grid_k, allowed[0]);
+        if (!split_k) err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, false, 1>, false, grid_k, allowed[1]);
         if (err == hipSuccess && grid_first > 0)
-            err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, true>, grid_first, allowed[1]);
+            err = launch(attention_grad_key_kernel<T, DP, VEC, BIAS, true, 1>, false, grid_first, allowed[2]);
         if (err != hipSuccess) return err;
         if (cut.kept() > 0) {
-            const dim3 grid(static_cast<uint32_t>(heads * cut.key_blocks), 2 * kOuter * DP / (4 * kThreads));
+            const dim3 grid(static_cast<uint32_t>(heads * cut.joined_blocks()), 2 * cut.rows * DP / (4 * kThreads));
             hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(kThreads), 0, stream, a, part, DP,
                                static_cast<T*>(x.dk), static_cast<T*>(x.dv), cut);
             err = hipGetLastError();
@@ -686,7 +741,9 @@ extern "C" {
 size_t pointops_attention_backward_workspace_bytes(const pointops_attention* in) {
     using namespace pointops::attn;
     Args a;
-    return read_args(in, &a) ? workspace_of(a, in->type).bytes : 0;
+    if (!read_args(in, &a)) return 0;
+    // Whether rows are read in 16-byte pieces depends on the gradient's strides too.
+    return std::max(workspace_of(a, in->type, true).bytes, workspace_of(a, in->type, false).bytes);
 }
 
 hipError_t pointops_attention_backward(const pointops_attention* in, const void* out, const float* lse,

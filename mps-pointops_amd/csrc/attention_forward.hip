@@ -71,32 +71,33 @@ __device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, 
     if (lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
 }
 
-template <typename T, int DP, bool VEC, bool BIAS>
+template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attention_forward_kernel(const Args a, T* __restrict__ out,
                                                                         float* __restrict__ lse_out) {
     using TileT = Tile<T, DP>;
-    constexpr int TK = kInner<T>, kSub = TK / 32, kOut = DP / 32;
+    constexpr int TK = Cut<T, SPLIT>::kInnerRows, kSub = Cut<T, SPLIT>::kSub, kRows = Cut<T, SPLIT>::kRows, kOut = DP / 32;
     constexpr int kTileBytes = TK * TileT::kStride;
     extern __shared__ char lds[];  // two pairs of a key and a value tile, the bias's table
     float* const table = reinterpret_cast<float*>(lds + 4 * kTileBytes);
 
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / kWave);
-    const int blocks = (a.Q + kOuter - 1) / kOuter;
+    const int wave_row = 32 * (wave % (kWaves / SPLIT)), sub = wave / (kWaves / SPLIT) * kSub;  // its rows, its pieces
+    const int blocks = (a.Q + kRows - 1) / kRows;
     const Place at = place(a.B * a.H, blocks);
     const int b = at.outer / a.H, h = at.outer % a.H, g = h / (a.H / a.G);
-    const int i0 = folded(at.inner, blocks) * kOuter;
+    const int i0 = folded(at.inner, blocks) * kRows;
     const int len = a.length(b), shift = a.N - a.Q;
 
     // The block's rows that exist, by position, and the tiles that they see.
-    const int rows = min(kOuter, a.Q - i0);
+    const int rows = min(kRows, a.Q - i0);
     const Walk walk(a, max(i0 + shift, 0), min(i0 + shift + rows, len) - 1, len, TK);
 
     // This wave's rows.
-    const int w0 = i0 + 32 * wave + shift;  // position of its first row
-    const int w_count = min(32, i0 + rows - (i0 + 32 * wave));
+    const int w0 = i0 + wave_row + shift;  // position of its first row
+    const int w_count = min(32, i0 + rows - (i0 + wave_row));
     const int w_first = max(w0, 0), w_last = min(w0 + w_count, len) - 1;
     const bool w_any = w_first <= w_last, w_whole = w_any && w0 >= 0 && w0 + w_count <= len;
-    const int row = i0 + 32 * wave + lane % 32, p = row + shift;
+    const int row = i0 + wave_row + lane % 32, p = row + shift;
     const Seen seen = seen_by(a, p, len);
 
     const T* const k = a.k.at<T>(b, g);
@@ -148,12 +149,12 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
                 RowFrags<T, DP> f;
-                f.load(ktile, 32 * u);
+                f.load(ktile, 32 * (sub + u));
                 keep_order();
                 s[u] = f.times(q);
             }
             ColumnFrags<T, DP> vf[2];  // of this chunk of keys and the next
-            vf[0].load(vtile, 0);
+            vf[0].load(vtile, 32 * sub);
             keep_order();
             if (scaled) {
 #pragma unroll
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
 #pragma unroll
                     for (int u = 0; u < kSub; ++u) s[u] += far;
                 } else {
-                    const float* from = table + near + lane % 32 - 4 * half + a.reach + kMargin;
+                    const float* from = table + near - 32 * sub + lane % 32 - 4 * half + a.reach + kMargin;
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
                 }
             }
             if (!whole) {
-                const int j = j0 + 4 * half;
+                const int j = j0 + 32 * sub + 4 * half;
 #pragma unroll
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             constexpr int kPer = 16 / kPerFrag<T>, kSteps = kSub * kPer;
 #pragma unroll
             for (int c = 0; c < kSteps; ++c) {
-                if (c + 1 < kSteps) vf[(c + 1) % 2].load(vtile, (c + 1) * TileT::kRowsPerFrag);
+                if (c + 1 < kSteps) vf[(c + 1) % 2].load(vtile, 32 * sub + (c + 1) * TileT::kRowsPerFrag);
                 keep_order();
                 vf[c % 2].add(as_fragment<T>(&w[c / kPer][c % kPer * kPerFrag<T>]), o);
             }
@@ -220,6 +221,22 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         __syncthreads();
     }
 
+    if constexpr (SPLIT == 2) {
+        // The later half's sums, brought to the pair's common maximum.
+        float* const other = reinterpret_cast<float*>(lds) + wave % 2 * (16 * kOut + 2) * kWave;
+        if (wave >= 2) {
+            put_sums(other + 2 * kWave, o);
+            other[lane] = m;
+            other[kWave + lane] = l;
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+        const float m2 = other[lane], top = fmaxf(m, m2), base = top == -kInf ? 0.f : top;
+        const float keep = exp2_fast(m - base), by = exp2_fast(m2 - base);
+        m = top;
+        l = l * keep + other[kWave + lane] * by;
+        get_sums(other + 2 * kWave, o, keep, by);
+    }
     l = halves_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float lse = l == 0.f ? kInf : m + log2f(l);
@@ -244,7 +261,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
     while (bad != 0) {
         const int r = __builtin_ctzll(bad);
         bad &= bad - 1;
-        const int i = i0 + 32 * wave + r;
+        const int i = i0 + wave_row + r;
         careful_row<T>(a, b, h, i, len, table, out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D,
                        lse_out == nullptr ? nullptr : lse_out + (static_cast<int64_t>(b) * a.H + h) * a.Q + i);
     }
@@ -252,21 +269,24 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
 
 template <typename T>
 hipError_t forward(const pointops_attention* in, const Args& a, void* out, float* lse, hipStream_t stream) {
-    const int64_t blocks = (in->Q + kOuter - 1) / kOuter * in->B * in->H;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
     return with_width(in->D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        constexpr size_t tiles = 4 * kInner<T> * Tile<T, DP>::kStride;
-        const size_t lds = tiles + (a.bias != nullptr ? 4 * (bias_entries(a.reach) + a.bk.n) : 0);
-        const bool vec = vector_rows<T>(a.q, a.D) && vector_rows<T>(a.k, a.D) && vector_rows<T>(a.v, a.D);
-        const dim3 grid(static_cast<uint32_t>(blocks));
         const bool bias = a.bias != nullptr;
-        const int which = !vec ? 0 : bias ? 1 : 2;
-        auto* const kernel = which == 0   ? attention_forward_kernel<T, DP, false, true>
-                             : which == 1 ? attention_forward_kernel<T, DP, true, true>
-                                          : attention_forward_kernel<T, DP, true, false>;
+        const bool split = kSplits<T, DP> && vec && few_blocks((in->Q + kOuter - 1) / kOuter * in->B * in->H);
+        const int64_t rows = split ? kOuter / 2 : kOuter, blocks = (in->Q + rows - 1) / rows * in->B * in->H;
+        if (blocks > INT32_MAX) return hipErrorInvalidValue;
+        const size_t tiles = static_cast<size_t>(4) * (split ? Cut<T, 2>::kInnerRows : kInner<T>) * Tile<T, DP>::kStride;
+        const size_t lds = tiles + (bias ? 4 * (bias_entries(a.reach) + a.bk.n) : 0);
+        const dim3 grid(static_cast<uint32_t>(blocks));
+        const int which = !vec ? 0 : (bias ? 1 : 2) + (split ? 2 : 0);
+        auto* kernel = which == 0   ? attention_forward_kernel<T, DP, false, true, 1>
+                       : which == 1 ? attention_forward_kernel<T, DP, true, true, 1>
+                                    : attention_forward_kernel<T, DP, true, false, 1>;
+        if constexpr (kSplits<T, DP>)
+            if (split) kernel = bias ? attention_forward_kernel<T, DP, true, true, 2> : attention_forward_kernel<T, DP, true, false, 2>;
         if (lds > kLdsFree) {
-            static std::atomic<uint64_t> allowed[3];
+            static std::atomic<uint64_t> allowed[5];
             const hipError_t err = allow_lds(kernel, allowed[which], tiles + 4 * (bias_entries(kMaxReach) + 255));
             if (err != hipSuccess) return err;
         }
