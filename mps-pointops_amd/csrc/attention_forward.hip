@@ -197,20 +197,25 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
                 for (int d = 0; d < kOut; ++d) o[d] *= keep;
             }
             const float base = m == -kInf ? 0.f : m;
-            float w[kSub][16];
-#pragma unroll
-            for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    w[u][r] = exp2_fast(__builtin_fmaf(s[u][r], factor, -base));
-                    l += w[u][r];
-                }
+            // A chunk's weights are formed while the products of the one before run.
             constexpr int kPer = 16 / kPerFrag<T>, kSteps = kSub * kPer;
+            i32x4 x[2];
+            auto weigh = [&](int c) {
+                float w[kPerFrag<T>];
+#pragma unroll
+                for (int r = 0; r < kPerFrag<T>; ++r) {
+                    w[r] = exp2_fast(__builtin_fmaf(s[c / kPer][c % kPer * kPerFrag<T> + r], factor, -base));
+                    l += w[r];
+                }
+                x[c % 2] = as_fragment<T>(w);
+            };
+            weigh(0);
 #pragma unroll
             for (int c = 0; c < kSteps; ++c) {
                 if (c + 1 < kSteps) vf[(c + 1) % 2].load(vtile, 32 * sub + (c + 1) * TileT::kRowsPerFrag);
                 keep_order();
-                vf[c % 2].add(as_fragment<T>(&w[c / kPer][c % kPer * kPerFrag<T>]), o);
+                vf[c % 2].add(x[c % 2], o);
+                if (c + 1 < kSteps) weigh(c + 1);
             }
         }
         ktile = ktile == lds ? lds + 2 * kTileBytes : lds;

@@ -96,6 +96,11 @@ def _check_table(table: Tensor, heads: int | None, max_distance: int | None, cau
 
 
 # ----------------------------------------------------------------- arguments
+def _like(t: Tensor) -> Tensor:
+    """Memory for a contiguous result of the tensor's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rows(t: Tensor) -> Tensor:
     """The tensor with its last dimension contiguous."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -176,7 +181,7 @@ def _tracked(*tensors: Tensor | None) -> bool:
 
 # ------------------------------------------------------------------ attention
 def _attend(q, k, v, bias, lengths, edges, window, sinks, causal, scale, lse):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _like(q)
     if out.numel():
         args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
         _native.call("pointops_attention_forward", args, out.data_ptr(), _native.ptr(lse), _native.stream(q.device))
@@ -199,10 +204,10 @@ class _WindowAttention(torch.autograd.Function):
         q, k, v, bias, lengths, out, lse = ctx.saved_tensors
         edges, window, sinks, causal, scale = ctx.rest
         grad = _rows(grad)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = _like(q), _like(k), _like(v)
         dbias = None
         if bias is not None and ctx.needs_input_grad[3]:
-            dbias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
+            dbias = _like(bias)
         if q.shape[0] and q.shape[2]:
             args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
             size = _native.size_query("pointops_attention_backward_workspace_bytes", args)
@@ -269,7 +274,7 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     q, k_cache, v_cache = _rows(q), _rows(k_cache), _rows(v_cache)
     bias = None if bias is None else bias.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _like(q)
     if out.numel():
         args = _pack(q, k_cache, v_cache, window, sinks, True, bias, edges, lengths,
                      q.shape[3] ** -0.5 if scale is None else float(scale))
@@ -353,8 +358,7 @@ def _pack_norm(q, k, q_weight, k_weight, cos, sin, eps) -> bytes:
 
 
 def _norm(q, k, q_weight, k_weight, cos, sin, eps):
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out, k_out = _like(q), _like(k)
     if q_out.numel() + k_out.numel():
         _native.call("pointops_qk_norm_rotate", _pack_norm(q, k, q_weight, k_weight, cos, sin, eps),
                      q_out.data_ptr(), k_out.data_ptr(), _native.stream(q.device))
@@ -373,8 +377,7 @@ class _QkNormRotate(torch.autograd.Function):
     def backward(ctx, q_grad: Tensor, k_grad: Tensor):
         q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
         q_grad, k_grad = _rows(q_grad), _rows(k_grad)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = _like(q), _like(k)
         weights = [w if need else None for w, need in zip((q_weight, k_weight), ctx.needs_input_grad[2:4])]
         # A weight without a row to sum over has a gradient of zeros.
         make = torch.empty_like if q.numel() + k.numel() else torch.zeros_like
