@@ -444,6 +444,13 @@ __device__ __forceinline__ float bias_log2(float v) {
     return w;
 }
 
+// One offset's bias for the whole wave, without a table.
+template <typename T>
+__device__ __forceinline__ float one_bias(const Args& a, int head, int offset) {
+    if (a.bias == nullptr) return 0.f;
+    return bias_log2(to_float(static_cast<const T*>(a.bias)[static_cast<int64_t>(bucket_of(a.bk, a.bk.edge, offset)) * a.H + head]));
+}
+
 // Fills the table for head `head` (edges: LDS, bk.n ints).  The caller's
 // next barrier makes it visible; this one has a barrier of its own.
 template <typename T>
@@ -488,6 +495,24 @@ struct CarefulRow {
         o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n]) : 0.f);
         o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + kWave]) : 0.f);
     }
+};
+
+// The same for gradients: one query and one key at a time, of which a wave holds
+// elements l and l + 64 in lane l.
+template <typename T>
+struct CarefulPair {
+    float x0 = 0.f, x1 = 0.f;
+    __device__ __forceinline__ void load(const T* row, int width) {
+        const int lane = lane_id();
+        x0 = lane < width ? to_float(row[lane]) : 0.f;
+        x1 = lane + kWave < width ? to_float(row[lane + kWave]) : 0.f;
+    }
+    __device__ __forceinline__ float dot(const CarefulPair& y) const { return wave_sum(x0 * y.x0 + x1 * y.x1); }
+    __device__ __forceinline__ void add(float w, const CarefulPair& y) {
+        x0 = __builtin_fmaf(w, y.x0, x0);
+        x1 = __builtin_fmaf(w, y.x1, x1);
+    }
+    __device__ __forceinline__ bool finite() const { return ballot(x0 * 0.f + x1 * 0.f != 0.f) == 0; }
 };
 
 // ---------------------------------------------------------------- dispatch

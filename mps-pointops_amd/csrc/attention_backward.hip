@@ -22,6 +22,61 @@ namespace pointops {
 namespace attn {
 namespace {
 
+// Gradients that are not finite are formed again pair by pair, where a product
+// with a masked pair's infinity or NaN may have spread: of one query over the
+// keys that it sees, and of one key over those of the rows i_from .. i_to - 1
+// of a head that see it.  By a whole wave.
+template <typename T>
+__device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, int b, int h, int i, int len, float lse,
+                                              float delta, T* dq) {
+    const int g = h / (a.H / a.G), p = i + a.N - a.Q;
+    const Seen seen = seen_by(a, p, len);
+    const T* const k = a.k.at<T>(b, g);
+    const T* const v = a.v.at<T>(b, g);
+    CarefulPair<T> q, go, sum;
+    q.load(a.q.at<T>(b, h) + i * a.q.n, a.D);
+    go.load(grad.at<T>(b, h) + i * grad.n, a.D);
+    auto key = [&](int64_t j) {
+        CarefulPair<T> kk, vv;
+        kk.load(k + j * a.k.n, a.D);
+        const float s = q.dot(kk) * a.scale_log2 + one_bias<T>(a, h, static_cast<int>(p - j));
+        if (s == -kInf) return;
+        vv.load(v + j * a.v.n, a.D);
+        sum.add(exp2_fast(s - lse) * (go.dot(vv) - delta), kk);
+    };
+    for (int j = 0; j < seen.first; ++j) key(j);
+    for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
+    const int lane = lane_id();
+    if (lane < a.D) dq[lane] = from_float<T>(sum.x0 * a.scale);
+    if (lane + kWave < a.D) dq[lane + kWave] = from_float<T>(sum.x1 * a.scale);
+}
+
+template <typename T>
+__device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, const float* lse_in, const float* delta_in, int b,
+                                            int h, int64_t j, int i_from, int i_to, bool beyond, int len,
+                                            CarefulPair<T>& dk, CarefulPair<T>& dv) {
+    const int g = h / (a.H / a.G);
+    const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
+    CarefulPair<T> k, v;
+    k.load(a.k.at<T>(b, g) + j * a.k.n, a.D);
+    v.load(a.v.at<T>(b, g) + j * a.v.n, a.D);
+    for (int64_t i = i_from; i < i_to; ++i) {
+        const int p = static_cast<int>(i) + a.N - a.Q, off = p - static_cast<int>(j);
+        const bool within = (off < 0 ? -off : off) < a.window;
+        if ((a.causal && off < 0) || within == beyond) continue;
+        const float lse = lse_in[stats + i];
+        if (lse == kInf) continue;
+        CarefulPair<T> q, go;
+        q.load(a.q.at<T>(b, h) + i * a.q.n, a.D);
+        const float s = q.dot(k) * a.scale_log2 + one_bias<T>(a, h, off);
+        if (s == -kInf) continue;
+        go.load(grad.at<T>(b, h) + i * grad.n, a.D);
+        const float w = exp2_fast(s - lse);
+        dv.add(w, go);
+        dk.add(w * (go.dot(v) - delta_in[stats + i]) * a.scale, q);
+    }
+}
+
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void attention_grad_query_kernel(
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
@@ -176,14 +231,28 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         rest += other[lane];
         get_sums(other + kWave, dq, 1.f, 1.f);
     }
-    if (row < a.Q) {
-        T* const dst = dq_out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
+    float odd = 0.f;  // NaN where anything is not finite
 #pragma unroll
-        for (int d = 0; d < kOut; ++d) {
-            dq[d] *= a.scale;
+    for (int d = 0; d < kOut; ++d) {
+        dq[d] *= a.scale;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd += dq[d][r] * 0.f;
+    }
+    uint64_t bad = ballot(exists && odd != 0.f);
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    T* const dst = dq_out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
+    if (row < a.Q && (bad >> (lane % 32) & 1) == 0) {
+#pragma unroll
+        for (int d = 0; d < kOut; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) store4<T, VEC>(dst, 32 * d + 8 * e + 4 * half, a.D, dq[d], 4 * e);
-        }
+    }
+    while (bad != 0) {
+        const int r = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const int i = i0 + wave_row + r;
+        careful_query<T>(a, grad, b, h, i, len, i2f(readlane(f2i(lse), r)), i2f(readlane(f2i(delta), r)),
+                         dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
     }
     // The weights of a row sum to 1, so that what is left of its ds is what the
     // rounded output took from delta.
@@ -506,13 +575,25 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         get_sums(other, dk, 1.f, 1.f);
         get_sums(other + 16 * kOut * kWave, dv, 1.f, 1.f);
     }
+    // Key `key` of the block, formed again.
+    auto again = [&](int key, CarefulPair<T>& ck, CarefulPair<T>& cv) {
+        for (int hh = 0; hh < group; ++hh) {
+            const int64_t before = static_cast<int64_t>(hh) * tiles;
+            const int from = t_first + static_cast<int>(max(share_low - before, int64_t(0)));
+            const int to = t_first + static_cast<int>(min(share_high - before, static_cast<int64_t>(tiles)));
+            careful_key<T>(a, grad, lse_in, delta_in, b, g * group + hh, j0 + key, i_low + from * TQ,
+                           min(i_low + to * TQ, i_high), FIRST, len, ck, cv);
+        }
+    };
     // Keys behind the cloud's length have no gradient.
+    float odd = 0.f;  // NaN where anything is not finite
 #pragma unroll
     for (int d = 0; d < kOut; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             dk[d][r] = j < len ? dk[d][r] * a.scale : 0.f;
             dv[d][r] = j < len ? dv[d][r] : 0.f;
+            odd += dk[d][r] * 0.f + dv[d][r] * 0.f;
         }
     float* const parts = part + bg * cut.floats(DP);
     if constexpr (FIRST) {
@@ -537,26 +618,66 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         }
         __syncthreads();
         float* const dst = parts + static_cast<int64_t>(cut.kept()) * 2 * cut.rows * DP + static_cast<int64_t>(unit) * 2 * 32 * DP;
-        for (int i = threadIdx.x; i < 2 * 32 * DP; i += kThreads) dst[i] = all[i / DP * kRow + i % DP];
-    } else if (cut.parted(block)) {
-        // (unit, dk or dv, key of the block, DP)
-        float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kRows + (j - j0)) * DP;
-#pragma unroll
-        for (int d = 0; d < kOut; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                store4<float, true>(dst, 32 * d + 8 * e + 4 * half, DP, dk[d], 4 * e);
-                store4<float, true>(dst + kRows * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
+        for (int key = wave; key < 32; key += kWaves) {
+            CarefulPair<T> ck, cv;
+            auto get = [&](int which, int d) { return d < DP ? all[(32 * which + key) * kRow + d] : 0.f; };
+            ck.x0 = get(0, lane), ck.x1 = get(0, lane + kWave), cv.x0 = get(1, lane), cv.x1 = get(1, lane + kWave);
+            if (!ck.finite() || !cv.finite()) {
+                ck = cv = CarefulPair<T>{};
+                if (j0 + key < exist) again(key, ck, cv);
             }
-    } else if (j < a.N) {
-        const int64_t to = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
+            auto set = [&](int which, int d, float x) {
+                if (d < DP) dst[(32 * which + key) * DP + d] = x;
+            };
+            set(0, lane, ck.x0), set(0, lane + kWave, ck.x1), set(1, lane, cv.x0), set(1, lane + kWave, cv.x1);
+        }
+        return;
+    }
+    uint64_t bad = ballot(odd != 0.f);
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    const bool parted = cut.parted(block);
+    // (unit, dk or dv, key of the block, DP), or the results.
+    float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kRows + (j - j0)) * DP;
+    const int64_t to = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
+    if ((bad >> (lane % 32) & 1) == 0) {
+        if (parted) {
 #pragma unroll
-        for (int d = 0; d < kOut; ++d)
+            for (int d = 0; d < kOut; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                store4<T, VEC>(dk_out + to, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
-                store4<T, VEC>(dv_out + to, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
+                for (int e = 0; e < 4; ++e) {
+                    store4<float, true>(dst, 32 * d + 8 * e + 4 * half, DP, dk[d], 4 * e);
+                    store4<float, true>(dst + kRows * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
+                }
+        } else if (j < a.N) {
+#pragma unroll
+            for (int d = 0; d < kOut; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    store4<T, VEC>(dk_out + to, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
+                    store4<T, VEC>(dv_out + to, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
+                }
+        }
+    }
+    while (bad != 0) {
+        const int r = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const int key = w0 - j0 + r;
+        CarefulPair<T> ck, cv;
+        again(key, ck, cv);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int d = lane + x * kWave;
+            const float yk = x == 0 ? ck.x0 : ck.x1, yv = x == 0 ? cv.x0 : cv.x1;
+            if (parted && d < DP) {
+                float* const at = parts + (static_cast<int64_t>(unit) * 2 * kRows + key) * DP + d;
+                at[0] = yk;
+                at[kRows * DP] = yv;
+            } else if (!parted && d < a.D) {
+                const int64_t at = ((static_cast<int64_t>(b) * a.N + j0 + key) * a.G + g) * a.D + d;
+                dk_out[at] = from_float<T>(yk);
+                dv_out[at] = from_float<T>(yv);
             }
+        }
     }
 }
 

@@ -71,7 +71,7 @@ def definition(q, k, v, grad, window=None, sinks=0, causal=False, bias=None, max
                 s = kk[at] @ q[b, i, h] * scale
                 if table is not None:
                     s = s + table[bucket[i, at], h]
-                    at, s = at[s > -math.inf], s[s > -math.inf]
+                    at, s = at[s != -math.inf], s[s != -math.inf]
                     if not len(at):
                         continue
                 p = torch.softmax(s, 0)
