@@ -174,11 +174,12 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_aligned_kernel(co
     add_buckets(bk, sums, kSpan, first + kThreads * V - 1 - i0 - (N - Q), dst);
 }
 
-// Eight lanes of parts for each of 32 buckets of a head.
+// 32 lanes of parts for each of 8 buckets of a head.
+constexpr int kJoinBuckets = 8;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_buckets_kernel(const float* __restrict__ part, int B, int64_t blocks,
                                                                 int count, T* __restrict__ grad) {
-    constexpr int kLanes = 8, kBuckets = kThreads / kLanes;
+    constexpr int kLanes = 32, kBuckets = kJoinBuckets;
     __shared__ float sums[kLanes][kBuckets];
     const int H = gridDim.x, h = blockIdx.x, x = threadIdx.x % kBuckets, y = threadIdx.x / kBuckets;
     const int bucket = blockIdx.y * kBuckets + x;
@@ -232,7 +233,7 @@ bool bias_sizes(int64_t Q, int64_t N, int64_t H, int32_t type) {
 
 hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, void* grad,
                         hipStream_t stream) {
-    const dim3 grid(H, (count + kThreads / 8 - 1) / (kThreads / 8));
+    const dim3 grid(H, (count + kJoinBuckets - 1) / kJoinBuckets);
     switch (type) {
         case POINTOPS_F32:
             hipLaunchKernelGGL(join_buckets_kernel<float>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
