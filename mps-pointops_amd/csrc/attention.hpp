@@ -554,15 +554,16 @@ bool read_buckets(const int32_t* edges, int n, int count, int64_t most, Buckets*
 
 // Adds a block's sums by offset (LDS, `entries` of them, offset o at entry o +
 // zero; the outermost buckets of a side take what lies beyond) by buckets:
-// dst[0 .. count - 1].  Eight lanes a bucket.
-__device__ __forceinline__ void add_buckets(const Buckets& bk, const float* sums, int entries, int zero, float* dst) {
+// dst[0 .. count - 1].  edge: bk.edge, or a copy of it.  Eight lanes a bucket.
+__device__ __forceinline__ void add_buckets(const Buckets& bk, const int* edge, const float* sums, int entries, int zero,
+                                            float* dst) {
     const int side = bk.n + 1;
     const bool two_sided = bk.count > side;
     for (int first = 0; first < bk.count; first += kThreads / 8) {
         const int bucket = first + static_cast<int>(threadIdx.x) / 8, e = bucket % side;
         float all = 0.f;
         if (bucket < bk.count) {
-            const int d_low = e == 0 ? 0 : bk.edge[e - 1], d_high = e == bk.n ? INT32_MAX : bk.edge[e] - 1;
+            const int d_low = e == 0 ? 0 : edge[e - 1], d_high = e == bk.n ? INT32_MAX : edge[e] - 1;
             int64_t low = static_cast<int64_t>(zero) + d_low, high = static_cast<int64_t>(zero) + d_high;
             if (bucket >= side) {
                 low = static_cast<int64_t>(zero) - d_high;
@@ -571,6 +572,7 @@ __device__ __forceinline__ void add_buckets(const Buckets& bk, const float* sums
                 low = 0;  // later keys have no buckets of their own
             }
             const int from = static_cast<int>(max(low, int64_t(0))), to = static_cast<int>(min(high, int64_t(entries - 1)));
+#pragma unroll 4
             for (int i = from + static_cast<int>(threadIdx.x) % 8; i <= to; i += 8) all += sums[i];
         }
         all = group_sum<8>(all);

@@ -559,7 +559,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 sums[i] = all;
             }
             __syncthreads();
-            add_buckets(a.bk, sums, entries, a.reach + kMargin, bucket_part);
+            add_buckets(a.bk, edges, sums, entries, a.reach + kMargin, bucket_part);
         }
     }
 

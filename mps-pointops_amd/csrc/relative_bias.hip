@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buck
     // Diagonal c has offset N - Q - c: entry 0 is diagonal c0 + kDiagSpan - 1.
     const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
     float* const dst = part + (h * static_cast<int64_t>(gridDim.x) * gridDim.y + block) * bk.count;
-    add_buckets(bk, sums, kDiagSpan, c0 + kDiagSpan - 1 - (N - Q), dst);
+    add_buckets(bk, bk.edge, sums, kDiagSpan, c0 + kDiagSpan - 1 - (N - Q), dst);
 }
 
 // The same where every row starts at a multiple of 16 bytes: a thread reads
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_aligned_kernel(co
     // A diagonal c (column less the tensor's row) has offset N - Q - c.
     const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
     float* const dst = part + (h * static_cast<int64_t>(gridDim.x) * gridDim.y + block) * bk.count;
-    add_buckets(bk, sums, kSpan, first + kThreads * V - 1 - i0 - (N - Q), dst);
+    add_buckets(bk, bk.edge, sums, kSpan, first + kThreads * V - 1 - i0 - (N - Q), dst);
 }
 
 // 32 lanes of parts for each of 8 buckets of a head.
