@@ -11,8 +11,17 @@
 // and passes over the queries that see them, all heads that share the key head
 // in turn (dk, dv and the bias's sums by offset).  The first keys, which every
 // query sees, have passes of their own for the queries beyond their window; they
-// and few blocks are cut into pieces whose 32-bit sums a last kernel joins.  ds and p are rounded to the inputs' type for the second
-// products, as the forward's weights are; the bias's sums take them unrounded.
+// and few blocks are cut into pieces whose 32-bit sums a last kernel joins.  ds and p
+// are rounded to the inputs' type for the second products, as the forward's weights
+// are (in float16, those below 6e-5 keep fewer bits: gradients that small are
+// scaled up by the caller's loss, as everywhere in that type); the bias's sums take
+// them unrounded.
+//
+// Bound by the matrix products (18 D operations a pair, with the scores' second
+// forming) and by the vector instructions of the weights between them.  Every
+// earlier key at 2 x 4096 queries, 8 heads of 128, bfloat16: dq 152 us, dk and dv
+// 245, the forward 128 (240 billion operations of the definition, 486 T/s with
+// all three; a large library product reaches 1204).
 #include <algorithm>
 #include <atomic>
 
@@ -75,6 +84,19 @@ __device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, con
         dv.add(w, go);
         dk.add(w * (go.dot(v) - delta_in[stats + i]) * a.scale, q);
     }
+}
+
+// A row's output is about as large as its values where it sees few keys, and its
+// rounding to 16 bits then takes as much from dq, through delta, as dq's own
+// (dq's error against 64 bits at 9 x 30 queries, 6 heads of 20, float16: 1.64
+// times a rounding's with it, 1.43 without).  Beyond this many keys the output is
+// an average of many, and the pass over them is not made twice.
+constexpr int kFewKeys = 128;
+
+// The most keys that a row up to position p_last sees.
+__device__ __forceinline__ int most_seen(const Args& a, int p_last, int len) {
+    const int side = min(a.window, kFewKeys + 1), first = min(a.sinks, kFewKeys + 1);
+    return a.causal ? min(side + first, p_last + 1) : min(2 * side - 1 + first, len);
 }
 
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
@@ -146,13 +168,22 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     }
     __syncthreads();
 
+    // The weights of a row sum to 1, so that what is left of its ds is what the
+    // rounded output took from delta: of few keys a pass ahead measures it.
+    auto left = [&] {
+        rest = halves_sum(rest);
+        return rest - rest == 0.f ? rest : 0.f;
+    };
     const float factor = biased ? 1.f : a.scale_log2;
     f32x16 dq[kOut] = {};
     char* ktile = lds;
+    bool ahead = sizeof(T) == 2 && most_seen(a, min(i0 + shift + rows, len) - 1, len) <= kFewKeys;
     while (t < walk.end) {
         char* const vtile = ktile + kTileBytes;
         const int j0 = t * TK;
         t = walk.after(t);
+        const bool turn = ahead && t >= walk.end;
+        if (turn) t = walk.begin();
         if (t < walk.end) {
             ks.load(k, a.k.n, t * TK, len, a.D);
             vs.load(v, a.v.n, t * TK, len, a.D);
@@ -199,10 +230,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                     for (int r = 0; r < 16; ++r)
                         if (!seen(j + 8 * (r / 4) + r % 4)) ds[r] = 0.f;
                 }
-                if (refine) {
+                if (refine || ahead) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) rest += ds[r];
                 }
+                if (ahead) continue;
                 constexpr int kSteps = 16 / kPerFrag<T>;
 #pragma unroll
                 for (int c = 0; c < kSteps; ++c) {
@@ -218,6 +250,18 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
             vs.store(ktile + kTileBytes);
         }
         __syncthreads();
+        if (turn) {
+            ahead = false;
+            float taken = left();
+            if constexpr (SPLIT == 2 && sizeof(T) == 2) {
+                __shared__ float parts[kWaves][32];
+                if (half == 0) parts[wave][lane] = taken;
+                __syncthreads();
+                taken = parts[wave % 2][lane % 32] + parts[wave % 2 + 2][lane % 32];
+            }
+            delta += taken;
+            rest = 0.f;
+        }
     }
 
     if constexpr (SPLIT == 2) {
@@ -254,9 +298,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         careful_query<T>(a, grad, b, h, i, len, i2f(readlane(f2i(lse), r)), i2f(readlane(f2i(delta), r)),
                          dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
     }
-    // The weights of a row sum to 1, so that what is left of its ds is what the
-    // rounded output took from delta.
-    if (refine) delta += halves_sum(rest);
+    if (refine) delta += left();
     if (row < a.Q && half == 0) delta_out[stat] = delta;
 }
 
