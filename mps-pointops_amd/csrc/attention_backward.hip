@@ -282,7 +282,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd += dq[d][r] * 0.f;
     }
-    uint64_t bad = ballot(exists && odd != 0.f);
+    // Rows that do not exist have met the tiles too, with weights of zero: 0 * inf.
+    uint64_t bad = ballot(row < a.Q && odd != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     T* const dst = dq_out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
     if (row < a.Q && (bad >> (lane % 32) & 1) == 0) {
