@@ -253,6 +253,21 @@ struct Stage {
             }
         }
     }
+    // Rows times by(row), row 0 being `first`.  Seldom called: what follows from the
+    // thread's number is worked out here, not kept in registers through a kernel's loop.
+    template <typename F>
+    __device__ __forceinline__ void scale(F by) {
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const float f = by((i * kThreads + thread) / kPerRow);
+            float x[kPerFrag<T>];
+#pragma unroll
+            for (int e = 0; e < kPerFrag<T>; ++e) x[e] = element<T>(r[i], e) * f;
+            r[i] = as_fragment<T>(x);
+        }
+    }
     __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {

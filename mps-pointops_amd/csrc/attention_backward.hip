@@ -31,13 +31,25 @@ namespace pointops {
 namespace attn {
 namespace {
 
+// The forward's lse is one 32-bit number.  Where a row's maximum is large (all of
+// its keys carry a mask of the type's lowest value, or their scores are that large)
+// the logarithm of the sum beside it is rounded, or lost altogether: exp2(s - lse)
+// are then the weights but for one factor a row.  From here on a row's
+// weights are added up ahead of its pass and both kernels divide by their sum; below,
+// the factor lies within 2^-18 of 1 (2^-14 for the 16-bit types).
+template <typename T>
+__device__ __forceinline__ bool coarse(float lse) {
+    const float size = __builtin_fabsf(lse);
+    return size >= (sizeof(T) == 4 ? 64.f : 1024.f) && size < kInf;
+}
+
 // Gradients that are not finite are formed again pair by pair, where a product
 // with a masked pair's infinity or NaN may have spread: of one query over the
 // keys that it sees, and of one key over those of the rows i_from .. i_to - 1
 // of a head that see it.  By a whole wave.
 template <typename T>
 __device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, int b, int h, int i, int len, float lse,
-                                              float delta, T* dq) {
+                                              float delta, float share, T* dq) {
     const int g = h / (a.H / a.G), p = i + a.N - a.Q;
     const Seen seen = seen_by(a, p, len);
     const T* const k = a.k.at<T>(b, g);
@@ -56,14 +68,15 @@ __device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, i
     for (int j = 0; j < seen.first; ++j) key(j);
     for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
     const int lane = lane_id();
-    if (lane < a.D) dq[lane] = from_float<T>(sum.x0 * a.scale);
-    if (lane + kWave < a.D) dq[lane + kWave] = from_float<T>(sum.x1 * a.scale);
+    const float by = a.scale * share;
+    if (lane < a.D) dq[lane] = from_float<T>(sum.x0 * by);
+    if (lane + kWave < a.D) dq[lane + kWave] = from_float<T>(sum.x1 * by);
 }
 
 template <typename T>
-__device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, const float* lse_in, const float* delta_in, int b,
-                                            int h, int64_t j, int i_from, int i_to, bool beyond, int len,
-                                            CarefulPair<T>& dk, CarefulPair<T>& dv) {
+__device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, const float* lse_in, const float* delta_in,
+                                            const float* share_in, int b, int h, int64_t j, int i_from, int i_to, bool beyond,
+                                            int len, CarefulPair<T>& dk, CarefulPair<T>& dv) {
     const int g = h / (a.H / a.G);
     const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
     CarefulPair<T> k, v;
@@ -80,7 +93,7 @@ __device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, con
         const float s = q.dot(k) * a.scale_log2 + one_bias<T>(a, h, off);
         if (s == -kInf) continue;
         go.load(grad.at<T>(b, h) + i * grad.n, a.D);
-        const float w = exp2_fast(s - lse);
+        const float w = exp2_fast(s - lse) * share_in[stats + i];
         dv.add(w, go);
         dk.add(w * (go.dot(v) - delta_in[stats + i]) * a.scale, q);
     }
@@ -99,10 +112,39 @@ __device__ __forceinline__ int most_seen(const Args& a, int p_last, int len) {
     return a.causal ? min(side + first, p_last + 1) : min(2 * side - 1 + first, len);
 }
 
+// The sum of a wave's rows' exp2(s - lse), with the scores as the pass over the keys
+// forms them; keys straight from memory, as few rows ask for it.
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ float exponents_sum(const Args& a, const i32x4 (&q)[Tile<T, DP>::kChunks], const T* k, const Walk& walk,
+                                               const Seen& seen, const float* table, int p, int len, float lse) {
+    const int lane = lane_id(), half = lane / 32;
+    const float factor = table != nullptr ? 1.f : a.scale_log2;
+    float sum = 0.f;
+    for (int t = walk.begin(); t < walk.end; t = walk.after(t)) {
+        const int row = 32 * t + lane % 32;
+        f32x16 s = {};
+#pragma unroll
+        for (int c = 0; c < Tile<T, DP>::kChunks; ++c) {
+            i32x4 key = {0, 0, 0, 0};
+            if (row < len) key = load_row<T, VEC>(k + row * a.k.n, (2 * c + half) * kPerFrag<T>, a.D);
+            s = mma<T>(key, q[c], s);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = 32 * t + 4 * half + 8 * (r / 4) + r % 4;
+            float x = s[r];
+            if (table != nullptr) x = x * a.scale_log2 + table[min(max(p - j, -a.reach), a.reach) + a.reach + kMargin];
+            if (seen(j)) sum += exp2_fast(__builtin_fmaf(x, factor, -lse));
+        }
+    }
+    return halves_sum(sum);
+}
+
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void attention_grad_query_kernel(
     const Args a, const T* __restrict__ out, const float* __restrict__ lse_in, const Rows grad,
-    float* __restrict__ delta_out, T* __restrict__ dq_out, const bool refine) {
+    float* __restrict__ delta_out, float* __restrict__ share_out, int* __restrict__ coarse_out,
+    T* __restrict__ dq_out, const bool refine) {
     using TileT = Tile<T, DP>;
     constexpr int TK = Cut<T, SPLIT>::kInnerRows, kSub = Cut<T, SPLIT>::kSub, kRows = Cut<T, SPLIT>::kRows;
     constexpr int kOut = DP / 32, kTileBytes = TK * TileT::kStride;
@@ -168,6 +210,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     }
     __syncthreads();
 
+    float share = 1.f;
+    const bool any_coarse = ballot(coarse<T>(lse)) != 0;
+    if (lane == 0 && row < a.Q) coarse_out[static_cast<int64_t>(b * a.H + h) * ((a.Q + 31) / 32) + row / 32] = any_coarse;
+    if (any_coarse) {
+        const float sum = exponents_sum<T, DP, VEC>(a, q, k, Walk(a, w_first, w_last, len, 32), seen, biased ? table : nullptr, p, len, lse);
+        if (coarse<T>(lse) && sum > 0.f && sum < kInf) share = 1.f / sum;
+    }
     // The weights of a row sum to 1, so that what is left of its ds is what the
     // rounded output took from delta: of few keys a pass ahead measures it.
     auto left = [&] {
@@ -259,7 +308,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                 __syncthreads();
                 taken = parts[wave % 2][lane % 32] + parts[wave % 2 + 2][lane % 32];
             }
-            delta += taken;
+            delta += taken * share;
             rest = 0.f;
         }
     }
@@ -278,7 +327,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     float odd = 0.f;  // NaN where anything is not finite
 #pragma unroll
     for (int d = 0; d < kOut; ++d) {
-        dq[d] *= a.scale;
+        dq[d] *= a.scale * share;
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd += dq[d][r] * 0.f;
     }
@@ -297,10 +346,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         bad &= bad - 1;
         const int i = i0 + wave_row + r;
         careful_query<T>(a, grad, b, h, i, len, i2f(readlane(f2i(lse), r)), i2f(readlane(f2i(delta), r)),
-                         dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
+                         i2f(readlane(f2i(share), r)), dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
     }
-    if (refine) delta += left();
-    if (row < a.Q && half == 0) delta_out[stat] = delta;
+    if (refine) delta += left() * share;
+    if (row < a.Q && half == 0) {
+        delta_out[stat] = delta;
+        share_out[stat] = share;
+    }
 }
 
 // How the passes of the keys are cut.  A key block of `rows` keys passes over the
@@ -337,7 +389,8 @@ constexpr int kSkewFloats = 16 + 16 * kSkewRow;
 // and take 32 queries each in turn; their sums are added at the end.
 template <typename T, int DP, bool VEC, bool BIAS, bool FIRST, int SPLIT>
 __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void attention_grad_key_kernel(
-    const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const Rows grad,
+    const Args a, const float* __restrict__ lse_in, const float* __restrict__ delta_in, const float* __restrict__ share_in,
+    const int* __restrict__ coarse_in, const Rows grad,
     T* __restrict__ dk_out, T* __restrict__ dv_out, float* __restrict__ part, float* __restrict__ dbias_part,
     const Pieces cut) {
     using TileT = Tile<T, DP>;
@@ -464,8 +517,13 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
         Stage<T, DP, TQ, VEC> qs, gs;
         float st = 0.f;
+        int odd_rows = 0;  // lanes 0 .. TQ / 32: whether any of the 32 rows that the tile meets there is a coarse one
+        const int groups_32 = (a.Q + 31) / 32;
+        const auto flags = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<int*>(coarse_in + (static_cast<int64_t>(b) * a.H + h) * groups_32), 0, 4 * groups_32, kRawBuffer);
         auto fetch = [&](int t) {
             const int i0 = i_low + t * TQ;
+            odd_rows = __builtin_amdgcn_raw_buffer_load_b32(flags, lane <= TQ / 32 ? 4u * (i0 / 32 + lane) : 0x80000000u, 0, 0);
             qs.load(q, a.q.n, i0, i_high, a.D);
             gs.load(go, grad.n, i0, i_high, a.D);
             if (threadIdx.x < 2 * TQ) {
@@ -476,13 +534,27 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             }
         };
         char* set = lds;
-        auto put = [&] {
+        // The shares of coarse rows (1 for others) are multiplied into their gradients and
+        // delta, on which all of a row's sums depend linearly: as factors of the
+        // weights they took 4 to 7 % more of the whole kernel.  16-bit gradients are
+        // rounded once more thereby.
+        auto put = [&](int t) {
             qs.store(set);
+            if (ballot(odd_rows != 0) != 0) {
+                auto share = [&](int row) {
+                    const int i = i_low + t * TQ + row;
+                    return i < i_high ? share_in[stats + i] : 1.f;
+                };
+                gs.scale(share);
+                int thread = threadIdx.x;
+                asm volatile("" : "+v"(thread));  // as in scale()
+                if (thread >= TQ && thread < 2 * TQ) st *= share(thread - TQ);
+            }
             gs.store(set + kTileBytes);
             if (threadIdx.x < 2 * TQ) reinterpret_cast<float*>(set + 2 * kTileBytes)[threadIdx.x] = st;
         };
         fetch(from);
-        put();
+        put(from);
         __syncthreads();
         for (int t = from; t < to; ++t) {
             if (t + 1 < to) fetch(t + 1);
@@ -577,7 +649,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                 }
             }
             set = set == lds ? lds + kSet : lds;
-            if (t + 1 < to) put();
+            if (t + 1 < to) put(t + 1);
             __syncthreads();
         }
         if (summed) {
@@ -624,7 +696,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
             const int64_t before = static_cast<int64_t>(hh) * tiles;
             const int from = t_first + static_cast<int>(max(share_low - before, int64_t(0)));
             const int to = t_first + static_cast<int>(min(share_high - before, static_cast<int64_t>(tiles)));
-            careful_key<T>(a, grad, lse_in, delta_in, b, g * group + hh, j0 + key, i_low + from * TQ,
+            careful_key<T>(a, grad, lse_in, delta_in, share_in, b, g * group + hh, j0 + key, i_low + from * TQ,
                            min(i_low + to * TQ, i_high), FIRST, len, ck, cv);
         }
     };
@@ -788,7 +860,7 @@ int padded(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
 
 struct Workspace {
     Pieces cut;
-    size_t delta, bias, part, bytes;
+    size_t delta, share, coarse, bias, part, bytes;
 };
 
 Workspace workspace_of(const Args& a, int type, bool may_split) {
@@ -798,7 +870,9 @@ Workspace workspace_of(const Args& a, int type, bool may_split) {
     w.cut = pieces_of(a, type == POINTOPS_F32 ? kInner<float> : kInner<f16>, may_split);
     const size_t units = static_cast<size_t>(w.cut.units()) + w.cut.first_units();
     w.delta = 0;
-    w.bias = up(rows * a.Q * sizeof(float));
+    w.share = up(rows * a.Q * sizeof(float));
+    w.coarse = 2 * w.share;
+    w.bias = w.coarse + up(rows * ((a.Q + 31) / 32) * sizeof(int));
     w.part = w.bias + (a.bias != nullptr ? up(rows * units * a.bk.count * sizeof(float)) : 0);
     w.bytes = w.part + static_cast<size_t>(a.B) * a.G * w.cut.floats(padded(a.D)) * sizeof(float);
     return w;
@@ -822,6 +896,8 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
     const Workspace w = workspace_of(a, kType<T>, kSplit);
     const Pieces cut = w.cut;
     float* const delta = reinterpret_cast<float*>(x.workspace + w.delta);
+    float* const share = reinterpret_cast<float*>(x.workspace + w.share);
+    int* const coarse = reinterpret_cast<int*>(x.workspace + w.coarse);
     float* const dbias_part = x.dbias != nullptr ? reinterpret_cast<float*>(x.workspace + w.bias) : nullptr;
     float* const part = reinterpret_cast<float*>(x.workspace + w.part);
     const int64_t heads = static_cast<int64_t>(a.B) * a.G, grid_k = cut.units() * heads, grid_first = cut.first_units() * heads;
@@ -844,7 +920,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
             if (err != hipSuccess) return err;
         }
         hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), lds, stream, a,
-                           static_cast<const T*>(x.out), x.lse, x.grad, delta, static_cast<T*>(x.dq), dbias_part != nullptr);
+                           static_cast<const T*>(x.out), x.lse, x.grad, delta, share, coarse, static_cast<T*>(x.dq), dbias_part != nullptr);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
@@ -861,7 +937,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
                 const hipError_t err = allow_lds(kernel, allowed, lds_for(split, bias_entries(kMaxReach), 255, true));
                 if (err != hipSuccess) return err;
             }
-            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), lds, stream, a, x.lse, delta, x.grad,
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), lds, stream, a, x.lse, delta, share, coarse, x.grad,
                                static_cast<T*>(x.dk), static_cast<T*>(x.dv), part, dbias_part, cut);
             return hipGetLastError();
         };
