@@ -482,8 +482,8 @@ __device__ __forceinline__ void fill_bias(const Args& a, int head, float* table,
 // ------------------------------------------------------------ careful rows
 // One query by a whole wave, key by key, for rows whose result is not finite:
 // there a product with a masked key's infinity or NaN may have spread.  Only
-// keys that the row sees are added (one whose score is -inf has no weight and
-// is left out).  Lane l holds elements l and l + 64.
+// keys that the row sees are added (one whose score is -inf, or whose bias is,
+// whatever it holds, has no weight and is left out).  Lane l holds elements l and l + 64.
 template <typename T>
 struct CarefulRow {
     const Args& a;
@@ -501,6 +501,7 @@ struct CarefulRow {
         q1 = d1 ? to_float(q[lane + kWave]) : 0.f;
     }
     __device__ __forceinline__ void add(int64_t j, float bias) {
+        if (bias == -kInf) return;
         const float k0 = d0 ? to_float(k[j * a.k.n]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + kWave]) : 0.f;
         const float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2 + bias;
         if (s == -kInf) return;
@@ -596,8 +597,9 @@ __device__ __forceinline__ void add_buckets(const Buckets& bk, const int* edge, 
 }
 
 // relative_bias.hip: grad[bucket][h] (of type POINTOPS_*) from part (B, H,
-// blocks, count).
-hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, void* grad,
+// blocks, count).  Given the bias itself (of the same type), entries of -inf have
+// gradients of zero, whatever masked places have left in their sums.
+hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, const void* bias, void* grad,
                         hipStream_t stream);
 
 // The device arguments of a call, and whether it is one that the kernels take.

@@ -59,8 +59,10 @@ __device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, i
     go.load(grad.at<T>(b, h) + i * grad.n, a.D);
     auto key = [&](int64_t j) {
         CarefulPair<T> kk, vv;
+        const float bias = one_bias<T>(a, h, static_cast<int>(p - j));
+        if (bias == -kInf) return;
         kk.load(k + j * a.k.n, a.D);
-        const float s = q.dot(kk) * a.scale_log2 + one_bias<T>(a, h, static_cast<int>(p - j));
+        const float s = q.dot(kk) * a.scale_log2 + bias;
         if (s == -kInf) return;
         vv.load(v + j * a.v.n, a.D);
         sum.add(exp2_fast(s - lse) * (go.dot(vv) - delta), kk);
@@ -88,9 +90,11 @@ __device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, con
         if ((a.causal && off < 0) || within == beyond) continue;
         const float lse = lse_in[stats + i];
         if (lse == kInf) continue;
+        const float bias = one_bias<T>(a, h, off);
+        if (bias == -kInf) continue;
         CarefulPair<T> q, go;
         q.load(a.q.at<T>(b, h) + i * a.q.n, a.D);
-        const float s = q.dot(k) * a.scale_log2 + one_bias<T>(a, h, off);
+        const float s = q.dot(k) * a.scale_log2 + bias;
         if (s == -kInf) continue;
         go.load(grad.at<T>(b, h) + i * grad.n, a.D);
         const float w = exp2_fast(s - lse) * share_in[stats + i];
@@ -132,9 +136,9 @@ __device__ __forceinline__ float exponents_sum(const Args& a, const i32x4 (&q)[T
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int j = 32 * t + 4 * half + 8 * (r / 4) + r % 4;
-            float x = s[r];
-            if (table != nullptr) x = x * a.scale_log2 + table[min(max(p - j, -a.reach), a.reach) + a.reach + kMargin];
-            if (seen(j)) sum += exp2_fast(__builtin_fmaf(x, factor, -lse));
+            const float bias = table != nullptr ? table[min(max(p - j, -a.reach), a.reach) + a.reach + kMargin] : 0.f;
+            const float x = table != nullptr ? s[r] * a.scale_log2 + bias : s[r];
+            if (seen(j) && bias != -kInf) sum += exp2_fast(__builtin_fmaf(x, factor, -lse));
         }
     }
     return halves_sum(sum);
@@ -219,10 +223,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     }
     // The weights of a row sum to 1, so that what is left of its ds is what the
     // rounded output took from delta: of few keys a pass ahead measures it.
-    auto left = [&] {
-        rest = halves_sum(rest);
-        return rest - rest == 0.f ? rest : 0.f;
-    };
+    // (Of a row beside a place that is no number it cannot be told.)
+    auto left = [](float all) { return all - all == 0.f ? all : 0.f; };
     const float factor = biased ? 1.f : a.scale_log2;
     f32x16 dq[kOut] = {};
     char* ktile = lds;
@@ -301,14 +303,14 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         __syncthreads();
         if (turn) {
             ahead = false;
-            float taken = left();
+            float taken = halves_sum(rest);
             if constexpr (SPLIT == 2 && sizeof(T) == 2) {
                 __shared__ float parts[kWaves][32];
                 if (half == 0) parts[wave][lane] = taken;
                 __syncthreads();
                 taken = parts[wave % 2][lane % 32] + parts[wave % 2 + 2][lane % 32];
             }
-            delta += taken * share;
+            delta += left(taken) * share;
             rest = 0.f;
         }
     }
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
         careful_query<T>(a, grad, b, h, i, len, i2f(readlane(f2i(lse), r)), i2f(readlane(f2i(delta), r)),
                          i2f(readlane(f2i(share), r)), dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
     }
-    if (refine) delta += left() * share;
+    if (refine) delta += left(halves_sum(rest)) * share;
     if (row < a.Q && half == 0) {
         delta_out[stat] = delta;
         share_out[stat] = share;
@@ -958,7 +960,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
         }
     }
     if (dbias_part == nullptr) return hipSuccess;
-    return join_buckets(dbias_part, a.B, a.H, cut.units() + cut.first_units(), a.bk.count, kType<T>, x.dbias, stream);
+    return join_buckets(dbias_part, a.B, a.H, cut.units() + cut.first_units(), a.bk.count, kType<T>, a.bias, x.dbias, stream);
 }
 
 template <typename T>

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_aligned_kernel(co
 constexpr int kJoinBuckets = 8;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_buckets_kernel(const float* __restrict__ part, int B, int64_t blocks,
-                                                                int count, T* __restrict__ grad) {
+                                                                int count, const T* __restrict__ bias, T* __restrict__ grad) {
     constexpr int kLanes = 32, kBuckets = kJoinBuckets;
     __shared__ float sums[kLanes][kBuckets];
     const int H = gridDim.x, h = blockIdx.x, x = threadIdx.x % kBuckets, y = threadIdx.x / kBuckets;
@@ -199,7 +199,9 @@ __global__ __launch_bounds__(kThreads) void join_buckets_kernel(const float* __r
         all = sums[0][x];
 #pragma unroll
         for (int i = 1; i < kLanes; ++i) all += sums[i][x];
-        grad[static_cast<int64_t>(bucket) * H + h] = from_float<T>(all);
+        const int64_t at = static_cast<int64_t>(bucket) * H + h;
+        if (bias != nullptr && to_float(bias[at]) == -kInf) all = 0.f;
+        grad[at] = from_float<T>(all);
     }
 }
 
@@ -234,21 +236,21 @@ bool bias_sizes(int64_t Q, int64_t N, int64_t H, int32_t type) {
 
 }  // namespace
 
-hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, void* grad,
+hipError_t join_buckets(const float* part, int B, int H, int64_t blocks, int count, int type, const void* bias, void* grad,
                         hipStream_t stream) {
     const dim3 grid(H, (count + kJoinBuckets - 1) / kJoinBuckets);
     switch (type) {
         case POINTOPS_F32:
             hipLaunchKernelGGL(join_buckets_kernel<float>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
-                               static_cast<float*>(grad));
+                               static_cast<const float*>(bias), static_cast<float*>(grad));
             break;
         case POINTOPS_F16:
             hipLaunchKernelGGL(join_buckets_kernel<f16>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
-                               static_cast<f16*>(grad));
+                               static_cast<const f16*>(bias), static_cast<f16*>(grad));
             break;
         default:
             hipLaunchKernelGGL(join_buckets_kernel<bf16>, grid, dim3(kThreads), 0, stream, part, B, blocks, count,
-                               static_cast<bf16*>(grad));
+                               static_cast<const bf16*>(bias), static_cast<bf16*>(grad));
     }
     return hipGetLastError();
 }
@@ -292,7 +294,7 @@ hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, i
     if (grad_table == nullptr || (Q > 0 && N > 0 && (grad == nullptr || workspace == nullptr))) return hipErrorInvalidValue;
     const int h = static_cast<int>(H), q = static_cast<int>(Q), n = static_cast<int>(N);
     float* const part = static_cast<float*>(workspace);
-    if (Q == 0 || N == 0) return join_buckets(nullptr, 0, h, 0, bk.count, type, grad_table, stream);
+    if (Q == 0 || N == 0) return join_buckets(nullptr, 0, h, 0, bk.count, type, nullptr, grad_table, stream);
     const int per = type == POINTOPS_F32 ? 4 : 8;
     const bool aligned = reinterpret_cast<uintptr_t>(grad) % 16 == 0 && stride_h % per == 0 && stride_i % per == 0 && N % per == 0;
     const dim3 grid = diagonal_grid(H, Q, N, aligned ? kThreads * per : kDiagSpan);
@@ -306,7 +308,7 @@ hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, i
     };
     const hipError_t err = type == POINTOPS_F32 ? sums(float{}) : type == POINTOPS_F16 ? sums(f16{}) : sums(bf16{});
     if (err != hipSuccess) return err;
-    return join_buckets(part, 1, h, static_cast<int64_t>(grid.x) * grid.y, bk.count, type, grad_table, stream);
+    return join_buckets(part, 1, h, static_cast<int64_t>(grid.x) * grid.y, bk.count, type, nullptr, grad_table, stream);
 }
 
 }  // extern "C"
