@@ -959,7 +959,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
             if (err != hipSuccess) return err;
         }
     }
-    if (dbias_part == nullptr) return hipSuccess;
+    if (x.dbias == nullptr || a.H == 0) return hipSuccess;
     return join_buckets(dbias_part, a.B, a.H, cut.units() + cut.first_units(), a.bk.count, kType<T>, a.bias, x.dbias, stream);
 }
 
@@ -994,12 +994,14 @@ hipError_t pointops_attention_backward(const pointops_attention* in, const void*
     using namespace pointops::attn;
     Args a;
     if (!read_args(in, &a)) return hipErrorInvalidValue;
-    if (a.B == 0 || a.H == 0 || (a.Q == 0 && a.N == 0)) return hipSuccess;
     if (dbias != nullptr && a.bias == nullptr) return hipErrorInvalidValue;
-    if (a.Q > 0 && (in->q == nullptr || out == nullptr || lse == nullptr || grad_out == nullptr || grad_stride == nullptr ||
-                    dq == nullptr || workspace == nullptr))
+    // (Of sides that are empty the others' gradients are zeros, written as any.)
+    const bool queries = a.B > 0 && a.H > 0 && a.Q > 0, keys = a.B > 0 && a.G > 0 && a.N > 0;
+    if (queries && (in->q == nullptr || out == nullptr || lse == nullptr || grad_out == nullptr || grad_stride == nullptr ||
+                    dq == nullptr))
         return hipErrorInvalidValue;
-    if (a.N > 0 && (in->k == nullptr || in->v == nullptr || dk == nullptr || dv == nullptr)) return hipErrorInvalidValue;
+    if (keys && (in->k == nullptr || in->v == nullptr || dk == nullptr || dv == nullptr)) return hipErrorInvalidValue;
+    if ((queries || keys) && workspace == nullptr && pointops_attention_backward_workspace_bytes(in) != 0) return hipErrorInvalidValue;
     Grads x{out, lse, {}, dq, dk, dv, dbias, static_cast<char*>(workspace)};
     if (grad_stride != nullptr) x.grad = {grad_out, grad_stride[0], grad_stride[1], grad_stride[2]};
     switch (in->type) {

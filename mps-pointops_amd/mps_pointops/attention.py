@@ -208,7 +208,7 @@ class _WindowAttention(torch.autograd.Function):
         dbias = None
         if bias is not None and ctx.needs_input_grad[3]:
             dbias = _like(bias)
-        if q.shape[0] and q.shape[2]:
+        if dq.numel() or dk.numel() or dbias is not None:
             args = _pack(q, k, v, window, sinks, causal, bias, edges, lengths, scale)
             size = _native.size_query("pointops_attention_backward_workspace_bytes", args)
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
@@ -216,9 +216,6 @@ class _WindowAttention(torch.autograd.Function):
             _native.call("pointops_attention_backward", args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(),
                          strides, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _native.ptr(dbias),
                          workspace.data_ptr(), _native.stream(q.device))
-        else:
-            for t in (dk, dv) if dbias is None else (dk, dv, dbias):
-                t.zero_()
         return dq, dk, dv, dbias, None, None, None, None, None, None
 
 
