@@ -622,7 +622,7 @@ hipError_t pointops_qk_norm_rotate(const pointops_qk_norm *in, void *q_out, void
                                    hipStream_t stream);
 
 /* Its gradients: dq, dk contiguous, of `type`; dq_weight, dk_weight (NULL: not
- * wanted) of weight_type.  `workspace` (NULL where no weight's gradient is
+ * wanted) of weight_type, zeros where there are no rows.  `workspace` (NULL where no weight's gradient is
  * wanted) holds pointops_qk_norm_rotate_backward_workspace_bytes(in) bytes. */
 size_t pointops_qk_norm_rotate_backward_workspace_bytes(const pointops_qk_norm *in);
 hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm *in, const void *q_grad,

@@ -324,7 +324,7 @@ Shape shape_of(const pointops_qk_norm& in) {
     s.units = (half + s.vec - 1) / s.vec + ((rest + s.vec - 1) / s.vec + 1) / 2;
     s.lanes = 1;
     while (s.lanes < s.units) s.lanes *= 2;
-    const int64_t tokens = in.B * in.N, heads = in.H + in.G, groups = kThreads / s.lanes;
+    const int64_t tokens = in.B * in.N, heads = std::max<int64_t>(1, in.H + in.G), groups = kThreads / s.lanes;
     s.blocks = std::min(kBlocks, (tokens * heads + groups - 1) / groups);
     s.blocks = std::max(s.blocks, (heads + groups - 1) / groups);
     s.step = std::min(tokens, s.blocks * groups / heads);
@@ -437,13 +437,14 @@ hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const vo
     if (!valid(in)) return hipErrorInvalidValue;
     if ((dq_weight != nullptr && in->q_weight == nullptr) || (dk_weight != nullptr && in->k_weight == nullptr))
         return hipErrorInvalidValue;
-    if (in->B == 0 || in->N == 0 || in->H + in->G == 0) return hipSuccess;
-    if ((in->H > 0 && (in->q == nullptr || dq == nullptr || q_grad == nullptr || q_grad_stride == nullptr)) ||
-        (in->G > 0 && (in->k == nullptr || dk == nullptr || k_grad == nullptr || k_grad_stride == nullptr)) ||
-        (in->R > 0 && (in->cos == nullptr || in->sin == nullptr)))
-        return hipErrorInvalidValue;
     const bool sums = dq_weight != nullptr || dk_weight != nullptr;
-    if (sums && workspace == nullptr) return hipErrorInvalidValue;
+    const bool none = in->B == 0 || in->N == 0 || in->H + in->G == 0;
+    if (none && !sums) return hipSuccess;
+    if (!none && ((in->H > 0 && (in->q == nullptr || dq == nullptr || q_grad == nullptr || q_grad_stride == nullptr)) ||
+        (in->G > 0 && (in->k == nullptr || dk == nullptr || k_grad == nullptr || k_grad_stride == nullptr)) ||
+        (in->R > 0 && (in->cos == nullptr || in->sin == nullptr))))
+        return hipErrorInvalidValue;
+    if (!none && sums && workspace == nullptr) return hipErrorInvalidValue;
     Rows gq{}, gk{};
     if (q_grad_stride != nullptr) gq = {q_grad, q_grad_stride[0], q_grad_stride[1], q_grad_stride[2]};
     if (k_grad_stride != nullptr) gk = {k_grad, k_grad_stride[0], k_grad_stride[1], k_grad_stride[2]};
@@ -455,12 +456,14 @@ hipError_t pointops_qk_norm_rotate_backward(const pointops_qk_norm* in, const vo
         using T = decltype(t);
         using W = decltype(w);
         constexpr int VEC = decltype(vec)::value, L = decltype(lanes)::value;
-        hipLaunchKernelGGL((qk_norm_grad_kernel<T, W, VEC, L>), dim3(static_cast<uint32_t>(s.blocks)), dim3(kThreads), 0,
-                           stream, a, gq, gk, static_cast<T*>(dq), static_cast<T*>(dk), part);
-        const hipError_t err = hipGetLastError();
-        if (err != hipSuccess || !sums) return err;
+        if (!none) {
+            hipLaunchKernelGGL((qk_norm_grad_kernel<T, W, VEC, L>), dim3(static_cast<uint32_t>(s.blocks)), dim3(kThreads), 0,
+                               stream, a, gq, gk, static_cast<T*>(dq), static_cast<T*>(dk), part);
+            const hipError_t err = hipGetLastError();
+            if (err != hipSuccess || !sums) return err;
+        }
         hipLaunchKernelGGL((qk_norm_weight_kernel<W, VEC, L>), dim3((4 * L * VEC + 7) / 8), dim3(kThreads), 0, stream, part,
-                           static_cast<int>(s.blocks), a.D, a.R, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
+                           none ? 0 : static_cast<int>(s.blocks), a.D, a.R, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
         return hipGetLastError();
     });
 }

@@ -376,10 +376,8 @@ class _QkNormRotate(torch.autograd.Function):
         q_grad, k_grad = _rows(q_grad), _rows(k_grad)
         dq, dk = _like(q), _like(k)
         weights = [w if need else None for w, need in zip((q_weight, k_weight), ctx.needs_input_grad[2:4])]
-        # A weight without a row to sum over has a gradient of zeros.
-        make = torch.empty_like if q.numel() + k.numel() else torch.zeros_like
-        dwq, dwk = (None if w is None else make(w) for w in weights)
-        if q.numel() + k.numel():
+        dwq, dwk = (None if w is None else torch.empty_like(w) for w in weights)
+        if q.numel() + k.numel() or dwq is not None or dwk is not None:
             args = _pack_norm(q, k, q_weight, k_weight, cos, sin, ctx.eps)
             workspace = None
             if dwq is not None or dwk is not None:

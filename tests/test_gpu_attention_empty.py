@@ -49,3 +49,29 @@ def test_the_entry_point_writes_everything(cuda_device, B, Q, N, H):
                  workspace.data_ptr(), _native.stream(cuda_device))
     for t in (dq, dk, dv, dbias):
         assert (t == 0).all()
+
+
+@pytest.mark.parametrize("B,N,H,G", [(0, 4, 2, 1), (3, 0, 2, 1), (3, 4, 0, 0), (0, 0, 0, 0), (3, 4, 0, 2)])
+@pytest.mark.parametrize("D,R", [(8, 8), (33, 6), (128, 128), (1, 0)])
+def test_weights_of_no_rows(cuda_device, B, N, H, G, D, R):
+    """qk_norm_rotate's weights, through the entry point and through autograd."""
+    from mps_pointops import _native, attention
+
+    q, k = torch.ones(B, N, H, D, device=cuda_device), torch.ones(B, N, G, D, device=cuda_device)
+    angle = torch.zeros(B, N, R // 2, device=cuda_device)
+    w = torch.ones(D, device=cuda_device)
+    dwq, dwk = (torch.full((D,), torch.nan, device=cuda_device) for _ in range(2))
+    dq, dk = torch.empty_like(q), torch.empty_like(k)
+    args = attention._pack_norm(q, k, w, w, angle, angle, 1e-6)
+    size = _native.size_query("pointops_qk_norm_rotate_backward_workspace_bytes", args)
+    workspace = torch.empty(size, dtype=torch.uint8, device=cuda_device)
+    three = ctypes.c_int64 * 3
+    _native.call("pointops_qk_norm_rotate_backward", args, q.data_ptr(), three(*q.stride()[:3]), k.data_ptr(),
+                 three(*k.stride()[:3]), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+                 workspace.data_ptr(), _native.stream(cuda_device))
+    leaves = [t.requires_grad_() for t in (q, k, w, w.clone())]
+    outs = attention.qk_norm_rotate(*leaves, angle, angle)
+    grads = torch.autograd.grad(outs, leaves, [torch.zeros_like(t) for t in outs])
+    assert all((t == 0).all() for t in (dwq, *grads))
+    if not k.numel():
+        assert (dwk == 0).all()
