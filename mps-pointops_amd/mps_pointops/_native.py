@@ -17,6 +17,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_NAME = "libpointops_hip.so"
 LIB_PATH = Path(__file__).resolve().with_name(LIB_NAME)
@@ -196,19 +197,28 @@ def size_query(name: str, *args) -> int:
     return int(getattr(library(), name)(*args))
 
 
+# What untraced() asks on every call, looked up once.
+_interpreter = torch._C._functorch.peek_interpreter_stack
+_modes = torch._C._len_torch_dispatch_stack
+_is_tracing = torch.jit.is_tracing
+_is_compiling = torch.compiler.is_compiling
+
+
+def untraced() -> bool:
+    """Whether nothing but the results themselves is asked of a call: outside
+    function transforms, forward-mode differentiation, tracing, compilation and
+    dispatch modes, all of which see tensor operations only."""
+    return (_interpreter() is None and forward_ad._current_level < 0 and _modes() == 0
+            and not _is_tracing() and not _is_compiling())
+
+
 def plain(*tensors: torch.Tensor) -> bool:
     """Whether kernels on raw pointers may stand in for tensor operations on
     these: no subclasses and no batched gradients (which may hold no memory of
-    their own; a backward's thread does not see the transform), and outside
-    function transforms, forward-mode differentiation, tracing, compilation and
-    dispatch modes, all of which see tensor operations only."""
+    their own; a backward's thread does not see the transform), and untraced."""
     return (all(type(t) in (torch.Tensor, torch.nn.Parameter) and torch._C._has_storage(t)
                 for t in tensors)
-            and torch._C._functorch.peek_interpreter_stack() is None
-            and torch.autograd.forward_ad._current_level < 0
-            and torch._C._len_torch_dispatch_stack() == 0
-            and not torch.jit.is_tracing()
-            and not torch.compiler.is_compiling())
+            and untraced())
 
 
 def outside(checks: list[tuple[torch.Tensor, int, int]]) -> list[bool]:

@@ -92,7 +92,7 @@ def _check_table(table: Tensor, heads: int | None, max_distance: int | None, cau
         raise ValueError(f"{name} must have at most {_MAX_SIDE} buckets for each side")
     if max_distance > limit:
         raise ValueError(f"max_distance must be at most {limit}")
-    return _edge_array(side, int(max_distance))
+    return _edge_array(int(side), int(max_distance))  # (a trace has tensors for sizes)
 
 
 # ----------------------------------------------------------------- arguments
@@ -179,6 +179,14 @@ def _tracked(*tensors: Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _by_function(*tensors: Tensor | None) -> bool:
+    """Whether a call goes through its autograd function: where its graph is
+    recorded, and where more than the tensors' memory is asked for.  A trace
+    records the function as a node, forward-mode differentiation and function
+    transforms refuse it; the kernels' call alone they would not see."""
+    return not _native.untraced() or _tracked(*tensors)
+
+
 # ------------------------------------------------------------------ attention
 def _attend(q, k, v, bias, lengths, edges, window, sinks, causal, scale, lse):
     out = _like(q)
@@ -248,7 +256,25 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = No
         scale = q.shape[3] ** -0.5
     args = (_rows(q), _rows(k), _rows(v), None if bias is None else bias.contiguous(),
             None if lengths is None else lengths.contiguous(), edges, window, sinks, causal, float(scale))
-    return _WindowAttention.apply(*args) if _tracked(q, k, v, bias) else _attend(*args, None)
+    return _WindowAttention.apply(*args) if _by_function(q, k, v, bias) else _attend(*args, None)
+
+
+def _step(q, k_cache, v_cache, bias, lengths, edges, window, sinks, scale):
+    out = _like(q)
+    if out.numel():
+        args = _pack(q, k_cache, v_cache, window, sinks, True, bias, edges, lengths, scale)
+        size = _native.size_query("pointops_attention_step_workspace_bytes", args)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _native.call("pointops_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(q.device))
+    return out
+
+
+class _WindowAttentionStep(torch.autograd.Function):
+    """A node for traces; without gradients."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _step(*args)
 
 
 def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor | None = None, *,
@@ -268,18 +294,10 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     if _tracked(q, k_cache, v_cache, bias):
         raise ValueError("window_attention_step has no gradients: call it under torch.no_grad(), "
                          "or use window_attention")
-    q, k_cache, v_cache = _rows(q), _rows(k_cache), _rows(v_cache)
-    bias = None if bias is None else bias.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    out = _like(q)
-    if out.numel():
-        args = _pack(q, k_cache, v_cache, window, sinks, True, bias, edges, lengths,
-                     q.shape[3] ** -0.5 if scale is None else float(scale))
-        size = _native.size_query("pointops_attention_step_workspace_bytes", args)
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _native.call("pointops_attention_step", args, out.data_ptr(), _native.ptr(workspace),
-                     _native.stream(q.device))
-    return out
+    args = (_rows(q), _rows(k_cache), _rows(v_cache), None if bias is None else bias.contiguous(),
+            None if lengths is None else lengths.contiguous(), edges, window, sinks,
+            float(q.shape[3] ** -0.5 if scale is None else scale))
+    return _step(*args) if _native.untraced() else _WindowAttentionStep.apply(*args)
 
 
 # ------------------------------------------------------------- relative bias
@@ -335,7 +353,7 @@ def relative_bias(table: Tensor, queries: int, keys: int, *, max_distance: int, 
         raise ValueError(f"relative_bias supports at most {_MAX_BIAS_TOKENS} queries and keys and 65535 heads")
     _native.require_device(table.device)
     args = table.contiguous(), edges, int(queries), int(keys)
-    return _RelativeBias.apply(*args) if _tracked(table) else _dense_bias(*args)
+    return _RelativeBias.apply(*args) if _by_function(table) else _dense_bias(*args)
 
 
 # --------------------------------------------------------- norm and rotation
@@ -446,7 +464,7 @@ def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
         cos, sin = cos.contiguous(), sin.contiguous()
     args = (_rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),
             None if k_weight is None else k_weight.contiguous(), cos, sin, float(eps))
-    return _QkNormRotate.apply(*args) if _tracked(q, k, q_weight, k_weight) else _norm(*args)
+    return _QkNormRotate.apply(*args) if _by_function(q, k, q_weight, k_weight) else _norm(*args)
 
 
 __all__ = ["bucket_edges", "qk_norm_rotate", "relative_bias", "window_attention", "window_attention_step"]
