@@ -43,12 +43,11 @@ _ARGS = struct.Struct("@6Q9q6q2q5if")
 # ------------------------------------------------------------------- buckets
 def _root_above(n: int, m: int) -> int:
     """The smallest d with d ** m >= n."""
-    d = max(1, int(round(n ** (1.0 / m)))) if n < 1 << 1000 else 1 << -(-n.bit_length() // m)
-    while d ** m >= n:
-        d -= 1
-    while d ** m < n:
-        d += 1
-    return d
+    low, high = 0, 1 << -(-n.bit_length() // m)  # low ** m < n <= high ** m
+    while high - low > 1:
+        mid = (low + high) // 2
+        low, high = (mid, high) if mid ** m < n else (low, mid)
+    return high
 
 
 @functools.lru_cache(maxsize=256)

@@ -4,7 +4,9 @@ from __future__ import annotations
 
 import ctypes
 
-from mps_pointops import _native
+import pytest
+
+from mps_pointops import _native, attention
 
 from test_attention_cpu import packed
 
@@ -16,3 +18,17 @@ def test_backward_needs_its_workspace_where_queries_are_none():
     lib = _native.library()
     assert lib.pointops_attention_backward_workspace_bytes(args) > 0
     assert lib.pointops_attention_backward(args, None, None, None, None, None, 8, 8, 8, None, None) == 1
+
+
+@pytest.mark.timeout(60)
+@pytest.mark.parametrize("buckets,max_distance", [(256, 1 << 30), (128, 1 << 30), (255, 1 << 20), (2, 1 << 30), (3, 2), (256, 129),
+                                                  (17, 10 ** 9 + 7), (64, 33)])
+def test_edges_of_large_distances(buckets, max_distance):
+    """Each edge against its definition in whole numbers: the least d with
+    (d / e) ** (buckets - e) >= (max_distance / e) ** t."""
+    edges = attention.bucket_edges(buckets, max_distance)
+    e = buckets // 2
+    steps = buckets - e
+    assert edges[:e] == tuple(range(1, e + 1)) and len(edges) == buckets - 1
+    for t, d in enumerate(edges[e:], 1):
+        assert d ** steps >= max_distance ** t * e ** (steps - t) > (d - 1) ** steps
