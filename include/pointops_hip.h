@@ -585,7 +585,7 @@ hipError_t pointops_attention_step(const pointops_attention *in, void *out, void
 
 /* The bias as a dense tensor: out[h][i][j] = table[bucket(N - Q + i - j)][h],
  * (H, Q, N) contiguous; table (buckets, H) contiguous, edges and buckets as in
- * pointops_attention, but edges up to 2^30.  Q, N < 2^22. */
+ * pointops_attention, but edges up to 2^30.  Q <= 4194240, N < 2^22, H <= 65535. */
 hipError_t pointops_relative_bias(const void *table, const int32_t *edges, int32_t n_edges,
                                   int32_t buckets, int32_t type, void *out, int64_t H, int64_t Q,
                                   int64_t N, hipStream_t stream);

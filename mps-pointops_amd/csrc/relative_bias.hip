@@ -211,7 +211,7 @@ hipError_t launch_bias(const Buckets& bk, const void* table, void* out, int H, i
     const int64_t x = static_cast<int64_t>(col_blocks) * H;
     const int rows = x * ((Q + kBiasRows - 1) / kBiasRows) >= 512 ? kBiasRows : kBiasRows / 8;
     const int64_t y = (static_cast<int64_t>(Q) + rows - 1) / rows;
-    if (x > INT32_MAX || y > 65535) return hipErrorInvalidValue;
+    if (x > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL(relative_bias_kernel<T>, dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(y)), dim3(kThreads), 0,
                        stream, bk, static_cast<const T*>(table), static_cast<T*>(out), H, Q, N, col_blocks, rows);
     return hipGetLastError();
@@ -228,9 +228,11 @@ dim3 diagonal_grid(int64_t H, int64_t Q, int64_t N, int64_t span) {
 }
 
 // Sizes that the kernels' launches hold.
-constexpr int64_t kBiasLimit = int64_t(1) << 22;  // rows of 64 in a grid's second dimension
+constexpr int64_t kMostRows = 65535 * int64_t(kBiasRows);  // a grid's second dimension
+constexpr int64_t kBiasLimit = int64_t(1) << 22;
+static_assert(kBiasRows == kDiagRows, "one limit for both directions");
 bool bias_sizes(int64_t Q, int64_t N, int64_t H, int32_t type) {
-    return Q >= 0 && N >= 0 && H >= 0 && Q < kBiasLimit && N < kBiasLimit && H <= 65535 && type >= POINTOPS_F32 &&
+    return Q >= 0 && N >= 0 && H >= 0 && Q <= kMostRows && N < kBiasLimit && H <= 65535 && type >= POINTOPS_F32 &&
            type <= POINTOPS_BF16;
 }
 
@@ -298,7 +300,6 @@ hipError_t pointops_relative_bias_backward(const void* grad, int64_t stride_h, i
     const int per = type == POINTOPS_F32 ? 4 : 8;
     const bool aligned = reinterpret_cast<uintptr_t>(grad) % 16 == 0 && stride_h % per == 0 && stride_i % per == 0 && N % per == 0;
     const dim3 grid = diagonal_grid(H, Q, N, aligned ? kThreads * per : kDiagSpan);
-    if (grid.y > 65535) return hipErrorInvalidValue;
     auto sums = [&](auto zero) {
         using T = decltype(zero);
         auto* const kernel = aligned ? relative_bias_grad_aligned_kernel<T> : relative_bias_grad_kernel<T>;

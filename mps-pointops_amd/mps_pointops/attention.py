@@ -300,7 +300,8 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
 
 
 # ------------------------------------------------------------- relative bias
-_MAX_BIAS_TOKENS = (1 << 22) - 1
+_MAX_BIAS_QUERIES = 65535 * 64
+_MAX_BIAS_KEYS = (1 << 22) - 1
 
 
 def _dense_bias(table, edges, queries, keys):
@@ -348,8 +349,8 @@ def relative_bias(table: Tensor, queries: int, keys: int, *, max_distance: int, 
     edges = _check_table(table, None, max_distance, causal, 1 << 30, "table")
     if queries < 0 or keys < 0:
         raise ValueError("queries and keys must be non-negative")
-    if max(queries, keys) > _MAX_BIAS_TOKENS or table.shape[1] > 65535:
-        raise ValueError(f"relative_bias supports at most {_MAX_BIAS_TOKENS} queries and keys and 65535 heads")
+    if queries > _MAX_BIAS_QUERIES or keys > _MAX_BIAS_KEYS or table.shape[1] > 65535:
+        raise ValueError(f"relative_bias supports at most {_MAX_BIAS_QUERIES} queries, {_MAX_BIAS_KEYS} keys and 65535 heads")
     _native.require_device(table.device)
     args = table.contiguous(), edges, int(queries), int(keys)
     return _RelativeBias.apply(*args) if _by_function(table) else _dense_bias(*args)

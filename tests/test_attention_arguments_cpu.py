@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
 from mps_pointops import _native, attention
 
@@ -32,3 +33,21 @@ def test_edges_of_large_distances(buckets, max_distance):
     assert edges[:e] == tuple(range(1, e + 1)) and len(edges) == buckets - 1
     for t, d in enumerate(edges[e:], 1):
         assert d ** steps >= max_distance ** t * e ** (steps - t) > (d - 1) ** steps
+
+
+def test_largest_dense_bias():
+    """The sizes that the launches hold, and one more of each."""
+    table = torch.zeros(8, 2)
+    for queries, keys in ((4194240, 3), (3, 4194303)):
+        with pytest.raises(ValueError, match="ROCm"):  # the next check
+            attention.relative_bias(table, queries, keys, max_distance=9)
+    for queries, keys in ((4194241, 3), (4194303, 3), (3, 4194304)):
+        with pytest.raises(ValueError, match="at most"):
+            attention.relative_bias(table, queries, keys, max_distance=9)
+    lib = _native.library()
+    edges = (ctypes.c_int32 * 1)(1)
+    for Q, N in ((4194241, 4), (4, 1 << 22)):
+        assert lib.pointops_relative_bias(8, edges, 1, 2, 0, 8, 0, Q, N, None) == 1
+        assert lib.pointops_relative_bias_backward(8, 1, 1, edges, 1, 2, 0, 8, 8, 0, Q, N, None) == 1
+        assert lib.pointops_relative_bias_backward_workspace_bytes(1, Q, N, 2) == 0
+    assert lib.pointops_relative_bias(8, edges, 1, 2, 0, 8, 0, 4194240, 4, None) == 0  # without heads: nothing to do
