@@ -480,10 +480,36 @@ __device__ __forceinline__ void fill_bias(const Args& a, int head, float* table,
 }
 
 // ------------------------------------------------------------ careful rows
+// Only what came out of the products not finite is formed again: finite values have
+// met no infinity or NaN.  And only until it is not finite again, which is then its
+// own: what a place that is no number in a seen pair costs ends there, and a pass
+// over all pairs is left to values that are finite without their masked neighbours.
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
+
+// A lane's values of a result that are not finite: bit 16 d + register.
+template <int N>
+__device__ __forceinline__ uint64_t odd_values(const f32x16 (&v)[N]) {
+    uint64_t odd = 0;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd |= finite(v[d][r]) ? 0 : uint64_t(1) << (16 * d + r);
+    return odd;
+}
+// Whether value `c` of the result's row (lane column) r is one of them, r uniform.
+__device__ __forceinline__ bool odd_value(uint64_t odd, int r, int c) {
+    const int low = static_cast<int>(odd), high = static_cast<int>(odd >> 32);
+    const uint64_t of[2] = {static_cast<uint32_t>(readlane(low, r)) | uint64_t(static_cast<uint32_t>(readlane(high, r))) << 32,
+                            static_cast<uint32_t>(readlane(low, r + 32)) | uint64_t(static_cast<uint32_t>(readlane(high, r + 32))) << 32};
+    const uint64_t mine = (c & 4) != 0 ? of[1] : of[0];
+    return (mine >> (c / 32 * 16 + c % 32 / 8 * 4 + c % 4) & 1) != 0;
+}
+
 // One query by a whole wave, key by key, for rows whose result is not finite:
 // there a product with a masked key's infinity or NaN may have spread.  Only
 // keys that the row sees are added (one whose score is -inf, or whose bias is,
-// whatever it holds, has no weight and is left out).  Lane l holds elements l and l + 64.
+// whatever it holds, has no weight and is left out).  Lane l holds elements l and
+// l + 64, of which it needs those that came out not finite (n0, n1).
 template <typename T>
 struct CarefulRow {
     const Args& a;
@@ -511,6 +537,10 @@ struct CarefulRow {
         o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n]) : 0.f);
         o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + kWave]) : 0.f);
     }
+    // Whether all that is needed has come out not finite again.
+    __device__ __forceinline__ bool settled(bool n0, bool n1) const {
+        return ballot((n0 && finite(o0)) || (n1 && finite(o1))) == 0;
+    }
 };
 
 // The same for gradients: one query and one key at a time, of which a wave holds
@@ -528,7 +558,6 @@ struct CarefulPair {
         x0 = __builtin_fmaf(w, y.x0, x0);
         x1 = __builtin_fmaf(w, y.x1, x1);
     }
-    __device__ __forceinline__ bool finite() const { return ballot(x0 * 0.f + x1 * 0.f != 0.f) == 0; }
 };
 
 // ---------------------------------------------------------------- dispatch

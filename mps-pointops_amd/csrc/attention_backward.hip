@@ -46,10 +46,11 @@ __device__ __forceinline__ bool coarse(float lse) {
 // Gradients that are not finite are formed again pair by pair, where a product
 // with a masked pair's infinity or NaN may have spread: of one query over the
 // keys that it sees, and of one key over those of the rows i_from .. i_to - 1
-// of a head that see it.  By a whole wave.
+// of a head that see it.  By a whole wave; n0 and so on are the values that a lane
+// needs.
 template <typename T>
 __device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, int b, int h, int i, int len, float lse,
-                                              float delta, float share, T* dq) {
+                                              float delta, float share, bool n0, bool n1, T* dq) {
     const int g = h / (a.H / a.G), p = i + a.N - a.Q;
     const Seen seen = seen_by(a, p, len);
     const T* const k = a.k.at<T>(b, g);
@@ -57,28 +58,38 @@ __device__ __forceinline__ void careful_query(const Args& a, const Rows& grad, i
     CarefulPair<T> q, go, sum;
     q.load(a.q.at<T>(b, h) + i * a.q.n, a.D);
     go.load(grad.at<T>(b, h) + i * grad.n, a.D);
-    auto key = [&](int64_t j) {
+    const int lane = lane_id();
+    n0 = n0 && lane < a.D;
+    n1 = n1 && lane + kWave < a.D;
+    auto settled = [&](int64_t j) {
         CarefulPair<T> kk, vv;
         const float bias = one_bias<T>(a, h, static_cast<int>(p - j));
-        if (bias == -kInf) return;
+        if (bias == -kInf) return false;
         kk.load(k + j * a.k.n, a.D);
         const float s = q.dot(kk) * a.scale_log2 + bias;
-        if (s == -kInf) return;
+        if (s == -kInf) return false;
         vv.load(v + j * a.v.n, a.D);
         sum.add(exp2_fast(s - lse) * (go.dot(vv) - delta), kk);
+        return ballot((n0 && finite(sum.x0)) || (n1 && finite(sum.x1))) == 0;
     };
-    for (int j = 0; j < seen.first; ++j) key(j);
-    for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
-    const int lane = lane_id();
+    bool done = false;
+    for (int j = 0; j < seen.first && !done; ++j) done = settled(j);
+    for (int j = max(seen.low, seen.first); j < seen.low + seen.count && !done; ++j) done = settled(j);
     const float by = a.scale * share;
-    if (lane < a.D) dq[lane] = from_float<T>(sum.x0 * by);
-    if (lane + kWave < a.D) dq[lane + kWave] = from_float<T>(sum.x1 * by);
+    if (n0) dq[lane] = from_float<T>(sum.x0 * by);
+    if (n1) dq[lane + kWave] = from_float<T>(sum.x1 * by);
 }
 
+// A key's values that are needed.
+struct Needed {
+    bool k0, k1, v0, v1;
+};
+
+// Whether all that is needed has come out not finite again.
 template <typename T>
-__device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, const float* lse_in, const float* delta_in,
+__device__ __forceinline__ bool careful_key(const Args& a, const Rows& grad, const float* lse_in, const float* delta_in,
                                             const float* share_in, int b, int h, int64_t j, int i_from, int i_to, bool beyond,
-                                            int len, CarefulPair<T>& dk, CarefulPair<T>& dv) {
+                                            int len, const Needed& need, CarefulPair<T>& dk, CarefulPair<T>& dv) {
     const int g = h / (a.H / a.G);
     const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
     CarefulPair<T> k, v;
@@ -100,7 +111,11 @@ __device__ __forceinline__ void careful_key(const Args& a, const Rows& grad, con
         const float w = exp2_fast(s - lse) * share_in[stats + i];
         dv.add(w, go);
         dk.add(w * (go.dot(v) - delta_in[stats + i]) * a.scale, q);
+        if (ballot((need.k0 && finite(dk.x0)) || (need.k1 && finite(dk.x1)) || (need.v0 && finite(dv.x0)) ||
+                   (need.v1 && finite(dv.x1))) == 0)
+            return true;
     }
+    return false;
 }
 
 // A row's output is about as large as its values where it sees few keys, and its
@@ -337,18 +352,26 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     uint64_t bad = ballot(row < a.Q && odd != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     T* const dst = dq_out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
-    if (row < a.Q && (bad >> (lane % 32) & 1) == 0) {
+    if (row < a.Q) {
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) store4<T, VEC>(dst, 32 * d + 8 * e + 4 * half, a.D, dq[d], 4 * e);
     }
-    while (bad != 0) {
-        const int r = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        const int i = i0 + wave_row + r;
-        careful_query<T>(a, grad, b, h, i, len, i2f(readlane(f2i(lse), r)), i2f(readlane(f2i(delta), r)),
-                         i2f(readlane(f2i(share), r)), dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
+    if (bad != 0) {
+        const uint64_t odd_dq = odd_values(dq);
+        __threadfence();  // what is written again comes behind the rows' stores
+        while (bad != 0) {
+            const int r = __builtin_ctzll(bad);
+            bad &= bad - 1;
+            // Where a row's own lse or delta is no number, so is every ds of its pairs, and all of dq as it lies.
+            const float row_lse = i2f(readlane(f2i(lse), r)), row_delta = i2f(readlane(f2i(delta), r));
+            if (row_lse != kInf && (!finite(row_lse) || !finite(row_delta))) continue;
+            const int i = i0 + wave_row + r;
+            careful_query<T>(a, grad, b, h, i, row_lse == kInf ? 0 : len, row_lse, row_delta, i2f(readlane(f2i(share), r)),
+                             odd_value(odd_dq, r, lane), odd_value(odd_dq, r, lane + kWave),
+                             dq_out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D);
+        }
     }
     if (refine) delta += left(halves_sum(rest)) * share;
     if (row < a.Q && half == 0) {
@@ -693,13 +716,16 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         get_sums(other + 16 * kOut * kWave, dv, 1.f, 1.f);
     }
     // Key `key` of the block, formed again.
-    auto again = [&](int key, CarefulPair<T>& ck, CarefulPair<T>& cv) {
+    auto again = [&](int key, Needed need, CarefulPair<T>& ck, CarefulPair<T>& cv) {
+        const bool d0 = lane < a.D, d1 = lane + kWave < a.D;
+        need = {need.k0 && d0, need.k1 && d1, need.v0 && d0, need.v1 && d1};
         for (int hh = 0; hh < group; ++hh) {
             const int64_t before = static_cast<int64_t>(hh) * tiles;
             const int from = t_first + static_cast<int>(max(share_low - before, int64_t(0)));
             const int to = t_first + static_cast<int>(min(share_high - before, static_cast<int64_t>(tiles)));
-            careful_key<T>(a, grad, lse_in, delta_in, share_in, b, g * group + hh, j0 + key, i_low + from * TQ,
-                           min(i_low + to * TQ, i_high), FIRST, len, ck, cv);
+            if (careful_key<T>(a, grad, lse_in, delta_in, share_in, b, g * group + hh, j0 + key, i_low + from * TQ,
+                               min(i_low + to * TQ, i_high), FIRST, len, need, ck, cv))
+                break;
         }
     };
     // Keys behind the cloud's length have no gradient.
@@ -735,18 +761,29 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
         }
         __syncthreads();
         float* const dst = parts + static_cast<int64_t>(cut.kept()) * 2 * cut.rows * DP + static_cast<int64_t>(unit) * 2 * 32 * DP;
+        auto get = [&](int which, int key, int d) { return d < DP ? all[(32 * which + key) * kRow + d] : 0.f; };
+        auto set = [&](int which, int key, int d, float x) {
+            if (d < DP) dst[(32 * which + key) * DP + d] = x;
+        };
+        uint32_t bad = 0;
         for (int key = wave; key < 32; key += kWaves) {
+            const float k0 = get(0, key, lane), k1 = get(0, key, lane + kWave), v0 = get(1, key, lane), v1 = get(1, key, lane + kWave);
+            set(0, key, lane, k0), set(0, key, lane + kWave, k1), set(1, key, lane, v0), set(1, key, lane + kWave, v1);
+            if (ballot(!finite((k0 + k1) + (v0 + v1))) != 0) bad |= 1u << key;
+        }
+        if (bad == 0) return;
+        __threadfence();  // what is written again comes behind these stores
+        while (bad != 0) {
+            const int key = __builtin_ctz(bad);
+            bad &= bad - 1;
+            const Needed need = {!finite(get(0, key, lane)), !finite(get(0, key, lane + kWave)), !finite(get(1, key, lane)),
+                                 !finite(get(1, key, lane + kWave))};
             CarefulPair<T> ck, cv;
-            auto get = [&](int which, int d) { return d < DP ? all[(32 * which + key) * kRow + d] : 0.f; };
-            ck.x0 = get(0, lane), ck.x1 = get(0, lane + kWave), cv.x0 = get(1, lane), cv.x1 = get(1, lane + kWave);
-            if (!ck.finite() || !cv.finite()) {
-                ck = cv = CarefulPair<T>{};
-                if (j0 + key < exist) again(key, ck, cv);
-            }
-            auto set = [&](int which, int d, float x) {
-                if (d < DP) dst[(32 * which + key) * DP + d] = x;
-            };
-            set(0, lane, ck.x0), set(0, lane + kWave, ck.x1), set(1, lane, cv.x0), set(1, lane + kWave, cv.x1);
+            if (j0 + key < exist) again(key, need, ck, cv);
+            if (need.k0) set(0, key, lane, ck.x0);
+            if (need.k1) set(0, key, lane + kWave, ck.x1);
+            if (need.v0) set(1, key, lane, cv.x0);
+            if (need.v1) set(1, key, lane + kWave, cv.x1);
         }
         return;
     }
@@ -756,43 +793,47 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
     // (unit, dk or dv, key of the block, DP), or the results.
     float* const dst = parts + (static_cast<int64_t>(unit) * 2 * kRows + (j - j0)) * DP;
     const int64_t to = ((static_cast<int64_t>(b) * a.N + j) * a.G + g) * a.D;
-    if ((bad >> (lane % 32) & 1) == 0) {
-        if (parted) {
+    if (parted) {
 #pragma unroll
-            for (int d = 0; d < kOut; ++d)
+        for (int d = 0; d < kOut; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    store4<float, true>(dst, 32 * d + 8 * e + 4 * half, DP, dk[d], 4 * e);
-                    store4<float, true>(dst + kRows * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
-                }
-        } else if (j < a.N) {
+            for (int e = 0; e < 4; ++e) {
+                store4<float, true>(dst, 32 * d + 8 * e + 4 * half, DP, dk[d], 4 * e);
+                store4<float, true>(dst + kRows * DP, 32 * d + 8 * e + 4 * half, DP, dv[d], 4 * e);
+            }
+    } else if (j < a.N) {
 #pragma unroll
-            for (int d = 0; d < kOut; ++d)
+        for (int d = 0; d < kOut; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    store4<T, VEC>(dk_out + to, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
-                    store4<T, VEC>(dv_out + to, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
-                }
-        }
+            for (int e = 0; e < 4; ++e) {
+                store4<T, VEC>(dk_out + to, 32 * d + 8 * e + 4 * half, a.D, dk[d], 4 * e);
+                store4<T, VEC>(dv_out + to, 32 * d + 8 * e + 4 * half, a.D, dv[d], 4 * e);
+            }
     }
+    if (bad == 0) return;
+    const uint64_t odd_k = odd_values(dk), odd_v = odd_values(dv);
+    __threadfence();  // what is written again comes behind the keys' stores
     while (bad != 0) {
         const int r = __builtin_ctzll(bad);
         bad &= bad - 1;
         const int key = w0 - j0 + r;
+        const Needed need = {odd_value(odd_k, r, lane), odd_value(odd_k, r, lane + kWave), odd_value(odd_v, r, lane),
+                             odd_value(odd_v, r, lane + kWave)};
         CarefulPair<T> ck, cv;
-        again(key, ck, cv);
+        again(key, need, ck, cv);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int d = lane + x * kWave;
             const float yk = x == 0 ? ck.x0 : ck.x1, yv = x == 0 ? cv.x0 : cv.x1;
+            const bool nk = x == 0 ? need.k0 : need.k1, nv = x == 0 ? need.v0 : need.v1;
             if (parted && d < DP) {
                 float* const at = parts + (static_cast<int64_t>(unit) * 2 * kRows + key) * DP + d;
-                at[0] = yk;
-                at[kRows * DP] = yv;
+                if (nk) at[0] = yk;
+                if (nv) at[kRows * DP] = yv;
             } else if (!parted && d < a.D) {
                 const int64_t at = ((static_cast<int64_t>(b) * a.N + j0 + key) * a.G + g) * a.D + d;
-                dk_out[at] = from_float<T>(yk);
-                dv_out[at] = from_float<T>(yv);
+                if (nk) dk_out[at] = from_float<T>(yk);
+                if (nv) dv_out[at] = from_float<T>(yv);
             }
         }
     }

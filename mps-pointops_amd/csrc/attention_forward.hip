@@ -60,22 +60,28 @@ bool read_args(const pointops_attention* in, Args* out) {
 
 namespace {
 
+// n0, n1: whether this lane's columns are needed; whole: so is lse (else it stays, as
+// the sum of the weights has not met masked pairs).
 template <typename T>
-__device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, int len, const float* table,
-                                            T* out, float* lse) {
+__device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, int len, const float* table, bool whole,
+                                            bool n0, bool n1, T* out, float* lse) {
     const int lane = lane_id(), p = i + a.N - a.Q;
     const Seen seen = seen_by(a, p, len);
     CarefulRow<T> row(a, b, h / (a.H / a.G), a.q.at<T>(b, h) + i * a.q.n);
-    auto key = [&](int j) {
+    n0 = n0 && row.d0;
+    n1 = n1 && row.d1;
+    auto settled = [&](int j) {
         const int off = min(max(p - j, -a.reach), a.reach);
         row.add(j, a.bias != nullptr ? table[off + a.reach + kMargin] : 0.f);
+        return whole ? row.l != row.l : row.settled(n0, n1);  // (then all that follows is NaN)
     };
-    for (int j = 0; j < seen.first; ++j) key(j);
-    for (int j = max(seen.low, seen.first); j < seen.low + seen.count; ++j) key(j);
+    bool done = false;
+    for (int j = 0; j < seen.first && !done; ++j) done = settled(j);
+    for (int j = max(seen.low, seen.first); j < seen.low + seen.count && !done; ++j) done = settled(j);
     const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
-    if (row.d0) out[lane] = from_float<T>(row.o0 * inv);
-    if (row.d1) out[lane + kWave] = from_float<T>(row.o1 * inv);
-    if (lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
+    if (n0) out[lane] = from_float<T>(row.o0 * inv);
+    if (n1) out[lane + kWave] = from_float<T>(row.o1 * inv);
+    if (whole && lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
 }
 
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
         }
     uint64_t bad = ballot(row < a.Q && odd != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
-    if (row < a.Q && (bad >> (lane % 32) & 1) == 0) {
+    if (row < a.Q) {
         T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row) * a.H + h) * a.D;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
@@ -270,11 +276,24 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) > 384 ? 1 : 2) void attent
             for (int e = 0; e < 4; ++e) store4<T, VEC>(dst, 32 * d + 8 * e + 4 * half, a.D, o[d], 4 * e);
         if (half == 0 && lse_out != nullptr) lse_out[(static_cast<int64_t>(b) * a.H + h) * a.Q + row] = lse;
     }
+    if (bad == 0) return;
+    // A sum of weights that is NaN comes from a seen pair, and all of its row is NaN as it
+    // lies, but where a bias of -inf masks that pair.
+    bool masks = false;
+    if (biased)
+        for (int x = lane; x < bias_entries(a.reach); x += kWave) masks |= table[x] == -kInf;
+    masks = ballot(masks) != 0;
+    const uint64_t odd_o = odd_values(o);
+    __threadfence();  // what is written again comes behind the rows' stores
     while (bad != 0) {
         const int r = __builtin_ctzll(bad);
         bad &= bad - 1;
+        const float sum = i2f(readlane(f2i(l), r));
+        if (sum != sum && !masks) continue;
         const int i = i0 + wave_row + r;
-        careful_row<T>(a, b, h, i, len, table, out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D,
+        const bool whole = sum != sum;
+        careful_row<T>(a, b, h, i, sum == 0.f ? 0 : len, table, whole, whole || odd_value(odd_o, r, lane),
+                       whole || odd_value(odd_o, r, lane + kWave), out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D,
                        lse_out == nullptr ? nullptr : lse_out + (static_cast<int64_t>(b) * a.H + h) * a.Q + i);
     }
 }

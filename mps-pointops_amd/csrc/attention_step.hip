@@ -215,16 +215,33 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
         float x0 = lane < a.D ? sums[row * kSumStride + lane] : 0.f;
         float x1 = lane + kWave < a.D ? sums[row * kSumStride + lane + kWave] : 0.f;
         float lm = tops[0][row], ll = totals[0][row];
-        if (ballot(x0 * 0.f + x1 * 0.f + ll * 0.f != 0.f) != 0) {
+        // A sum of weights that is NaN comes from a seen pair, and all of its row is NaN as it
+        // lies, but where a bias of -inf masks that pair.
+        const bool whole = ll != ll;
+        bool masks = false;
+        if (whole && biased)
+            for (int x = lane; x < a.bk.count; x += kWave) masks |= table[x * kTile + row] == -kInf;
+        const bool n0 = whole || !finite(x0), n1 = whole || !finite(x1);
+        if (ll == 0.f) {
+            x0 = x1 = 0.f;
+        } else if (whole ? ballot(masks) != 0 : ballot(n0 || n1) != 0) {
             CarefulRow<T> c(a, b, g, a.q.at<T>(b, hh) + ii * a.q.n);
             const Seen sees = seen_by(a, shift + ii, len);
-            for (int t = begin; t < end; ++t)
-                for (int j = tiles.key(t); j < tiles.key(t) + kTile; ++j)
-                    if (sees(j)) c.add(j, biased ? bias_at(shift + ii - j, row) : 0.f);
-            x0 = c.o0;
-            x1 = c.o1;
-            lm = c.m;
-            ll = c.l;
+            bool done = false;
+            for (int t = begin; t < end && !done; ++t)
+                for (int j = tiles.key(t); j < tiles.key(t) + kTile && !done; ++j)
+                    if (sees(j)) {
+                        c.add(j, biased ? bias_at(shift + ii - j, row) : 0.f);
+                        done = whole ? c.l != c.l : c.settled(n0, n1);
+                    }
+            if (whole) {
+                lm = c.m;
+                ll = c.l;
+            }
+            // To the maximum of the products' sums.
+            const float by = whole ? 1.f : exp2_fast(c.m - lm);
+            x0 = n0 ? c.o0 * by : x0;
+            x1 = n1 ? c.o1 * by : x1;
         }
         if (splits == 1) {
             const float inv = ll == 0.f ? 0.f : 1.f / ll;
