@@ -186,6 +186,15 @@ struct Tile {
 // for LDS (at one wave a SIMD that was two thirds of the time).
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
 
+// Between a wave's stores to LDS and its other lanes' reads of them (or the next
+// stores): the hardware keeps a wave's LDS accesses in order, and neither the compiler's
+// memory passes nor its scheduler may change it.  No instruction.
+__device__ __forceinline__ void lanes_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Row operands of a tile's rows row0 .. row0 + 31, all chunks.
 template <typename T, int DP>
 struct RowFrags {

@@ -665,10 +665,12 @@ __global__ __launch_bounds__(kThreads, DP * sizeof(T) <= 128 ? 2 : 1) void atten
                                     *reinterpret_cast<f32x4*>(skew + lane % 16 * kSkewRow + 8 * e + 4 * half) =
                                         f32x4{ds[4 * e], ds[4 * e + 1], ds[4 * e + 2], ds[4 * e + 3]};
                             }
+                            lanes_exchange();
                             float all[4] = {};
 #pragma unroll
                             for (int r = 0; r < 16; ++r) all[r % 4] += skew[r * (kSkewRow + 1) + lane - 16];
                             mine[near + own - 16 * x + lane - 16 + a.reach + kMargin] += (all[0] + all[1]) + (all[2] + all[3]);
+                            lanes_exchange();
                         }
                     }
                 }

@@ -165,6 +165,7 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
             w[x] = exp2_fast(s[x] - base);
             l += w[x];
         }
+        lanes_exchange();
 #pragma unroll
         for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
             const i32x4 f = as_fragment<T>(&w[c * kPerFrag<T>]);
@@ -172,6 +173,7 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
             for (int d = 0; d < kOut; ++d)
                 o[d] = mma<T>(TileT::columns(vtile, c * TileT::kRowsPerFrag, 32 * d), f, o[d]);
         }
+        lanes_exchange();
     }
     l = halves_sum(l);
 
