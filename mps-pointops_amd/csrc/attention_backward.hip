@@ -122,7 +122,9 @@ __device__ __forceinline__ bool careful_key(const Args& a, const Rows& grad, con
 // rounding to 16 bits then takes as much from dq, through delta, as dq's own
 // (dq's error against 64 bits at 9 x 30 queries, 6 heads of 20, float16: 1.64
 // times a rounding's with it, 1.43 without).  Beyond this many keys the output is
-// an average of many, and the pass over them is not made twice.
+// an average of many, and the pass over them is not made twice.  (With a bias, whose
+// sums are small beside their terms, dk and the bias take delta with what the pass over
+// the keys measured: `refine`, whether or not the bias's gradient is asked for.)
 constexpr int kFewKeys = 128;
 
 // The most keys that a row up to position p_last sees.
@@ -965,7 +967,7 @@ hipError_t launch_backward(const Args& a, const Grads& x, hipStream_t stream) {
             if (err != hipSuccess) return err;
         }
         hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid_q)), dim3(kThreads), lds, stream, a,
-                           static_cast<const T*>(x.out), x.lse, x.grad, delta, share, coarse, static_cast<T*>(x.dq), dbias_part != nullptr);
+                           static_cast<const T*>(x.out), x.lse, x.grad, delta, share, coarse, static_cast<T*>(x.dq), a.bias != nullptr);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
