@@ -9,6 +9,12 @@
 // piece of LDS (for the transposing read), without a barrier in the loop.  The
 // keys are split over the block's waves and, where the batch is small, over
 // blocks, whose maxima, sums and outputs (32-bit) a second kernel joins.
+//
+// As the products wait for memory, 16-bit weights keep their bits: values are
+// multiplied by the rounded weights and by what the rounding left, so that outputs
+// carry the result's rounding alone (bfloat16, error against 64 bits over one
+// rounding's: 1.35 -> 1.0; 4 x 65536 keys, 32 heads over 8 of 128, 166.8 -> 168.7 us,
+// 4 x 2048, 8 heads over 2 of 64, window 512, 12.1 -> 12.6).
 #include <algorithm>
 
 #include "attention.hpp"
@@ -169,9 +175,19 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
 #pragma unroll
         for (int c = 0; c < 16 / kPerFrag<T>; ++c) {
             const i32x4 f = as_fragment<T>(&w[c * kPerFrag<T>]);
+            i32x4 rest;
+            if constexpr (sizeof(T) == 2) {
+                float left[kPerFrag<T>];
 #pragma unroll
-            for (int d = 0; d < kOut; ++d)
-                o[d] = mma<T>(TileT::columns(vtile, c * TileT::kRowsPerFrag, 32 * d), f, o[d]);
+                for (int e = 0; e < kPerFrag<T>; ++e) left[e] = w[c * kPerFrag<T> + e] - element<T>(f, e);
+                rest = as_fragment<T>(left);
+            }
+#pragma unroll
+            for (int d = 0; d < kOut; ++d) {
+                const i32x4 values = TileT::columns(vtile, c * TileT::kRowsPerFrag, 32 * d);
+                o[d] = mma<T>(values, f, o[d]);
+                if constexpr (sizeof(T) == 2) o[d] = mma<T>(values, rest, o[d]);
+            }
         }
         lanes_exchange();
     }
