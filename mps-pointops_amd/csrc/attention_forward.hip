@@ -11,10 +11,12 @@
 // sums and outputs are 32-bit; the weights p are rounded to the values' type
 // for the second product, as its matrix instruction takes them.
 //
-// Bound by the products and the exponentials between them: 16384 queries, 8
-// heads over 2 of 128, window 2048, bfloat16, takes 170 us, 763 T/s of the pairs
-// seen (a large library product: 1204); every earlier key at 2 x 4096 queries, 8
-// heads of 128, 128 us.  32 queries a wave keep their output and operands in
+// Bound by the operands' reads from LDS and the products, which take as long as each
+// other and of which two waves a SIMD overlap a part: the matrix cores are busy for
+// 37 % of a compute unit's busy cycles, LDS for 37 % (every earlier key: 33 and 33 %).
+// 16384 queries, 8 heads over 2 of 128, window 2048, bfloat16, takes 170 to 177 us, 733
+// to 765 T/s of the pairs seen (a large library product: 1204); every earlier key at 2 x
+// 4096 queries, 8 heads of 128, 118 to 128 us.  32 queries a wave keep their output and operands in
 // registers beside a whole tile's scores; with the tiles in two LDS buffers one
 // barrier a tile is left.
 #include "attention.hpp"

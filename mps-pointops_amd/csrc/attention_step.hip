@@ -337,7 +337,9 @@ struct Plan {
 };
 
 // Splits of the keys that give every compute unit four blocks, with at least
-// two tiles a wave.
+// two tiles a wave.  By the cache's size: the lengths are on the device, and a call
+// does not wait for it (4 clouds of 500 tokens, 32 heads over 8 of 128: 24 us in a cache
+// of 65536, 16 in one of 512).
 Plan plan_of(const Args& a, int type) {
     const int64_t rows = static_cast<int64_t>(a.Q) * (a.H / a.G), row_blocks = (rows + kTile - 1) / kTile;
     const int64_t all = (static_cast<int64_t>(a.N) + kTile - 1) / kTile;

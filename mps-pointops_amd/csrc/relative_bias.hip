@@ -76,7 +76,8 @@ constexpr int kDiagSpan = kThreads * kDiagonals;
 
 // kDiagonals values at any address, read past the caches' order of use: what
 // the forward has just written fills them, and the gradient is read once (16 x
-// 2048 x 2048, float32, aligned rows: 87 us with ordinary loads, 52 = 5.2 TB/s).
+// 2048 x 2048, float32, aligned rows: 87 us with ordinary loads, 52 with these; 48 =
+// 5.5 TB/s since the buckets' bounds come from LDS).
 template <typename T>
 struct Values {
     T e[kDiagonals];
@@ -129,8 +130,8 @@ __global__ __launch_bounds__(kThreads) void relative_bias_grad_kernel(const Buck
 // The same where every row starts at a multiple of 16 bytes: a thread reads
 // aligned pieces of V values, the same columns for V rows and V columns further
 // for the next V, so that 2 V - 1 diagonals stay in its registers; its
-// neighbour's share of them is added at the end.  16 x 2048 x 2048, float32: 60 us
-// by the kernel above, by this one 52.
+// neighbour's share of them is added at the end.  16 x 2048 x 2048, float32: 48 us,
+// where the kernel above took 60 to this one's 52.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void relative_bias_grad_aligned_kernel(const Buckets bk, const T* __restrict__ grad,
                                                                               int64_t stride_h, int64_t stride_i,
