@@ -94,3 +94,14 @@ def test_other_calls_leave_the_function_out(launches, monkeypatch, name):
     shapes, call = CALLS[name]
     call(*(shape(*s) for s in shapes))
     assert len(launches) == 1
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_transforms_are_refused(launches, name):
+    shapes, call = CALLS[name]
+    args = tuple(torch.zeros(3, *s) for s in shapes)
+    with pytest.raises(RuntimeError):
+        torch.vmap(call)(*args)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.grad(lambda x, *rest: outputs(call(x, *rest))[0].sum())(*(shape(*s) for s in shapes))
+    assert not launches
