@@ -131,6 +131,14 @@ __device__ __forceinline__ bool careful_key(const Args& a, const Rows& grad, con
 // the keys measured: `refine`, whether or not the bias's gradient is asked for.)
 constexpr int kFewKeys = 128;
 
+// A row's ds add up to zero, and in heads of few columns dq cancels the more by it: with
+// ds rounded, its error is 1.45 to 1.6 times one rounding's at widths 16 to 24 (1.41 to
+// 1.46 from 32 on).  There the second product is made again with what the rounding
+// left (16-bit types; 1.1 times; 462 queries over 924 keys, 3 x 6 heads of 20: 23.2 ->
+// 24.5 us of the kernel by queries).  Width 32 would pay 36.3 -> 44.8 us for it (4 x
+// 4096 queries, 8 heads over 2, window 512).
+constexpr int kNarrow = 24;
+
 // The most keys that a row up to position p_last sees.
 __device__ __forceinline__ int most_seen(const Args& a, int p_last, int len) {
     const int side = min(a.window, kFewKeys + 1), first = min(a.sinks, kFewKeys + 1);
@@ -246,6 +254,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
     // rounded output took from delta: of few keys a pass ahead measures it.
     // (Of a row beside a place that is no number it cannot be told.)
     auto left = [](float all) { return all - all == 0.f ? all : 0.f; };
+    const bool narrow = a.D <= kNarrow;
     const float factor = biased ? 1.f : a.scale_log2;
     f32x16 dq[kOut] = {};
     char* ktile = lds;
@@ -312,7 +321,14 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && DP > 64) ? 1 : 2) void
                 for (int c = 0; c < kSteps; ++c) {
                     if (c + 1 < kSteps) cf[(c + 1) % 2].load(ktile, own + (c + 1) * TileT::kRowsPerFrag);
                     keep_order();
-                    cf[c % 2].add(as_fragment<T>(&ds[c * kPerFrag<T>]), dq);
+                    const i32x4 x = as_fragment<T>(&ds[c * kPerFrag<T>]);
+                    cf[c % 2].add(x, dq);
+                    if (sizeof(T) == 2 && DP == 32 && narrow) {
+                        float rounded[kPerFrag<T>];
+#pragma unroll
+                        for (int e = 0; e < kPerFrag<T>; ++e) rounded[e] = ds[c * kPerFrag<T> + e] - element<T>(x, e);
+                        cf[c % 2].add(as_fragment<T>(rounded), dq);
+                    }
                 }
             }
         }
