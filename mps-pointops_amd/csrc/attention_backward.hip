@@ -96,13 +96,33 @@ __device__ __forceinline__ bool careful_key(const Args& a, const Rows& grad, con
                                             int len, const Needed& need, CarefulPair<T>& dk, CarefulPair<T>& dv) {
     const int g = h / (a.H / a.G);
     const int64_t stats = (static_cast<int64_t>(b) * a.H + h) * a.Q;
+    auto settled = [&] {
+        return ballot((need.k0 && finite(dk.x0)) || (need.k1 && finite(dk.x1)) || (need.v0 && finite(dv.x0)) ||
+                      (need.v1 && finite(dv.x1))) == 0;
+    };
+    auto sees = [&](int64_t i) {
+        const int off = static_cast<int>(i) + a.N - a.Q - static_cast<int>(j);
+        return !(a.causal && off < 0) && ((off < 0 ? -off : off) < a.window) != beyond;
+    };
+    // A row whose lse is no number makes all of a key that it sees none, one whose delta
+    // is not finite its dk: 64 rows at a time.
+    bool odd_lse = false, odd_delta = false;
+    for (int64_t i = i_from + lane_id(); i < i_to; i += kWave) {
+        const float lse = lse_in[stats + i], delta = delta_in[stats + i];
+        if ((lse == lse && finite(delta)) || lse == kInf || !sees(i)) continue;
+        if (one_bias<T>(a, h, static_cast<int>(i) + a.N - a.Q - static_cast<int>(j)) == -kInf) continue;
+        odd_lse |= lse != lse;
+        odd_delta = true;
+    }
+    if (ballot(odd_delta) != 0) dk.x0 = dk.x1 = __builtin_nanf("");
+    if (ballot(odd_lse) != 0) dv.x0 = dv.x1 = __builtin_nanf("");
+    if (settled()) return true;
     CarefulPair<T> k, v;
     k.load(a.k.at<T>(b, g) + j * a.k.n, a.D);
     v.load(a.v.at<T>(b, g) + j * a.v.n, a.D);
     for (int64_t i = i_from; i < i_to; ++i) {
-        const int p = static_cast<int>(i) + a.N - a.Q, off = p - static_cast<int>(j);
-        const bool within = (off < 0 ? -off : off) < a.window;
-        if ((a.causal && off < 0) || within == beyond) continue;
+        if (!sees(i)) continue;
+        const int off = static_cast<int>(i) + a.N - a.Q - static_cast<int>(j);
         const float lse = lse_in[stats + i];
         if (lse == kInf) continue;
         const float bias = one_bias<T>(a, h, off);
@@ -115,9 +135,7 @@ __device__ __forceinline__ bool careful_key(const Args& a, const Rows& grad, con
         const float w = exp2_fast(s - lse) * share_in[stats + i];
         dv.add(w, go);
         dk.add(w * (go.dot(v) - delta_in[stats + i]) * a.scale, q);
-        if (ballot((need.k0 && finite(dk.x0)) || (need.k1 && finite(dk.x1)) || (need.v0 && finite(dv.x0)) ||
-                   (need.v1 && finite(dv.x1))) == 0)
-            return true;
+        if (settled()) return true;
     }
     return false;
 }

@@ -89,3 +89,42 @@ def test_times(cuda_device, kind, biased, sinks):
         took, results = best(step, *[torch.full_like(t, value) for t in (q, k, v, g)])
         assert took < 10 * usual + 0.5
         assert not torch.isfinite(results[0]).any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_one_token(cuda_device, kind, biased):
+    """A NaN token in the middle, with a finite gradient: all that meets it is NaN,
+    which is found without going through the pairs before it; what does not keeps its
+    values, those of the clouds without it."""
+    from mps_pointops.attention import window_attention
+
+    N, at = 4096, 2048
+    q, k, v, g, bias = tensors(63, 1, N, N, 4, 2, 64, TYPES[kind], 16 if biased else 0)
+    how = dict(bias=bias, max_distance=100 if biased else None, causal=True)
+
+    def train(*tensors):
+        leaves = [t.detach().requires_grad_() for t in tensors]
+        out = window_attention(*leaves, **how)
+        return out, *torch.autograd.grad(out, leaves, g)
+
+    def best(*tensors):
+        times = []
+        for _ in range(4):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            results = train(*tensors)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times[1:]), results
+
+    usual, whole = best(q, k, v)
+    for t in (q, k, v):
+        t[:, at] = math.nan
+    took, got = best(q, k, v)
+    assert took < 10 * usual + 0.5, (took, usual)
+    for x, y in zip(got[:2], whole):  # rows before it do not see it
+        assert torch.isnan(x[:, at:]).all()
+        assert (x[:, :at].double() - y[:, :at].double()).norm() <= LIMIT[kind] * y[:, :at].double().norm()
+    assert torch.isnan(got[2]).all() and torch.isnan(got[3]).all()  # every key is seen by its row or a later one
