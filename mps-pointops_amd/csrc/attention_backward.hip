@@ -20,9 +20,9 @@
 // Bound by the matrix products (18 D operations a pair, with the scores' second
 // forming) and, as long, by their operands' reads from LDS, with the vector
 // instructions of the weights between them.  Every earlier key at 2 x 4096 queries, 8
-// heads of 128, bfloat16: dq 150 us, dk and dv 234, the forward 123, each as traced; all
-// three pass in 495 (240 billion operations of the definition, 486 T/s; a large library
-// product reaches 1204).  Matrix cores and LDS are each busy for 39 and 33 % of a
+// heads of 128, bfloat16: dq 150 us, dk and dv 240, the forward 123, each as traced; a
+// pass of all three takes 495 to 502 (240 billion operations of the definition, 480 to
+// 486 T/s; a large library product reaches 1204).  Matrix cores and LDS are each busy for 39 and 33 % of a
 // compute unit's busy cycles in dq, 33 and 34 in dk and dv (one wave a SIMD at width
 // 128, two at 64).  Registers that do not fit: 6 to 16 in the key kernel of width 64
 // with a bias, 5 to 12 in the query kernel of width 128 with one.
