@@ -584,6 +584,76 @@ size_t pointops_attention_step_workspace_bytes(const pointops_attention *in);
 hipError_t pointops_attention_step(const pointops_attention *in, void *out, void *workspace,
                                    hipStream_t stream);
 
+/* A cache of keys and values in 8 or 4 bits, given by a HOST pointer: a row of D <=
+ * 128 values is P * bits / 8 bytes of codes (P: D rounded up to a multiple of 32, codes
+ * behind D zero) and P / 32 bytes of scales, rows of a key head one behind the other;
+ * batch_stride and head_stride count rows, in codes and scales alike.  k and v are
+ * multiples of 16, k_scales and v_scales of P / 32 where that is 2 or 4.
+ *
+ * Values v of a group of 32 (the last may be shorter) have the scale X = 2^x, the
+ * smallest x >= -127 with max |v| <= M X, held as the byte x + 127, and codes v / X
+ * rounded to the nearest value of the type, to even codes at ties: bits = 8: E4M3
+ * (M = 448), bits = 4: E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6; M = 6; value 2 i in the low
+ * half of byte i).  A group with an infinity or NaN has the byte 255 and reads as NaN. */
+typedef struct {
+    void *k, *v;
+    uint8_t *k_scales, *v_scales;
+    int64_t batch_stride, head_stride;
+    int64_t B, N, G, D;
+    int32_t bits;
+} pointops_cache;
+
+/* Writes `tokens` rows of k and v (B, tokens, G, D) of `type`, strides of batch, token
+ * and head in elements, D contiguous: token t of sequence b to position starts[b] + t
+ * where that lies in [0, lengths[b]); all else stays as it is.  lengths and starts: int32
+ * or int64 (their *_bits), B values; lengths NULL: N (values are clamped to [0, N]);
+ * starts NULL: lengths[b] - tokens. */
+hipError_t pointops_cache_write(const pointops_cache *cache, const void *k,
+                                const int64_t *k_stride, const void *v, const int64_t *v_stride,
+                                int64_t tokens, const void *lengths, int32_t length_bits,
+                                const void *starts, int32_t start_bits, int32_t type,
+                                hipStream_t stream);
+
+/* The whole cache as k and v (B, N, G, D) of `type`, contiguous, each value rounded once. */
+hipError_t pointops_cache_read(const pointops_cache *cache, void *k, void *v, int32_t type,
+                               hipStream_t stream);
+
+/* Keys and values that a step reads: rows of its type, strides of batch, token and head
+ * in elements, or (scales not NULL) those of a pointops_cache, k_stride = {batch_stride,
+ * 1, head_stride} in rows.  N = 0: none. */
+typedef struct {
+    const void *k, *v;
+    const uint8_t *k_scales, *v_scales;
+    int64_t k_stride[3], v_stride[3];
+    int64_t N;
+} pointops_keys;
+
+/* Attention of the last Q tokens of each sequence over what is kept of it, given by a HOST
+ * pointer: first the `start`'s keys, common to all sequences (its batch strides are not
+ * read), then its own, the first lengths[b] of `own` (int32 or int64; NULL: all; clamped
+ * to [0, own.N]).  As pointops_attention_step over both one behind the other, with
+ * lengths start.N + lengths[b]; q (B, Q, H, D), window, sinks, bias and edges as there.
+ * `bits`: 0 (rows of `type`), 8 or 4, of both. */
+typedef struct {
+    const void *q;
+    pointops_keys start, own;
+    const void *bias;
+    const void *lengths;
+    const int32_t *edges;
+    int64_t q_stride[3];
+    int64_t B, Q, H, G, D;
+    int64_t window, sinks;
+    int32_t n_edges, buckets, length_bits, type, bits;
+    float scale;
+} pointops_cache_attention;
+
+/* out (B, Q, H, D) contiguous; `workspace` holds
+ * pointops_cache_attention_step_workspace_bytes(in) bytes at a multiple of 16 (NULL where
+ * that is 0). */
+size_t pointops_cache_attention_step_workspace_bytes(const pointops_cache_attention *in);
+hipError_t pointops_cache_attention_step(const pointops_cache_attention *in, void *out,
+                                         void *workspace, hipStream_t stream);
+
 /* The bias as a dense tensor: out[h][i][j] = table[bucket(N - Q + i - j)][h],
  * (H, Q, N) contiguous; table (buckets, H) contiguous, edges and buckets as in
  * pointops_attention, but edges up to 2^30.  Q <= 4194240, N < 2^22, H <= 65535. */

@@ -1,0 +1,9 @@
+// Attention over caches in the tokens' own type, f16.
+#include "attention_cache.hpp"
+
+namespace pointops {
+namespace attn {
+template hipError_t launch_cache_form<f16, kAligned>(const CacheArgs&, const CachePlan&, void*, float*, hipStream_t);
+template hipError_t launch_cache_form<f16, kAny>(const CacheArgs&, const CachePlan&, void*, float*, hipStream_t);
+}  // namespace attn
+}  // namespace pointops

@@ -1,0 +1,259 @@
+// A cache in 8 or 4 bits: writing new tokens to it and reading it back.
+//
+// Both are bound by memory.  Four neighbouring lanes hold a group of 32 values,
+// eight each (16 bytes of a 16-bit type), and find its scale among themselves;
+// neighbouring lanes are pieces of a row, then the tokens behind it, so that codes
+// are written and read in whole lines (rows of 64 bytes for 4 bits and 128 values).
+#include "quantized_cache.hpp"
+
+namespace pointops {
+namespace attn {
+namespace {
+
+// One side (keys, values) of the cache and of the tokens.
+struct Side {
+    const void* rows;   // of the tokens, strides in elements
+    int64_t b, n, h;
+    uint8_t *codes, *scales;
+};
+
+struct CacheCall {
+    Side side[2];
+    const void *lengths, *starts;
+    int length_bits, start_bits;
+    int64_t cache_b, cache_h;  // strides of the cache, in rows
+    int B, G, D, N, T;         // T: tokens of the call
+    bool vec;                  // rows at multiples of 16 bytes, D a multiple of 8
+};
+
+__device__ __forceinline__ int64_t value_at(const void* p, int bits, int b) {
+    return bits == 64 ? static_cast<const int64_t*>(p)[b] : static_cast<const int32_t*>(p)[b];
+}
+
+// Lanes of a row of D values, eight each, a whole number of groups.
+__host__ __device__ constexpr int lanes_of(int D) { return padded(D) / 8; }
+
+struct Piece {
+    int side, b, g, t, at;  // at: the first of its eight values
+    bool any;
+};
+
+// A block's pieces: 256 in a row's lanes, then tokens, of one key head.
+__device__ __forceinline__ Piece piece_of(const CacheCall& c, int tokens, uint32_t blocks) {
+    const uint32_t chunk = blockIdx.x % blocks, unit = blockIdx.x / blocks;
+    const int lanes = lanes_of(c.D);
+    const int64_t at = static_cast<int64_t>(chunk) * kThreads + threadIdx.x;
+    Piece p;
+    p.t = static_cast<int>(at / lanes);
+    p.at = static_cast<int>(at % lanes) * 8;
+    p.any = p.t < tokens;
+    p.side = static_cast<int>(unit % 2);
+    p.g = static_cast<int>(unit / 2 % c.G);
+    p.b = static_cast<int>(unit / 2 / c.G);
+    return p;
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheCall c, uint32_t blocks) {
+    const Piece p = piece_of(c, c.T, blocks);
+    const Side& s = c.side[p.side];
+    int64_t length = c.N;
+    if (c.lengths != nullptr) length = min(max(value_at(c.lengths, c.length_bits, p.b), int64_t(0)), int64_t(c.N));
+    // (A start that far off leaves nothing to write, and none of its sums passes 64 bits.)
+    int64_t start = length - c.T;
+    if (c.starts != nullptr) start = min(max(value_at(c.starts, c.start_bits, p.b), -int64_t(c.T)), int64_t(c.N));
+    const int64_t place = start + p.t;
+    const bool here = p.any && place >= 0 && place < length;  // of a row's lanes all or none
+
+    float x[8];
+    const T* const row = static_cast<const T*>(s.rows) + p.b * s.b + p.t * s.n + p.g * s.h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    if (here) {
+        if (c.vec) {
+            if (p.at < c.D) {
+                T piece[8];
+                __builtin_memcpy(piece, __builtin_assume_aligned(row + p.at, 16), sizeof piece);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = to_float(piece[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (p.at + e < c.D) x[e] = to_float(row[p.at + e]);
+        }
+    }
+    // As whole numbers, magnitudes are in their order, infinity and NaN above all.
+    int most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, f2i(x[e]) & 0x7fffffff);
+    most = max(most, dpp<kDppQuadXor1>(most));
+    most = max(most, dpp<kDppQuadXor2>(most));
+    if (!here) return;
+    const uint32_t byte = scale_byte<BITS>(i2f(most));
+    // The codes of a group that is no number are zeros: its scale says so.
+    const float scale = scale_of(byte);
+    const int64_t at = p.b * c.cache_b + p.g * c.cache_h + place;
+    if constexpr (BITS == 8) {
+        s16x2 low = {0, 0}, high = {0, 0};
+        if (byte != kNoNumber) {
+            low = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(low, x[0], x[1], scale, false);
+            low = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(low, x[2], x[3], scale, true);
+            high = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(high, x[4], x[5], scale, false);
+            high = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(high, x[6], x[7], scale, true);
+        }
+        *reinterpret_cast<i32x2*>(s.codes + at * padded(c.D) + p.at) =
+            i32x2{__builtin_bit_cast(int, low), __builtin_bit_cast(int, high)};
+    } else {
+        uint32_t codes = 0;
+        if (byte != kNoNumber) {
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+        }
+        *reinterpret_cast<uint32_t*>(s.codes + at * (padded(c.D) / 2) + p.at / 2) = codes;
+    }
+    if (p.at % kGroup == 0) s.scales[at * (padded(c.D) / kGroup) + p.at / kGroup] = static_cast<uint8_t>(byte);
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(const CacheCall c, T* __restrict__ k, T* __restrict__ v,
+                                                              uint32_t blocks) {
+    const Piece p = piece_of(c, c.N, blocks);
+    if (!p.any || p.at >= c.D) return;
+    const Side& s = c.side[p.side];
+    const int64_t at = p.b * c.cache_b + p.g * c.cache_h + p.t;
+    const float scale = scale_of(s.scales[at * (padded(c.D) / kGroup) + p.at / kGroup]);
+    f32x2 x[4];
+    if constexpr (BITS == 8) {
+        const i32x2 codes = *reinterpret_cast<const i32x2*>(s.codes + at * padded(c.D) + p.at);
+        x[0] = decode<8, 0>(codes[0], scale);
+        x[1] = decode<8, 1>(codes[0], scale);
+        x[2] = decode<8, 0>(codes[1], scale);
+        x[3] = decode<8, 1>(codes[1], scale);
+    } else {
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(s.codes + at * (padded(c.D) / 2) + p.at / 2);
+        x[0] = decode<4, 0>(codes, scale);
+        x[1] = decode<4, 1>(codes, scale);
+        x[2] = decode<4, 2>(codes, scale);
+        x[3] = decode<4, 3>(codes, scale);
+    }
+    T piece[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) piece[e] = from_float<T>(x[e / 2][e % 2]);
+    T* const row = (p.side == 0 ? k : v) + ((static_cast<int64_t>(p.b) * c.N + p.t) * c.G + p.g) * c.D + p.at;
+    if (c.vec) {
+        __builtin_memcpy(__builtin_assume_aligned(row, 16), piece, sizeof piece);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (p.at + e < c.D) row[e] = piece[e];
+    }
+}
+
+bool read_cache(const pointops_cache* in, CacheCall* c) {
+    const int64_t limit = (int64_t(1) << 30) - 1024;
+    if (in == nullptr || in->B < 0 || in->N < 0 || in->G < 0 || in->D < 1 || in->D > kMaxHead) return false;
+    if (in->B > limit || in->N > limit || in->G > limit || (in->bits != 8 && in->bits != 4)) return false;
+    c->side[0] = {nullptr, 0, 0, 0, static_cast<uint8_t*>(in->k), in->k_scales};
+    c->side[1] = {nullptr, 0, 0, 0, static_cast<uint8_t*>(in->v), in->v_scales};
+    c->lengths = c->starts = nullptr;
+    c->length_bits = c->start_bits = 0;
+    c->cache_b = in->batch_stride;
+    c->cache_h = in->head_stride;
+    c->B = static_cast<int>(in->B);
+    c->G = static_cast<int>(in->G);
+    c->D = static_cast<int>(in->D);
+    c->N = static_cast<int>(in->N);
+    c->T = 0;
+    c->vec = false;
+    return in->B == 0 || in->N == 0 || in->G == 0 ||
+           (in->k != nullptr && in->v != nullptr && in->k_scales != nullptr && in->v_scales != nullptr &&
+            codes_aligned(in->k, in->k_scales, c->D) && codes_aligned(in->v, in->v_scales, c->D));
+}
+
+// Blocks of one key head's tokens; false if the launch would not hold them all.
+bool blocks_of(const CacheCall& c, int tokens, uint32_t* each, uint32_t* all) {
+    const int64_t n = (static_cast<int64_t>(tokens) * lanes_of(c.D) + kThreads - 1) / kThreads;
+    const int64_t units = int64_t(2) * c.B * c.G;
+    if (units > INT32_MAX || n > INT32_MAX / units) return false;
+    *each = static_cast<uint32_t>(n);
+    *all = static_cast<uint32_t>(n * units);
+    return true;
+}
+
+template <typename F>
+hipError_t with_type(int32_t type, int bits, F f) {
+    auto of = [&](auto t) {
+        return bits == 8 ? f(t, std::integral_constant<int, 8>{}) : f(t, std::integral_constant<int, 4>{});
+    };
+    switch (type) {
+        case POINTOPS_F32: return of(float{});
+        case POINTOPS_F16: return of(f16{});
+        default: return of(bf16{});
+    }
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace attn
+}  // namespace pointops
+
+extern "C" {
+
+hipError_t pointops_cache_write(const pointops_cache* cache, const void* k, const int64_t* k_stride, const void* v,
+                                const int64_t* v_stride, int64_t tokens, const void* lengths, int32_t length_bits,
+                                const void* starts, int32_t start_bits, int32_t type, hipStream_t stream) {
+    using namespace pointops::attn;
+    CacheCall c;
+    if (!read_cache(cache, &c) || tokens < 0 || tokens > (int64_t(1) << 30) - 1024) return hipErrorInvalidValue;
+    if (type < POINTOPS_F32 || type > POINTOPS_BF16) return hipErrorInvalidValue;
+    if ((lengths != nullptr && length_bits != 32 && length_bits != 64) ||
+        (starts != nullptr && start_bits != 32 && start_bits != 64))
+        return hipErrorInvalidValue;
+    if (c.B == 0 || c.G == 0 || c.N == 0 || tokens == 0) return hipSuccess;
+    if (k == nullptr || v == nullptr || k_stride == nullptr || v_stride == nullptr) return hipErrorInvalidValue;
+    const int64_t per = 16 / (type == POINTOPS_F32 ? 4 : 2);
+    c.vec = aligned(k) && aligned(v) && c.D % 8 == 0;
+    for (int i = 0; i < 3; ++i) c.vec = c.vec && k_stride[i] % per == 0 && v_stride[i] % per == 0;
+    c.side[0].rows = k;
+    c.side[1].rows = v;
+    for (int i = 0; i < 2; ++i) {
+        const int64_t* const stride = i == 0 ? k_stride : v_stride;
+        c.side[i].b = stride[0];
+        c.side[i].n = stride[1];
+        c.side[i].h = stride[2];
+    }
+    c.lengths = lengths;
+    c.starts = starts;
+    c.length_bits = length_bits;
+    c.start_bits = start_bits;
+    c.T = static_cast<int>(tokens);
+    uint32_t each, all;
+    if (!blocks_of(c, c.T, &each, &all)) return hipErrorInvalidValue;
+    return with_type(type, cache->bits, [&](auto t, auto bits) {
+        hipLaunchKernelGGL((cache_write_kernel<decltype(t), decltype(bits)::value>), dim3(all), dim3(kThreads), 0, stream, c, each);
+        return hipGetLastError();
+    });
+}
+
+hipError_t pointops_cache_read(const pointops_cache* cache, void* k, void* v, int32_t type, hipStream_t stream) {
+    using namespace pointops::attn;
+    CacheCall c;
+    if (!read_cache(cache, &c) || type < POINTOPS_F32 || type > POINTOPS_BF16) return hipErrorInvalidValue;
+    if (c.B == 0 || c.G == 0 || c.N == 0) return hipSuccess;
+    if (k == nullptr || v == nullptr) return hipErrorInvalidValue;
+    c.vec = aligned(k) && aligned(v) && c.D % 8 == 0;
+    uint32_t each, all;
+    if (!blocks_of(c, c.N, &each, &all)) return hipErrorInvalidValue;
+    return with_type(type, cache->bits, [&](auto t, auto bits) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((cache_read_kernel<T, decltype(bits)::value>), dim3(all), dim3(kThreads), 0, stream, c,
+                           static_cast<T*>(k), static_cast<T*>(v), each);
+        return hipGetLastError();
+    });
+}
+
+}  // extern "C"

@@ -78,6 +78,9 @@ _SIGNATURES: dict[str, list] = {
     "pointops_attention_forward": [_vp, _vp, _vp, _vp],
     "pointops_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "pointops_attention_step": [_vp, _vp, _vp, _vp],
+    "pointops_cache_write": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _i32, _vp],
+    "pointops_cache_read": [_vp, _vp, _vp, _i32, _vp],
+    "pointops_cache_attention_step": [_vp, _vp, _vp, _vp],
     "pointops_relative_bias": [_vp, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp],
     "pointops_relative_bias_backward": [_vp, _i64, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i64, _i64,
                                         _i64, _vp],
@@ -107,6 +110,7 @@ _SIZE_QUERIES: dict[str, list] = {
     "pointops_group_points_backward_workspace_bytes": [_i64, _i64, _i64, _i64],
     "pointops_attention_backward_workspace_bytes": [_vp],
     "pointops_attention_step_workspace_bytes": [_vp],
+    "pointops_cache_attention_step_workspace_bytes": [_vp],
     "pointops_relative_bias_backward_workspace_bytes": [_i64, _i64, _i64, _i32],
     "pointops_qk_norm_rotate_backward_workspace_bytes": [_vp],
 }

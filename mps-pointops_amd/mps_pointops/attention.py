@@ -10,7 +10,11 @@ layer over such sequences asks for beside its matrix products:
 * ``window_attention_step``: the same for one or a few new tokens over a cache;
 * ``qk_norm_rotate``: the norm of each head's query and key and their rotation
   by the token's position in one pass, with its gradients;
-* ``relative_bias``: the learned bias as a dense tensor, with its gradient.
+* ``relative_bias``: the learned bias as a dense tensor, with its gradient;
+* ``QuantizedCache``, ``cache_write``, ``cache_read``: keys and values kept in 8
+  or 4 bits, and ``quantized_attention_step``, the step over them;
+* ``prefix_attention_step``: the step of a batch whose clouds continue one common
+  start, which is kept and read once for all.
 
 Tensors are (batch, tokens, heads, width) in float32, float16 or bfloat16 on
 ``device='cuda'``, with any strides; fewer key heads than query heads are
@@ -307,6 +311,319 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     return _step(*args) if _native.untraced() else _WindowAttentionStep.apply(*args)
 
 
+# ------------------------------------------------------------ quantized cache
+# pointops_cache, pointops_keys and pointops_cache_attention of pointops_hip.h.
+_CACHE = struct.Struct("@4Q6qi4x")
+_KEYS = struct.Struct("@4Q7q")
+_CACHE_ARGS = struct.Struct("@Q88s88s3Q3q5q2q5if")
+_GROUP = 32
+
+
+class QuantizedCache:
+    """Keys and values of ``batch`` clouds of up to ``tokens`` positions, in 8 or
+    4 bits a value.
+
+    Each row of ``width`` values (at most 128) of one of the ``heads`` key heads is
+    held as codes and a scale ``2 ** x`` for each 32 of them: the smallest one,
+    x >= -127, with which the group's largest magnitude is at most 448 (8 bits: 3
+    fraction bits, exponents from -6 to 8, even steps of 2 ** -9 below) or 6 (4 bits:
+    0, 0.5, 1, 1.5, 2, 3, 4, 6) times it.  Quotients are rounded to the nearest value,
+    to even codes at ties: by at most 1/16 of a value in 8 bits, 1/4 in 4 (below the
+    smallest exponents by half a step).  A group with an infinity or NaN reads as NaN.
+
+    ``k_codes, v_codes (batch, heads, tokens, bytes)`` and ``k_scales, v_scales (batch,
+    heads, tokens, groups)`` are uint8 and zeros (values of zero) at first; a row's
+    bytes are ``width`` rounded up to a multiple of 32, or half of that.
+    """
+
+    def __init__(self, batch: int, tokens: int, heads: int, width: int, *, bits: int = 8,
+                 device: torch.device | str = "cuda"):
+        if bits not in (8, 4):
+            raise ValueError("bits must be 8 or 4")
+        if not 1 <= width <= _MAX_HEAD:
+            raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
+        if min(batch, tokens, heads) < 0 or max(batch, tokens, heads) > _MAX_TOKENS:
+            raise ValueError(f"sizes must lie in [0, {_MAX_TOKENS}]")
+        self.width, self.bits = int(width), int(bits)
+        groups = -(-width // _GROUP)
+        self.k_codes, self.v_codes = (torch.zeros((batch, heads, tokens, groups * _GROUP * bits // 8), dtype=torch.uint8,
+                                                  device=device) for _ in range(2))
+        self.k_scales, self.v_scales = (torch.zeros((batch, heads, tokens, groups), dtype=torch.uint8, device=device)
+                                        for _ in range(2))
+
+    @property
+    def batch(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def heads(self) -> int:
+        return self.k_codes.shape[1]
+
+    @property
+    def tokens(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def device(self) -> torch.device:
+        return self.k_codes.device
+
+    def _view(self, dim: int, first: int, count: int) -> QuantizedCache:
+        if first < 0 or count < 0 or first + count > self.k_codes.shape[dim]:
+            raise ValueError(f"there are {self.k_codes.shape[dim]} of these")
+        view = object.__new__(QuantizedCache)
+        view.width, view.bits = self.width, self.bits
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+            setattr(view, name, getattr(self, name).narrow(dim, first, count))
+        return view
+
+    def first(self, tokens: int) -> QuantizedCache:
+        """The first ``tokens`` positions, in the same memory."""
+        return self._view(2, 0, tokens)
+
+    def cloud(self, index: int) -> QuantizedCache:
+        """One cloud's cache (a batch of one), in the same memory."""
+        return self._view(0, index, 1)
+
+    def _check(self) -> None:
+        """The tensors are those of the constructor or views of them."""
+        row = -(-self.width // _GROUP)
+        shape = self.k_codes.shape
+        for t, size in ((self.k_codes, row * _GROUP * self.bits // 8), (self.v_codes, row * _GROUP * self.bits // 8),
+                        (self.k_scales, row), (self.v_scales, row)):
+            if (t.dtype != torch.uint8 or t.shape != (*shape[:3], size) or t.device != self.k_codes.device
+                    or (t.numel() and (t.stride(3) != 1 and size > 1 or t.stride(2) != size and shape[2] > 1
+                                       or t.stride(0) * row != self.k_scales.stride(0) * size
+                                       or t.stride(1) * row != self.k_scales.stride(1) * size))):
+                raise ValueError("the cache's tensors must keep their types, shapes and strides")
+
+    def _strides(self) -> tuple[int, int]:
+        """Of batch and key head, in rows."""
+        row = self.k_scales.shape[3]
+        return self.k_scales.stride(0) // row, self.k_scales.stride(1) // row
+
+    def _pack(self) -> bytes:
+        return _CACHE.pack(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scales.data_ptr(),
+                           self.v_scales.data_ptr(), *self._strides(), *self.k_codes.shape[:1], self.tokens, self.heads,
+                           self.width, self.bits)
+
+    def __repr__(self) -> str:
+        return (f"QuantizedCache(batch={self.batch}, tokens={self.tokens}, heads={self.heads}, width={self.width}, "
+                f"bits={self.bits}, device='{self.device}')")
+
+
+def _check_places(batch: int, device: torch.device, **places) -> None:
+    for name, t in places.items():
+        if t is None:
+            continue
+        if not isinstance(t, Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name} must be int32 or int64")
+        if t.shape != (batch,):
+            raise ValueError(f"{name} must have shape (batch,)")
+        if t.device != device:
+            raise ValueError(f"{name} must be on the same device")
+
+
+def _not_traced(name: str) -> None:
+    if not _native.untraced():
+        raise RuntimeError(f"{name} works on a cache's memory: traces, transforms and forward-mode differentiation "
+                           "do not see it")
+
+
+def _cache_of(cache, name: str = "cache") -> QuantizedCache:
+    if not isinstance(cache, QuantizedCache):
+        raise TypeError(f"{name} must be a QuantizedCache")
+    cache._check()
+    return cache
+
+
+def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | None = None, *,
+                starts: Tensor | None = None) -> None:
+    """Writes the keys and values of new tokens ``k, v (B, T, G, D)`` to a cache.
+
+    The T tokens of a cloud are the last of its first ``lengths (B,)`` positions
+    (int32 or int64, clamped to [0, tokens]; None: all), or, with ``starts (B,)``, token t
+    goes to position ``starts + t`` where that lies in [0, lengths): a batch of
+    prompts padded to T has starts of 0 and their own lengths.  All other positions
+    stay as they are.  k and v are float32, float16 or bfloat16 with any strides; the
+    rounding to codes has no gradient.
+    """
+    _not_traced("cache_write")
+    _cache_of(cache)
+    _check_heads({"k": k, "v": v})
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    if (k.shape[0], k.shape[2], k.shape[3]) != (cache.batch, cache.heads, cache.width):
+        raise ValueError("k and v must have the cache's batch size, heads and width")
+    if k.shape[1] > _MAX_TOKENS:
+        raise ValueError(f"sizes must be at most {_MAX_TOKENS}")
+    if k.device != cache.device:
+        raise ValueError("k and v must be on the cache's device")
+    _check_places(cache.batch, cache.device, lengths=lengths, starts=starts)
+    _native.require_device(k.device)
+    if _tracked(k, v):
+        raise ValueError("cache_write has no gradients: call it under torch.no_grad()")
+    if not k.numel() or not cache.tokens:
+        return
+    k, v = _rows(k), _rows(v)
+    lengths, starts = (None if t is None else t.contiguous() for t in (lengths, starts))
+    three = ctypes.c_int64 * 3
+    _native.call("pointops_cache_write", cache._pack(), k.data_ptr(), three(*k.stride()[:3]), v.data_ptr(),
+                 three(*v.stride()[:3]), k.shape[1], _native.ptr(lengths),
+                 0 if lengths is None else 8 * lengths.element_size(), _native.ptr(starts),
+                 0 if starts is None else 8 * starts.element_size(), _TYPES[k.dtype], _native.stream(k.device))
+
+
+def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
+    """All keys and values of a cache (``cache.first(n)``: of its first n positions),
+    ``(B, tokens, G, D)`` each, in float32, float16 or bfloat16, rounded once; float32
+    and bfloat16 hold every value exactly but those below their smallest normal
+    numbers, float16 those from 2 ** -14 to 65504.
+    """
+    _not_traced("cache_read")
+    _cache_of(cache)
+    if dtype not in _TYPES:
+        raise TypeError("dtype must be float32, float16 or bfloat16")
+    _native.require_device(cache.device)
+    shape = cache.batch, cache.tokens, cache.heads, cache.width
+    k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    if k.numel():
+        _native.call("pointops_cache_read", cache._pack(), k.data_ptr(), v.data_ptr(), _TYPES[dtype],
+                     _native.stream(cache.device))
+    return k, v
+
+
+def _pack_keys(kept) -> bytes:
+    if kept is None:
+        return bytes(_KEYS.size)
+    if isinstance(kept, QuantizedCache):
+        batch, head = kept._strides()
+        return _KEYS.pack(kept.k_codes.data_ptr(), kept.v_codes.data_ptr(), kept.k_scales.data_ptr(),
+                          kept.v_scales.data_ptr(), batch, 1, head, batch, 1, head, kept.tokens)
+    k, v = kept
+    return _KEYS.pack(k.data_ptr(), v.data_ptr(), 0, 0, *k.stride()[:3], *v.stride()[:3], k.shape[1])
+
+
+def _cache_step(name: str, q: Tensor, start, own, lengths, bits, window, sinks, bias, max_distance, scale) -> Tensor:
+    """The step over checked keys: of the start (a batch of one; None) and own."""
+    batch, queries, heads, width = q.shape
+    key_heads = own.heads if bits else own[0].shape[2]
+    edges = None
+    if heads and (key_heads == 0 or heads % key_heads):
+        raise ValueError("the number of query heads must be a multiple of the number of key heads")
+    tokens = own.tokens if bits else own[0].shape[1]
+    if start is not None:
+        tokens += start.tokens if bits else start[0].shape[1]
+    if max(batch * queries * max(heads, 1), tokens) > _MAX_TOKENS:
+        raise ValueError(f"queries of all heads and keys must be at most {_MAX_TOKENS}")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1")
+    if sinks < 0:
+        raise ValueError("sinks must be non-negative")
+    if bias is not None:
+        if not isinstance(bias, Tensor):
+            raise TypeError("bias must be a tensor")
+        if bias.dtype != q.dtype:
+            raise TypeError("bias must have q's type")
+        if bias.device != q.device:
+            raise ValueError("bias must be on q's device")
+        edges = _check_table(bias, heads, max_distance, True, _MAX_REACH, "bias")
+        bias = bias.contiguous()
+    _check_places(batch, q.device, lengths=lengths)
+    _native.require_device(q.device)
+    if _tracked(q, bias, *(() if bits else (*(start or ()), *own))):
+        raise ValueError(f"{name} has no gradients: call it under torch.no_grad()")
+    out = _like(q)
+    if not out.numel():
+        return out
+    q = _rows(q)
+    if not bits:
+        start, own = (None if pair is None else [_rows(t) for t in pair] for pair in (start, own))
+    lengths = None if lengths is None else lengths.contiguous()
+    args = _CACHE_ARGS.pack(
+        q.data_ptr(), _pack_keys(start), _pack_keys(own), 0 if bias is None else bias.data_ptr(),
+        0 if lengths is None else lengths.data_ptr(), 0 if edges is None else ctypes.addressof(edges), *q.stride()[:3],
+        batch, queries, heads, key_heads, width, tokens + 1 if window is None else min(int(window), tokens + 1),
+        min(int(sinks), tokens), 0 if edges is None else len(edges), 0 if bias is None else bias.shape[0],
+        0 if lengths is None else 8 * lengths.element_size(), _TYPES[q.dtype], bits,
+        float(width ** -0.5 if scale is None else scale))
+    size = _native.size_query("pointops_cache_attention_step_workspace_bytes", args)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    _native.call("pointops_cache_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(q.device))
+    return out
+
+
+def _check_coded(q: Tensor, cache: QuantizedCache, name: str, batch: int) -> None:
+    _cache_of(cache, name)
+    if cache.device != q.device:
+        raise ValueError(f"{name} must be on q's device")
+    if cache.batch != batch:
+        raise ValueError(f"{name} must have a batch of {batch}")
+    if cache.width != q.shape[3]:
+        raise ValueError(f"{name} must have q's head width")
+
+
+def quantized_attention_step(q: Tensor, cache: QuantizedCache, lengths: Tensor | None = None, *,
+                             window: int | None = None, sinks: int = 0, bias: Tensor | None = None,
+                             max_distance: int | None = None, scale: float | None = None) -> Tensor:
+    """``window_attention_step`` over keys and values in 8 or 4 bits: of the values
+    that the cache holds, without a further rounding of them, of the queries or of
+    the weights.  ``q (B, Q, H, D)`` is float32, float16 or bfloat16.
+    """
+    _not_traced("quantized_attention_step")
+    _check_heads({"q": q})
+    _check_coded(q, cache, "cache", q.shape[0])
+    return _cache_step("quantized_attention_step", q, None, cache, lengths, cache.bits, window, sinks, bias, max_distance,
+                       scale)
+
+
+def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = None, *, window: int | None = None,
+                          sinks: int = 0, bias: Tensor | None = None, max_distance: int | None = None,
+                          scale: float | None = None) -> Tensor:
+    """``window_attention_step`` of a batch whose clouds continue one common start.
+
+    ``prefix`` is the start's keys and values, two tensors ``(P, G, D)``, and
+    ``cache`` each cloud's own behind them, two tensors ``(B, N, G, D)`` of which the
+    first ``lengths (B,)`` hold tokens, the new ones' own among them: the cloud's
+    positions are 0 .. P + lengths - 1, and ``q (B, Q, H, D)`` stands at the last Q.
+    Or both are a ``QuantizedCache`` of the same bits, the prefix with a batch of one.
+    The start's keys are read once for all queries of the batch.  Without gradients.
+    """
+    _not_traced("prefix_attention_step")
+    _check_heads({"q": q})
+    coded = isinstance(prefix, QuantizedCache)
+    if coded != isinstance(cache, QuantizedCache):
+        raise TypeError("prefix and cache must both be a QuantizedCache, or both pairs of tensors")
+    if coded:
+        _check_coded(q, prefix, "prefix", 1)
+        _check_coded(q, cache, "cache", q.shape[0])
+        if prefix.bits != cache.bits or prefix.heads != cache.heads:
+            raise ValueError("prefix and cache must have the same bits and heads")
+        return _cache_step("prefix_attention_step", q, prefix, cache, lengths, cache.bits, window, sinks, bias, max_distance,
+                           scale)
+    for name, pair in (("prefix", prefix), ("cache", cache)):
+        if not isinstance(pair, (tuple, list)) or len(pair) != 2 or not all(isinstance(t, Tensor) for t in pair):
+            raise TypeError(f"{name} must be a pair of tensors or a QuantizedCache")
+    if any(t.ndim != 3 for t in prefix):
+        raise ValueError("prefix must be two tensors of shape (tokens, heads, width)")
+    start, own = [t[None] for t in prefix], list(cache)
+    _check_heads({"q": q, "prefix's keys": start[0], "prefix's values": start[1], "cache's keys": own[0],
+                  "cache's values": own[1]})
+    for name, (k, v) in (("prefix", start), ("cache", own)):
+        if k.shape != v.shape:
+            raise ValueError(f"{name}'s keys and values must have the same shape")
+        if k.shape[3] != q.shape[3]:
+            raise ValueError(f"{name} must have q's head width")
+    if not 1 <= q.shape[3] <= _MAX_HEAD:
+        raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
+    if own[0].shape[0] != q.shape[0]:
+        raise ValueError("cache must have q's batch size")
+    if start[0].shape[2] != own[0].shape[2]:
+        raise ValueError("prefix and cache must have the same heads")
+    return _cache_step("prefix_attention_step", q, start, own, lengths, 0, window, sinks, bias, max_distance, scale)
+
+
 # ------------------------------------------------------------- relative bias
 _MAX_BIAS_QUERIES = 65535 * 64
 _MAX_BIAS_KEYS = (1 << 22) - 1
@@ -475,4 +792,5 @@ def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     return _QkNormRotate.apply(*args) if _by_function(q, k, q_weight, k_weight) else _norm(*args)
 
 
-__all__ = ["bucket_edges", "qk_norm_rotate", "relative_bias", "window_attention", "window_attention_step"]
+__all__ = ["QuantizedCache", "bucket_edges", "cache_read", "cache_write", "prefix_attention_step", "qk_norm_rotate",
+           "quantized_attention_step", "relative_bias", "window_attention", "window_attention_step"]
