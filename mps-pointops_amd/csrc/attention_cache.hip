@@ -34,7 +34,7 @@ __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const Ca
     const int64_t all = static_cast<int64_t>(a.B) * per, in_g = id % all;
     const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / per), row = static_cast<int>(in_g % per);
     // Of each kind: the row's first part, and from one to the next.
-    const int start_rows = 16 * plan.start_cols, own_rows = 16 * plan.own_cols;
+    const int start_rows = plan.start_rows, own_rows = plan.own_rows;
     const int64_t start_unit = static_cast<int64_t>(g) * plan.start_blocks + in_g / start_rows;
     const int64_t own_unit = (static_cast<int64_t>(b) * a.G + g) * plan.own_blocks + row / own_rows;
     const float* const start = parts + (start_unit * plan.start_splits * start_rows + in_g % start_rows) * width;
@@ -152,8 +152,9 @@ bool read_call(const pointops_cache_attention* in, CacheArgs* out) {
     return true;
 }
 
-bool pieces(const void* p, int64_t b, int64_t n, int64_t h) {  // strides in bytes
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % 16 == 0 && n % 16 == 0 && h % 16 == 0;
+// (Strides in bytes.  A tile of 32 rows lies within 2 GiB, on one side of its first.)
+bool pieces(const void* p, int64_t b, int64_t n, int64_t h) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % 16 == 0 && n % 16 == 0 && h % 16 == 0 && n >= 0 && n < (1 << 26);
 }
 bool pieces(const Kept& k) { return k.tokens == 0 || (pieces(k.k, k.kb, k.kn, k.kh) && pieces(k.v, k.vb, k.vn, k.vh)); }
 
@@ -166,26 +167,49 @@ int form_of(const pointops_cache_attention& in, CacheArgs* a) {
     return whole && pieces(a->start) && pieces(a->own) ? kAligned : kAny;
 }
 
+#ifndef TARGET1
+#define TARGET1 1024
+#endif
+// Where what a sequence's rows see are so many tiles at most, and so many of all sequences (whose
+// blocks each read the start's keys), one launch of whole rows is shorter than parts and their join.
+constexpr int kDirectTiles = 40, kDirectWork = 16384;
+
+#ifndef TARGET2
+#define TARGET2 512
+#endif
 // Parts that give every compute unit its blocks (four of 16 rows, two of more), at least
 // two tiles a wave; the start's and the caches' as their work is to each other.  By
 // the caches' sizes: the lengths are on the device, and a call does not wait for it.
 CachePlan plan_of(const CacheArgs& a, int form) {
     CachePlan p = {};
-    const int many = kManyCols;
     const int64_t per = static_cast<int64_t>(a.Q) * (a.H / a.G), all = per * a.B;
-    p.own_cols = per <= 16 && form != kAny ? 1 : many;
-    p.start_cols = a.start.tokens == 0 || (all <= 16 && form != kAny) ? p.own_cols : many;
-    auto blocks = [](int64_t rows, int cols) { return static_cast<int>((rows + 16 * cols - 1) / (16 * cols)); };
-    p.own_blocks = blocks(per, p.own_cols);
-    p.start_blocks = blocks(all, p.start_cols);
-    p.own_units = static_cast<int64_t>(a.B) * a.G * p.own_blocks;
-    p.start_units = a.start.tokens == 0 ? 0 : static_cast<int64_t>(a.G) * p.start_blocks;
+    const bool some = a.start.tokens != 0;
     const int64_t seen = (static_cast<int64_t>(a.window) + a.Q - 1) / kKeys + 2 + (a.sinks + kKeys - 1) / kKeys;
     auto tiles = [&](int tokens) { return std::min<int64_t>((static_cast<int64_t>(tokens) + kKeys - 1) / kKeys, seen); };
     const int64_t start_tiles = tiles(a.start.tokens), own_tiles = tiles(a.own.tokens);
-    const double start_work = static_cast<double>(p.start_units) * start_tiles * p.start_cols;
-    const double own_work = static_cast<double>(p.own_units) * own_tiles * p.own_cols;
-    const double target = p.start_cols > 1 ? 512 : 1024, sum = std::max(1.0, start_work + own_work);
+    // (A window over both sees no more than one over either.)
+    const int64_t all_tiles = std::min(start_tiles + own_tiles, seen + 1);
+    if (form == kAny) p.shape = kTwoTwo;
+    else if (per <= 16 && all_tiles <= kDirectTiles && all_tiles * a.B * a.G <= kDirectWork) p.shape = kDirect;
+    else if (per > 16) p.shape = some && all > 32 ? kPairsTwo : kTwoTwo;
+    else if (!some || all <= 16) p.shape = kOne;
+    else p.shape = all <= 32 ? kTwo : kPairs;
+    const ShapeRows rows = kShapeRows[p.shape];
+    p.start_rows = 16 * rows.cols * rows.row_waves;
+    p.own_rows = 16 * rows.own_cols;
+    auto blocks = [](int64_t rows, int each) { return static_cast<int>((rows + each - 1) / each); };
+    p.own_blocks = blocks(per, p.own_rows);
+    p.own_units = static_cast<int64_t>(a.B) * a.G * p.own_blocks;
+    if (p.shape == kDirect) {
+        p.own_splits = 1;
+        p.direct = true;
+        return p;
+    }
+    p.start_blocks = blocks(all, p.start_rows);
+    p.start_units = some ? static_cast<int64_t>(a.G) * p.start_blocks : 0;
+    const double start_work = static_cast<double>(p.start_units) * start_tiles * std::max(1, rows.row_waves);
+    const double own_work = static_cast<double>(p.own_units) * own_tiles;
+    const double target = some ? TARGET2 : TARGET1, sum = std::max(1.0, start_work + own_work);
     auto splits = [&](double work, int64_t units, int64_t count) {
         const int64_t wanted = static_cast<int64_t>(target * (work / sum) / std::max<int64_t>(1, units) + 0.999);
         return static_cast<int>(std::max<int64_t>(1, std::min(wanted, count / (2 * kStepWaves))));
@@ -193,13 +217,13 @@ CachePlan plan_of(const CacheArgs& a, int form) {
     p.start_splits = p.start_units == 0 ? 0 : splits(start_work, p.start_units, start_tiles);
     p.own_splits = splits(own_work, p.own_units, own_tiles);
     p.direct = p.start_splits == 0 && p.own_splits == 1;
-    p.start_floats = p.start_units * p.start_splits * 16 * p.start_cols * part_width(padded(a.D));
+    p.start_floats = p.start_units * p.start_splits * p.start_rows * part_width(padded(a.D));
     return p;
 }
 
 size_t workspace_of(const CacheArgs& a, const CachePlan& p) {
     if (p.direct) return 0;
-    return sizeof(float) * (p.start_floats + p.own_units * p.own_splits * 16 * p.own_cols * part_width(padded(a.D)));
+    return sizeof(float) * (p.start_floats + p.own_units * p.own_splits * p.own_rows * part_width(padded(a.D)));
 }
 
 template <typename T>

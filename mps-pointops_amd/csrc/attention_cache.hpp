@@ -59,13 +59,15 @@ struct CacheArgs {
 
 constexpr int kStepWaves = 4, kStepThreads = kStepWaves * kWave;
 constexpr int kKeys = 32;  // of a wave at a time
+constexpr size_t kMostLds = 160 * 1024;
 
 // Parts of a sum over keys: of a unit (key head with 16 COLS rows), `splits` of them,
 // each `rows` long; a part is its maximum and its sum, two unused, then the values.
 __host__ __device__ constexpr int part_width(int DP) { return DP + 4; }
 
 struct CachePlan {
-    int start_cols, own_cols;             // 16-row columns of a block
+    int shape;                            // of Shape
+    int start_rows, own_rows;             // of a block
     int start_blocks, own_blocks;         // blocks of rows of a key head (of a sequence's key head)
     int start_splits, own_splits;         // 0: no start
     int64_t start_units, own_units;       // key heads by blocks of rows (by sequences)
@@ -108,8 +110,8 @@ struct Products {
     static constexpr int kWeight = sizeof(T) == 2 ? 2 : kCoded ? 3 : 1;
 };
 
-// x as N fragments of C that add up to it.
-template <typename C, int N>
+// x as N fragments of C that add up to it (of an infinity, FINITE: all but the first are NaN).
+template <typename C, int N, bool FINITE>
 __device__ __forceinline__ void split(const float* x, i32x4 (&out)[N]) {
     float left[kPerFrag<C>];
 #pragma unroll
@@ -121,7 +123,7 @@ __device__ __forceinline__ void split(const float* x, i32x4 (&out)[N]) {
 #pragma unroll
             for (int e = 0; e < kPerFrag<C>; ++e) {
                 const float taken = element<C>(out[n], e);
-                left[e] = finite(taken) ? left[e] - taken : 0.f;
+                left[e] = FINITE || finite(taken) ? left[e] - taken : 0.f;
             }
         }
     }
@@ -153,7 +155,7 @@ struct Incoming {
 
     i32x4 kr[kCoded ? 1 : 2][kCoded ? 1 : kFrags], vr[kCoded ? 1 : kPieces];
     uint32_t kc[kCoded ? 2 : 1][kCoded ? kFrags * kWords : 1], vc[kCoded ? kCodePieces : 1][kCoded ? 2 * kWords : 1];
-    uint32_t ks[kCoded ? 2 : 1][kCoded ? kScales : 1], vs[kCoded ? kCodePieces : 1];
+    uint32_t ks[kCoded ? 2 : 1], vs[kCoded ? kCodePieces : 1];
 
     template <int N>
     __device__ static __forceinline__ void words(const uint8_t* p, uint32_t* out) {
@@ -170,58 +172,60 @@ struct Incoming {
         }
     }
 
-    // Keys j0 .. j0 + 31 of the head at k and v; from `limit` (>= 1) on the last one again, for which
-    // the caller's scores are masked.
+    // Keys j0 .. j0 + 31 of the head at k and v; from `limit` (> j0) on the last one again, for which
+    // the caller's scores are masked.  A tile's base is uniform, its rows lie within 2 GiB of it.
     __device__ __forceinline__ void load(const Kept& kept, const char* k, const char* v, const uint8_t* k_scales,
                                          const uint8_t* v_scales, int j0, int limit, int width) {
-        const int lane = lane_id(), col = lane % 16, quad = lane / 16;
+        const int lane = lane_id(), col = lane % 16, quad = lane / 16, last = min(limit - 1 - j0, kKeys - 1);
         if constexpr (!kCoded) {
+            const char* const k0 = k + j0 * kept.kn;
+            const char* const v0 = v + j0 * kept.vn;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const T* const row = reinterpret_cast<const T*>(k + min(j0 + 16 * u + col, limit - 1) * kept.kn);
+                const T* const row = reinterpret_cast<const T*>(k0 + at_row(min(16 * u + col, last), kept.kn));
 #pragma unroll
                 for (int c = 0; c < kFrags; ++c) kr[u][c] = load_row<T, FORM == kAligned>(row, column(c, quad), width);
             }
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
                 const int at = x * kWave + lane;
-                const T* const row = reinterpret_cast<const T*>(v + min(j0 + at / kPerRow, limit - 1) * kept.vn);
+                const T* const row = reinterpret_cast<const T*>(v0 + at_row(min(at / kPerRow, last), kept.vn));
                 vr[x] = load_row<T, FORM == kAligned>(row, at % kPerRow * kPerFrag<T>, width);
             }
         } else {
+            const uint8_t* const k0 = reinterpret_cast<const uint8_t*>(k) + static_cast<int64_t>(j0) * kRowBytes;
+            const uint8_t* const v0 = reinterpret_cast<const uint8_t*>(v) + static_cast<int64_t>(j0) * kRowBytes;
+            const uint8_t* const ks0 = k_scales + static_cast<int64_t>(j0) * kScales;
+            const uint8_t* const vs0 = v_scales + static_cast<int64_t>(j0) * kScales;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int64_t j = min(j0 + 16 * u + col, limit - 1);
-                const uint8_t* const row = reinterpret_cast<const uint8_t*>(k) + j * kRowBytes;
+                const uint32_t row = min(16 * u + col, last);
 #pragma unroll
-                for (int c = 0; c + 1 < kFrags; c += 2) words<2 * kWords>(row + column(c, quad) * kWords / 2, kc[u] + c * kWords);
+                for (int c = 0; c + 1 < kFrags; c += 2)
+                    words<2 * kWords>(k0 + (row * kRowBytes + column(c, quad) * kWords / 2), kc[u] + c * kWords);
                 if constexpr (kFrags % 2 != 0)
-                    words<kWords>(row + column(kFrags - 1, quad) * kWords / 2, kc[u] + (kFrags - 1) * kWords);
-                load_scales(k_scales + j * kScales, ks[u]);
+                    words<kWords>(k0 + (row * kRowBytes + column(kFrags - 1, quad) * kWords / 2), kc[u] + (kFrags - 1) * kWords);
+                ks[u] = load_scales(ks0 + row * kScales);
             }
 #pragma unroll
             for (int x = 0; x < kCodePieces; ++x) {
-                const int at = x * kWave + lane, piece = at % kCodePerRow;
-                const int64_t j = min(j0 + at / kCodePerRow, limit - 1);
-                words<2 * kWords>(reinterpret_cast<const uint8_t*>(v) + j * kRowBytes + piece * 8 * kWords, vc[x]);
-                vs[x] = v_scales[j * kScales + piece / 2];
+                const uint32_t at = x * kWave + lane, piece = at % kCodePerRow, row = min(static_cast<int>(at / kCodePerRow), last);
+                words<2 * kWords>(v0 + (row * kRowBytes + piece * 8 * kWords), vc[x]);
+                vs[x] = vs0[row * kScales + piece / 2];
             }
         }
     }
-    // The scales of a row's groups, as bytes in one word or (96 values) one by one.
-    __device__ static __forceinline__ void load_scales(const uint8_t* p, uint32_t* out) {
-        if constexpr (kScales == 4) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = x >> (8 * i) & 255;
-        } else if constexpr (kScales == 2) {
-            const uint32_t x = *reinterpret_cast<const uint16_t*>(p);
-            out[0] = x & 255;
-            out[1] = x >> 8;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kScales; ++i) out[i] = p[i];
-        }
+    // Rows of any stride (kAny), or of one whose tile lies within 2 GiB.
+    __device__ static __forceinline__ int64_t at_row(int row, int64_t stride) {
+        if constexpr (FORM == kAligned) return static_cast<uint32_t>(row) * static_cast<uint32_t>(stride);
+        else return row * stride;
+    }
+    // The scales of a row's groups, a byte each.
+    __device__ static __forceinline__ uint32_t load_scales(const uint8_t* p) {
+        if constexpr (kScales == 4) return *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (kScales == 3) return p[0] | p[1] << 8 | p[2] << 16;
+        else if constexpr (kScales == 2) return *reinterpret_cast<const uint16_t*>(p);
+        else return p[0];
     }
 
     // Row operand: keys 16 u + lane % 16, fragment c.
@@ -229,9 +233,8 @@ struct Incoming {
         if constexpr (!kCoded) {
             return kr[u][c];
         } else {
-            const int quad = lane_id() / 16;
-            const uint32_t byte = c < DP / 64 * 2 ? (quad < 2 ? ks[u][c / 2 * 2] : ks[u][c / 2 * 2 + 1]) : ks[u][c];
-            return decode8<FORM>(kc[u] + c * kWords, scale_of(byte));
+            const int group = c < DP / 64 * 2 ? c / 2 * 2 + lane_id() / 32 : c;
+            return decode8<FORM>(kc[u] + c * kWords, scale_of(ks[u] >> (8 * group) & 255));
         }
     }
 
@@ -314,21 +317,98 @@ struct CarefulKept {
     }
 };
 
+// ------------------------------------------------- keys that waves share
+// 32 KW keys and values of the common start on their way through a block's registers to
+// LDS, where its waves read both.  Rows behind `limit` are zeros (a descriptor that ends
+// with the last row), for which the caller's scores are masked.
+template <typename T, int FORM, int DP, int KW>
+struct Shared {
+    using C = typename Products<T, FORM>::C;
+    static constexpr bool kCoded = Products<T, FORM>::kCoded;
+    using TileT = Tile<C, DP>;
+    static constexpr int kRows = kKeys * KW, kBytes = 2 * kRows * TileT::kStride;
+    static constexpr int kPerRow = kCoded ? DP / 16 : DP * static_cast<int>(sizeof(C)) / 16;
+    static constexpr int kPieces = (kRows * kPerRow + kStepThreads - 1) / kStepThreads;
+    static constexpr bool kAll = kRows * kPerRow % kStepThreads == 0;
+    static constexpr int kWords = FORM == kEight ? 2 : 1, kRowBytes = FORM == kEight ? DP : DP / 2, kScales = DP / kGroup;
+    static constexpr int kPieceBytes = kCoded ? 8 * kWords : 16;
+    i32x4 r[2][kPieces];
+    uint32_t scale[kCoded ? 2 : 1][kCoded ? kPieces : 1];
+
+    __device__ __forceinline__ void load(const Kept& kept, const char* k, const char* v, const uint8_t* k_scales,
+                                         const uint8_t* v_scales, int j0, int limit, int width) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int64_t stride = kCoded ? kRowBytes : side == 0 ? kept.kn : kept.vn;
+            const int64_t bytes = (limit - 1 - j0) * stride + (kCoded ? kRowBytes : width * static_cast<int>(sizeof(T)));
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((side == 0 ? k : v) + j0 * stride), 0,
+                                                                static_cast<int>(min(bytes, int64_t(INT32_MAX))), kRawBuffer);
+            const auto scales = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<uint8_t*>((side == 0 ? k_scales : v_scales) + static_cast<int64_t>(j0) * kScales), 0,
+                static_cast<int>(min(static_cast<int64_t>(limit - j0) * kScales, int64_t(INT32_MAX))), kRawBuffer);
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) {
+                const uint32_t at = x * kStepThreads + threadIdx.x, row = at / kPerRow, piece = at % kPerRow;
+                const bool here = (kAll || row < kRows) && (kCoded || static_cast<int>(piece) * kPerFrag<T> < width);
+                const uint32_t offset = here ? row * static_cast<uint32_t>(stride) + piece * kPieceBytes : 0x80000000u;
+                if constexpr (kPieceBytes == 16) r[side][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+                else {
+                    const i32x2 y = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0));
+                    r[side][x] = i32x4{y[0], y[1], 0, 0};
+                }
+                if constexpr (kCoded)
+                    scale[side][x] = __builtin_amdgcn_raw_buffer_load_b8(scales, here ? row * kScales + piece / 2 : 0x80000000u, 0, 0);
+            }
+        }
+    }
+    // Keys, then values.
+    __device__ __forceinline__ void store(char* tiles) const {
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) {
+                const int at = x * kStepThreads + static_cast<int>(threadIdx.x), row = at / kPerRow;
+                if (!kAll && row >= kRows) continue;
+                i32x4* const to = reinterpret_cast<i32x4*>(tiles + (side * kRows + row) * TileT::kStride + at % kPerRow * (kCoded ? 32 : 16));
+                if constexpr (kCoded) {
+                    const uint32_t codes[4] = {static_cast<uint32_t>(r[side][x][0]), static_cast<uint32_t>(r[side][x][1]),
+                                               static_cast<uint32_t>(r[side][x][2]), static_cast<uint32_t>(r[side][x][3])};
+                    to[0] = decode8<FORM>(codes, scale_of(scale[side][x]));
+                    to[1] = decode8<FORM>(codes + kWords, scale_of(scale[side][x]));
+                } else {
+                    to[0] = r[side][x];
+                }
+            }
+    }
+    // Row operand: key `row` + lane % 16 of those in LDS, fragment c: values from column(c, lane / 16) on.
+    __device__ static __forceinline__ int column(int c, int quad) { return (4 * c + quad) * kPerFrag<C>; }
+    __device__ static __forceinline__ i32x4 keys(const char* tiles, int row, int c) {
+        const int lane = lane_id();
+        return *reinterpret_cast<const i32x4*>(tiles + (row + lane % 16) * TileT::kStride + 64 * c + 16 * (lane / 16));
+    }
+};
+
 // ------------------------------------------------------------------ a part
-template <int COLS, int DP>
-constexpr int kSumBytes = 16 * COLS * (DP + 4) * 4;
-// The waves' tiles, then their sums in the same place; maxima and sums of the weights; then
-// the bias: [buckets][heads of the rows], the buckets of 0 .. reach, the edges.
-template <typename T, int FORM, int DP, int COLS>
-constexpr int kTilesBytes = kStepWaves * Incoming<T, FORM, DP>::kTileBytes > kSumBytes<COLS, DP>
-                                ? kStepWaves * Incoming<T, FORM, DP>::kTileBytes : kSumBytes<COLS, DP>;
-template <typename T, int FORM, int DP, int COLS>
-constexpr int kStepLds = kTilesBytes<T, FORM, DP, COLS> + 2 * kStepWaves * 16 * COLS * 4;
-inline int bias_heads(int group, int cols) { return group < 16 * cols ? group : 16 * cols; }
-constexpr size_t bias_most(int cols) { return 4 * (256 * 16 * cols) + (kMaxReach + 4) / 4 * 4 + 4 * 255; }
-inline size_t bias_lds(const CacheArgs& a, int cols) {
+// The rows and keys of a block: the common start with rows of all sequences, a sequence's
+// cache with its rows, or its rows with both, one behind the other.
+enum Kind { kStart, kOwn, kBoth };
+
+// A block's waves: ROW_WAVES hold 16 COLS rows each, and so many of them share 32 keys at
+// a time; 1: every wave has the same rows and takes its own keys.
+template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int WAVES>
+struct StepLds {
+    static constexpr int kKeyWaves = WAVES / ROW_WAVES, kRows = 16 * COLS * ROW_WAVES;
+    static constexpr int kSums = kRows * (DP + 4) * 4;
+    static constexpr int kTiles = ROW_WAVES == 1 ? WAVES * Incoming<T, FORM, DP>::kTileBytes
+                                                 : 2 * Shared<T, FORM, DP, kKeyWaves>::kBytes;
+    // The tiles, then the sums in the same place; maxima and sums of the weights; then the
+    // bias: [buckets][heads of the rows], the buckets of 0 .. reach, the edges.
+    static constexpr int kPlace = kTiles > kSums ? kTiles : kSums;
+    static constexpr int kBytes = kPlace + 2 * kKeyWaves * kRows * 4;
+};
+inline size_t bias_lds(const CacheArgs& a, int rows) {
     if (a.bias == nullptr) return 0;
-    return 4 * static_cast<size_t>(a.bk.count) * bias_heads(a.H / a.G, cols) + (a.reach + 4) / 4 * 4 + 4 * a.bk.n;
+    return 4 * static_cast<size_t>(a.bk.count) * std::min(a.H / a.G, rows) + (a.reach + 4) / 4 * 4 + 4 * a.bk.n;
 }
 
 // Keys of `kept` that the query at position p sees: as Seen, in the kept keys' own numbers.
@@ -338,83 +418,140 @@ __device__ __forceinline__ Seen seen_of(const CacheArgs& a, int p, int base, int
     return {low, max(0, high - low + 1), max(0, min(min(a.sinks, p + 1) - base, limit))};
 }
 
-// One block's part of one unit.  START: the common start (rows of all sequences), else the
-// cache of sequence b.
-template <typename T, int FORM, int DP, int COLS, bool START>
+// What a block reads of one of the kept: keys 0 .. limit - 1 at positions `base` on, of
+// which its rows see the first `first_tiles` tiles and those from `low_tile` on.
+template <int TILE, int COLS>
+struct Range {
+    const Kept* kept;
+    const char *k, *v;
+    const uint8_t *k_scales, *v_scales;
+    int base, limit, first_tiles, low_tile, tiles;
+    int low_most, high_least;  // keys in between are seen by all of the wave's rows
+    Seen seen[COLS];
+
+    __device__ __forceinline__ int first_key(int tile) const {
+        return (tile < first_tiles ? tile : tile - first_tiles + low_tile) * TILE;
+    }
+    __device__ __forceinline__ void tiles_of(int first, int low, int high) {
+        first_tiles = (first + TILE - 1) / TILE;
+        low_tile = high < 0 ? first_tiles : max(first_tiles, low / TILE);
+        tiles = first_tiles + max(0, (high < 0 ? 0 : high / TILE + 1) - low_tile);
+    }
+};
+
+// One block's part of one unit.
+template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int WAVES, int KIND>
 __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict__ out, float* __restrict__ part, int b0,
                                                int g, int r0, int split_at, int splits, char* lds) {
+    using Lds = StepLds<T, FORM, DP, COLS, ROW_WAVES, WAVES>;
+    constexpr int kKeyWaves = Lds::kKeyWaves, kRows = Lds::kRows, kThreads = kWave * WAVES;
+    constexpr bool kShared = ROW_WAVES > 1, kManySequences = KIND == kStart;
     using In = Incoming<T, FORM, DP>;
+    using Sh = Shared<T, FORM, DP, kKeyWaves>;
     using C = typename In::C;
     constexpr int kQ = Products<T, FORM>::kQuery, kW = Products<T, FORM>::kWeight, kFrags = In::kFrags;
-    constexpr int kOut = DP / 16, kSumStride = DP + 4, kRows = 16 * COLS;
-    const Kept& kept = START ? a.start : a.own;
+    constexpr int kOut = DP / 16, kSumStride = DP + 4, kTile = kShared ? kKeys * kKeyWaves : kKeys;
+    constexpr int kRanges = KIND == kBoth ? 2 : 1;
     const int lane = lane_id(), col = lane % 16, quad = lane / 16, wave = uniform(threadIdx.x / kWave);
-    const int group = a.H / a.G, per = a.Q * group, total = START ? a.B * per : per;
-    const int rows = min(kRows, total - r0), base = START ? 0 : a.start.tokens;
-    float* const tops = reinterpret_cast<float*>(lds + kTilesBytes<T, FORM, DP, COLS>);
-    float* const totals = tops + kStepWaves * kRows;
-    float* const table = totals + kStepWaves * kRows;
+    const int row_wave = wave % ROW_WAVES, key_wave = wave / ROW_WAVES;
+    const int w0 = 16 * COLS * row_wave;  // this wave's first row in the block
+    const int group = a.H / a.G, per = a.Q * group, total = kManySequences ? a.B * per : per;
+    const int rows = min(kRows, total - r0);
+    float* const tops = reinterpret_cast<float*>(lds + Lds::kPlace);
+    float* const totals = tops + kKeyWaves * kRows;
+    float* const table = totals + kKeyWaves * kRows;
 
     // Rows: this lane's columns.
-    const int own_length = START ? 0 : uniform(a.length(b0));
-    const int limit = START ? kept.tokens : own_length;
-    int p[COLS];
-    Seen seen[COLS];
-    int first = 0, low = INT32_MAX, high = -1, low_most = 0, high_least = INT32_MAX, p_least = INT32_MAX;
+    const int own_length = kManySequences ? 0 : uniform(a.length(b0));
+    int p[COLS], p_least = INT32_MAX;
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        const int r = r0 + 16 * n + col;
-        const bool mine = 16 * n + col < rows;
+        const int r = r0 + w0 + 16 * n + col;
         p[n] = -1;
-        if (mine) {
-            const int length = START ? a.length(r / per) : own_length;
-            p[n] = a.start.tokens + length - a.Q + (START ? r % per : r) / group;
-        }
-        seen[n] = seen_of(a, p[n], base, limit);
-        first = max(first, seen[n].first);
-        if (seen[n].count > 0) {
-            low = min(low, seen[n].low);
-            high = max(high, seen[n].low + seen[n].count - 1);
-        }
-        if (mine) {
-            // (A row that sees nothing of these is masked in every tile.)
-            low_most = max(low_most, seen[n].low);
-            high_least = min(high_least, seen[n].low + seen[n].count - 1);
+        if (w0 + 16 * n + col < rows) {
+            const int length = kManySequences ? a.length(r / per) : own_length;
+            p[n] = a.start.tokens + length - a.Q + (kManySequences ? r % per : r) / group;
             p_least = min(p_least, p[n]);
         }
     }
-    first = wave_max_i32_l63(first);
-    low = -wave_max_i32_l63(-low);
-    high = wave_max_i32_l63(high);
-    low_most = wave_max_i32_l63(low_most);
-    high_least = -wave_max_i32_l63(-high_least);
     p_least = -wave_max_i32_l63(-p_least);
-    // Tiles of keys: the first keys', then the window's.
-    const int first_tiles = (first + kKeys - 1) / kKeys;
-    const int low_tile = high < 0 ? first_tiles : max(first_tiles, low / kKeys);
-    const int tiles = first_tiles + max(0, (high < 0 ? 0 : high / kKeys + 1) - low_tile);
+    Range<kTile, COLS> range[kRanges];
+#pragma unroll
+    for (int x = 0; x < kRanges; ++x) {
+        Range<kTile, COLS>& at = range[x];
+        const bool start = KIND == kStart || (KIND == kBoth && x == 0);
+        at.kept = start ? &a.start : &a.own;
+        at.base = start ? 0 : a.start.tokens;
+        at.limit = start ? a.start.tokens : own_length;
+        const int64_t b = start ? 0 : b0;
+        at.k = at.kept->k + b * at.kept->kb + g * at.kept->kh;
+        at.v = at.kept->v + b * at.kept->vb + g * at.kept->vh;
+        at.k_scales = at.kept->k_scales + b * at.kept->sb + g * at.kept->sh;
+        at.v_scales = at.kept->v_scales + b * at.kept->sb + g * at.kept->sh;
+        int first = 0, low = INT32_MAX, high = -1, low_most = 0, high_least = INT32_MAX;
+#pragma unroll
+        for (int n = 0; n < COLS; ++n) {
+            const Seen seen = seen_of(a, p[n], at.base, at.limit);
+            at.seen[n] = seen;
+            first = max(first, seen.first);
+            if (seen.count > 0) {
+                low = min(low, seen.low);
+                high = max(high, seen.low + seen.count - 1);
+            }
+            if (w0 + 16 * n + col < rows) {
+                // (A row that sees nothing of these is masked in every tile.)
+                low_most = max(low_most, seen.low);
+                high_least = min(high_least, seen.low + seen.count - 1);
+            }
+        }
+        first = wave_max_i32_l63(first);
+        low = -wave_max_i32_l63(-low);
+        high = wave_max_i32_l63(high);
+        at.low_most = wave_max_i32_l63(low_most);
+        at.high_least = -wave_max_i32_l63(-high_least);
+        if constexpr (kShared) {
+            // What any of the block's rows sees.
+            int* const ends = reinterpret_cast<int*>(tops);
+            if (lane == 0) {
+                ends[3 * wave] = first;
+                ends[3 * wave + 1] = low;
+                ends[3 * wave + 2] = high;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < WAVES; ++y) {
+                first = max(first, ends[3 * y]);
+                low = min(low, ends[3 * y + 1]);
+                high = max(high, ends[3 * y + 2]);
+            }
+            first = uniform(first);
+            low = uniform(low);
+            high = uniform(high);
+            __syncthreads();
+        }
+        at.tiles_of(first, low, high);
+    }
+    const int first_range = range[0].tiles, tiles = kRanges == 2 ? first_range + range[kRanges - 1].tiles : first_range;
     const int begin = static_cast<int>(static_cast<int64_t>(tiles) * split_at / splits);
     const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split_at + 1) / splits);
-    auto first_key = [&](int tile) { return (tile < first_tiles ? tile : tile - first_tiles + low_tile) * kKeys; };
-
-    const int64_t b = START ? 0 : b0;
-    const char* const k = kept.k + b * kept.kb + g * kept.kh;
-    const char* const v = kept.v + b * kept.vb + g * kept.vh;
-    const uint8_t* const k_scales = kept.k_scales + b * kept.sb + g * kept.sh;
-    const uint8_t* const v_scales = kept.v_scales + b * kept.sb + g * kept.sh;
-    In in;
-    int tile = begin + wave;
-    if (tile < end) in.load(kept, k, v, k_scales, v_scales, first_key(tile), limit, a.D);
+    std::conditional_t<kShared, Sh, In> in;
+    auto fetch = [&](int tile) {
+        const bool second = kRanges == 2 && tile >= first_range;
+        const Range<kTile, COLS>& at = range[second ? kRanges - 1 : 0];
+        in.load(*at.kept, at.k, at.v, at.k_scales, at.v_scales, at.first_key(second ? tile - first_range : tile), at.limit, a.D);
+    };
+    int tile = kShared ? begin : begin + wave;
+    if (tile < end) fetch(tile);
 
     i32x4 q[COLS][kFrags][kQ];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        const int r = r0 + 16 * n + col, in_b = START ? r % per : r;
-        const bool mine = 16 * n + col < rows;
-        const T* const row = a.q.at<T>(START ? r / per : b0, g * group + in_b % group) + in_b / group * a.q.n;
+        const int r = r0 + w0 + 16 * n + col, in_b = kManySequences ? r % per : r;
+        const bool mine = w0 + 16 * n + col < rows;
+        const T* const row = a.q.at<T>(kManySequences ? r / per : b0, g * group + in_b % group) + in_b / group * a.q.n;
 #pragma unroll
         for (int c = 0; c < kFrags; ++c) {
-            const int at = In::column(c, quad);
+            const int at = kShared ? Sh::column(c, quad) : In::column(c, quad);
             float x[kPerFrag<C>];
 #pragma unroll
             for (int e = 0; e < kPerFrag<C>; ++e) x[e] = 0.f;
@@ -432,7 +569,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                         if (at + e < a.D) x[e] = to_float(row[at + e]);
                 }
             }
-            split<C, kQ>(x, q[n][c]);
+            split<C, kQ, false>(x, q[n][c]);
         }
     }
 
@@ -443,18 +580,17 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     float far[COLS];
     if (biased) {
         int* const edges = reinterpret_cast<int*>(ids + (a.reach + 4) / 4 * 4);
-        for (int x = threadIdx.x; x < a.bk.n; x += kStepThreads) edges[x] = a.bk.edge[x];
-        const int h0 = g * group + (heads < group ? r0 % group : 0);
-        for (int x = threadIdx.x; x < a.bk.count * heads; x += kStepThreads) {
-            const int h = heads < group ? g * group + (r0 + x % heads) % group : h0 + x % heads;
+        for (int x = threadIdx.x; x < a.bk.n; x += kThreads) edges[x] = a.bk.edge[x];
+        for (int x = threadIdx.x; x < a.bk.count * heads; x += kThreads) {
+            const int h = g * group + (heads < group ? (r0 + x % heads) % group : x % heads);
             table[x] = bias_log2(to_float(static_cast<const T*>(a.bias)[static_cast<int64_t>(x / heads) * a.H + h]));
         }
         __syncthreads();
-        for (int x = threadIdx.x; x <= a.reach; x += kStepThreads) ids[x] = static_cast<uint8_t>(bucket_of(a.bk, edges, x));
+        for (int x = threadIdx.x; x <= a.reach; x += kThreads) ids[x] = static_cast<uint8_t>(bucket_of(a.bk, edges, x));
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            head[n] = heads < group ? 16 * n + col : (r0 + 16 * n + col) % group;
+            head[n] = heads < group ? w0 + 16 * n + col : (r0 + w0 + 16 * n + col) % group;
             far[n] = table[a.bk.n * heads + head[n]];
         }
     }
@@ -464,7 +600,6 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     // and a negative scale turns their order.
     const bool scaled = biased || !(a.scale_log2 > 0.f);
     const float factor = scaled ? 1.f : a.scale_log2;
-    char* const values = lds + wave * In::kTileBytes;
     f32x4 o[kOut][COLS];
     float m[COLS], l[COLS];
 #pragma unroll
@@ -474,74 +609,140 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 #pragma unroll
         for (int d = 0; d < kOut; ++d) o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (; tile < end; tile += kStepWaves) {
-        const int j0 = first_key(tile);
-        f32x4 s[COLS][2];
+    f32x4 s[COLS][2];
+    i32x4 w[COLS][8 / kPerFrag<C>][kW];
+    auto score = [&](auto&& keys) {
 #pragma unroll
         for (int n = 0; n < COLS; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kFrags; ++c)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const i32x4 f = in.keys(u, c);
+                const i32x4 f = keys(u, c);
 #pragma unroll
                 for (int n = 0; n < COLS; ++n)
 #pragma unroll
                     for (int x = 0; x < kQ; ++x) s[n][u] = mma16<C>(f, q[n][c][x], s[n][u]);
             }
-        in.store_values(values);
-        if (tile + kStepWaves < end) in.load(kept, k, v, k_scales, v_scales, first_key(tile + kStepWaves), limit, a.D);
-        const bool whole = j0 >= low_most && j0 + kKeys - 1 <= high_least;
-        const bool all_far = p_least - (base + j0 + kKeys - 1) >= a.reach;
-        i32x4 w[COLS][8 / kPerFrag<C>][kW];
+    };
+    // Of the 32 keys from j0 on.
+    auto weigh = [&](const Range<kTile, COLS>& at, int j0) {
+        const int j = j0 + 4 * quad;  // register e of half u: key j + 16 u + e
+        if (scaled) {
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[n][u] *= a.scale_log2;
+        }
+        if (biased) {
+            if (p_least - (at.base + j0 + kKeys - 1) >= a.reach) {
+#pragma unroll
+                for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) s[n][u] += far[n];
+            } else {
+#pragma unroll
+                for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[n][e / 4][e % 4] += bias_at(p[n] - at.base - (j + e / 4 * 16 + e % 4), head[n]);
+            }
+        }
+        if (j0 < at.low_most || j0 + kKeys - 1 > at.high_least) {
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[n][e / 4][e % 4] = at.seen[n](j + e / 4 * 16 + e % 4) ? s[n][e / 4][e % 4] : -kInf;
+        }
+        float top[COLS];
+        bool rises = false;
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            float x[8];  // keys 16 u + 4 quad + e, as u, e
+            float t = s[n][0][0];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = scaled ? s[n][e / 4][e % 4] * a.scale_log2 : s[n][e / 4][e % 4];
-            const int j = j0 + 4 * quad;
-            if (biased) {
+            for (int e = 1; e < 8; ++e) t = fmaxf(t, s[n][e / 4][e % 4]);
+            top[n] = quads_max(t) * factor;
+            rises |= top[n] > m[n] + kSlack;
+        }
+        if (ballot(rises) != 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] += all_far ? far[n] : bias_at(p[n] - base - (j + e / 4 * 16 + e % 4), head[n]);
-            }
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!seen[n](j + e / 4 * 16 + e % 4)) x[e] = -kInf;
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
-            top = quads_max(top) * factor;
-            if (ballot(top > m[n] + kSlack) != 0) {
-                const float next = fmaxf(m[n], top);
+            for (int n = 0; n < COLS; ++n) {
+                const float next = fmaxf(m[n], top[n]);
                 const float keep = m[n] == next ? 1.f : exp2_fast(m[n] - next);
                 m[n] = next;
                 l[n] *= keep;
 #pragma unroll
                 for (int d = 0; d < kOut; ++d) o[d][n] *= keep;
             }
-            const float less = m[n] == -kInf ? 0.f : m[n];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = exp2_fast(__builtin_fmaf(x[e], factor, -less));
-                l[n] += x[e];
-            }
-#pragma unroll
-            for (int f = 0; f < 8 / kPerFrag<C>; ++f) split<C, kW>(x + f * kPerFrag<C>, w[n][f]);
         }
-        lanes_exchange();
 #pragma unroll
-        for (int d = 0; d < kOut; ++d)
+        for (int n = 0; n < COLS; ++n) {
+            const float less = m[n] == -kInf ? 0.f : m[n];
+            float x[8];
 #pragma unroll
-            for (int f = 0; f < 8 / kPerFrag<C>; ++f) {
-                const i32x4 x = In::values(values, f, d);
+            for (int e = 0; e < 8; ++e) x[e] = exp2_fast(__builtin_fmaf(s[n][e / 4][e % 4], factor, -less));
+            l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-                for (int n = 0; n < COLS; ++n)
+            for (int f = 0; f < 8 / kPerFrag<C>; ++f) split<C, kW, true>(x + f * kPerFrag<C>, w[n][f]);
+        }
+    };
+    // The values' operands are read two ahead of their products, the first ones before the
+    // weights are formed.
+    constexpr int kHalves = 8 / kPerFrag<C>, kSteps = kOut * kHalves, kBefore = 2;
+    i32x4 vf[kBefore];
+    auto ahead = [&](const char* values) {
 #pragma unroll
-                    for (int y = 0; y < kW; ++y) o[d][n] = mma16<C>(x, w[n][f][y], o[d][n]);
-            }
-        lanes_exchange();
+        for (int x = 0; x < kBefore; ++x) vf[x] = In::values(values, x % kHalves, x / kHalves);
+    };
+    auto add = [&](const char* values) {
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x) {
+            const i32x4 f = vf[x % kBefore];
+            const int then = x + kBefore;
+            if (then < kSteps) vf[x % kBefore] = In::values(values, then % kHalves, then / kHalves);
+            keep_order();
+#pragma unroll
+            for (int n = 0; n < COLS; ++n)
+#pragma unroll
+                for (int y = 0; y < kW; ++y) o[x / kHalves][n] = mma16<C>(f, w[n][x % kHalves][y], o[x / kHalves][n]);
+        }
+    };
+    if constexpr (kShared) {
+        // Two sets of tiles in LDS: one barrier a tile.
+        char* now = lds;
+        if (tile < end) in.store(now);
+        __syncthreads();
+        for (; tile < end; ++tile) {
+            if (tile + 1 < end) fetch(tile + 1);
+            const int at = kKeys * key_wave;
+            const char* const values = now + (Sh::kRows + at) * Sh::TileT::kStride;
+            i32x4 kf[2][kFrags];
+#pragma unroll
+            for (int c = 0; c < kFrags; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) kf[u][c] = Sh::keys(now, at + 16 * u, c);
+            keep_order();
+            score([&](int u, int c) { return kf[u][c]; });
+            ahead(values);
+            keep_order();
+            weigh(range[0], range[0].first_key(tile) + at);
+            add(values);
+            now = now == lds ? lds + Sh::kBytes : lds;
+            if (tile + 1 < end) in.store(now);
+            __syncthreads();
+        }
+    } else {
+        char* const values = lds + wave * In::kTileBytes;
+        for (; tile < end; tile += WAVES) {
+            score([&](int u, int c) { return in.keys(u, c); });
+            in.store_values(values);
+            if (tile + WAVES < end) fetch(tile + WAVES);
+            lanes_exchange();
+            ahead(values);
+            if (kRanges == 2 && tile >= first_range) weigh(range[kRanges - 1], range[kRanges - 1].first_key(tile - first_range));
+            else weigh(range[0], range[0].first_key(tile));
+            add(values);
+            lanes_exchange();
+        }
     }
 
     // The waves' parts, brought to their common maximum and added in order.
@@ -550,31 +751,32 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     for (int n = 0; n < COLS; ++n) {
         l[n] = quads_sum(l[n]);
         if (quad == 0) {
-            tops[wave * kRows + 16 * n + col] = m[n];
-            totals[wave * kRows + 16 * n + col] = l[n];
+            tops[key_wave * kRows + w0 + 16 * n + col] = m[n];
+            totals[key_wave * kRows + w0 + 16 * n + col] = l[n];
         }
     }
     __syncthreads();  // also: the tiles' LDS is free
     float top[COLS], sum[COLS];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        top[n] = tops[16 * n + col];
+        top[n] = tops[w0 + 16 * n + col];
 #pragma unroll
-        for (int x = 1; x < kStepWaves; ++x) top[n] = fmaxf(top[n], tops[x * kRows + 16 * n + col]);
+        for (int x = 1; x < kKeyWaves; ++x) top[n] = fmaxf(top[n], tops[x * kRows + w0 + 16 * n + col]);
         const float less = top[n] == -kInf ? 0.f : top[n];
         sum[n] = 0.f;
 #pragma unroll
-        for (int x = 0; x < kStepWaves; ++x) sum[n] += totals[x * kRows + 16 * n + col] * exp2_fast(tops[x * kRows + 16 * n + col] - less);
+        for (int x = 0; x < kKeyWaves; ++x)
+            sum[n] += totals[x * kRows + w0 + 16 * n + col] * exp2_fast(tops[x * kRows + w0 + 16 * n + col] - less);
         mine_by[n] = exp2_fast(m[n] - less);
     }
     float* const sums = reinterpret_cast<float*>(lds);
-    for (int x = 0; x < kStepWaves; ++x) {
-        if (x == wave) {
+    for (int x = 0; x < kKeyWaves; ++x) {
+        if (x == key_wave) {
 #pragma unroll
             for (int n = 0; n < COLS; ++n)
 #pragma unroll
                 for (int d = 0; d < kOut; ++d) {
-                    f32x4* const at = reinterpret_cast<f32x4*>(sums + (16 * n + col) * kSumStride + 16 * d + 4 * quad);
+                    f32x4* const at = reinterpret_cast<f32x4*>(sums + (w0 + 16 * n + col) * kSumStride + 16 * d + 4 * quad);
                     f32x4 y = x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : *at;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[d][n][e], mine_by[n], y[e]);
@@ -583,17 +785,17 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         }
         __syncthreads();
     }
-    if (quad == 0 && wave == 0) {
+    if (quad == 0 && key_wave == 0) {
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            tops[16 * n + col] = top[n];
-            totals[16 * n + col] = sum[n];
+            tops[w0 + 16 * n + col] = top[n];
+            totals[w0 + 16 * n + col] = sum[n];
         }
     }
     __syncthreads();
     // Rows of the block, one a wave at a time: out, or the split's part of it.
-    for (int row = wave; row < rows; row += kStepWaves) {
-        const int r = r0 + row, in_b = START ? r % per : r, bb = START ? r / per : b0;
+    for (int row = wave; row < rows; row += WAVES) {
+        const int r = r0 + row, in_b = kManySequences ? r % per : r, bb = kManySequences ? r / per : b0;
         const int i = in_b / group, h = g * group + in_b % group;
         float x0 = lane < a.D ? sums[row * kSumStride + lane] : 0.f;
         float x1 = lane + kWave < a.D ? sums[row * kSumStride + lane + kWave] : 0.f;
@@ -610,17 +812,22 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
             x0 = x1 = 0.f;
         } else if (none ? ballot(masks) != 0 : ballot(n0 || n1) != 0) {
             CarefulKept<T, FORM> c(a, a.q.at<T>(bb, h) + i * a.q.n);
-            const int at = a.start.tokens + (START ? uniform(a.length(bb)) : own_length) - a.Q + i;
-            const Seen sees = seen_of(a, at, base, limit);
+            const int place = a.start.tokens + (kManySequences ? uniform(a.length(bb)) : own_length) - a.Q + i;
             bool done = false;
-            for (int t = begin; t < end && !done; ++t)
-                for (int j = first_key(t); j < first_key(t) + kKeys && !done; ++j)
-                    if (sees(j)) {
-                        const int64_t n = j;
-                        c.add(k + n * kept.kn, v + n * kept.vn, k_scales + n * In::kScales, v_scales + n * In::kScales,
-                              biased ? bias_at(at - base - j, column) : 0.f);
-                        done = none ? c.l != c.l : c.settled(n0, n1);
-                    }
+#pragma unroll
+            for (int x = 0; x < kRanges; ++x) {
+                const Range<kTile, COLS>& at = range[x];
+                const Seen sees = seen_of(a, place, at.base, at.limit);
+                const int before = x == 0 ? 0 : first_range;
+                for (int t = max(begin - before, 0); t < min(end - before, at.tiles) && !done; ++t)
+                    for (int j = at.first_key(t); j < at.first_key(t) + kTile && !done; ++j)
+                        if (sees(j)) {
+                            const int64_t n = j;
+                            c.add(at.k + n * at.kept->kn, at.v + n * at.kept->vn, at.k_scales + n * In::kScales,
+                                  at.v_scales + n * In::kScales, biased ? bias_at(place - at.base - j, column) : 0.f);
+                            done = none ? c.l != c.l : c.settled(n0, n1);
+                        }
+            }
             if (none) {
                 lm = c.m;
                 ll = c.l;
@@ -648,55 +855,92 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 }
 
 // The start's blocks, then the caches'.
-template <typename T, int FORM, int DP, int START_COLS, int OWN_COLS>
-__global__ __launch_bounds__(kStepThreads, START_COLS > 1 || OWN_COLS > 1 || sizeof(T) == 4 ? 1 : 2) void attention_cache_kernel(
+template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int OWN_COLS>
+__global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (FORM < kFour || COLS * ROW_WAVES > 1)) ? 1 : 2) void attention_cache_kernel(
     const CacheArgs a, const CachePlan plan, T* __restrict__ out, float* __restrict__ parts) {
     extern __shared__ __attribute__((aligned(16))) char cache_lds[];
+    constexpr int kStartRows = 16 * COLS * ROW_WAVES, kOwnRows = 16 * OWN_COLS;
     const int64_t block = blockIdx.x, start = plan.start_units * plan.start_splits;
     if (block < start) {
-        const int split_at = static_cast<int>(block % plan.start_splits);
-        const int unit = static_cast<int>(block / plan.start_splits);
-        attention_part<T, FORM, DP, START_COLS, true>(
-            a, out, parts + block * (16 * START_COLS) * part_width(DP), 0, unit / plan.start_blocks,
-            unit % plan.start_blocks * (16 * START_COLS), split_at, plan.start_splits, cache_lds);
+        // The row blocks of the same keys are eight blocks apart, on one XCD (whose L2 then
+        // holds the keys for all of them).
+        const uint32_t all = static_cast<uint32_t>(a.G * plan.start_splits), eights = 8u * plan.start_blocks;
+        const uint32_t some = static_cast<uint32_t>(block) / eights, left = min(8u, all - 8 * some), in = static_cast<uint32_t>(block) % eights;
+        const uint32_t keys = 8 * some + in % left, row_block = in / left;
+        const int split_at = static_cast<int>(keys % plan.start_splits), g = static_cast<int>(keys / plan.start_splits);
+        const int64_t place = (static_cast<int64_t>(g) * plan.start_blocks + row_block) * plan.start_splits + split_at;
+        attention_part<T, FORM, DP, COLS, ROW_WAVES, kStepWaves, kStart>(a, out, parts + place * kStartRows * part_width(DP), 0, g,
+                                                           static_cast<int>(row_block) * kStartRows, split_at, plan.start_splits, cache_lds);
     } else {
         const int64_t at = block - start;
         const int split_at = static_cast<int>(at % plan.own_splits);
         const int64_t unit = at / plan.own_splits, bg = unit / plan.own_blocks;
-        attention_part<T, FORM, DP, OWN_COLS, false>(
-            a, out, plan.direct ? nullptr : parts + plan.start_floats + at * (16 * OWN_COLS) * part_width(DP),
-            static_cast<int>(bg / a.G), static_cast<int>(bg % a.G), static_cast<int>(unit % plan.own_blocks) * (16 * OWN_COLS),
-            split_at, plan.own_splits, cache_lds);
+        attention_part<T, FORM, DP, OWN_COLS, 1, kStepWaves, kOwn>(
+            a, out, plan.direct ? nullptr : parts + plan.start_floats + at * kOwnRows * part_width(DP), static_cast<int>(bg / a.G),
+            static_cast<int>(bg % a.G), static_cast<int>(unit % plan.own_blocks) * kOwnRows, split_at, plan.own_splits, cache_lds);
     }
 }
 
-// Columns of 16 rows that one wave takes at once where there are more than 16 rows: as
-// many as its registers hold.
-constexpr int kManyCols = 2;
+// Few keys: a sequence's rows with all that they see, the start's keys among them, in
+// one block, without parts.  Eight waves, so that each has few tiles one after the other;
+// four where the registers do not hold more.
+constexpr int direct_waves(int size, int form, int DP) { return size == 4 && form < kFour && DP > 64 ? 4 : 8; }
+
+template <typename T, int FORM, int DP>
+__global__ __launch_bounds__(kWave * direct_waves(sizeof(T), FORM, DP), direct_waves(sizeof(T), FORM, DP) / 4) void attention_direct_kernel(
+    const CacheArgs a, T* __restrict__ out) {
+    extern __shared__ __attribute__((aligned(16))) char cache_lds[];
+    attention_part<T, FORM, DP, 1, 1, direct_waves(sizeof(T), FORM, DP), kBoth>(
+        a, out, nullptr, static_cast<int>(blockIdx.x / a.G), static_cast<int>(blockIdx.x % a.G), 0, 0, 1, cache_lds);
+}
+
+// Kernels: rows of a start's block, 16 COLS of ROW_WAVES waves, and 16 OWN_COLS of a cache's.
+enum Shape { kDirect, kOne, kTwo, kTwoTwo, kPairs, kPairsTwo, kShapes };
+struct ShapeRows {
+    int cols, row_waves, own_cols;
+};
+constexpr ShapeRows kShapeRows[kShapes] = {{1, 1, 1}, {1, 1, 1}, {2, 1, 1}, {2, 1, 2}, {2, 2, 1}, {2, 2, 2}};
 
 template <typename T, int FORM>
 hipError_t launch_cache_form(const CacheArgs& a, const CachePlan& plan, void* out, float* parts, hipStream_t stream) {
-    constexpr int M = kManyCols;
-    const int64_t blocks = plan.start_units * plan.start_splits + plan.own_units * plan.own_splits;
     return with_width(a.D, [&](auto width) {
         constexpr int DP = decltype(width)::value;
-        const int which = plan.start_cols == 1 ? 0 : plan.own_cols == 1 ? 1 : 2;
-        auto* kernel = attention_cache_kernel<T, FORM, DP, M, M>;
+        auto launch = [&](auto* kernel, std::atomic<uint64_t>& allowed, int64_t blocks, int waves, size_t lds, auto... rest) {
+            if (lds > kMostLds) return hipErrorInvalidValue;
+            if (lds > kLdsFree) {
+                const hipError_t err = allow_lds(kernel, allowed, kMostLds);
+                if (err != hipSuccess) return err;
+            }
+            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kWave * waves), lds, stream, a, rest...);
+            return hipGetLastError();
+        };
+        auto parted = [&](auto shape) {
+            constexpr ShapeRows R = kShapeRows[decltype(shape)::value];
+            using Start = StepLds<T, FORM, DP, R.cols, R.row_waves, kStepWaves>;
+            using Own = StepLds<T, FORM, DP, R.own_cols, 1, kStepWaves>;
+            static std::atomic<uint64_t> allowed;
+            return launch(attention_cache_kernel<T, FORM, DP, R.cols, R.row_waves, R.own_cols>, allowed,
+                          plan.start_units * plan.start_splits + plan.own_units * plan.own_splits, kStepWaves,
+                          std::max(Start::kBytes + bias_lds(a, Start::kRows), Own::kBytes + bias_lds(a, Own::kRows)), plan,
+                          static_cast<T*>(out), parts);
+        };
         if constexpr (FORM != kAny) {  // (whose plans have no others)
-            if (which == 0) kernel = attention_cache_kernel<T, FORM, DP, 1, 1>;
-            if (which == 1) kernel = attention_cache_kernel<T, FORM, DP, M, 1>;
+            switch (plan.shape) {
+                case kDirect: {
+                    constexpr int W = direct_waves(sizeof(T), FORM, DP);
+                    using L = StepLds<T, FORM, DP, 1, 1, W>;
+                    static std::atomic<uint64_t> allowed;
+                    return launch(attention_direct_kernel<T, FORM, DP>, allowed, plan.own_units, W,
+                                  L::kBytes + bias_lds(a, L::kRows), static_cast<T*>(out));
+                }
+                case kOne: return parted(std::integral_constant<int, kOne>{});
+                case kTwo: return parted(std::integral_constant<int, kTwo>{});
+                case kPairs: return parted(std::integral_constant<int, kPairs>{});
+                case kPairsTwo: return parted(std::integral_constant<int, kPairsTwo>{});
+                default: break;
+            }
         }
-        const size_t one = kStepLds<T, FORM, DP, 1> + bias_lds(a, 1), many = kStepLds<T, FORM, DP, M> + bias_lds(a, M);
-        const size_t lds = which == 0 ? one : which == 1 ? std::max(one, many) : many;
-        if (lds > kLdsFree) {
-            static std::atomic<uint64_t> allowed[3];
-            const size_t most = std::max(kStepLds<T, FORM, DP, 1> + bias_most(1), kStepLds<T, FORM, DP, M> + bias_most(M));
-            const hipError_t err = allow_lds(kernel, allowed[which], most);
-            if (err != hipSuccess) return err;
-        }
-        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kStepThreads), lds, stream, a, plan,
-                           static_cast<T*>(out), parts);
-        return hipGetLastError();
+        return parted(std::integral_constant<int, kTwoTwo>{});
     });
 }
 

@@ -312,10 +312,14 @@ def window_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
 
 
 # ------------------------------------------------------------ quantized cache
-# pointops_cache, pointops_keys and pointops_cache_attention of pointops_hip.h.
+# pointops_cache, pointops_keys and pointops_cache_attention of pointops_hip.h; of the
+# last, with both keys given as they are or packed.
 _CACHE = struct.Struct("@4Q6qi4x")
 _KEYS = struct.Struct("@4Q7q")
-_CACHE_ARGS = struct.Struct("@Q88s88s3Q3q5q2q5if")
+_STEP_RAW = struct.Struct("@Q4Q7q4Q7q3Q3q5q2q5if")
+_STEP_CODED = struct.Struct("@Q88s88s3Q3q5q2q5if")
+_NO_KEYS = bytes(_KEYS.size)
+_THREE = ctypes.c_int64 * 3
 _GROUP = 32
 
 
@@ -333,8 +337,12 @@ class QuantizedCache:
 
     ``k_codes, v_codes (batch, heads, tokens, bytes)`` and ``k_scales, v_scales (batch,
     heads, tokens, groups)`` are uint8 and zeros (values of zero) at first; a row's
-    bytes are ``width`` rounded up to a multiple of 32, or half of that.
+    bytes are ``width`` rounded up to a multiple of 32, or half of that.  Their contents
+    may be copied and changed, the tensors themselves stay.
     """
+
+    __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales", "batch", "tokens", "heads", "width", "bits", "device",
+                 "_pointers", "_keys", "_packed")
 
     def __init__(self, batch: int, tokens: int, heads: int, width: int, *, bits: int = 8,
                  device: torch.device | str = "cuda"):
@@ -344,98 +352,79 @@ class QuantizedCache:
             raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
         if min(batch, tokens, heads) < 0 or max(batch, tokens, heads) > _MAX_TOKENS:
             raise ValueError(f"sizes must lie in [0, {_MAX_TOKENS}]")
-        self.width, self.bits = int(width), int(bits)
         groups = -(-width // _GROUP)
-        self.k_codes, self.v_codes = (torch.zeros((batch, heads, tokens, groups * _GROUP * bits // 8), dtype=torch.uint8,
-                                                  device=device) for _ in range(2))
-        self.k_scales, self.v_scales = (torch.zeros((batch, heads, tokens, groups), dtype=torch.uint8, device=device)
-                                        for _ in range(2))
+        self._hold([torch.zeros((batch, heads, tokens, size), dtype=torch.uint8, device=device)
+                    for size in (groups * _GROUP * bits // 8, groups * _GROUP * bits // 8, groups, groups)], width, bits)
 
-    @property
-    def batch(self) -> int:
-        return self.k_codes.shape[0]
+    def _hold(self, tensors: list[Tensor], width: int, bits: int) -> None:
+        shape = tensors[0].shape
+        pointers = tuple(t.data_ptr() for t in tensors)
+        row = tensors[2].shape[3]
+        batch, head = (stride // row for stride in tensors[2].stride()[:2])  # in rows, of all four alike
+        values = (*tensors, shape[0], shape[2], shape[1], int(width), int(bits), tensors[0].device, pointers,
+                  _KEYS.pack(*pointers, batch, 1, head, batch, 1, head, shape[2]),
+                  _CACHE.pack(*pointers, batch, head, shape[0], shape[2], shape[1], width, bits))
+        for name, value in zip(self.__slots__, values):
+            object.__setattr__(self, name, value)
 
-    @property
-    def heads(self) -> int:
-        return self.k_codes.shape[1]
-
-    @property
-    def tokens(self) -> int:
-        return self.k_codes.shape[2]
-
-    @property
-    def device(self) -> torch.device:
-        return self.k_codes.device
+    def __setattr__(self, name: str, value) -> None:
+        raise AttributeError(f"a cache's {name} stays as it was made: copy into its tensors")
 
     def _view(self, dim: int, first: int, count: int) -> QuantizedCache:
         if first < 0 or count < 0 or first + count > self.k_codes.shape[dim]:
             raise ValueError(f"there are {self.k_codes.shape[dim]} of these")
         view = object.__new__(QuantizedCache)
-        view.width, view.bits = self.width, self.bits
-        for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
-            setattr(view, name, getattr(self, name).narrow(dim, first, count))
+        view._hold([t.narrow(dim, first, count) for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales)],
+                   self.width, self.bits)
         return view
 
-    def first(self, tokens: int) -> QuantizedCache:
-        """The first ``tokens`` positions, in the same memory."""
-        return self._view(2, 0, tokens)
+    def positions(self, start: int, stop: int) -> QuantizedCache:
+        """Positions start .. stop - 1 as a cache, in the same memory."""
+        return self._view(2, start, stop - start)
 
     def cloud(self, index: int) -> QuantizedCache:
         """One cloud's cache (a batch of one), in the same memory."""
         return self._view(0, index, 1)
-
-    def _check(self) -> None:
-        """The tensors are those of the constructor or views of them."""
-        row = -(-self.width // _GROUP)
-        shape = self.k_codes.shape
-        for t, size in ((self.k_codes, row * _GROUP * self.bits // 8), (self.v_codes, row * _GROUP * self.bits // 8),
-                        (self.k_scales, row), (self.v_scales, row)):
-            if (t.dtype != torch.uint8 or t.shape != (*shape[:3], size) or t.device != self.k_codes.device
-                    or (t.numel() and (t.stride(3) != 1 and size > 1 or t.stride(2) != size and shape[2] > 1
-                                       or t.stride(0) * row != self.k_scales.stride(0) * size
-                                       or t.stride(1) * row != self.k_scales.stride(1) * size))):
-                raise ValueError("the cache's tensors must keep their types, shapes and strides")
-
-    def _strides(self) -> tuple[int, int]:
-        """Of batch and key head, in rows."""
-        row = self.k_scales.shape[3]
-        return self.k_scales.stride(0) // row, self.k_scales.stride(1) // row
-
-    def _pack(self) -> bytes:
-        return _CACHE.pack(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scales.data_ptr(),
-                           self.v_scales.data_ptr(), *self._strides(), *self.k_codes.shape[:1], self.tokens, self.heads,
-                           self.width, self.bits)
 
     def __repr__(self) -> str:
         return (f"QuantizedCache(batch={self.batch}, tokens={self.tokens}, heads={self.heads}, width={self.width}, "
                 f"bits={self.bits}, device='{self.device}')")
 
 
-def _check_places(batch: int, device: torch.device, **places) -> None:
-    for name, t in places.items():
-        if t is None:
-            continue
-        if not isinstance(t, Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"{name} must be int32 or int64")
-        if t.shape != (batch,):
-            raise ValueError(f"{name} must have shape (batch,)")
-        if t.device != device:
-            raise ValueError(f"{name} must be on the same device")
-
-
-def _not_traced(name: str) -> None:
-    if not _native.untraced():
-        raise RuntimeError(f"{name} works on a cache's memory: traces, transforms and forward-mode differentiation "
-                           "do not see it")
-
-
-def _cache_of(cache, name: str = "cache") -> QuantizedCache:
-    if not isinstance(cache, QuantizedCache):
+def _check_cache(cache, name: str = "cache") -> None:
+    if type(cache) is not QuantizedCache:
         raise TypeError(f"{name} must be a QuantizedCache")
-    cache._check()
-    return cache
+    if cache._pointers != (cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scales.data_ptr(),
+                           cache.v_scales.data_ptr()):
+        raise ValueError(f"{name}'s tensors have lost their memory")
+
+
+def _check_places(name: str, places, batch: int, device: torch.device) -> None:
+    if not isinstance(places, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if places.dtype not in _PLACES:
+        raise TypeError(f"{name} must be int32 or int64")
+    if places.shape != (batch,):
+        raise ValueError(f"{name} must have shape (batch,)")
+    if places.device != device:
+        raise ValueError(f"{name} must be on the same device")
+
+
+_PLACES = {torch.int32: 32, torch.int64: 64}
+
+
+def _place_args(places: Tensor | None) -> tuple[Tensor | None, int, int]:
+    """The tensor, its address and its bits."""
+    if places is None:
+        return None, 0, 0
+    places = places.contiguous()
+    return places, places.data_ptr(), _PLACES[places.dtype]
+
+
+def _check_untraced(name: str) -> None:
+    if not _native.untraced():
+        raise RuntimeError(f"{name} works on kept memory: traces, transforms and forward-mode differentiation "
+                           "do not see it")
 
 
 def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | None = None, *,
@@ -449,113 +438,125 @@ def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | N
     stay as they are.  k and v are float32, float16 or bfloat16 with any strides; the
     rounding to codes has no gradient.
     """
-    _not_traced("cache_write")
-    _cache_of(cache)
-    _check_heads({"k": k, "v": v})
-    if k.shape != v.shape:
+    _check_untraced("cache_write")
+    _check_cache(cache)
+    if not isinstance(k, Tensor) or not isinstance(v, Tensor):
+        raise TypeError("k and v must be tensors")
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.ndim != 4:
+        raise ValueError("k and v must have shape (batch, tokens, heads, width)")
+    if v.shape != shape:
         raise ValueError("k and v must have the same shape")
-    if (k.shape[0], k.shape[2], k.shape[3]) != (cache.batch, cache.heads, cache.width):
+    if dtype not in _TYPES:
+        raise TypeError("k and v must be float32, float16 or bfloat16")
+    if v.dtype != dtype:
+        raise TypeError("k and v must have the same type")
+    batch, tokens, heads, width = shape
+    if batch != cache.batch or heads != cache.heads or width != cache.width:
         raise ValueError("k and v must have the cache's batch size, heads and width")
-    if k.shape[1] > _MAX_TOKENS:
+    if tokens > _MAX_TOKENS:
         raise ValueError(f"sizes must be at most {_MAX_TOKENS}")
-    if k.device != cache.device:
+    device = k.device
+    if device != cache.device or v.device != device:
         raise ValueError("k and v must be on the cache's device")
-    _check_places(cache.batch, cache.device, lengths=lengths, starts=starts)
-    _native.require_device(k.device)
+    if lengths is not None:
+        _check_places("lengths", lengths, batch, device)
+    if starts is not None:
+        _check_places("starts", starts, batch, device)
+    _native.require_device(device)
     if _tracked(k, v):
         raise ValueError("cache_write has no gradients: call it under torch.no_grad()")
-    if not k.numel() or not cache.tokens:
+    if not (batch and tokens and heads and cache.tokens):
         return
     k, v = _rows(k), _rows(v)
-    lengths, starts = (None if t is None else t.contiguous() for t in (lengths, starts))
-    three = ctypes.c_int64 * 3
-    _native.call("pointops_cache_write", cache._pack(), k.data_ptr(), three(*k.stride()[:3]), v.data_ptr(),
-                 three(*v.stride()[:3]), k.shape[1], _native.ptr(lengths),
-                 0 if lengths is None else 8 * lengths.element_size(), _native.ptr(starts),
-                 0 if starts is None else 8 * starts.element_size(), _TYPES[k.dtype], _native.stream(k.device))
+    lengths, length_at, length_bits = _place_args(lengths)
+    starts, start_at, start_bits = _place_args(starts)
+    _native.call("pointops_cache_write", cache._packed, k.data_ptr(), _THREE(*k.stride()[:3]), v.data_ptr(),
+                 _THREE(*v.stride()[:3]), tokens, length_at, length_bits, start_at, start_bits, _TYPES[dtype],
+                 _native.stream(device))
 
 
 def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
-    """All keys and values of a cache (``cache.first(n)``: of its first n positions),
+    """All keys and values of a cache (of a part: ``cache.positions(start, stop)``),
     ``(B, tokens, G, D)`` each, in float32, float16 or bfloat16, rounded once; float32
     and bfloat16 hold every value exactly but those below their smallest normal
     numbers, float16 those from 2 ** -14 to 65504.
     """
-    _not_traced("cache_read")
-    _cache_of(cache)
+    _check_untraced("cache_read")
+    _check_cache(cache)
     if dtype not in _TYPES:
         raise TypeError("dtype must be float32, float16 or bfloat16")
-    _native.require_device(cache.device)
+    device = cache.device
+    _native.require_device(device)
     shape = cache.batch, cache.tokens, cache.heads, cache.width
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     if k.numel():
-        _native.call("pointops_cache_read", cache._pack(), k.data_ptr(), v.data_ptr(), _TYPES[dtype],
-                     _native.stream(cache.device))
+        _native.call("pointops_cache_read", cache._packed, k.data_ptr(), v.data_ptr(), _TYPES[dtype],
+                     _native.stream(device))
     return k, v
 
 
-def _pack_keys(kept) -> bytes:
-    if kept is None:
-        return bytes(_KEYS.size)
-    if isinstance(kept, QuantizedCache):
-        batch, head = kept._strides()
-        return _KEYS.pack(kept.k_codes.data_ptr(), kept.v_codes.data_ptr(), kept.k_scales.data_ptr(),
-                          kept.v_scales.data_ptr(), batch, 1, head, batch, 1, head, kept.tokens)
-    k, v = kept
-    return _KEYS.pack(k.data_ptr(), v.data_ptr(), 0, 0, *k.stride()[:3], *v.stride()[:3], k.shape[1])
-
-
-def _cache_step(name: str, q: Tensor, start, own, lengths, bits, window, sinks, bias, max_distance, scale) -> Tensor:
-    """The step over checked keys: of the start (a batch of one; None) and own."""
+def _check_step(q, key_heads: int, tokens: int, window, sinks, bias, max_distance, lengths):
+    """The bias's edges."""
     batch, queries, heads, width = q.shape
-    key_heads = own.heads if bits else own[0].shape[2]
-    edges = None
+    if not 1 <= width <= _MAX_HEAD:
+        raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
     if heads and (key_heads == 0 or heads % key_heads):
         raise ValueError("the number of query heads must be a multiple of the number of key heads")
-    tokens = own.tokens if bits else own[0].shape[1]
-    if start is not None:
-        tokens += start.tokens if bits else start[0].shape[1]
-    if max(batch * queries * max(heads, 1), tokens) > _MAX_TOKENS:
+    if batch * queries * heads > _MAX_TOKENS or max(batch, queries, heads, tokens) > _MAX_TOKENS:
         raise ValueError(f"queries of all heads and keys must be at most {_MAX_TOKENS}")
     if window is not None and window < 1:
         raise ValueError("window must be at least 1")
     if sinks < 0:
         raise ValueError("sinks must be non-negative")
-    if bias is not None:
-        if not isinstance(bias, Tensor):
-            raise TypeError("bias must be a tensor")
-        if bias.dtype != q.dtype:
-            raise TypeError("bias must have q's type")
-        if bias.device != q.device:
-            raise ValueError("bias must be on q's device")
-        edges = _check_table(bias, heads, max_distance, True, _MAX_REACH, "bias")
-        bias = bias.contiguous()
-    _check_places(batch, q.device, lengths=lengths)
-    _native.require_device(q.device)
-    if _tracked(q, bias, *(() if bits else (*(start or ()), *own))):
-        raise ValueError(f"{name} has no gradients: call it under torch.no_grad()")
+    if lengths is not None:
+        _check_places("lengths", lengths, batch, q.device)
+    if bias is None:
+        return None
+    if not isinstance(bias, Tensor):
+        raise TypeError("bias must be a tensor")
+    if bias.dtype != q.dtype:
+        raise TypeError("bias must have q's type")
+    if bias.device != q.device:
+        raise ValueError("bias must be on q's device")
+    return _check_table(bias, heads, max_distance, True, _MAX_REACH, "bias")
+
+
+def _check_query(q) -> None:
+    if not isinstance(q, Tensor):
+        raise TypeError("q must be a tensor")
+    if q.ndim != 4:
+        raise ValueError("q must have shape (batch, tokens, heads, width)")
+    if q.dtype not in _TYPES:
+        raise TypeError("q must be float32, float16 or bfloat16")
+
+
+def _kept_step(q, keys, key_heads, tokens, bits, lengths, window, sinks, bias, edges, scale) -> Tensor:
+    """The step over checked keys: the arguments of pointops_keys of the start and of the
+    clouds' own, in one list, or both packed."""
     out = _like(q)
+    shape, device = q.shape, q.device
     if not out.numel():
         return out
     q = _rows(q)
-    if not bits:
-        start, own = (None if pair is None else [_rows(t) for t in pair] for pair in (start, own))
-    lengths = None if lengths is None else lengths.contiguous()
-    args = _CACHE_ARGS.pack(
-        q.data_ptr(), _pack_keys(start), _pack_keys(own), 0 if bias is None else bias.data_ptr(),
-        0 if lengths is None else lengths.data_ptr(), 0 if edges is None else ctypes.addressof(edges), *q.stride()[:3],
-        batch, queries, heads, key_heads, width, tokens + 1 if window is None else min(int(window), tokens + 1),
-        min(int(sinks), tokens), 0 if edges is None else len(edges), 0 if bias is None else bias.shape[0],
-        0 if lengths is None else 8 * lengths.element_size(), _TYPES[q.dtype], bits,
-        float(width ** -0.5 if scale is None else scale))
+    if bias is not None:
+        bias = bias.contiguous()
+    lengths, length_at, length_bits = _place_args(lengths)
+    stride = q.stride()
+    args = (_STEP_CODED if bits else _STEP_RAW).pack(
+        q.data_ptr(), *keys, 0 if bias is None else bias.data_ptr(), length_at,
+        0 if edges is None else ctypes.addressof(edges), stride[0], stride[1], stride[2], shape[0], shape[1], shape[2],
+        key_heads, shape[3], tokens + 1 if window is None else min(int(window), tokens + 1), min(int(sinks), tokens),
+        0 if edges is None else len(edges), 0 if bias is None else bias.shape[0], length_bits, _TYPES[q.dtype], bits,
+        float(shape[3] ** -0.5 if scale is None else scale))
     size = _native.size_query("pointops_cache_attention_step_workspace_bytes", args)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _native.call("pointops_cache_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(q.device))
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _native.call("pointops_cache_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(device))
     return out
 
 
-def _check_coded(q: Tensor, cache: QuantizedCache, name: str, batch: int) -> None:
-    _cache_of(cache, name)
+def _check_coded(q: Tensor, cache, name: str, batch: int) -> None:
+    _check_cache(cache, name)
     if cache.device != q.device:
         raise ValueError(f"{name} must be on q's device")
     if cache.batch != batch:
@@ -571,11 +572,15 @@ def quantized_attention_step(q: Tensor, cache: QuantizedCache, lengths: Tensor |
     that the cache holds, without a further rounding of them, of the queries or of
     the weights.  ``q (B, Q, H, D)`` is float32, float16 or bfloat16.
     """
-    _not_traced("quantized_attention_step")
-    _check_heads({"q": q})
+    _check_untraced("quantized_attention_step")
+    _check_query(q)
     _check_coded(q, cache, "cache", q.shape[0])
-    return _cache_step("quantized_attention_step", q, None, cache, lengths, cache.bits, window, sinks, bias, max_distance,
-                       scale)
+    edges = _check_step(q, cache.heads, cache.tokens, window, sinks, bias, max_distance, lengths)
+    _native.require_device(q.device)
+    if _tracked(q, bias):
+        raise ValueError("quantized_attention_step has no gradients: call it under torch.no_grad()")
+    return _kept_step(q, (_NO_KEYS, cache._keys), cache.heads, cache.tokens, cache.bits, lengths, window, sinks, bias,
+                      edges, scale)
 
 
 def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = None, *, window: int | None = None,
@@ -588,40 +593,58 @@ def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = Non
     first ``lengths (B,)`` hold tokens, the new ones' own among them: the cloud's
     positions are 0 .. P + lengths - 1, and ``q (B, Q, H, D)`` stands at the last Q.
     Or both are a ``QuantizedCache`` of the same bits, the prefix with a batch of one.
-    The start's keys are read once for all queries of the batch.  Without gradients.
+    Where they are long, the start's keys are read once for all queries of the batch.
+    Without gradients.
     """
-    _not_traced("prefix_attention_step")
-    _check_heads({"q": q})
-    coded = isinstance(prefix, QuantizedCache)
-    if coded != isinstance(cache, QuantizedCache):
-        raise TypeError("prefix and cache must both be a QuantizedCache, or both pairs of tensors")
-    if coded:
+    _check_untraced("prefix_attention_step")
+    _check_query(q)
+    if type(prefix) is QuantizedCache or type(cache) is QuantizedCache:
+        if type(prefix) is not type(cache):
+            raise TypeError("prefix and cache must both be a QuantizedCache, or both pairs of tensors")
         _check_coded(q, prefix, "prefix", 1)
         _check_coded(q, cache, "cache", q.shape[0])
         if prefix.bits != cache.bits or prefix.heads != cache.heads:
             raise ValueError("prefix and cache must have the same bits and heads")
-        return _cache_step("prefix_attention_step", q, prefix, cache, lengths, cache.bits, window, sinks, bias, max_distance,
-                           scale)
-    for name, pair in (("prefix", prefix), ("cache", cache)):
-        if not isinstance(pair, (tuple, list)) or len(pair) != 2 or not all(isinstance(t, Tensor) for t in pair):
+        tokens = prefix.tokens + cache.tokens
+        edges = _check_step(q, cache.heads, tokens, window, sinks, bias, max_distance, lengths)
+        _native.require_device(q.device)
+        if _tracked(q, bias):
+            raise ValueError("prefix_attention_step has no gradients: call it under torch.no_grad()")
+        return _kept_step(q, (prefix._keys, cache._keys), cache.heads, tokens, cache.bits, lengths, window, sinks, bias,
+                          edges, scale)
+    dtype, device = q.dtype, q.device
+    for name, pair, dims, shape in (("prefix", prefix, 3, "(tokens, heads, width)"),
+                                    ("cache", cache, 4, "(batch, tokens, heads, width)")):
+        if not isinstance(pair, (tuple, list)) or len(pair) != 2:
             raise TypeError(f"{name} must be a pair of tensors or a QuantizedCache")
-    if any(t.ndim != 3 for t in prefix):
-        raise ValueError("prefix must be two tensors of shape (tokens, heads, width)")
-    start, own = [t[None] for t in prefix], list(cache)
-    _check_heads({"q": q, "prefix's keys": start[0], "prefix's values": start[1], "cache's keys": own[0],
-                  "cache's values": own[1]})
-    for name, (k, v) in (("prefix", start), ("cache", own)):
-        if k.shape != v.shape:
-            raise ValueError(f"{name}'s keys and values must have the same shape")
-        if k.shape[3] != q.shape[3]:
-            raise ValueError(f"{name} must have q's head width")
-    if not 1 <= q.shape[3] <= _MAX_HEAD:
-        raise ValueError(f"the head width must lie in [1, {_MAX_HEAD}]")
-    if own[0].shape[0] != q.shape[0]:
+        for t in pair:
+            if not isinstance(t, Tensor):
+                raise TypeError(f"{name} must be a pair of tensors or a QuantizedCache")
+            if t.ndim != dims:
+                raise ValueError(f"{name} must be two tensors of shape {shape}")
+            if t.dtype != dtype:
+                raise TypeError(f"{name} must have the same type as q")
+            if t.device != device:
+                raise ValueError(f"{name} must be on q's device")
+    (pk, pv), (ck, cv) = prefix, cache
+    start, own = pk.shape, ck.shape
+    if pv.shape != start or cv.shape != own:
+        raise ValueError("keys and values must have the same shape")
+    if own[0] != q.shape[0]:
         raise ValueError("cache must have q's batch size")
-    if start[0].shape[2] != own[0].shape[2]:
+    if start[1] != own[2]:
         raise ValueError("prefix and cache must have the same heads")
-    return _cache_step("prefix_attention_step", q, start, own, lengths, 0, window, sinks, bias, max_distance, scale)
+    if start[2] != q.shape[3] or own[3] != q.shape[3]:
+        raise ValueError("prefix and cache must have q's head width")
+    tokens = start[0] + own[1]
+    edges = _check_step(q, own[2], tokens, window, sinks, bias, max_distance, lengths)
+    _native.require_device(device)
+    if _tracked(q, bias, pk, pv, ck, cv):
+        raise ValueError("prefix_attention_step has no gradients: call it under torch.no_grad()")
+    pk, pv, ck, cv = _rows(pk), _rows(pv), _rows(ck), _rows(cv)
+    keys = (pk.data_ptr(), pv.data_ptr(), 0, 0, 0, *pk.stride()[:2], 0, *pv.stride()[:2], start[0],
+            ck.data_ptr(), cv.data_ptr(), 0, 0, *ck.stride()[:3], *cv.stride()[:3], own[1])
+    return _kept_step(q, keys, own[2], tokens, 0, lengths, window, sinks, bias, edges, scale)
 
 
 # ------------------------------------------------------------- relative bias

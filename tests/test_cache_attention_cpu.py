@@ -29,12 +29,11 @@ def test_layout(width, bits, row, groups):
     assert c.k_scales.shape == c.v_scales.shape == (3, 2, 5, groups)
     assert not c.k_codes.any() and not c.v_scales.any()
     assert (c.batch, c.tokens, c.heads, c.width, c.bits, c.device.type) == (3, 5, 2, width, bits, "cpu")
-    part = c.cloud(2).first(4)
+    part = c.cloud(2).positions(0, 4)
     assert (part.batch, part.tokens, part.heads, part.width, part.bits) == (1, 4, 2, width, bits)
     part.k_codes.fill_(9)
     assert (c.k_codes[2, :, :4] == 9).all() and not c.k_codes[:2].any() and not c.k_codes[2, :, 4].any()
-    for c in (c, part, c.first(0), cache(0, 3, 2, width, bits), cache(1, 1, 1, width, bits)):
-        c._check()
+    assert c.positions(2, 5).k_codes.data_ptr() == c.k_codes.data_ptr() + 2 * row and c.positions(5, 5).tokens == 0
     assert "bits=%d" % bits in repr(part)
 
 
@@ -43,16 +42,18 @@ def test_cache_refusals():
                             ((1, 1, 1, 8), dict(bits=5), "bits")]:
         with pytest.raises(ValueError, match=text):
             QuantizedCache(*args, device="cpu", **how)
-    for wrong in (lambda c: c.first(8), lambda c: c.first(-1), lambda c: c.cloud(2), lambda c: c.cloud(-1)):
+    for wrong in (lambda c: c.positions(0, 8), lambda c: c.positions(-1, 2), lambda c: c.positions(3, 2), lambda c: c.cloud(2), lambda c: c.cloud(-1)):
         with pytest.raises(ValueError, match="there are"):
             wrong(cache())
-    for name, t in (("k_codes", torch.zeros(2, 2, 7, 32)), ("v_codes", torch.zeros(2, 2, 7, 16, dtype=torch.uint8)),
-                    ("k_scales", torch.zeros(2, 2, 8, 1, dtype=torch.uint8)), ("v_scales", torch.zeros(2, 7, 2, 1, dtype=torch.uint8).transpose(1, 2)),
-                    ("k_codes", torch.zeros(2, 2, 7, 64, dtype=torch.uint8)[..., :32])):
-        c = cache()
-        setattr(c, name, t)
-        with pytest.raises(ValueError, match="strides"):
-            attention.cache_write(c, rows(2, 3, 2, 8), rows(2, 3, 2, 8))
+    c = cache()
+    for name in ("k_codes", "v_scales", "width", "other"):
+        with pytest.raises(AttributeError, match="stays"):
+            setattr(c, name, 3)
+    c.v_codes.set_(torch.zeros(1, dtype=torch.uint8))  # memory that a call would read past
+    for call in (lambda: attention.cache_write(c, rows(2, 3, 2, 8), rows(2, 3, 2, 8)), lambda: attention.cache_read(c),
+                 lambda: attention.quantized_attention_step(rows(2, 1, 4, 8), c)):
+        with pytest.raises(ValueError, match="memory"):
+            call()
 
 
 def test_write_refusals():
@@ -194,7 +195,7 @@ def test_c_step_refusals():
         assert step(args) == 1, args
     assert lib.pointops_cache_attention_step_workspace_bytes(None) == 0
     assert step(out=None) == 1
-    parts = packed(start=packed_keys())
+    parts = packed(start=packed_keys(N=100000), window=1 << 20)
     assert lib.pointops_cache_attention_step_workspace_bytes(parts) > 0 and step(parts, workspace=None) == 1
     long = packed(bits=8, window=1 << 20, own=packed_keys(ks=16, vs=16, N=100000))
     assert lib.pointops_cache_attention_step_workspace_bytes(long) > 0 and step(long, workspace=None) == 1

@@ -193,13 +193,13 @@ def test_views(cuda_device):
 
     x = make(7, 3, 20, 2, 72)
     cache = new_cache(3, 20, 2, 72, 4)
-    cache_write(cache.first(5), x[:, :5], x[:, 5:10])
-    cache_write(cache.cloud(1).first(9), x[1:2, 11:], x[1:2, 2:11])
+    cache_write(cache.positions(0, 5), x[:, :5], x[:, 5:10])
+    cache_write(cache.cloud(1).positions(0, 9), x[1:2, 11:], x[1:2, 2:11])
     want = torch.zeros(2, 3, 20, 2, 72, dtype=torch.float64)
     want[0, :, :5], want[1, :, :5] = held(x[:, :5], 4)[0], held(x[:, 5:10], 4)[0]
     want[0, 1, :9], want[1, 1, :9] = held(x[1, 11:], 4)[0], held(x[1, 2:11], 4)[0]
-    for part, cut in ((cache, want), (cache.first(7), want[:, :, :7]), (cache.cloud(2), want[:, 2:3]), (cache.first(0), want[:, :, :0]),
-                      (cache.cloud(1).first(9), want[:, 1:2, :9])):
+    for part, cut in ((cache, want), (cache.positions(3, 7), want[:, :, 3:7]), (cache.cloud(2), want[:, 2:3]), (cache.positions(20, 20), want[:, :, :0]),
+                      (cache.cloud(1).positions(0, 9), want[:, 1:2, :9])):
         k, v = cache_read(part, dtype=torch.float32)
         same(k, cut[0].float())
         same(v, cut[1].float())
@@ -212,9 +212,7 @@ def test_offsets_beyond_32_bits(cuda_device):
     cache = new_cache(1, N, 1, 128, 8)  # 2^32 bytes of codes and more
     x = make(8, 1, 70, 1, 128, dtype=torch.bfloat16)
     cache_write(cache, x, x)
-    tail = cache.first(N)
-    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
-        setattr(tail, name, getattr(cache, name)[:, :, -70:])
+    tail = cache.positions(N - 70, N)
     k, v = cache_read(tail, dtype=torch.float32)
     same(k, held(x, 8)[0].float())
     same(v, held(x, 8)[0].float())
