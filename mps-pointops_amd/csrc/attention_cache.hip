@@ -23,31 +23,50 @@ POINTOPS_FORM(bf16, kFour)
 
 namespace {
 
+struct JoinArgs {
+    int B, Q, H, G, D, group, per, width;
+    int start_rows, own_rows, start_blocks, own_blocks, start_splits, own_splits;
+    int64_t start_floats;
+};
+
 // One wave a row: its parts, of the start's keys and of its own, brought to their common
-// maximum and added in order.
+// maximum and added in order.  The first ones' values are asked for beside the maxima.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const CacheArgs a, const CachePlan plan,
-                                                                        const float* __restrict__ parts, T* __restrict__ out) {
-    const int lane = lane_id(), group = a.H / a.G, per = a.Q * group, width = part_width(padded(a.D));
+__global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const JoinArgs a, const float* __restrict__ parts,
+                                                                        T* __restrict__ out) {
+    const int lane = lane_id(), width = a.width;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;  // (g, b, row)
-    if (id >= static_cast<int64_t>(a.G) * a.B * per) return;
-    const int64_t all = static_cast<int64_t>(a.B) * per, in_g = id % all;
-    const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / per), row = static_cast<int>(in_g % per);
+    const int64_t all = static_cast<int64_t>(a.B) * a.per, in_g = id % all;
+    if (id >= a.G * all) return;
+    const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / a.per), row = static_cast<int>(in_g % a.per);
     // Of each kind: the row's first part, and from one to the next.
-    const int start_rows = plan.start_rows, own_rows = plan.own_rows;
-    const int64_t start_unit = static_cast<int64_t>(g) * plan.start_blocks + in_g / start_rows;
-    const int64_t own_unit = (static_cast<int64_t>(b) * a.G + g) * plan.own_blocks + row / own_rows;
-    const float* const start = parts + (start_unit * plan.start_splits * start_rows + in_g % start_rows) * width;
-    const float* const own = parts + plan.start_floats + (own_unit * plan.own_splits * own_rows + row % own_rows) * width;
-    const int64_t start_step = static_cast<int64_t>(start_rows) * width, own_step = static_cast<int64_t>(own_rows) * width;
-    const int count = plan.start_splits + plan.own_splits;
-    auto part = [&](int s) { return s < plan.start_splits ? start + s * start_step : own + (s - plan.start_splits) * own_step; };
+    const int64_t start_unit = static_cast<int64_t>(g) * a.start_blocks + in_g / a.start_rows;
+    const int64_t own_unit = (static_cast<int64_t>(b) * a.G + g) * a.own_blocks + row / a.own_rows;
+    const float* const start = parts + (start_unit * a.start_splits * a.start_rows + in_g % a.start_rows) * width;
+    const float* const own = parts + a.start_floats + (own_unit * a.own_splits * a.own_rows + row % a.own_rows) * width;
+    const int start_step = a.start_rows * width, own_step = a.own_rows * width;
+    const int count = a.start_splits + a.own_splits;
+    auto part = [&](int s) {
+        return s < a.start_splits ? start + static_cast<int64_t>(s) * start_step
+                                  : own + static_cast<int64_t>(s - a.start_splits) * own_step;
+    };
+    const int c0 = 4 + min(lane, a.D - 1), c1 = 4 + min(lane + kWave, a.D - 1);
+    constexpr int kAtOnce = 16;
+    float y0[kAtOnce], y1[kAtOnce];
+    auto ask = [&](int from) {  // (past the end: the last one again, for which the factor is not used)
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const float* const at = part(min(from + k, count - 1));
+            y0[k] = at[c0];
+            y1[k] = at[c1];
+        }
+    };
+    ask(0);
     float top = -kInf;
     for (int s = lane; s < count; s += kWave) top = fmaxf(top, part(s)[0]);
     top = wave_max(top);
     const float less = top == -kInf ? 0.f : top;
     float sum = 0.f, x0 = 0.f, x1 = 0.f;
-    const int c0 = min(lane, a.D - 1), c1 = min(lane + kWave, a.D - 1);
     for (int from = 0; from < count; from += kWave) {
         // A lane's part: its factor; then the parts' rows one after another.
         const int s = from + lane;
@@ -57,20 +76,12 @@ __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const Ca
             sum = __builtin_fmaf(part(s)[1], by, sum);
         }
         const int some = min(kWave, count - from);
-        constexpr int kAtOnce = 8;
         for (int i = 0; i < some; i += kAtOnce) {
-            float y0[kAtOnce], y1[kAtOnce];
+            if (from + i > 0) ask(from + i);
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
-                const float* const at = part(from + min(i + k, some - 1)) + 4;
-                y0[k] = at[c0];
-                y1[k] = at[c1];
-            }
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                const float f = i + k < some ? i2f(readlane(f2i(by), min(i + k, some - 1))) : 0.f;
-                // (The last part is read again past the end; a factor of 0 does not take away what is no number.)
                 if (i + k < some) {
+                    const float f = i2f(readlane(f2i(by), i + k));
                     x0 = __builtin_fmaf(y0[k], f, x0);
                     x1 = __builtin_fmaf(y1[k], f, x1);
                 }
@@ -79,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const Ca
     }
     sum = wave_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row / group) * a.H + g * group + row % group) * a.D;
+    T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row / a.group) * a.H + g * a.group + row % a.group) * a.D;
     if (lane < a.D) dst[lane] = from_float<T>(x0 * inv);
     if (lane + kWave < a.D) dst[lane + kWave] = from_float<T>(x1 * inv);
 }
@@ -152,9 +163,9 @@ bool read_call(const pointops_cache_attention* in, CacheArgs* out) {
     return true;
 }
 
-// (Strides in bytes.  A tile of 32 rows lies within 2 GiB, on one side of its first.)
+// (Strides in bytes.  A tile of up to 64 rows lies within 2 GiB behind its first.)
 bool pieces(const void* p, int64_t b, int64_t n, int64_t h) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % 16 == 0 && n % 16 == 0 && h % 16 == 0 && n >= 0 && n < (1 << 26);
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % 16 == 0 && n % 16 == 0 && h % 16 == 0 && n >= 0 && n < (1 << 25);
 }
 bool pieces(const Kept& k) { return k.tokens == 0 || (pieces(k.k, k.kb, k.kn, k.kh) && pieces(k.v, k.vb, k.vn, k.vh)); }
 
@@ -167,18 +178,12 @@ int form_of(const pointops_cache_attention& in, CacheArgs* a) {
     return whole && pieces(a->start) && pieces(a->own) ? kAligned : kAny;
 }
 
-#ifndef TARGET1
-#define TARGET1 1024
-#endif
 // Where what a sequence's rows see are so many tiles at most, and so many of all sequences (whose
 // blocks each read the start's keys), one launch of whole rows is shorter than parts and their join.
 constexpr int kDirectTiles = 40, kDirectWork = 16384;
 
-#ifndef TARGET2
-#define TARGET2 512
-#endif
-// Parts that give every compute unit its blocks (four of 16 rows, two of more), at least
-// two tiles a wave; the start's and the caches' as their work is to each other.  By
+// Parts that give every compute unit the two blocks that its registers hold (4 x 65536 tokens in
+// 8 bits: 98 us by 512 blocks, 104 by 1024 in two rounds), at least two tiles a wave; the start's and the caches' as their work is to each other.  By
 // the caches' sizes: the lengths are on the device, and a call does not wait for it.
 CachePlan plan_of(const CacheArgs& a, int form) {
     CachePlan p = {};
@@ -209,7 +214,7 @@ CachePlan plan_of(const CacheArgs& a, int form) {
     p.start_units = some ? static_cast<int64_t>(a.G) * p.start_blocks : 0;
     const double start_work = static_cast<double>(p.start_units) * start_tiles * std::max(1, rows.row_waves);
     const double own_work = static_cast<double>(p.own_units) * own_tiles;
-    const double target = some ? TARGET2 : TARGET1, sum = std::max(1.0, start_work + own_work);
+    const double target = 512, sum = std::max(1.0, start_work + own_work);
     auto splits = [&](double work, int64_t units, int64_t count) {
         const int64_t wanted = static_cast<int64_t>(target * (work / sum) / std::max<int64_t>(1, units) + 0.999);
         return static_cast<int>(std::max<int64_t>(1, std::min(wanted, count / (2 * kStepWaves))));
@@ -240,8 +245,10 @@ hipError_t cache_step(const CacheArgs& a, int form, void* out, void* workspace, 
     const hipError_t err = launch(a, plan, out, parts, stream);
     if (err != hipSuccess || plan.direct) return err;
     const int64_t rows = static_cast<int64_t>(a.B) * a.Q * a.H;
+    const JoinArgs join = {a.B, a.Q, a.H, a.G, a.D, a.H / a.G, a.Q * (a.H / a.G), part_width(padded(a.D)), plan.start_rows, plan.own_rows,
+                           plan.start_blocks, plan.own_blocks, plan.start_splits, plan.own_splits, plan.start_floats};
     hipLaunchKernelGGL(attention_cache_join_kernel<T>, dim3(static_cast<uint32_t>((rows + kWaves - 1) / kWaves)),
-                       dim3(kThreads), 0, stream, a, plan, parts, static_cast<T*>(out));
+                       dim3(kThreads), 0, stream, join, static_cast<const float*>(parts), static_cast<T*>(out));
     return hipGetLastError();
 }
 

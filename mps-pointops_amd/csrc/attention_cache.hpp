@@ -110,23 +110,63 @@ struct Products {
     static constexpr int kWeight = sizeof(T) == 2 ? 2 : kCoded ? 3 : 1;
 };
 
+// Two values rounded to C in one word.
+template <typename C>
+__device__ __forceinline__ int pair_of(float x, float y) {
+    if constexpr (__is_same(C, bf16)) {
+        return __builtin_bit_cast(int, __builtin_convertvector((f32x2{x, y}), bf16x2));
+    } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(int, __builtin_convertvector((f32x2{x, y}), f16x2));
+    }
+}
+template <typename C>
+__device__ __forceinline__ float half_of(int pair, int which) {
+    if constexpr (__is_same(C, bf16)) return i2f(which == 0 ? pair << 16 : pair & static_cast<int>(0xffff0000u));
+    else return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(which == 0 ? pair : pair >> 16)));
+}
+
 // x as N fragments of C that add up to it (of an infinity, FINITE: all but the first are NaN).
 template <typename C, int N, bool FINITE>
 __device__ __forceinline__ void split(const float* x, i32x4 (&out)[N]) {
-    float left[kPerFrag<C>];
+    if constexpr (sizeof(C) == 4) {
+        out[0] = as_fragment<C>(x);
+    } else {
+        float left[8];
 #pragma unroll
-    for (int e = 0; e < kPerFrag<C>; ++e) left[e] = x[e];
+        for (int e = 0; e < 8; ++e) left[e] = x[e];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        out[n] = as_fragment<C>(left);
-        if (n + 1 < N) {
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < kPerFrag<C>; ++e) {
-                const float taken = element<C>(out[n], e);
-                left[e] = FINITE || finite(taken) ? left[e] - taken : 0.f;
+            for (int i = 0; i < 4; ++i) {
+                out[n][i] = pair_of<C>(left[2 * i], left[2 * i + 1]);
+#pragma unroll
+                for (int e = 2 * i; n + 1 < N && e < 2 * i + 2; ++e) {
+                    const float taken = half_of<C>(out[n][i], e % 2);
+                    left[e] = FINITE || finite(taken) ? left[e] - taken : 0.f;
+                }
             }
-        }
     }
+}
+
+// Buffer loads of what is read once and in whole lines: it does not stay in the caches.
+// Of a wave's own values (all its loads at 64 x 2048 bfloat16 tokens, 8 heads of 128, kept: 120 us,
+// values alone past the caches 94, keys too, of whose lines a load takes the half, 121;
+// 4 x 65536 in 8 bits 110, 93, 95; 32 x 8192 in 4 bits 53, 52, 55).
+constexpr int kOnce = 2;
+// An offset behind every buffer: reads there give zeros and touch nothing.
+constexpr uint32_t kNothing = 0x80000000u;
+// A value that stays in its register: left to itself the compiler chooses between two
+// offsets by a branch at every load, each with a wait for the loads before.
+__device__ __forceinline__ uint32_t fixed(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// Rows j0 .. limit - 1 (of `bytes` each; j0 < limit) of those at `base`, as a buffer that ends with the last.
+__device__ __forceinline__ auto rows_from(const void* base, int64_t stride, int j0, int limit, int bytes) {
+    const int64_t all = (limit - 1 - j0) * stride + bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + j0 * stride), 0,
+                                             static_cast<int>(min(all, int64_t(INT32_MAX))), kRawBuffer);
 }
 
 // ------------------------------------------------- 32 keys on their way in
@@ -139,9 +179,11 @@ struct Incoming {
     static constexpr int kFrags = DP * static_cast<int>(sizeof(C)) / 64;  // of a key's row
     using TileT = Tile<C, DP>;
     static constexpr int kTileBytes = kKeys * TileT::kStride;
+    static constexpr bool kWhole = FORM == kFour && DP == 128;  // a row's four lanes hold a group of 32 each
 
     __device__ static __forceinline__ int column(int c, int quad) {
         if constexpr (!kCoded) return (4 * c + quad) * kPerFrag<C>;
+        else if constexpr (kWhole) return quad * 32 + c * 8;
         else return c < DP / 64 * 2 ? c / 2 * 64 + quad * 16 + c % 2 * 8 : c * 32 + quad * 8;
     }
 
@@ -157,75 +199,119 @@ struct Incoming {
     uint32_t kc[kCoded ? 2 : 1][kCoded ? kFrags * kWords : 1], vc[kCoded ? kCodePieces : 1][kCoded ? 2 * kWords : 1];
     uint32_t ks[kCoded ? 2 : 1], vs[kCoded ? kCodePieces : 1];
 
-    template <int N>
-    __device__ static __forceinline__ void words(const uint8_t* p, uint32_t* out) {
-        if constexpr (N == 4) {
-            const i32x4 x = *reinterpret_cast<const i32x4*>(p);
+    // Offsets of this lane's pieces in a tile: of its key in either half, of its first value
+    // and (rows of 96 values) its others, of scales; what lies behind a row's width: kNothing.
+    static constexpr int kVectors = kCoded ? kCodePieces : kPieces, kVectorsPerRow = kCoded ? kCodePerRow : kPerRow;
+    static constexpr bool kSteps = kWave % kVectorsPerRow == 0;  // a lane's values are in one column
+    uint32_t k_at[2], v_at[kSteps ? 1 : kVectors], ks_at[kCoded ? 2 : 1], vs_at[!kCoded ? 1 : kSteps ? 1 : kVectors];
+    uint32_t behind;  // of the last 32 columns of a key's row: kNothing in a lane past the width, else 0 (a bit each of two)
+
+    __device__ __forceinline__ void set(const Kept& kept, int width) {
+        const int lane = lane_id(), col = lane % 16, quad = lane / 16;
+        const uint32_t kn = kCoded ? kRowBytes : static_cast<uint32_t>(kept.kn), vn = kCoded ? kRowBytes : static_cast<uint32_t>(kept.vn);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = x[i];
-        } else if constexpr (N == 2) {
-            const i32x2 x = *reinterpret_cast<const i32x2*>(p);
-            out[0] = x[0];
-            out[1] = x[1];
-        } else {
-            out[0] = *reinterpret_cast<const uint32_t*>(p);
+        for (int u = 0; u < 2; ++u) {
+            k_at[u] = fixed((16 * u + col) * kn + (kCoded ? column(0, quad) * kWords / 2 : 16 * quad));
+            if constexpr (kCoded) ks_at[u] = fixed((16 * u + col) * kScales);
+        }
+#pragma unroll
+        for (int x = 0; x < (kSteps ? 1 : kVectors); ++x) {
+            const uint32_t at = x * kWave + lane, row = at / kVectorsPerRow, piece = at % kVectorsPerRow;
+            const bool past = !kCoded && static_cast<int>(piece) * kPerFrag<T> >= width;
+            v_at[x] = fixed(past ? kNothing : row * vn + piece * (kCoded ? 8 * kWords : 16));
+            if constexpr (kCoded) vs_at[x] = fixed(row * kScales + piece / 2);
+        }
+        if constexpr (!kCoded) {
+            behind = 0;
+#pragma unroll
+            for (int c = kFrags - kLast; c < kFrags; ++c)
+                if (column(c, quad) >= width) behind |= kNothing >> (kFrags - 1 - c);
+            behind = fixed(behind);
         }
     }
+    static constexpr int kLast = static_cast<int>(sizeof(C)) / 2;  // fragments of 32 columns
 
-    // Keys j0 .. j0 + 31 of the head at k and v; from `limit` (> j0) on the last one again, for which
-    // the caller's scores are masked.  A tile's base is uniform, its rows lie within 2 GiB of it.
+    // Keys j0 .. j0 + 31 of the head at k and v; zeros from `limit` (> j0) on, for which the
+    // caller's scores are masked.
     __device__ __forceinline__ void load(const Kept& kept, const char* k, const char* v, const uint8_t* k_scales,
                                          const uint8_t* v_scales, int j0, int limit, int width) {
-        const int lane = lane_id(), col = lane % 16, quad = lane / 16, last = min(limit - 1 - j0, kKeys - 1);
-        if constexpr (!kCoded) {
-            const char* const k0 = k + j0 * kept.kn;
-            const char* const v0 = v + j0 * kept.vn;
+        const int lane = lane_id(), col = lane % 16, quad = lane / 16;
+        if constexpr (FORM == kAny) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const T* const row = reinterpret_cast<const T*>(k0 + at_row(min(16 * u + col, last), kept.kn));
+                const int j = min(j0 + 16 * u + col, limit - 1);
 #pragma unroll
-                for (int c = 0; c < kFrags; ++c) kr[u][c] = load_row<T, FORM == kAligned>(row, column(c, quad), width);
+                for (int c = 0; c < kFrags; ++c) kr[u][c] = load_row<T, false>(reinterpret_cast<const T*>(k + j * kept.kn), column(c, quad), width);
             }
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
-                const int at = x * kWave + lane;
-                const T* const row = reinterpret_cast<const T*>(v0 + at_row(min(at / kPerRow, last), kept.vn));
-                vr[x] = load_row<T, FORM == kAligned>(row, at % kPerRow * kPerFrag<T>, width);
+                const int at = x * kWave + lane, j = min(j0 + at / kPerRow, limit - 1);
+                vr[x] = load_row<T, false>(reinterpret_cast<const T*>(v + j * kept.vn), at % kPerRow * kPerFrag<T>, width);
             }
+        } else if constexpr (FORM == kAligned) {
+            const auto ks = rows_from(k, kept.kn, j0, limit, width * static_cast<int>(sizeof(T)));
+            const auto vs = rows_from(v, kept.vn, j0, limit, width * static_cast<int>(sizeof(T)));
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < kFrags; ++c) {
+                    const uint32_t past = c < kFrags - kLast ? 0 : behind << (kFrags - 1 - c) & kNothing;
+                    kr[u][c] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ks, (k_at[u] + 64 * c) | past, 0, 0));
+                }
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x)
+                vr[x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    vs, kSteps ? v_at[0] + x * (kWave / kPerRow) * static_cast<uint32_t>(kept.vn) : v_at[x], 0, kOnce));
         } else {
-            const uint8_t* const k0 = reinterpret_cast<const uint8_t*>(k) + static_cast<int64_t>(j0) * kRowBytes;
-            const uint8_t* const v0 = reinterpret_cast<const uint8_t*>(v) + static_cast<int64_t>(j0) * kRowBytes;
-            const uint8_t* const ks0 = k_scales + static_cast<int64_t>(j0) * kScales;
-            const uint8_t* const vs0 = v_scales + static_cast<int64_t>(j0) * kScales;
+            const auto k0 = rows_from(k, kRowBytes, j0, limit, kRowBytes), v0 = rows_from(v, kRowBytes, j0, limit, kRowBytes);
+            const auto ks0 = rows_from(k_scales, kScales, j0, limit, kScales), vs0 = rows_from(v_scales, kScales, j0, limit, kScales);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t row = min(16 * u + col, last);
+                if constexpr (kWhole) words<4, 0>(k0, k_at[u], kc[u]);
+                else {
 #pragma unroll
-                for (int c = 0; c + 1 < kFrags; c += 2)
-                    words<2 * kWords>(k0 + (row * kRowBytes + column(c, quad) * kWords / 2), kc[u] + c * kWords);
+                    for (int c = 0; c + 1 < kFrags; c += 2) words<2 * kWords, 0>(k0, k_at[u] + c * 16 * kWords, kc[u] + c * kWords);
+                }
+                // (The last 32 columns: eight a lane, not sixteen.)
                 if constexpr (kFrags % 2 != 0)
-                    words<kWords>(k0 + (row * kRowBytes + column(kFrags - 1, quad) * kWords / 2), kc[u] + (kFrags - 1) * kWords);
-                ks[u] = load_scales(ks0 + row * kScales);
+                    words<kWords, 0>(k0, k_at[u] + (column(kFrags - 1, quad) - (kFrags > 1 ? column(0, quad) : quad * 8)) * kWords / 2,
+                                  kc[u] + (kFrags - 1) * kWords);
+                ks[u] = scale_bytes(ks0, ks_at[u]);
             }
 #pragma unroll
             for (int x = 0; x < kCodePieces; ++x) {
-                const uint32_t at = x * kWave + lane, piece = at % kCodePerRow, row = min(static_cast<int>(at / kCodePerRow), last);
-                words<2 * kWords>(v0 + (row * kRowBytes + piece * 8 * kWords), vc[x]);
-                vs[x] = vs0[row * kScales + piece / 2];
+                words<2 * kWords, kOnce>(v0, kSteps ? v_at[0] + x * (kWave / kCodePerRow) * kRowBytes : v_at[x], vc[x]);
+                vs[x] = __builtin_amdgcn_raw_buffer_load_b8(vs0, kSteps ? vs_at[0] + x * (kWave / kCodePerRow) * kScales : vs_at[x], 0, 0);
             }
         }
     }
-    // Rows of any stride (kAny), or of one whose tile lies within 2 GiB.
-    __device__ static __forceinline__ int64_t at_row(int row, int64_t stride) {
-        if constexpr (FORM == kAligned) return static_cast<uint32_t>(row) * static_cast<uint32_t>(stride);
-        else return row * stride;
+    template <int N, int POLICY, typename R>
+    __device__ static __forceinline__ void words(R rows, uint32_t at, uint32_t* out) {
+        if constexpr (N == 4) {
+            const i32x4 x = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, 0, POLICY));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = x[i];
+        } else if constexpr (N == 2) {
+            const i32x2 x = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, POLICY));
+            out[0] = x[0];
+            out[1] = x[1];
+        } else {
+            out[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, POLICY);
+        }
     }
     // The scales of a row's groups, a byte each.
-    __device__ static __forceinline__ uint32_t load_scales(const uint8_t* p) {
-        if constexpr (kScales == 4) return *reinterpret_cast<const uint32_t*>(p);
-        else if constexpr (kScales == 3) return p[0] | p[1] << 8 | p[2] << 16;
-        else if constexpr (kScales == 2) return *reinterpret_cast<const uint16_t*>(p);
-        else return p[0];
+    template <typename R>
+    __device__ static __forceinline__ uint32_t scale_bytes(R rows, uint32_t at) {
+        if constexpr (kScales == 4) return __builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0);
+        else if constexpr (kScales == 2) return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0));
+        else if constexpr (kScales == 1) return static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rows, at, 0, 0));
+        else {
+            uint32_t all = 0;
+#pragma unroll
+            for (int i = 0; i < kScales; ++i)
+                all |= static_cast<uint32_t>(static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rows, at + i, 0, 0))) << (8 * i);
+            return all;
+        }
     }
 
     // Row operand: keys 16 u + lane % 16, fragment c.
@@ -233,7 +319,7 @@ struct Incoming {
         if constexpr (!kCoded) {
             return kr[u][c];
         } else {
-            const int group = c < DP / 64 * 2 ? c / 2 * 2 + lane_id() / 32 : c;
+            const int group = kWhole ? lane_id() / 16 : c < DP / 64 * 2 ? c / 2 * 2 + lane_id() / 32 : c;
             return decode8<FORM>(kc[u] + c * kWords, scale_of(ks[u] >> (8 * group) & 255));
         }
     }
@@ -335,29 +421,39 @@ struct Shared {
     i32x4 r[2][kPieces];
     uint32_t scale[kCoded ? 2 : 1][kCoded ? kPieces : 1];
 
+    uint32_t at[2][kPieces], scale_at[kCoded ? kPieces : 1];
+
+    __device__ __forceinline__ void set(const Kept& kept, int width) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) {
+                const uint32_t stride = kCoded ? kRowBytes : static_cast<uint32_t>(side == 0 ? kept.kn : kept.vn);
+                const uint32_t n = x * kStepThreads + threadIdx.x, row = n / kPerRow, piece = n % kPerRow;
+                const bool here = (kAll || row < kRows) && (kCoded || static_cast<int>(piece) * kPerFrag<T> < width);
+                at[side][x] = fixed(here ? row * stride + piece * kPieceBytes : kNothing);
+                if constexpr (kCoded)
+                    if (side == 0) scale_at[x] = fixed(here ? row * kScales + piece / 2 : kNothing);
+            }
+    }
     __device__ __forceinline__ void load(const Kept& kept, const char* k, const char* v, const uint8_t* k_scales,
                                          const uint8_t* v_scales, int j0, int limit, int width) {
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-            const int64_t stride = kCoded ? kRowBytes : side == 0 ? kept.kn : kept.vn;
-            const int64_t bytes = (limit - 1 - j0) * stride + (kCoded ? kRowBytes : width * static_cast<int>(sizeof(T)));
-            const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((side == 0 ? k : v) + j0 * stride), 0,
-                                                                static_cast<int>(min(bytes, int64_t(INT32_MAX))), kRawBuffer);
-            const auto scales = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint8_t*>((side == 0 ? k_scales : v_scales) + static_cast<int64_t>(j0) * kScales), 0,
-                static_cast<int>(min(static_cast<int64_t>(limit - j0) * kScales, int64_t(INT32_MAX))), kRawBuffer);
+            const auto rows = rows_from(side == 0 ? k : v, kCoded ? kRowBytes : side == 0 ? kept.kn : kept.vn, j0, limit,
+                                        kCoded ? kRowBytes : width * static_cast<int>(sizeof(T)));
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
-                const uint32_t at = x * kStepThreads + threadIdx.x, row = at / kPerRow, piece = at % kPerRow;
-                const bool here = (kAll || row < kRows) && (kCoded || static_cast<int>(piece) * kPerFrag<T> < width);
-                const uint32_t offset = here ? row * static_cast<uint32_t>(stride) + piece * kPieceBytes : 0x80000000u;
-                if constexpr (kPieceBytes == 16) r[side][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+                if constexpr (kPieceBytes == 16) r[side][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at[side][x], 0, 0));
                 else {
-                    const i32x2 y = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0));
+                    const i32x2 y = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, at[side][x], 0, 0));
                     r[side][x] = i32x4{y[0], y[1], 0, 0};
                 }
-                if constexpr (kCoded)
-                    scale[side][x] = __builtin_amdgcn_raw_buffer_load_b8(scales, here ? row * kScales + piece / 2 : 0x80000000u, 0, 0);
+            }
+            if constexpr (kCoded) {
+                const auto scales = rows_from(side == 0 ? k_scales : v_scales, kScales, j0, limit, kScales);
+#pragma unroll
+                for (int x = 0; x < kPieces; ++x) scale[side][x] = __builtin_amdgcn_raw_buffer_load_b8(scales, scale_at[x], 0, 0);
             }
         }
     }
@@ -535,10 +631,17 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     const int begin = static_cast<int>(static_cast<int64_t>(tiles) * split_at / splits);
     const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split_at + 1) / splits);
     std::conditional_t<kShared, Sh, In> in;
+    in.set(*range[0].kept, a.D);
+    bool in_second = false;
     auto fetch = [&](int tile) {
         const bool second = kRanges == 2 && tile >= first_range;
         const Range<kTile, COLS>& at = range[second ? kRanges - 1 : 0];
-        in.load(*at.kept, at.k, at.v, at.k_scales, at.v_scales, at.first_key(second ? tile - first_range : tile), at.limit, a.D);
+        if (second && !in_second) {  // (whose strides may be others)
+            in.set(*at.kept, a.D);
+            in_second = true;
+        }
+        const int from = at.first_key(second ? tile - first_range : tile);
+        in.load(*at.kept, at.k, at.v, at.k_scales, at.v_scales, from, at.limit, a.D);
     };
     int tile = kShared ? begin : begin + wave;
     if (tile < end) fetch(tile);
