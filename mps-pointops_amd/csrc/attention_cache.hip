@@ -24,75 +24,24 @@ POINTOPS_FORM(bf16, kFour)
 namespace {
 
 struct JoinArgs {
-    int B, Q, H, G, D, group, per, width;
-    int start_rows, own_rows, start_blocks, own_blocks, start_splits, own_splits;
-    int64_t start_floats;
+    int B, Q, H, G, D;
+    Parts start, own;
 };
 
-// One wave a row: its parts, of the start's keys and of its own, brought to their common
-// maximum and added in order.  The first ones' values are asked for beside the maxima.
+// One wave a row: its parts, of the start's keys and of its own.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const JoinArgs a, const float* __restrict__ parts,
                                                                         T* __restrict__ out) {
-    const int lane = lane_id(), width = a.width;
+    const int group = a.H / a.G, per = a.Q * group, width = part_width(padded(a.D));
     const int64_t id = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;  // (g, b, row)
-    const int64_t all = static_cast<int64_t>(a.B) * a.per, in_g = id % all;
+    const int64_t all = static_cast<int64_t>(a.B) * per, in_g = id % all;
     if (id >= a.G * all) return;
-    const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / a.per), row = static_cast<int>(in_g % a.per);
-    // Of each kind: the row's first part, and from one to the next.
-    const int64_t start_unit = static_cast<int64_t>(g) * a.start_blocks + in_g / a.start_rows;
-    const int64_t own_unit = (static_cast<int64_t>(b) * a.G + g) * a.own_blocks + row / a.own_rows;
-    const float* const start = parts + (start_unit * a.start_splits * a.start_rows + in_g % a.start_rows) * width;
-    const float* const own = parts + a.start_floats + (own_unit * a.own_splits * a.own_rows + row % a.own_rows) * width;
-    const int start_step = a.start_rows * width, own_step = a.own_rows * width;
-    const int count = a.start_splits + a.own_splits;
-    auto part = [&](int s) {
-        return s < a.start_splits ? start + static_cast<int64_t>(s) * start_step
-                                  : own + static_cast<int64_t>(s - a.start_splits) * own_step;
-    };
-    const int c0 = 4 + min(lane, a.D - 1), c1 = 4 + min(lane + kWave, a.D - 1);
-    constexpr int kAtOnce = 16;
-    float y0[kAtOnce], y1[kAtOnce];
-    auto ask = [&](int from) {  // (past the end: the last one again, for which the factor is not used)
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            const float* const at = part(min(from + k, count - 1));
-            y0[k] = at[c0];
-            y1[k] = at[c1];
-        }
-    };
-    ask(0);
-    float top = -kInf;
-    for (int s = lane; s < count; s += kWave) top = fmaxf(top, part(s)[0]);
-    top = wave_max(top);
-    const float less = top == -kInf ? 0.f : top;
-    float sum = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int from = 0; from < count; from += kWave) {
-        // A lane's part: its factor; then the parts' rows one after another.
-        const int s = from + lane;
-        float by = 0.f;
-        if (s < count) {
-            by = exp2_fast(part(s)[0] - less);
-            sum = __builtin_fmaf(part(s)[1], by, sum);
-        }
-        const int some = min(kWave, count - from);
-        for (int i = 0; i < some; i += kAtOnce) {
-            if (from + i > 0) ask(from + i);
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                if (i + k < some) {
-                    const float f = i2f(readlane(f2i(by), i + k));
-                    x0 = __builtin_fmaf(y0[k], f, x0);
-                    x1 = __builtin_fmaf(y1[k], f, x1);
-                }
-            }
-        }
-    }
-    sum = wave_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row / a.group) * a.H + g * a.group + row % a.group) * a.D;
-    if (lane < a.D) dst[lane] = from_float<T>(x0 * inv);
-    if (lane + kWave < a.D) dst[lane + kWave] = from_float<T>(x1 * inv);
+    const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / per), row = static_cast<int>(in_g % per);
+    RowSum sum;
+    sum.add(a.start.first(parts, g, in_g, width), static_cast<int64_t>(a.start.rows) * width, a.start.splits, a.D);
+    sum.add(a.own.first(parts + a.start.floats, static_cast<int64_t>(b) * a.G + g, row, width),
+            static_cast<int64_t>(a.own.rows) * width, a.own.splits, a.D);
+    sum.write(out + ((static_cast<int64_t>(b) * a.Q + row / group) * a.H + g * group + row % group) * a.D, a.D);
 }
 
 int size_of(int type) { return type == POINTOPS_F32 ? 4 : 2; }
@@ -142,6 +91,8 @@ bool read_call(const pointops_cache_attention* in, CacheArgs* out) {
     if (keys > limit || in->B * in->Q > limit || in->B * in->Q * in->H > limit) return false;
     a.q = {in->q, in->q_stride[0], in->q_stride[1], in->q_stride[2]};
     a.q_vec = false;
+    a.group = Divisor::of(in->H > 0 ? in->H / in->G : 1);
+    a.per = Divisor::of(in->H > 0 && in->Q > 0 ? in->H / in->G * in->Q : 1);
     a.bias = in->bias;
     a.lengths = in->lengths;
     a.length_bits = in->length_bits;
@@ -178,75 +129,74 @@ int form_of(const pointops_cache_attention& in, CacheArgs* a) {
     return whole && pieces(a->start) && pieces(a->own) ? kAligned : kAny;
 }
 
+// LDS of a start's block whose waves share their keys: two sets of tiles (or the sums), the bias.
+size_t pairs_lds(const CacheArgs& a, int size) {
+    const size_t bytes = padded(a.D) * size, stride = bytes + (bytes == 256 ? 48 : 16), key_waves = kStepWaves / kShapeRows[kPairs].row_waves;
+    const size_t rows = kShapeRows[kPairs].start(), tiles = 4 * kKeys * key_waves * stride, sums = rows * part_width(padded(a.D)) * 4;
+    return std::max(tiles, sums) + 2 * key_waves * rows * 4 + bias_lds(a, static_cast<int>(rows));
+}
+
 // Where what a sequence's rows see are so many tiles at most, and so many of all sequences (whose
 // blocks each read the start's keys), one launch of whole rows is shorter than parts and their join.
 constexpr int kDirectTiles = 40, kDirectWork = 16384;
 
 // Parts that give every compute unit the two blocks that its registers hold (4 x 65536 tokens in
-// 8 bits: 98 us by 512 blocks, 104 by 1024 in two rounds), at least two tiles a wave; the start's and the caches' as their work is to each other.  By
-// the caches' sizes: the lengths are on the device, and a call does not wait for it.
-CachePlan plan_of(const CacheArgs& a, int form) {
+// 8 bits: 98 us by 512 blocks, 104 by 1024 in two rounds), at least two tiles a wave; the start's and
+// the caches' as their work is to each other.  By the caches' sizes: the lengths are on the device, and
+// a call does not wait for it.
+CachePlan plan_of(const CacheArgs& a, int type, int form) {
     CachePlan p = {};
-    const int64_t per = static_cast<int64_t>(a.Q) * (a.H / a.G), all = per * a.B;
-    const bool some = a.start.tokens != 0;
+    const int64_t per = a.per.d, all = per * a.B, width = part_width(padded(a.D));
     const int64_t seen = (static_cast<int64_t>(a.window) + a.Q - 1) / kKeys + 2 + (a.sinks + kKeys - 1) / kKeys;
     auto tiles = [&](int tokens) { return std::min<int64_t>((static_cast<int64_t>(tokens) + kKeys - 1) / kKeys, seen); };
     const int64_t start_tiles = tiles(a.start.tokens), own_tiles = tiles(a.own.tokens);
     // (A window over both sees no more than one over either.)
-    const int64_t all_tiles = std::min(start_tiles + own_tiles, seen + 1);
+    const int64_t both = std::min(start_tiles + own_tiles, seen + 1), heads = static_cast<int64_t>(a.B) * a.G;
+    const bool some = a.start.tokens != 0, pairs = pairs_lds(a, form == kAligned && type == POINTOPS_F32 ? 4 : 2) <= kMostLds;
     if (form == kAny) p.shape = kTwoTwo;
-    else if (per <= 16 && all_tiles <= kDirectTiles && all_tiles * a.B * a.G <= kDirectWork) p.shape = kDirect;
-    else if (per > 16) p.shape = some && all > 32 ? kPairsTwo : kTwoTwo;
+    else if (per <= 16 && both <= kDirectTiles && both * heads <= kDirectWork) p.shape = kDirect;
+    else if (per > 16) p.shape = some && all > 32 && pairs ? kPairsTwo : kTwoTwo;
     else if (!some || all <= 16) p.shape = kOne;
-    else p.shape = all <= 32 ? kTwo : kPairs;
+    else p.shape = all > 32 && pairs ? kPairs : kTwo;
     const ShapeRows rows = kShapeRows[p.shape];
-    p.start_rows = 16 * rows.cols * rows.row_waves;
-    p.own_rows = 16 * rows.own_cols;
-    auto blocks = [](int64_t rows, int each) { return static_cast<int>((rows + each - 1) / each); };
-    p.own_blocks = blocks(per, p.own_rows);
-    p.own_units = static_cast<int64_t>(a.B) * a.G * p.own_blocks;
-    if (p.shape == kDirect) {
-        p.own_splits = 1;
-        p.direct = true;
-        return p;
-    }
-    p.start_blocks = blocks(all, p.start_rows);
-    p.start_units = some ? static_cast<int64_t>(a.G) * p.start_blocks : 0;
-    const double start_work = static_cast<double>(p.start_units) * start_tiles * std::max(1, rows.row_waves);
-    const double own_work = static_cast<double>(p.own_units) * own_tiles;
-    const double target = 512, sum = std::max(1.0, start_work + own_work);
-    auto splits = [&](double work, int64_t units, int64_t count) {
-        const int64_t wanted = static_cast<int64_t>(target * (work / sum) / std::max<int64_t>(1, units) + 0.999);
-        return static_cast<int>(std::max<int64_t>(1, std::min(wanted, count / (2 * kStepWaves))));
+    auto cut = [&](Parts& parts, int each, int64_t rows, int64_t heads) {
+        parts.rows = each;
+        parts.blocks = static_cast<int>((rows + each - 1) / each);
+        parts.units = heads * parts.blocks;
     };
-    p.start_splits = p.start_units == 0 ? 0 : splits(start_work, p.start_units, start_tiles);
-    p.own_splits = splits(own_work, p.own_units, own_tiles);
-    p.direct = p.start_splits == 0 && p.own_splits == 1;
-    p.start_floats = p.start_units * p.start_splits * p.start_rows * part_width(padded(a.D));
+    cut(p.own, rows.own(), per, heads);
+    p.own.splits = 1;
+    if (p.shape == kDirect) return p;
+    if (some) cut(p.start, rows.start(), all, a.G);
+    const double start_work = static_cast<double>(p.start.units) * start_tiles * rows.row_waves;
+    const double own_work = static_cast<double>(p.own.units) * own_tiles, sum = std::max(1.0, start_work + own_work);
+    auto split = [&](Parts& parts, double work, int64_t count) {
+        const int64_t wanted = static_cast<int64_t>(512 * (work / sum) / std::max<int64_t>(1, parts.units) + 0.999);
+        parts.splits = static_cast<int>(std::max<int64_t>(1, std::min(wanted, count / (2 * kStepWaves))));
+        parts.floats = parts.units * parts.splits * parts.rows * width;
+    };
+    if (some) split(p.start, start_work, start_tiles);
+    split(p.own, own_work, own_tiles);
+    p.joined = some || p.own.splits > 1;
     return p;
 }
 
-size_t workspace_of(const CacheArgs& a, const CachePlan& p) {
-    if (p.direct) return 0;
-    return sizeof(float) * (p.start_floats + p.own_units * p.own_splits * p.own_rows * part_width(padded(a.D)));
-}
+size_t workspace_of(const CachePlan& p) { return sizeof(float) * (p.start.floats + (p.joined ? p.own.floats : 0)); }
 
 template <typename T>
-hipError_t cache_step(const CacheArgs& a, int form, void* out, void* workspace, hipStream_t stream) {
-    const CachePlan plan = plan_of(a, form);
-    if (workspace == nullptr && workspace_of(a, plan) != 0) return hipErrorInvalidValue;
-    const int64_t blocks = plan.start_units * plan.start_splits + plan.own_units * plan.own_splits;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+hipError_t cache_step(const CacheArgs& a, int type, int form, void* out, void* workspace, hipStream_t stream) {
+    const CachePlan plan = plan_of(a, type, form);
+    if (workspace == nullptr && workspace_of(plan) != 0) return hipErrorInvalidValue;
+    if (plan.start.units * plan.start.splits + plan.own.units * plan.own.splits > INT32_MAX) return hipErrorInvalidValue;
     float* const parts = static_cast<float*>(workspace);
     const auto launch = form == kAligned ? launch_cache_form<T, kAligned>
                         : form == kAny   ? launch_cache_form<T, kAny>
                         : form == kEight ? launch_cache_form<T, kEight>
                                          : launch_cache_form<T, kFour>;
     const hipError_t err = launch(a, plan, out, parts, stream);
-    if (err != hipSuccess || plan.direct) return err;
+    if (err != hipSuccess || !plan.joined) return err;
     const int64_t rows = static_cast<int64_t>(a.B) * a.Q * a.H;
-    const JoinArgs join = {a.B, a.Q, a.H, a.G, a.D, a.H / a.G, a.Q * (a.H / a.G), part_width(padded(a.D)), plan.start_rows, plan.own_rows,
-                           plan.start_blocks, plan.own_blocks, plan.start_splits, plan.own_splits, plan.start_floats};
+    const JoinArgs join = {a.B, a.Q, a.H, a.G, a.D, plan.start, plan.own};
     hipLaunchKernelGGL(attention_cache_join_kernel<T>, dim3(static_cast<uint32_t>((rows + kWaves - 1) / kWaves)),
                        dim3(kThreads), 0, stream, join, static_cast<const float*>(parts), static_cast<T*>(out));
     return hipGetLastError();
@@ -271,7 +221,7 @@ size_t pointops_cache_attention_step_workspace_bytes(const pointops_cache_attent
     CacheArgs a;
     if (!read_call(in, &a) || a.B == 0 || a.H == 0 || a.Q == 0) return 0;
     const int form = form_of(*in, &a);
-    return workspace_of(a, plan_of(a, form));
+    return workspace_of(plan_of(a, in->type, form));
 }
 
 hipError_t pointops_cache_attention_step(const pointops_cache_attention* in, void* out, void* workspace, hipStream_t stream) {
@@ -283,9 +233,9 @@ hipError_t pointops_cache_attention_step(const pointops_cache_attention* in, voi
     if (in->bits != 0 && (!kept_aligned(a.start, a.D) || !kept_aligned(a.own, a.D))) return hipErrorInvalidValue;
     const int form = form_of(*in, &a);
     switch (in->type) {
-        case POINTOPS_F32: return cache_step<float>(a, form, out, workspace, stream);
-        case POINTOPS_F16: return cache_step<f16>(a, form, out, workspace, stream);
-        default: return cache_step<bf16>(a, form, out, workspace, stream);
+        case POINTOPS_F32: return cache_step<float>(a, in->type, form, out, workspace, stream);
+        case POINTOPS_F16: return cache_step<f16>(a, in->type, form, out, workspace, stream);
+        default: return cache_step<bf16>(a, in->type, form, out, workspace, stream);
     }
 }
 

@@ -39,7 +39,23 @@ struct Kept {
     int tokens;
 };
 
+// Division of 0 .. 2^31 - 1 by a number of the call, as a product and a shift (a division
+// by what the compiler does not know is some thirty instructions, and a row asks for several):
+// n / d = (n m / 2^32 + n) / 2^s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1.
+struct Divisor {
+    uint32_t d, m, s;
+    static Divisor of(int64_t d) {
+        uint32_t s = 0;
+        while ((int64_t(1) << s) < d) ++s;
+        return {static_cast<uint32_t>(d), static_cast<uint32_t>((((uint64_t(1) << s) - d) << 32) / d + 1), s};
+    }
+    __device__ __forceinline__ int of_row(int n) const {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> s);
+    }
+};
+
 struct CacheArgs {
+    Divisor group, per;  // heads of a key head, rows of a sequence's key head (those by its queries)
     Rows q;
     bool q_vec;
     Kept own, start;
@@ -59,30 +75,37 @@ struct CacheArgs {
 
 constexpr int kStepWaves = 4, kStepThreads = kStepWaves * kWave;
 constexpr int kKeys = 32;  // of a wave at a time
+constexpr float kMostWeight = 256.f;  // the running maximum may lie 8 (in units of log 2) below the true one
 constexpr size_t kMostLds = 160 * 1024;
 
-// Parts of a sum over keys: of a unit (key head with 16 COLS rows), `splits` of them,
+// Parts of a sum over keys: of a unit (a key head with a block of rows), `splits` of them,
 // each `rows` long; a part is its maximum and its sum, two unused, then the values.
 __host__ __device__ constexpr int part_width(int DP) { return DP + 4; }
 
+struct Parts {
+    int rows, blocks, splits;  // of a block, blocks of rows of a key head, parts of each (0: none)
+    int64_t units;             // key heads (the caches': of all sequences) by blocks of rows
+    int64_t floats;
+    __device__ __forceinline__ const float* first(const float* parts, int64_t head, int64_t row, int width) const {
+        return parts + ((head * blocks + row / rows) * splits * rows + row % rows) * width;
+    }
+};
+
 struct CachePlan {
-    int shape;                            // of Shape
-    int start_rows, own_rows;             // of a block
-    int start_blocks, own_blocks;         // blocks of rows of a key head (of a sequence's key head)
-    int start_splits, own_splits;         // 0: no start
-    int64_t start_units, own_units;       // key heads by blocks of rows (by sequences)
-    int64_t start_floats;                 // of the start's parts, ahead of the own ones
-    bool direct;                          // one part: no join
+    int shape;         // of Shape
+    Parts start, own;  // the caches' parts lie behind the start's
+    bool joined;       // a launch of its own joins the parts
 };
 
 // ------------------------------------------------------------ small pieces
+// acc += A B of 32 values of 16 bits, or step e of four of 16 values of 32 bits.  An instruction
+// waits for the one before it on the same registers: the callers go round several.
 template <typename T>
-__device__ __forceinline__ f32x4 mma16(i32x4 a, i32x4 b, f32x4 acc) {
+constexpr int kMmaSteps = sizeof(T) == 4 ? 4 : 1;
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(i32x4 a, i32x4 b, f32x4 acc, int e) {
     if constexpr (sizeof(T) == 4) {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
-        return acc;
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[e], __builtin_bit_cast(f32x4, b)[e], acc, 0, 0, 0);
     } else if constexpr (__is_same(T, bf16)) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
     } else {
@@ -162,11 +185,12 @@ __device__ __forceinline__ uint32_t fixed(uint32_t v) {
     asm volatile("" : "+v"(v));
     return v;
 }
-// Rows j0 .. limit - 1 (of `bytes` each; j0 < limit) of those at `base`, as a buffer that ends with the last.
-__device__ __forceinline__ auto rows_from(const void* base, int64_t stride, int j0, int limit, int bytes) {
-    const int64_t all = (limit - 1 - j0) * stride + bytes;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + j0 * stride), 0,
-                                             static_cast<int>(min(all, int64_t(INT32_MAX))), kRawBuffer);
+// `rows` rows (of `bytes` each, at least one) from j0 on of those at `base`, as a buffer that ends with
+// the last.  A tile of rows lies within 2 GiB.
+__device__ __forceinline__ auto rows_from(const void* base, uint32_t stride, int j0, int rows, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(static_cast<const char*>(base) + static_cast<uint64_t>(static_cast<uint32_t>(j0)) * stride), 0,
+        static_cast<int>(static_cast<uint32_t>(rows - 1) * stride) + bytes, kRawBuffer);
 }
 
 // ------------------------------------------------- 32 keys on their way in
@@ -249,8 +273,9 @@ struct Incoming {
                 vr[x] = load_row<T, false>(reinterpret_cast<const T*>(v + j * kept.vn), at % kPerRow * kPerFrag<T>, width);
             }
         } else if constexpr (FORM == kAligned) {
-            const auto ks = rows_from(k, kept.kn, j0, limit, width * static_cast<int>(sizeof(T)));
-            const auto vs = rows_from(v, kept.vn, j0, limit, width * static_cast<int>(sizeof(T)));
+            const int rows = min(limit - j0, kKeys), bytes = width * static_cast<int>(sizeof(T));
+            const auto ks = rows_from(k, static_cast<uint32_t>(kept.kn), j0, rows, bytes);
+            const auto vs = rows_from(v, static_cast<uint32_t>(kept.vn), j0, rows, bytes);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -263,8 +288,9 @@ struct Incoming {
                 vr[x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
                     vs, kSteps ? v_at[0] + x * (kWave / kPerRow) * static_cast<uint32_t>(kept.vn) : v_at[x], 0, kOnce));
         } else {
-            const auto k0 = rows_from(k, kRowBytes, j0, limit, kRowBytes), v0 = rows_from(v, kRowBytes, j0, limit, kRowBytes);
-            const auto ks0 = rows_from(k_scales, kScales, j0, limit, kScales), vs0 = rows_from(v_scales, kScales, j0, limit, kScales);
+            const int rows = min(limit - j0, kKeys);
+            const auto k0 = rows_from(k, kRowBytes, j0, rows, kRowBytes), v0 = rows_from(v, kRowBytes, j0, rows, kRowBytes);
+            const auto ks0 = rows_from(k_scales, kScales, j0, rows, kScales), vs0 = rows_from(v_scales, kScales, j0, rows, kScales);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if constexpr (kWhole) words<4, 0>(k0, k_at[u], kc[u]);
@@ -407,15 +433,15 @@ struct CarefulKept {
 // 32 KW keys and values of the common start on their way through a block's registers to
 // LDS, where its waves read both.  Rows behind `limit` are zeros (a descriptor that ends
 // with the last row), for which the caller's scores are masked.
-template <typename T, int FORM, int DP, int KW>
+template <typename T, int FORM, int DP, int KW, int THREADS>
 struct Shared {
     using C = typename Products<T, FORM>::C;
     static constexpr bool kCoded = Products<T, FORM>::kCoded;
     using TileT = Tile<C, DP>;
     static constexpr int kRows = kKeys * KW, kBytes = 2 * kRows * TileT::kStride;
     static constexpr int kPerRow = kCoded ? DP / 16 : DP * static_cast<int>(sizeof(C)) / 16;
-    static constexpr int kPieces = (kRows * kPerRow + kStepThreads - 1) / kStepThreads;
-    static constexpr bool kAll = kRows * kPerRow % kStepThreads == 0;
+    static constexpr int kPieces = (kRows * kPerRow + THREADS - 1) / THREADS;
+    static constexpr bool kAll = kRows * kPerRow % THREADS == 0;
     static constexpr int kWords = FORM == kEight ? 2 : 1, kRowBytes = FORM == kEight ? DP : DP / 2, kScales = DP / kGroup;
     static constexpr int kPieceBytes = kCoded ? 8 * kWords : 16;
     i32x4 r[2][kPieces];
@@ -429,7 +455,7 @@ struct Shared {
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
                 const uint32_t stride = kCoded ? kRowBytes : static_cast<uint32_t>(side == 0 ? kept.kn : kept.vn);
-                const uint32_t n = x * kStepThreads + threadIdx.x, row = n / kPerRow, piece = n % kPerRow;
+                const uint32_t n = x * THREADS + threadIdx.x, row = n / kPerRow, piece = n % kPerRow;
                 const bool here = (kAll || row < kRows) && (kCoded || static_cast<int>(piece) * kPerFrag<T> < width);
                 at[side][x] = fixed(here ? row * stride + piece * kPieceBytes : kNothing);
                 if constexpr (kCoded)
@@ -440,8 +466,9 @@ struct Shared {
                                          const uint8_t* v_scales, int j0, int limit, int width) {
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-            const auto rows = rows_from(side == 0 ? k : v, kCoded ? kRowBytes : side == 0 ? kept.kn : kept.vn, j0, limit,
-                                        kCoded ? kRowBytes : width * static_cast<int>(sizeof(T)));
+            const int count = min(limit - j0, kRows);
+            const auto rows = rows_from(side == 0 ? k : v, kCoded ? kRowBytes : static_cast<uint32_t>(side == 0 ? kept.kn : kept.vn), j0,
+                                        count, kCoded ? kRowBytes : width * static_cast<int>(sizeof(T)));
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
                 if constexpr (kPieceBytes == 16) r[side][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at[side][x], 0, 0));
@@ -451,7 +478,7 @@ struct Shared {
                 }
             }
             if constexpr (kCoded) {
-                const auto scales = rows_from(side == 0 ? k_scales : v_scales, kScales, j0, limit, kScales);
+                const auto scales = rows_from(side == 0 ? k_scales : v_scales, kScales, j0, count, kScales);
 #pragma unroll
                 for (int x = 0; x < kPieces; ++x) scale[side][x] = __builtin_amdgcn_raw_buffer_load_b8(scales, scale_at[x], 0, 0);
             }
@@ -463,7 +490,7 @@ struct Shared {
         for (int side = 0; side < 2; ++side)
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
-                const int at = x * kStepThreads + static_cast<int>(threadIdx.x), row = at / kPerRow;
+                const int at = x * THREADS + static_cast<int>(threadIdx.x), row = at / kPerRow;
                 if (!kAll && row >= kRows) continue;
                 i32x4* const to = reinterpret_cast<i32x4*>(tiles + (side * kRows + row) * TileT::kStride + at % kPerRow * (kCoded ? 32 : 16));
                 if constexpr (kCoded) {
@@ -484,6 +511,66 @@ struct Shared {
     }
 };
 
+// ------------------------------------------------------------- joining parts
+// A row's sum over keys, in a wave: lane l holds values l and l + 64.
+struct RowSum {
+    float m = -kInf, l = 0.f, x0 = 0.f, x1 = 0.f;
+
+    // Adds `count` parts, `step` floats from one to the next, in order.
+    __device__ __forceinline__ void add(const float* first, int64_t step, int count, int D) {
+        if (count == 0) return;
+        const int lane = lane_id(), c0 = 4 + min(lane, D - 1), c1 = 4 + min(lane + kWave, D - 1);
+        constexpr int kAtOnce = 16;
+        float y0[kAtOnce], y1[kAtOnce];
+        auto ask = [&](int from) {  // (past the end: the last one again, for which the factor is not used)
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float* const at = first + min(from + k, count - 1) * step;
+                y0[k] = at[c0];
+                y1[k] = at[c1];
+            }
+        };
+        ask(0);  // (beside the maxima)
+        float top = -kInf;
+        for (int s = lane; s < count; s += kWave) top = fmaxf(top, first[s * step]);
+        top = fmaxf(m, wave_max(top));
+        const float less = top == -kInf ? 0.f : top, keep = exp2_fast(m - less);
+        m = top;
+        x0 *= keep;
+        x1 *= keep;
+        float sum = 0.f;
+        for (int from = 0; from < count; from += kWave) {
+            // A lane's part: its factor; then the parts' rows one after another.
+            const int s = from + lane;
+            float by = 0.f;
+            if (s < count) {
+                by = exp2_fast(first[s * step] - less);
+                sum = __builtin_fmaf(first[s * step + 1], by, sum);
+            }
+            const int some = min(kWave, count - from);
+            for (int i = 0; i < some; i += kAtOnce) {
+                if (from + i > 0) ask(from + i);
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    if (i + k < some) {
+                        const float f = i2f(readlane(f2i(by), i + k));
+                        x0 = __builtin_fmaf(y0[k], f, x0);
+                        x1 = __builtin_fmaf(y1[k], f, x1);
+                    }
+                }
+            }
+        }
+        l = __builtin_fmaf(l, keep, wave_sum(sum));
+    }
+    template <typename T>
+    __device__ __forceinline__ void write(T* dst, int D) const {
+        const int lane = lane_id();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (lane < D) dst[lane] = from_float<T>(x0 * inv);
+        if (lane + kWave < D) dst[lane + kWave] = from_float<T>(x1 * inv);
+    }
+};
+
 // ------------------------------------------------------------------ a part
 // The rows and keys of a block: the common start with rows of all sequences, a sequence's
 // cache with its rows, or its rows with both, one behind the other.
@@ -496,7 +583,7 @@ struct StepLds {
     static constexpr int kKeyWaves = WAVES / ROW_WAVES, kRows = 16 * COLS * ROW_WAVES;
     static constexpr int kSums = kRows * (DP + 4) * 4;
     static constexpr int kTiles = ROW_WAVES == 1 ? WAVES * Incoming<T, FORM, DP>::kTileBytes
-                                                 : 2 * Shared<T, FORM, DP, kKeyWaves>::kBytes;
+                                                 : 2 * Shared<T, FORM, DP, kKeyWaves, kWave * WAVES>::kBytes;
     // The tiles, then the sums in the same place; maxima and sums of the weights; then the
     // bias: [buckets][heads of the rows], the buckets of 0 .. reach, the edges.
     static constexpr int kPlace = kTiles > kSums ? kTiles : kSums;
@@ -543,7 +630,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     constexpr int kKeyWaves = Lds::kKeyWaves, kRows = Lds::kRows, kThreads = kWave * WAVES;
     constexpr bool kShared = ROW_WAVES > 1, kManySequences = KIND == kStart;
     using In = Incoming<T, FORM, DP>;
-    using Sh = Shared<T, FORM, DP, kKeyWaves>;
+    using Sh = Shared<T, FORM, DP, kKeyWaves, kWave * WAVES>;
     using C = typename In::C;
     constexpr int kQ = Products<T, FORM>::kQuery, kW = Products<T, FORM>::kWeight, kFrags = In::kFrags;
     constexpr int kOut = DP / 16, kSumStride = DP + 4, kTile = kShared ? kKeys * kKeyWaves : kKeys;
@@ -551,7 +638,15 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     const int lane = lane_id(), col = lane % 16, quad = lane / 16, wave = uniform(threadIdx.x / kWave);
     const int row_wave = wave % ROW_WAVES, key_wave = wave / ROW_WAVES;
     const int w0 = 16 * COLS * row_wave;  // this wave's first row in the block
-    const int group = a.H / a.G, per = a.Q * group, total = kManySequences ? a.B * per : per;
+    const int group = a.group.d, per = a.per.d, total = kManySequences ? a.B * per : per;
+    // A row's sequence, query and head in the group.
+    struct Row {
+        int b, i, h;
+    };
+    auto row_of = [&](int r) {
+        const int b = kManySequences ? a.per.of_row(r) : b0, in = kManySequences ? r - b * per : r, i = a.group.of_row(in);
+        return Row{b, i, in - i * group};
+    };
     const int rows = min(kRows, total - r0);
     float* const tops = reinterpret_cast<float*>(lds + Lds::kPlace);
     float* const totals = tops + kKeyWaves * kRows;
@@ -559,14 +654,16 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 
     // Rows: this lane's columns.
     const int own_length = kManySequences ? 0 : uniform(a.length(b0));
+    Row mine[COLS];
     int p[COLS], p_least = INT32_MAX;
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        const int r = r0 + w0 + 16 * n + col;
+        // (Columns without a row: the block's first, whose values they do not read.)
+        const bool any = w0 + 16 * n + col < rows;
+        mine[n] = row_of(any ? r0 + w0 + 16 * n + col : r0);
         p[n] = -1;
-        if (w0 + 16 * n + col < rows) {
-            const int length = kManySequences ? a.length(r / per) : own_length;
-            p[n] = a.start.tokens + length - a.Q + (kManySequences ? r % per : r) / group;
+        if (any) {
+            p[n] = a.start.tokens + (kManySequences ? a.length(mine[n].b) : own_length) - a.Q + mine[n].i;
             p_least = min(p_least, p[n]);
         }
     }
@@ -649,16 +746,15 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     i32x4 q[COLS][kFrags][kQ];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        const int r = r0 + w0 + 16 * n + col, in_b = kManySequences ? r % per : r;
-        const bool mine = w0 + 16 * n + col < rows;
-        const T* const row = a.q.at<T>(kManySequences ? r / per : b0, g * group + in_b % group) + in_b / group * a.q.n;
+        const bool any = w0 + 16 * n + col < rows;
+        const T* const row = a.q.at<T>(mine[n].b, g * group + mine[n].h) + mine[n].i * a.q.n;
 #pragma unroll
         for (int c = 0; c < kFrags; ++c) {
             const int at = kShared ? Sh::column(c, quad) : In::column(c, quad);
             float x[kPerFrag<C>];
 #pragma unroll
             for (int e = 0; e < kPerFrag<C>; ++e) x[e] = 0.f;
-            if (mine) {
+            if (any) {
                 if (a.q_vec) {
 #pragma unroll
                     for (int e = 0; e < kPerFrag<C>; e += kPerFrag<T>) {
@@ -685,7 +781,8 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         int* const edges = reinterpret_cast<int*>(ids + (a.reach + 4) / 4 * 4);
         for (int x = threadIdx.x; x < a.bk.n; x += kThreads) edges[x] = a.bk.edge[x];
         for (int x = threadIdx.x; x < a.bk.count * heads; x += kThreads) {
-            const int h = g * group + (heads < group ? (r0 + x % heads) % group : x % heads);
+            const int at = x % heads, in = r0 + at - a.group.of_row(r0 + at) * group;
+            const int h = g * group + (heads < group ? in : at);
             table[x] = bias_log2(to_float(static_cast<const T*>(a.bias)[static_cast<int64_t>(x / heads) * a.H + h]));
         }
         __syncthreads();
@@ -693,7 +790,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            head[n] = heads < group ? w0 + 16 * n + col : (r0 + w0 + 16 * n + col) % group;
+            head[n] = heads < group ? w0 + 16 * n + col : mine[n].h;
             far[n] = table[a.bk.n * heads + head[n]];
         }
     }
@@ -707,7 +804,11 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     float m[COLS], l[COLS];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        m[n] = -kInf;
+        // (A row that sees nothing needs no maximum: its weights are zeros by any.)
+        bool sees = false;
+#pragma unroll
+        for (int x = 0; x < kRanges; ++x) sees |= range[x].seen[n].count > 0 || range[x].seen[n].first > 0;
+        m[n] = sees ? -kInf : 0.f;
         l[n] = 0.f;
 #pragma unroll
         for (int d = 0; d < kOut; ++d) o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -715,18 +816,37 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     f32x4 s[COLS][2];
     i32x4 w[COLS][8 / kPerFrag<C>][kW];
     auto score = [&](auto&& keys) {
+        // (One column: two sums, of even and of odd fragments.)
+        constexpr int kSums = COLS == 1 && kFrags > 1 ? 2 : 1;
+        f32x4 sum[kSums][COLS][2];
 #pragma unroll
-        for (int n = 0; n < COLS; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < kSums; ++t)
 #pragma unroll
-        for (int c = 0; c < kFrags; ++c)
+            for (int n = 0; n < COLS; ++n) sum[t][n][0] = sum[t][n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const i32x4 f = keys(u, c);
+        for (int c = 0; c < kFrags; c += kSums) {
+            i32x4 f[kSums][2];
 #pragma unroll
-                for (int n = 0; n < COLS; ++n)
+            for (int t = 0; t < kSums; ++t)
 #pragma unroll
-                    for (int x = 0; x < kQ; ++x) s[n][u] = mma16<C>(f, q[n][c][x], s[n][u]);
-            }
+                for (int u = 0; u < 2; ++u)
+                    if (c + t < kFrags) f[t][u] = keys(u, c + t);
+#pragma unroll
+            for (int x = 0; x < kQ; ++x)
+#pragma unroll
+                for (int e = 0; e < kMmaSteps<C>; ++e)
+#pragma unroll
+                    for (int t = 0; t < kSums; ++t)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int n = 0; n < COLS; ++n)
+                                if (c + t < kFrags) sum[t][n][u] = mma16<C>(f[t][u], q[n][c + t][x], sum[t][n][u], e);
+        }
+#pragma unroll
+        for (int n = 0; n < COLS; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[n][u] = kSums == 2 ? sum[0][n][u] + sum[kSums - 1][n][u] : sum[0][n][u];
     };
     // Of the 32 keys from j0 on.
     auto weigh = [&](const Range<kTile, COLS>& at, int j0) {
@@ -756,57 +876,75 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[n][e / 4][e % 4] = at.seen[n](j + e / 4 * 16 + e % 4) ? s[n][e / 4][e % 4] : -kInf;
         }
-        float top[COLS];
+        float x[COLS][8];
+        auto form = [&]() {
+#pragma unroll
+            for (int n = 0; n < COLS; ++n) {
+                const float less = m[n] == -kInf ? 0.f : m[n];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[n][e] = exp2_fast(__builtin_fmaf(s[n][e / 4][e % 4], factor, -less));
+            }
+        };
+        // The weights by the maximum so far; where one of them has outgrown it (or there is none
+        // yet), by a new one.  So the scores' own maximum is seldom asked for.
+        form();
         bool rises = false;
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            float t = s[n][0][0];
+            float most = x[n][0];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) t = fmaxf(t, s[n][e / 4][e % 4]);
-            top[n] = quads_max(t) * factor;
-            rises |= top[n] > m[n] + kSlack;
+            for (int e = 1; e < 8; ++e) most = fmaxf(most, x[n][e]);
+            rises |= most > kMostWeight || m[n] == -kInf;
         }
         if (ballot(rises) != 0) {
 #pragma unroll
             for (int n = 0; n < COLS; ++n) {
-                const float next = fmaxf(m[n], top[n]);
+                float top = s[n][0][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, s[n][e / 4][e % 4]);
+                const float next = fmaxf(m[n], quads_max(top) * factor);
                 const float keep = m[n] == next ? 1.f : exp2_fast(m[n] - next);
                 m[n] = next;
                 l[n] *= keep;
 #pragma unroll
                 for (int d = 0; d < kOut; ++d) o[d][n] *= keep;
             }
+            form();
         }
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            const float less = m[n] == -kInf ? 0.f : m[n];
-            float x[8];
+            l[n] += ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3])) + ((x[n][4] + x[n][5]) + (x[n][6] + x[n][7]));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = exp2_fast(__builtin_fmaf(s[n][e / 4][e % 4], factor, -less));
-            l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-#pragma unroll
-            for (int f = 0; f < 8 / kPerFrag<C>; ++f) split<C, kW, true>(x + f * kPerFrag<C>, w[n][f]);
+            for (int f = 0; f < 8 / kPerFrag<C>; ++f) split<C, kW, true>(x[n] + f * kPerFrag<C>, w[n][f]);
         }
     };
-    // The values' operands are read two ahead of their products, the first ones before the
+    // The values' operands are read a batch ahead of their products, the first before the
     // weights are formed.
-    constexpr int kHalves = 8 / kPerFrag<C>, kSteps = kOut * kHalves, kBefore = 2;
-    i32x4 vf[kBefore];
-    auto ahead = [&](const char* values) {
+    constexpr int kHalves = 8 / kPerFrag<C>, kBatch = COLS > 1 ? 2 : kOut % 4 == 0 ? 4 : kOut % 3 == 0 ? 3 : 2;
+    static_assert(kOut % kBatch == 0);
+    i32x4 vf[2][kBatch][kHalves];
+    auto ask = [&](const char* values, int d, i32x4 (&f)[kBatch][kHalves]) {
 #pragma unroll
-        for (int x = 0; x < kBefore; ++x) vf[x] = In::values(values, x % kHalves, x / kHalves);
+        for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) f[x][h] = In::values(values, h, d + x);
     };
     auto add = [&](const char* values) {
 #pragma unroll
-        for (int x = 0; x < kSteps; ++x) {
-            const i32x4 f = vf[x % kBefore];
-            const int then = x + kBefore;
-            if (then < kSteps) vf[x % kBefore] = In::values(values, then % kHalves, then / kHalves);
+        for (int d = 0; d < kOut; d += kBatch) {
+            const auto& f = vf[d / kBatch % 2];
+            if (d + kBatch < kOut) ask(values, d + kBatch, vf[(d / kBatch + 1) % 2]);
             keep_order();
 #pragma unroll
-            for (int n = 0; n < COLS; ++n)
+            for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                for (int y = 0; y < kW; ++y) o[x / kHalves][n] = mma16<C>(f, w[n][x % kHalves][y], o[x / kHalves][n]);
+                for (int y = 0; y < kW; ++y)
+#pragma unroll
+                    for (int e = 0; e < kMmaSteps<C>; ++e)
+#pragma unroll
+                        for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+                            for (int n = 0; n < COLS; ++n) o[d + x][n] = mma16<C>(f[x][h], w[n][h][y], o[d + x][n], e);
         }
     };
     if constexpr (kShared) {
@@ -825,7 +963,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                 for (int u = 0; u < 2; ++u) kf[u][c] = Sh::keys(now, at + 16 * u, c);
             keep_order();
             score([&](int u, int c) { return kf[u][c]; });
-            ahead(values);
+            ask(values, 0, vf[0]);
             keep_order();
             weigh(range[0], range[0].first_key(tile) + at);
             add(values);
@@ -840,7 +978,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
             in.store_values(values);
             if (tile + WAVES < end) fetch(tile + WAVES);
             lanes_exchange();
-            ahead(values);
+            ask(values, 0, vf[0]);
             if (kRanges == 2 && tile >= first_range) weigh(range[kRanges - 1], range[kRanges - 1].first_key(tile - first_range));
             else weigh(range[0], range[0].first_key(tile));
             add(values);
@@ -853,6 +991,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
         l[n] = quads_sum(l[n]);
+        if (l[n] == 0.f) m[n] = -kInf;
         if (quad == 0) {
             tops[key_wave * kRows + w0 + 16 * n + col] = m[n];
             totals[key_wave * kRows + w0 + 16 * n + col] = l[n];
@@ -898,24 +1037,25 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     __syncthreads();
     // Rows of the block, one a wave at a time: out, or the split's part of it.
     for (int row = wave; row < rows; row += WAVES) {
-        const int r = r0 + row, in_b = kManySequences ? r % per : r, bb = kManySequences ? r / per : b0;
-        const int i = in_b / group, h = g * group + in_b % group;
         float x0 = lane < a.D ? sums[row * kSumStride + lane] : 0.f;
         float x1 = lane + kWave < a.D ? sums[row * kSumStride + lane + kWave] : 0.f;
         float lm = tops[row], ll = totals[row];
         // A sum of weights that is NaN comes from a seen pair, and all of its row is NaN as it
         // lies, but where a bias of -inf masks that pair.
         const bool none = ll != ll;
-        const int column = heads < group ? row : in_b % group;
         bool masks = false;
-        if (none && biased)
+        if (none && biased) {
+            const int column = heads < group ? row : row_of(r0 + row).h;
             for (int x = lane; x < a.bk.count; x += kWave) masks |= table[x * heads + column] == -kInf;
+        }
         const bool n0 = none || !finite(x0), n1 = none || !finite(x1);
         if (ll == 0.f) {
             x0 = x1 = 0.f;
         } else if (none ? ballot(masks) != 0 : ballot(n0 || n1) != 0) {
-            CarefulKept<T, FORM> c(a, a.q.at<T>(bb, h) + i * a.q.n);
-            const int place = a.start.tokens + (kManySequences ? uniform(a.length(bb)) : own_length) - a.Q + i;
+            const Row at_row = row_of(r0 + row);
+            const int column = heads < group ? row : at_row.h;
+            CarefulKept<T, FORM> c(a, a.q.at<T>(at_row.b, g * group + at_row.h) + at_row.i * a.q.n);
+            const int place = a.start.tokens + (kManySequences ? uniform(a.length(at_row.b)) : own_length) - a.Q + at_row.i;
             bool done = false;
 #pragma unroll
             for (int x = 0; x < kRanges; ++x) {
@@ -940,11 +1080,10 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
             x0 = n0 ? c.o0 * by : x0;
             x1 = n1 ? c.o1 * by : x1;
         }
-        if (part == nullptr) {
-            const float inv = ll == 0.f ? 0.f : 1.f / ll;
-            T* const dst = out + ((static_cast<int64_t>(bb) * a.Q + i) * a.H + h) * a.D;
-            if (lane < a.D) dst[lane] = from_float<T>(x0 * inv);
-            if (lane + kWave < a.D) dst[lane + kWave] = from_float<T>(x1 * inv);
+        if (KIND == kBoth || part == nullptr) {
+            const Row at_row = row_of(r0 + row);
+            const RowSum all{lm, ll, x0, x1};
+            all.write(out + ((static_cast<int64_t>(at_row.b) * a.Q + at_row.i) * a.H + g * group + at_row.h) * a.D, a.D);
         } else {
             float* const dst = part + static_cast<int64_t>(row) * part_width(DP);
             if (lane == 0) {
@@ -957,30 +1096,32 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     }
 }
 
-// The start's blocks, then the caches'.
+// Parts: the start's blocks, then the caches', which fill the compute units beside and behind
+// them (64 sequences of 512 tokens behind 16384, 32 heads over 8 of 128, bfloat16: 62 us, by two
+// launches 73).  A start's block has 16 COLS rows of ROW_WAVES waves, a cache's 16 OWN_COLS.
+// Registers: two waves a SIMD, one for 32-bit values, whose products take four times the operands.
 template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int OWN_COLS>
-__global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (FORM < kFour || COLS * ROW_WAVES > 1)) ? 1 : 2) void attention_cache_kernel(
+__global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (FORM < kFour || COLS * OWN_COLS > 1)) ? 1 : 2) void attention_cache_kernel(
     const CacheArgs a, const CachePlan plan, T* __restrict__ out, float* __restrict__ parts) {
     extern __shared__ __attribute__((aligned(16))) char cache_lds[];
     constexpr int kStartRows = 16 * COLS * ROW_WAVES, kOwnRows = 16 * OWN_COLS;
-    const int64_t block = blockIdx.x, start = plan.start_units * plan.start_splits;
-    if (block < start) {
+    const int64_t block = blockIdx.x, first = plan.start.units * plan.start.splits;
+    if (block < first) {
         // The row blocks of the same keys are eight blocks apart, on one XCD (whose L2 then
         // holds the keys for all of them).
-        const uint32_t all = static_cast<uint32_t>(a.G * plan.start_splits), eights = 8u * plan.start_blocks;
+        const uint32_t all = static_cast<uint32_t>(a.G * plan.start.splits), eights = 8u * plan.start.blocks;
         const uint32_t some = static_cast<uint32_t>(block) / eights, left = min(8u, all - 8 * some), in = static_cast<uint32_t>(block) % eights;
         const uint32_t keys = 8 * some + in % left, row_block = in / left;
-        const int split_at = static_cast<int>(keys % plan.start_splits), g = static_cast<int>(keys / plan.start_splits);
-        const int64_t place = (static_cast<int64_t>(g) * plan.start_blocks + row_block) * plan.start_splits + split_at;
+        const int split_at = static_cast<int>(keys % plan.start.splits), g = static_cast<int>(keys / plan.start.splits);
+        const int64_t place = (static_cast<int64_t>(g) * plan.start.blocks + row_block) * plan.start.splits + split_at;
         attention_part<T, FORM, DP, COLS, ROW_WAVES, kStepWaves, kStart>(a, out, parts + place * kStartRows * part_width(DP), 0, g,
-                                                           static_cast<int>(row_block) * kStartRows, split_at, plan.start_splits, cache_lds);
+                                                                         static_cast<int>(row_block) * kStartRows, split_at, plan.start.splits, cache_lds);
     } else {
-        const int64_t at = block - start;
-        const int split_at = static_cast<int>(at % plan.own_splits);
-        const int64_t unit = at / plan.own_splits, bg = unit / plan.own_blocks;
+        const int64_t at = block - first, unit = at / plan.own.splits, bg = unit / plan.own.blocks;
         attention_part<T, FORM, DP, OWN_COLS, 1, kStepWaves, kOwn>(
-            a, out, plan.direct ? nullptr : parts + plan.start_floats + at * kOwnRows * part_width(DP), static_cast<int>(bg / a.G),
-            static_cast<int>(bg % a.G), static_cast<int>(unit % plan.own_blocks) * kOwnRows, split_at, plan.own_splits, cache_lds);
+            a, out, plan.joined ? parts + plan.start.floats + at * kOwnRows * part_width(DP) : nullptr, static_cast<int>(bg / a.G),
+            static_cast<int>(bg % a.G), static_cast<int>(unit % plan.own.blocks) * kOwnRows, static_cast<int>(at % plan.own.splits),
+            plan.own.splits, cache_lds);
     }
 }
 
@@ -997,12 +1138,14 @@ __global__ __launch_bounds__(kWave * direct_waves(sizeof(T), FORM, DP), direct_w
         a, out, nullptr, static_cast<int>(blockIdx.x / a.G), static_cast<int>(blockIdx.x % a.G), 0, 0, 1, cache_lds);
 }
 
-// Kernels: rows of a start's block, 16 COLS of ROW_WAVES waves, and 16 OWN_COLS of a cache's.
-enum Shape { kDirect, kOne, kTwo, kTwoTwo, kPairs, kPairsTwo, kShapes };
+// Kernels, by the rows of a start's block and of a cache's.
+enum Shape { kDirect, kOne, kTwo, kPairs, kTwoTwo, kPairsTwo, kShapes };
 struct ShapeRows {
     int cols, row_waves, own_cols;
+    constexpr int start() const { return 16 * cols * row_waves; }
+    constexpr int own() const { return 16 * own_cols; }
 };
-constexpr ShapeRows kShapeRows[kShapes] = {{1, 1, 1}, {1, 1, 1}, {2, 1, 1}, {2, 1, 2}, {2, 2, 1}, {2, 2, 2}};
+constexpr ShapeRows kShapeRows[kShapes] = {{1, 1, 1}, {1, 1, 1}, {2, 1, 1}, {2, 2, 1}, {2, 1, 2}, {2, 2, 2}};
 
 template <typename T, int FORM>
 hipError_t launch_cache_form(const CacheArgs& a, const CachePlan& plan, void* out, float* parts, hipStream_t stream) {
@@ -1021,29 +1164,31 @@ hipError_t launch_cache_form(const CacheArgs& a, const CachePlan& plan, void* ou
             constexpr ShapeRows R = kShapeRows[decltype(shape)::value];
             using Start = StepLds<T, FORM, DP, R.cols, R.row_waves, kStepWaves>;
             using Own = StepLds<T, FORM, DP, R.own_cols, 1, kStepWaves>;
+            const size_t own_lds = Own::kBytes + bias_lds(a, Own::kRows);
             static std::atomic<uint64_t> allowed;
             return launch(attention_cache_kernel<T, FORM, DP, R.cols, R.row_waves, R.own_cols>, allowed,
-                          plan.start_units * plan.start_splits + plan.own_units * plan.own_splits, kStepWaves,
-                          std::max(Start::kBytes + bias_lds(a, Start::kRows), Own::kBytes + bias_lds(a, Own::kRows)), plan,
+                          plan.start.units * plan.start.splits + plan.own.units * plan.own.splits, kStepWaves,
+                          plan.start.units == 0 ? own_lds : std::max(Start::kBytes + bias_lds(a, Start::kRows), own_lds), plan,
                           static_cast<T*>(out), parts);
         };
-        if constexpr (FORM != kAny) {  // (whose plans have no others)
+        if constexpr (FORM == kAny) {  // (whose plans have no others)
+            return parted(std::integral_constant<int, kTwoTwo>{});
+        } else {
             switch (plan.shape) {
                 case kDirect: {
                     constexpr int W = direct_waves(sizeof(T), FORM, DP);
                     using L = StepLds<T, FORM, DP, 1, 1, W>;
                     static std::atomic<uint64_t> allowed;
-                    return launch(attention_direct_kernel<T, FORM, DP>, allowed, plan.own_units, W,
-                                  L::kBytes + bias_lds(a, L::kRows), static_cast<T*>(out));
+                    return launch(attention_direct_kernel<T, FORM, DP>, allowed, plan.own.units, W, L::kBytes + bias_lds(a, L::kRows),
+                                  static_cast<T*>(out));
                 }
                 case kOne: return parted(std::integral_constant<int, kOne>{});
                 case kTwo: return parted(std::integral_constant<int, kTwo>{});
                 case kPairs: return parted(std::integral_constant<int, kPairs>{});
                 case kPairsTwo: return parted(std::integral_constant<int, kPairsTwo>{});
-                default: break;
+                default: return parted(std::integral_constant<int, kTwoTwo>{});
             }
         }
-        return parted(std::integral_constant<int, kTwoTwo>{});
     });
 }
 

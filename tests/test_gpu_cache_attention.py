@@ -184,6 +184,16 @@ def test_bias_masks(cuda_device, bits):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("bits", FORMS)
+def test_large_tables(cuda_device, kind, bits):
+    """The most buckets with many heads a key head, whose table and the widest
+    rows' tiles do not fit one block together."""
+    for B, H, D, P in ((3, 64, 128, 1500), (2, 128, 100, 1400), (3, 9, 128, 1500), (40, 4, 128, 1300)):
+        q, prefix, own, bias = make(15, kind, B, 1, P, 9, H, 1, D, 256)
+        run(kind, q, prefix, own, None, bits, bias=bias, max_distance=1000)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_strides_and_alignment(cuda_device, kind):
     """Heads before tokens, rows that start anywhere, one start broadcast over its
     heads, queries cut from a projection, a last dimension that is not contiguous."""
