@@ -10,7 +10,9 @@ keys are normed and rotated by the point's three coordinates
 two (``window_attention``, with a bias learned by buckets of the offset).  The
 trained model then continues a cloud point by point over a cache of keys and
 values (``window_attention_step``); fed the same points, the steps give the
-whole pass's logits.  ``Layer.weights`` shows what a head attends to, from
+whole pass's logits.  The cache may hold its keys and values in 8 or 4 bits
+(``QuantizedCache``, ``cache_write``, ``quantized_attention_step``), and one start can
+be continued in many ways that share its cache (``prefix_attention_step``).  ``Layer.weights`` shows what a head attends to, from
 ordinary products and the dense bias (``relative_bias``).
 """
 
@@ -28,6 +30,8 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "mps-pointops_amd")
 
 import mps_pointops as mp  # noqa: E402
 from mps_pointops import attention  # noqa: E402
+
+Cache = "tuple[Tensor, Tensor] | attention.QuantizedCache"  # a layer's keys and values
 
 GRID = 16
 WIDTH, HEADS, KEY_HEADS, HEAD = 128, 4, 2, 32
@@ -97,13 +101,25 @@ class Layer(nn.Module):
         return self.rest(x, attention.window_attention(q, k, v, window=WINDOW, sinks=FIRST, causal=True,
                                                        bias=self.bias, max_distance=REACH))
 
-    def step(self, x: Tensor, cos: Tensor, sin: Tensor, keys: Tensor, values: Tensor, at: int) -> Tensor:
-        """One token for each cloud, its key and value written to the cache."""
+    def step(self, x: Tensor, cos: Tensor, sin: Tensor, cache: Cache, at: int, prefix: Cache | None = None) -> Tensor:
+        """A few tokens for each cloud, their keys and values written to the cache from place
+        `at` on, behind a prefix that all clouds share."""
         q, k, v = self.heads(x, cos, sin)
-        keys[:, at:at + 1], values[:, at:at + 1] = k, v
-        lengths = torch.full((len(x),), at + 1, dtype=torch.int32, device=x.device)
-        return self.rest(x, attention.window_attention_step(q, keys, values, lengths, window=WINDOW, sinks=FIRST,
-                                                            bias=self.bias, max_distance=REACH))
+        end = at + x.shape[1]
+        lengths = torch.full((len(x),), end, dtype=torch.int32, device=x.device)
+        coded = isinstance(cache, attention.QuantizedCache)
+        if coded:
+            attention.cache_write(cache, k, v, lengths)
+        else:
+            cache[0][:, at:end], cache[1][:, at:end] = k, v
+        how = dict(window=WINDOW, sinks=FIRST, bias=self.bias, max_distance=REACH)
+        if prefix is not None:
+            seen = attention.prefix_attention_step(q, prefix, cache, lengths, **how)
+        elif coded:
+            seen = attention.quantized_attention_step(q, cache, lengths, **how)
+        else:
+            seen = attention.window_attention_step(q, *cache, lengths, **how)
+        return self.rest(x, seen)
 
     def weights(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
         """(batch, heads, tokens, tokens) weights, for inspection."""
@@ -129,17 +145,21 @@ class Generator(nn.Module):
             x = layer(x, *turn)
         return self.head(x)
 
-    def cache(self, batch: int, tokens: int) -> list[tuple[Tensor, Tensor]]:
+    def cache(self, batch: int, tokens: int, bits: int = 32) -> list[Cache]:
+        """One of each layer, in float32 or in 8 or 4 bits."""
         like = self.token.weight
+        if bits != 32:
+            return [attention.QuantizedCache(batch, tokens, KEY_HEADS, HEAD, bits=bits, device=like.device)
+                    for _ in self.layers]
         return [(like.new_zeros(batch, tokens, KEY_HEADS, HEAD), like.new_zeros(batch, tokens, KEY_HEADS, HEAD))
                 for _ in self.layers]
 
     @torch.no_grad()
-    def step(self, token: Tensor, cache: list[tuple[Tensor, Tensor]], at: int) -> Tensor:
-        """Logits after the (batch, 1) tokens at place `at` of the cache."""
+    def step(self, token: Tensor, cache: list[Cache], at: int, prefix: list[Cache] | None = None) -> Tensor:
+        """Logits after the (batch, few) tokens from place `at` of the cache on."""
         x, turn = self.token(token), angles(place(token))
-        for layer, (keys, values) in zip(self.layers, cache):
-            x = layer.step(x, *turn, keys, values, at)
+        for n, layer in enumerate(self.layers):
+            x = layer.step(x, *turn, cache[n], at, None if prefix is None else prefix[n])
         return self.head(x)
 
 
@@ -157,21 +177,39 @@ def train(model: Generator, steps: int, points: int, batch: int = 16) -> list[fl
 
 
 @torch.no_grad()
-def replay(model: Generator, token: Tensor) -> Tensor:
+def replay(model: Generator, token: Tensor, bits: int = 32) -> Tensor:
     """The whole pass's logits, step by step."""
-    cache = model.cache(*token.shape)
+    cache = model.cache(*token.shape, bits)
     return torch.cat([model.step(token[:, n:n + 1], cache, n) for n in range(token.shape[1])], 1)
 
 
 @torch.no_grad()
-def generate(model: Generator, start: Tensor, points: int) -> Tensor:
+def generate(model: Generator, start: Tensor, points: int, bits: int = 32) -> Tensor:
     """The start continued with the likeliest next cells."""
-    cache = model.cache(len(start), points)
+    cache = model.cache(len(start), points, bits)
     token = start
     for n in range(points):
         logits = model.step(token[:, n:n + 1], cache, n)
         if n + 1 == token.shape[1] and n + 1 < points:
             token = torch.cat([token, logits[:, -1:].argmax(-1)], 1)
+    return token
+
+
+@torch.no_grad()
+def continue_many(model: Generator, start: Tensor, ways: int, points: int, bits: int = 32, seed: int = 0) -> Tensor:
+    """One start (tokens) continued in several ways, drawn from the model: the start's keys and
+    values are computed and kept once, and each way keeps its own points alone."""
+    gen = torch.Generator(device=start.device).manual_seed(seed)
+    prefix = model.cache(1, len(start), bits)
+    logits = model.step(start[None], prefix, 0)[:, -1].expand(ways, -1)
+    if bits == 32:
+        prefix = [(k[0], v[0]) for k, v in prefix]
+    cache = model.cache(ways, points, bits)
+    token = start.expand(ways, -1)
+    for n in range(points):
+        token = torch.cat([token, torch.multinomial(logits.softmax(-1), 1, generator=gen)], 1)
+        if n + 1 < points:
+            logits = model.step(token[:, -1:], cache, n, prefix)[:, -1]
     return token
 
 
@@ -191,6 +229,12 @@ def main() -> None:
     made = generate(model, token[:, :args.points // 2], args.points)
     kept = (made[:, 1:] != made[:, :-1]).float().mean()
     print(f"continued {tuple(made.shape)} cells; {100 * kept:.0f}% of them move on")
+    for bits in (8, 4):
+        with torch.no_grad():
+            coded = replay(model, token, bits)
+        print(f"over a cache in {bits} bits the steps differ by {(whole - coded).norm() / whole.norm():.1e}")
+    many = continue_many(model, token[0, :args.points // 2], 8, args.points // 2, bits=8)
+    print(f"one start continued in {len(many)} ways: {tuple(many.shape)} cells")
 
 
 if __name__ == "__main__":

@@ -816,37 +816,20 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     f32x4 s[COLS][2];
     i32x4 w[COLS][8 / kPerFrag<C>][kW];
     auto score = [&](auto&& keys) {
-        // (One column: two sums, of even and of odd fragments.)
-        constexpr int kSums = COLS == 1 && kFrags > 1 ? 2 : 1;
-        f32x4 sum[kSums][COLS][2];
 #pragma unroll
-        for (int t = 0; t < kSums; ++t)
+        for (int n = 0; n < COLS; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < COLS; ++n) sum[t][n][0] = sum[t][n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kFrags; c += kSums) {
-            i32x4 f[kSums][2];
-#pragma unroll
-            for (int t = 0; t < kSums; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (c + t < kFrags) f[t][u] = keys(u, c + t);
+        for (int c = 0; c < kFrags; ++c) {
+            const i32x4 f[2] = {keys(0, c), keys(1, c)};
 #pragma unroll
             for (int x = 0; x < kQ; ++x)
 #pragma unroll
                 for (int e = 0; e < kMmaSteps<C>; ++e)
 #pragma unroll
-                    for (int t = 0; t < kSums; ++t)
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int n = 0; n < COLS; ++n)
-                                if (c + t < kFrags) sum[t][n][u] = mma16<C>(f[t][u], q[n][c + t][x], sum[t][n][u], e);
+                        for (int n = 0; n < COLS; ++n) s[n][u] = mma16<C>(f[u], q[n][c][x], s[n][u], e);
         }
-#pragma unroll
-        for (int n = 0; n < COLS; ++n)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) s[n][u] = kSums == 2 ? sum[0][n][u] + sum[kSums - 1][n][u] : sum[0][n][u];
     };
     // Of the 32 keys from j0 on.
     auto weigh = [&](const Range<kTile, COLS>& at, int j0) {
@@ -920,7 +903,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     };
     // The values' operands are read a batch ahead of their products, the first before the
     // weights are formed.
-    constexpr int kHalves = 8 / kPerFrag<C>, kBatch = COLS > 1 ? 2 : kOut % 4 == 0 ? 4 : kOut % 3 == 0 ? 3 : 2;
+    constexpr int kHalves = 8 / kPerFrag<C>, kBatch = 2;
     static_assert(kOut % kBatch == 0);
     i32x4 vf[2][kBatch][kHalves];
     auto ask = [&](const char* values, int d, i32x4 (&f)[kBatch][kHalves]) {

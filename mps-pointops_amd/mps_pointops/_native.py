@@ -189,6 +189,16 @@ def call(name: str, *args) -> None:
     _enqueue(name, *args)
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` for tensors of ``device``, which need not be the current one (the
+    kernel's code and limits are those of the current device)."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
 def _enqueue(name: str, *args) -> None:
     status = getattr(library(), name)(*args)
     if status != 0:

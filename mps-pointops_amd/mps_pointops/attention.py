@@ -386,9 +386,19 @@ class QuantizedCache:
         """One cloud's cache (a batch of one), in the same memory."""
         return self._view(0, index, 1)
 
+    def __reduce__(self):
+        return _restore, (self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.width, self.bits)
+
     def __repr__(self) -> str:
         return (f"QuantizedCache(batch={self.batch}, tokens={self.tokens}, heads={self.heads}, width={self.width}, "
                 f"bits={self.bits}, device='{self.device}')")
+
+
+def _restore(*args) -> QuantizedCache:
+    """A cache of four tensors, from a copy or a file."""
+    cache = object.__new__(QuantizedCache)
+    cache._hold([t.contiguous() for t in args[:4]], *args[4:])
+    return cache
 
 
 def _check_cache(cache, name: str = "cache") -> None:
@@ -471,7 +481,7 @@ def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | N
     k, v = _rows(k), _rows(v)
     lengths, length_at, length_bits = _place_args(lengths)
     starts, start_at, start_bits = _place_args(starts)
-    _native.call("pointops_cache_write", cache._packed, k.data_ptr(), _THREE(*k.stride()[:3]), v.data_ptr(),
+    _native.call_on(device, "pointops_cache_write", cache._packed, k.data_ptr(), _THREE(*k.stride()[:3]), v.data_ptr(),
                  _THREE(*v.stride()[:3]), tokens, length_at, length_bits, start_at, start_bits, _TYPES[dtype],
                  _native.stream(device))
 
@@ -491,7 +501,7 @@ def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) ->
     shape = cache.batch, cache.tokens, cache.heads, cache.width
     k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     if k.numel():
-        _native.call("pointops_cache_read", cache._packed, k.data_ptr(), v.data_ptr(), _TYPES[dtype],
+        _native.call_on(device, "pointops_cache_read", cache._packed, k.data_ptr(), v.data_ptr(), _TYPES[dtype],
                      _native.stream(device))
     return k, v
 
@@ -551,7 +561,7 @@ def _kept_step(q, keys, key_heads, tokens, bits, lengths, window, sinks, bias, e
         float(shape[3] ** -0.5 if scale is None else scale))
     size = _native.size_query("pointops_cache_attention_step_workspace_bytes", args)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _native.call("pointops_cache_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(device))
+    _native.call_on(device, "pointops_cache_attention_step", args, out.data_ptr(), _native.ptr(workspace), _native.stream(device))
     return out
 
 

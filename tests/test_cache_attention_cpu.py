@@ -3,7 +3,9 @@ no GPU: refusals of the public calls, the C ABI's before any launch, layouts."""
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 import struct
 
 import pytest
@@ -35,6 +37,22 @@ def test_layout(width, bits, row, groups):
     assert (c.k_codes[2, :, :4] == 9).all() and not c.k_codes[:2].any() and not c.k_codes[2, :, 4].any()
     assert c.positions(2, 5).k_codes.data_ptr() == c.k_codes.data_ptr() + 2 * row and c.positions(5, 5).tokens == 0
     assert "bits=%d" % bits in repr(part)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_copies(bits):
+    """Of a cache and of a part, by copy and by pickle, in memory of their own."""
+    c = cache(3, 5, 2, 40, bits)
+    c.k_codes.random_(0, 100)
+    c.v_scales.random_(0, 100)
+    for part in (c, c.cloud(1), c.positions(2, 4)):
+        for new in (copy.deepcopy(part), pickle.loads(pickle.dumps(part))):
+            assert (new.batch, new.tokens, new.heads, new.width, new.bits) == (part.batch, part.tokens, part.heads, 40, bits)
+            for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+                assert torch.equal(getattr(new, name), getattr(part, name))
+                assert getattr(new, name).data_ptr() != getattr(part, name).data_ptr()
+            with pytest.raises(ValueError, match="ROCm"):  # the next check
+                attention.cache_read(new)
 
 
 def test_cache_refusals():
