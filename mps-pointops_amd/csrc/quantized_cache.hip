@@ -1,10 +1,11 @@
 // A cache in 8 or 4 bits: writing new tokens to it and reading it back.
 //
 // Both are bound by memory: 8 x 16384 tokens of 8 heads of 128, float16 to 8 bits and back, take 160
-// and 152 us, 5.1 and 5.4 TB/s of what they read and write (a large copy: 4.7).  Four neighbouring lanes hold a group of 32 values,
-// eight each (16 bytes of a 16-bit type), and find its scale among themselves;
-// neighbouring lanes are pieces of a row, then the tokens behind it, so that codes
-// are written and read in whole lines (rows of 64 bytes for 4 bits and 128 values).
+// and 152 us, 5.1 and 5.4 TB/s of what they read and write (a large copy: 4.7).  Four
+// neighbouring lanes hold a group of 32 values, eight each (16 bytes of a 16-bit type),
+// and find its scale among themselves; neighbouring lanes are pieces of a row, then the
+// tokens behind it, so that codes are written and read in whole lines (rows of 64 bytes
+// for 4 bits and 128 values).
 #include <algorithm>
 
 #include "quantized_cache.hpp"
@@ -41,15 +42,16 @@ struct Piece {
     bool any;
 };
 
-// A block's pieces: 256 in a row's lanes, then tokens, of one key head.
+// A block's pieces: whole rows of one key head's tokens (of 96 values 21, four threads
+// are left over), so that no thread divides by more than a row's lanes.
+__host__ __device__ constexpr int rows_of(int D) { return kThreads / lanes_of(D); }
 __device__ __forceinline__ Piece piece_of(const CacheCall& c, int tokens, uint32_t blocks) {
-    const uint32_t chunk = blockIdx.x % blocks, unit = blockIdx.x / blocks;
-    const int lanes = lanes_of(c.D);
-    const int64_t at = static_cast<int64_t>(chunk) * kThreads + threadIdx.x;
+    const uint32_t chunk = blockIdx.x % blocks, unit = blockIdx.x / blocks, lanes = lanes_of(c.D);
+    const uint32_t row = threadIdx.x * (65536 / lanes + 1) >> 16;  // of fewer than 256 threads, exactly
     Piece p;
-    p.t = static_cast<int>(at / lanes);
-    p.at = static_cast<int>(at % lanes) * 8;
-    p.any = p.t < tokens;
+    p.t = static_cast<int>(chunk * rows_of(c.D) + row);
+    p.at = static_cast<int>(threadIdx.x - row * lanes) * 8;
+    p.any = static_cast<int>(row) < rows_of(c.D) && p.t < tokens;
     p.side = static_cast<int>(unit % 2);
     p.g = static_cast<int>(unit / 2 % c.G);
     p.b = static_cast<int>(unit / 2 / c.G);
@@ -215,7 +217,7 @@ bool read_cache(const pointops_cache* in, CacheCall* c) {
 
 // Blocks of one key head's tokens; false if the launch would not hold them all.
 bool blocks_of(const CacheCall& c, int tokens, uint32_t* each, uint32_t* all) {
-    const int64_t n = (static_cast<int64_t>(tokens) * lanes_of(c.D) + kThreads - 1) / kThreads;
+    const int64_t n = (static_cast<int64_t>(tokens) + rows_of(c.D) - 1) / rows_of(c.D);
     const int64_t units = int64_t(2) * c.B * c.G;
     if (units > INT32_MAX || n > INT32_MAX / units) return false;
     *each = static_cast<uint32_t>(n);
