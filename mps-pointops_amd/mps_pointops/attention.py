@@ -319,7 +319,7 @@ _KEYS = struct.Struct("@4Q7q")
 _STEP_RAW = struct.Struct("@Q4Q7q4Q7q3Q3q5q2q5if")
 _STEP_CODED = struct.Struct("@Q88s88s3Q3q5q2q5if")
 _NO_KEYS = bytes(_KEYS.size)
-_THREE = ctypes.c_int64 * 3
+_THREE = struct.Struct("@3q")
 _GROUP = 32
 
 
@@ -481,9 +481,9 @@ def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | N
     k, v = _rows(k), _rows(v)
     lengths, length_at, length_bits = _place_args(lengths)
     starts, start_at, start_bits = _place_args(starts)
-    _native.call_on(device, "pointops_cache_write", cache._packed, k.data_ptr(), _THREE(*k.stride()[:3]), v.data_ptr(),
-                 _THREE(*v.stride()[:3]), tokens, length_at, length_bits, start_at, start_bits, _TYPES[dtype],
-                 _native.stream(device))
+    _native.call_on(device, "pointops_cache_write", cache._packed, k.data_ptr(), _THREE.pack(*k.stride()[:3]), v.data_ptr(),
+                    _THREE.pack(*v.stride()[:3]), tokens, length_at, length_bits, start_at, start_bits, _TYPES[dtype],
+                    _native.stream(device))
 
 
 def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
@@ -502,7 +502,7 @@ def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) ->
     k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     if k.numel():
         _native.call_on(device, "pointops_cache_read", cache._packed, k.data_ptr(), v.data_ptr(), _TYPES[dtype],
-                     _native.stream(device))
+                        _native.stream(device))
     return k, v
 
 
@@ -632,7 +632,7 @@ def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = Non
                 raise TypeError(f"{name} must be a pair of tensors or a QuantizedCache")
             if t.ndim != dims:
                 raise ValueError(f"{name} must be two tensors of shape {shape}")
-            if t.dtype != dtype:
+            if t.dtype is not dtype:
                 raise TypeError(f"{name} must have the same type as q")
             if t.device != device:
                 raise ValueError(f"{name} must be on q's device")
@@ -651,9 +651,12 @@ def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = Non
     _native.require_device(device)
     if _tracked(q, bias, pk, pv, ck, cv):
         raise ValueError("prefix_attention_step has no gradients: call it under torch.no_grad()")
-    pk, pv, ck, cv = _rows(pk), _rows(pv), _rows(ck), _rows(cv)
-    keys = (pk.data_ptr(), pv.data_ptr(), 0, 0, 0, *pk.stride()[:2], 0, *pv.stride()[:2], start[0],
-            ck.data_ptr(), cv.data_ptr(), 0, 0, *ck.stride()[:3], *cv.stride()[:3], own[1])
+    a, b, c, d = pk.stride(), pv.stride(), ck.stride(), cv.stride()
+    if own[3] > 1 and not a[2] == b[2] == c[3] == d[3] == 1:
+        pk, pv, ck, cv = _rows(pk), _rows(pv), _rows(ck), _rows(cv)
+        a, b, c, d = pk.stride(), pv.stride(), ck.stride(), cv.stride()
+    keys = (pk.data_ptr(), pv.data_ptr(), 0, 0, 0, a[0], a[1], 0, b[0], b[1], start[0],
+            ck.data_ptr(), cv.data_ptr(), 0, 0, c[0], c[1], c[2], d[0], d[1], d[2], own[1])
     return _kept_step(q, keys, own[2], tokens, 0, lengths, window, sinks, bias, edges, scale)
 
 
