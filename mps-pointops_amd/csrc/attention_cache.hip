@@ -24,7 +24,8 @@ POINTOPS_FORM(bf16, kFour)
 namespace {
 
 struct JoinArgs {
-    int B, Q, H, G, D;
+    Divisor all, per, group;  // rows of a key head, of a sequence's, heads of a key head
+    int rows, Q, H, G, D;
     Parts start, own;
 };
 
@@ -32,16 +33,15 @@ struct JoinArgs {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const JoinArgs a, const float* __restrict__ parts,
                                                                         T* __restrict__ out) {
-    const int group = a.H / a.G, per = a.Q * group, width = part_width(padded(a.D));
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;  // (g, b, row)
-    const int64_t all = static_cast<int64_t>(a.B) * per, in_g = id % all;
-    if (id >= a.G * all) return;
-    const int g = static_cast<int>(id / all), b = static_cast<int>(in_g / per), row = static_cast<int>(in_g % per);
+    const int width = part_width(padded(a.D)), id = uniform(static_cast<int>(blockIdx.x * kWaves + threadIdx.x / kWave));  // (g, b, row)
+    if (id >= a.rows) return;
+    const int g = a.all.of_row(id), in_g = id - g * static_cast<int>(a.all.d);
+    const int b = a.per.of_row(in_g), row = in_g - b * static_cast<int>(a.per.d), i = a.group.of_row(row);
     RowSum sum;
     sum.add(a.start.first(parts, g, in_g, width), static_cast<int64_t>(a.start.rows) * width, a.start.splits, a.D);
-    sum.add(a.own.first(parts + a.start.floats, static_cast<int64_t>(b) * a.G + g, row, width),
-            static_cast<int64_t>(a.own.rows) * width, a.own.splits, a.D);
-    sum.write(out + ((static_cast<int64_t>(b) * a.Q + row / group) * a.H + g * group + row % group) * a.D, a.D);
+    sum.add(a.own.first(parts + a.start.floats, b * a.G + g, row, width), static_cast<int64_t>(a.own.rows) * width, a.own.splits, a.D);
+    const int h = g * static_cast<int>(a.group.d) + row - i * static_cast<int>(a.group.d);
+    sum.write(out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D, a.D);
 }
 
 int size_of(int type) { return type == POINTOPS_F32 ? 4 : 2; }
@@ -161,6 +161,7 @@ CachePlan plan_of(const CacheArgs& a, int type, int form) {
     const ShapeRows rows = kShapeRows[p.shape];
     auto cut = [&](Parts& parts, int each, int64_t rows, int64_t heads) {
         parts.rows = each;
+        while ((1 << parts.shift) < each) ++parts.shift;
         parts.blocks = static_cast<int>((rows + each - 1) / each);
         parts.units = heads * parts.blocks;
     };
@@ -195,8 +196,8 @@ hipError_t cache_step(const CacheArgs& a, int type, int form, void* out, void* w
                                          : launch_cache_form<T, kFour>;
     const hipError_t err = launch(a, plan, out, parts, stream);
     if (err != hipSuccess || !plan.joined) return err;
-    const int64_t rows = static_cast<int64_t>(a.B) * a.Q * a.H;
-    const JoinArgs join = {a.B, a.Q, a.H, a.G, a.D, plan.start, plan.own};
+    const int64_t rows = static_cast<int64_t>(a.B) * a.Q * a.H;  // (at most 2^30)
+    const JoinArgs join = {Divisor::of(rows / a.G), a.per, a.group, static_cast<int>(rows), a.Q, a.H, a.G, a.D, plan.start, plan.own};
     hipLaunchKernelGGL(attention_cache_join_kernel<T>, dim3(static_cast<uint32_t>((rows + kWaves - 1) / kWaves)),
                        dim3(kThreads), 0, stream, join, static_cast<const float*>(parts), static_cast<T*>(out));
     return hipGetLastError();

@@ -83,11 +83,12 @@ constexpr size_t kMostLds = 160 * 1024;
 __host__ __device__ constexpr int part_width(int DP) { return DP + 4; }
 
 struct Parts {
-    int rows, blocks, splits;  // of a block, blocks of rows of a key head, parts of each (0: none)
-    int64_t units;             // key heads (the caches': of all sequences) by blocks of rows
+    int rows, shift, blocks, splits;  // of a block (2^shift), blocks of rows of a key head, parts of each (0: none)
+    int64_t units;                    // key heads (the caches': of all sequences) by blocks of rows
     int64_t floats;
-    __device__ __forceinline__ const float* first(const float* parts, int64_t head, int64_t row, int width) const {
-        return parts + ((head * blocks + row / rows) * splits * rows + row % rows) * width;
+    __device__ __forceinline__ const float* first(const float* parts, int head, int row, int width) const {
+        const int64_t unit = static_cast<int64_t>(head) * blocks + (row >> shift);
+        return parts + (unit * splits * rows + (row & (rows - 1))) * width;
     }
 };
 
@@ -725,8 +726,9 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         at.tiles_of(first, low, high);
     }
     const int first_range = range[0].tiles, tiles = kRanges == 2 ? first_range + range[kRanges - 1].tiles : first_range;
-    const int begin = static_cast<int>(static_cast<int64_t>(tiles) * split_at / splits);
-    const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split_at + 1) / splits);
+    // The first `over` parts have one tile more.
+    const int each = tiles / splits, over = tiles - each * splits;
+    const int begin = split_at * each + min(split_at, over), end = begin + each + (split_at < over ? 1 : 0);
     std::conditional_t<kShared, Sh, In> in;
     in.set(*range[0].kept, a.D);
     bool in_second = false;
@@ -1088,23 +1090,24 @@ __global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (F
     const CacheArgs a, const CachePlan plan, T* __restrict__ out, float* __restrict__ parts) {
     extern __shared__ __attribute__((aligned(16))) char cache_lds[];
     constexpr int kStartRows = 16 * COLS * ROW_WAVES, kOwnRows = 16 * OWN_COLS;
-    const int64_t block = blockIdx.x, first = plan.start.units * plan.start.splits;
+    // (A launch has fewer than 2^31 blocks; divisions of 64 bits are a hundred instructions each.)
+    const uint32_t block = blockIdx.x, first = static_cast<uint32_t>(plan.start.units) * plan.start.splits;
     if (block < first) {
         // The row blocks of the same keys are eight blocks apart, on one XCD (whose L2 then
         // holds the keys for all of them).
-        const uint32_t all = static_cast<uint32_t>(a.G * plan.start.splits), eights = 8u * plan.start.blocks;
-        const uint32_t some = static_cast<uint32_t>(block) / eights, left = min(8u, all - 8 * some), in = static_cast<uint32_t>(block) % eights;
-        const uint32_t keys = 8 * some + in % left, row_block = in / left;
-        const int split_at = static_cast<int>(keys % plan.start.splits), g = static_cast<int>(keys / plan.start.splits);
-        const int64_t place = (static_cast<int64_t>(g) * plan.start.blocks + row_block) * plan.start.splits + split_at;
-        attention_part<T, FORM, DP, COLS, ROW_WAVES, kStepWaves, kStart>(a, out, parts + place * kStartRows * part_width(DP), 0, g,
-                                                                         static_cast<int>(row_block) * kStartRows, split_at, plan.start.splits, cache_lds);
+        const uint32_t splits = plan.start.splits, all = a.G * splits, eights = 8u * plan.start.blocks;
+        const uint32_t some = block / eights, left = min(8u, all - 8 * some), in = block - some * eights;
+        const uint32_t row_block = in / left, keys = 8 * some + in - row_block * left, g = keys / splits, split_at = keys - g * splits;
+        const int64_t place = (static_cast<int64_t>(g) * plan.start.blocks + row_block) * splits + split_at;
+        attention_part<T, FORM, DP, COLS, ROW_WAVES, kStepWaves, kStart>(
+            a, out, parts + place * kStartRows * part_width(DP), 0, static_cast<int>(g), static_cast<int>(row_block) * kStartRows,
+            static_cast<int>(split_at), plan.start.splits, cache_lds);
     } else {
-        const int64_t at = block - first, unit = at / plan.own.splits, bg = unit / plan.own.blocks;
+        const uint32_t at = block - first, unit = at / plan.own.splits, bg = unit / plan.own.blocks, b = bg / a.G;
         attention_part<T, FORM, DP, OWN_COLS, 1, kStepWaves, kOwn>(
-            a, out, plan.joined ? parts + plan.start.floats + at * kOwnRows * part_width(DP) : nullptr, static_cast<int>(bg / a.G),
-            static_cast<int>(bg % a.G), static_cast<int>(unit % plan.own.blocks) * kOwnRows, static_cast<int>(at % plan.own.splits),
-            plan.own.splits, cache_lds);
+            a, out, plan.joined ? parts + plan.start.floats + static_cast<int64_t>(at) * kOwnRows * part_width(DP) : nullptr,
+            static_cast<int>(b), static_cast<int>(bg - b * a.G), static_cast<int>(unit - bg * plan.own.blocks) * kOwnRows,
+            static_cast<int>(at - unit * plan.own.splits), plan.own.splits, cache_lds);
     }
 }
 
