@@ -130,8 +130,9 @@ int form_of(const pointops_cache_attention& in, CacheArgs* a) {
 }
 
 // LDS of a start's block whose waves share their keys: two sets of tiles (or the sums), the bias.
-size_t pairs_lds(const CacheArgs& a, int size) {
-    const size_t bytes = padded(a.D) * size, stride = bytes + (bytes == 256 ? 48 : 16), key_waves = kStepWaves / kShapeRows[kPairs].row_waves;
+size_t pairs_lds(const CacheArgs& a, int type, int form) {
+    const bool words = form == kAligned && type == POINTOPS_F32, streamed = form == kAligned && !words;
+    const size_t bytes = padded(a.D) * (words ? 4 : 2), stride = streamed ? bytes : bytes + (bytes == 256 ? 48 : 16), key_waves = kStepWaves / kShapeRows[kPairs].row_waves;
     const size_t rows = kShapeRows[kPairs].start(), tiles = 4 * kKeys * key_waves * stride, sums = rows * part_width(padded(a.D)) * 4;
     return std::max(tiles, sums) + 2 * key_waves * rows * 4 + bias_lds(a, static_cast<int>(rows));
 }
@@ -152,7 +153,7 @@ CachePlan plan_of(const CacheArgs& a, int type, int form) {
     const int64_t start_tiles = tiles(a.start.tokens), own_tiles = tiles(a.own.tokens);
     // (A window over both sees no more than one over either.)
     const int64_t both = std::min(start_tiles + own_tiles, seen + 1), heads = static_cast<int64_t>(a.B) * a.G;
-    const bool some = a.start.tokens != 0, pairs = pairs_lds(a, form == kAligned && type == POINTOPS_F32 ? 4 : 2) <= kMostLds;
+    const bool some = a.start.tokens != 0, pairs = pairs_lds(a, type, form) <= kMostLds;
     if (form == kAny) p.shape = kTwoTwo;
     else if (per <= 16 && both <= kDirectTiles && both * heads <= kDirectWork) p.shape = kDirect;
     else if (per > 16) p.shape = some && all > 32 && pairs ? kPairsTwo : kTwoTwo;

@@ -512,6 +512,94 @@ struct Shared {
     }
 };
 
+// The same for rows of 16 bits, which memory loads write to LDS themselves: 64 lanes' pieces of
+// 16 bytes one behind the other, so that rows have no room between them.  Each lane asks for the
+// piece that belongs there: within a row, piece p lies at p ^ turn(row), with which the row operands'
+// reads of 8 rows and the transposing reads of 4 rows and 2 pieces fall on all banks.  What lies
+// behind a row's width is cleared once; loads past the descriptor's end bring zeros.
+// 64 sequences behind 65536 tokens of width 128, in turn: 167 us through registers, 146 to 151 so (LDS
+// instructions 15 to 6 % of the time, the matrix units 37 to 40 % busy); 32 behind 32768 of width
+// 96 37 and 35, of 64 30 to 31 either way.
+template <typename T, int DP, int KW, int WAVES>
+struct Streamed {
+    static constexpr int kRows = kKeys * KW, kRowBytes = DP * 2, kPerRow = DP / 8, kBytes = 2 * kRows * kRowBytes;
+    static constexpr int kLoads = kRows * kPerRow / kWave / WAVES;  // of a wave and side, 1 KB each
+    static_assert(kRows * kPerRow % (kWave * WAVES) == 0);
+    // Rows of a multiple of 128 bytes have 8 pieces and more to change places among, others 4.
+    __device__ static __forceinline__ uint32_t turn(uint32_t row) {
+        if constexpr (kPerRow % 8 == 0) return (row & 3) << 1 | (row >> 2 & 1);
+        else return (row >> 1 & 1) << 1 | (row >> 2 & 1);
+    }
+    uint32_t at[2][kLoads];  // of this lane's pieces in a tile of rows; kNothing: none
+    uint32_t key_at[2], value_at[4];
+    int wave;
+
+    __device__ __forceinline__ uint32_t row_of(int x) const { return (static_cast<uint32_t>(x * WAVES + wave) * kWave + lane_id()) / kPerRow; }
+    __device__ __forceinline__ uint32_t piece_of(int x) const {
+        const uint32_t n = static_cast<uint32_t>(x * WAVES + wave) * kWave + lane_id();
+        return n % kPerRow ^ turn(n / kPerRow);
+    }
+    __device__ __forceinline__ void set(const Kept& kept, int width) {
+        wave = uniform(threadIdx.x / kWave);
+        const uint32_t lane = lane_id(), col = lane % 16, quad = lane / 16;
+#pragma unroll
+        for (int x = 0; x < kLoads; ++x) {
+            const bool here = static_cast<int>(piece_of(x)) * 8 < width;
+            at[0][x] = fixed(here ? row_of(x) * static_cast<uint32_t>(kept.kn) + piece_of(x) * 16 : kNothing);
+            at[1][x] = fixed(here ? row_of(x) * static_cast<uint32_t>(kept.vn) + piece_of(x) * 16 : kNothing);
+        }
+        // Key lane % 16's piece 4 c + quad, of even and of odd c.
+        const uint32_t turned = turn(col), high = turned / 4 * 64;
+        key_at[0] = col * kRowBytes + (quad ^ turned % 4) * 16 + high;
+        key_at[1] = col * kRowBytes + (quad ^ turned % 4) * 16 - high;
+        // Of keys 4 quad + i / 4 (i = lane % 16) columns 16 d + 4 (i % 4) .. + 3, of d % 4 = 0 .. 3.
+        const uint32_t row = 4 * quad + col / 4, by = turn(row);
+#pragma unroll
+        for (uint32_t d = 0; d < 4; ++d)
+            value_at[d] = row * kRowBytes + (d ^ by / 2) * 32 + (col % 4 / 2 ^ by % 2) * 16 + col % 2 * 8;
+    }
+    template <typename Rows>
+    __device__ static __forceinline__ void bring(Rows rows, char* to, uint32_t from) {
+        typedef __attribute__((address_space(3))) void lds_t;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_t*)to, 16, from, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const Kept& kept, const char* k, const char* v, int j0, int limit, int width, char* tiles) const {
+        const int count = min(limit - j0, kRows), bytes = width * 2;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const uint32_t stride = static_cast<uint32_t>(side == 0 ? kept.kn : kept.vn);
+            const auto rows = rows_from(side == 0 ? k : v, stride, j0, count, bytes);
+            char* const to = tiles + side * kRows * kRowBytes + wave * (kWave * 16);
+            if (count == kRows) {
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) bring(rows, to + x * WAVES * kWave * 16, at[side][x]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) {
+                    // Behind the last row: that row again (its scores are masked).
+                    const uint32_t row = min(row_of(x), static_cast<uint32_t>(count - 1));
+                    bring(rows, to + x * WAVES * kWave * 16, at[side][x] == kNothing ? kNothing : row * stride + piece_of(x) * 16);
+                }
+            }
+        }
+    }
+    // What this wave has asked for lies in LDS (vmcnt 0, the other counters left alone).
+    __device__ __forceinline__ void arrived() const { __builtin_amdgcn_s_waitcnt(0x0f70); }
+    // Row operand: key `row` + lane % 16 (row a multiple of 16), fragment c.
+    __device__ __forceinline__ i32x4 keys(const char* tiles, int row, int c) const {
+        return *reinterpret_cast<const i32x4*>(tiles + row * kRowBytes + 64 * c + key_at[c % 2]);
+    }
+    // Transposed operand of the 32 keys from `row` on: Incoming's order.
+    __device__ __forceinline__ i32x4 values(const char* tiles, int row, int d) const {
+        const char* const p = tiles + (kRows + row) * kRowBytes + d / 4 * 128 + value_at[d % 4];
+        typedef __attribute__((address_space(3))) s16x4 lds4;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * kRowBytes));
+        const i32x2 a = __builtin_bit_cast(i32x2, x), b = __builtin_bit_cast(i32x2, y);
+        return i32x4{a[0], a[1], b[0], b[1]};
+    }
+};
+
 // ------------------------------------------------------------- joining parts
 // A row's sum over keys, in a wave: lane l holds values l and l + 64.
 struct RowSum {
@@ -583,7 +671,9 @@ template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int WAVES>
 struct StepLds {
     static constexpr int kKeyWaves = WAVES / ROW_WAVES, kRows = 16 * COLS * ROW_WAVES;
     static constexpr int kSums = kRows * (DP + 4) * 4;
+    static constexpr bool kStreamed = ROW_WAVES > 1 && FORM == kAligned && sizeof(T) == 2;
     static constexpr int kTiles = ROW_WAVES == 1 ? WAVES * Incoming<T, FORM, DP>::kTileBytes
+                                  : kStreamed    ? 2 * Streamed<T, DP, kKeyWaves, WAVES>::kBytes
                                                  : 2 * Shared<T, FORM, DP, kKeyWaves, kWave * WAVES>::kBytes;
     // The tiles, then the sums in the same place; maxima and sums of the weights; then the
     // bias: [buckets][heads of the rows], the buckets of 0 .. reach, the edges.
@@ -629,7 +719,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                                                int g, int r0, int split_at, int splits, char* lds) {
     using Lds = StepLds<T, FORM, DP, COLS, ROW_WAVES, WAVES>;
     constexpr int kKeyWaves = Lds::kKeyWaves, kRows = Lds::kRows, kThreads = kWave * WAVES;
-    constexpr bool kShared = ROW_WAVES > 1, kManySequences = KIND == kStart;
+    constexpr bool kShared = ROW_WAVES > 1, kManySequences = KIND == kStart, kStreamed = Lds::kStreamed;
     using In = Incoming<T, FORM, DP>;
     using Sh = Shared<T, FORM, DP, kKeyWaves, kWave * WAVES>;
     using C = typename In::C;
@@ -729,10 +819,10 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     // The first `over` parts have one tile more.
     const int each = tiles / splits, over = tiles - each * splits;
     const int begin = split_at * each + min(split_at, over), end = begin + each + (split_at < over ? 1 : 0);
-    std::conditional_t<kShared, Sh, In> in;
+    std::conditional_t<kStreamed, Streamed<T, DP, kKeyWaves, WAVES>, std::conditional_t<kShared, Sh, In>> in;
     in.set(*range[0].kept, a.D);
     bool in_second = false;
-    auto fetch = [&](int tile) {
+    auto fetch = [&](int tile, char* to) {
         const bool second = kRanges == 2 && tile >= first_range;
         const Range<kTile, COLS>& at = range[second ? kRanges - 1 : 0];
         if (second && !in_second) {  // (whose strides may be others)
@@ -740,10 +830,17 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
             in_second = true;
         }
         const int from = at.first_key(second ? tile - first_range : tile);
-        in.load(*at.kept, at.k, at.v, at.k_scales, at.v_scales, from, at.limit, a.D);
+        if constexpr (kStreamed) in.load(*at.kept, at.k, at.v, from, at.limit, a.D, to);
+        else in.load(*at.kept, at.k, at.v, at.k_scales, at.v_scales, from, at.limit, a.D);
     };
     int tile = kShared ? begin : begin + wave;
-    if (tile < end) fetch(tile);
+    if constexpr (kStreamed) {
+        if (a.D < DP) {
+            for (int x = threadIdx.x; x < Lds::kTiles / 16; x += kThreads) reinterpret_cast<i32x4*>(lds)[x] = i32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
+    }
+    if (tile < end) fetch(tile, lds);
 
     i32x4 q[COLS][kFrags][kQ];
 #pragma unroll
@@ -912,7 +1009,10 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 #pragma unroll
         for (int x = 0; x < kBatch; ++x)
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) f[x][h] = In::values(values, h, d + x);
+            for (int h = 0; h < kHalves; ++h) {
+                if constexpr (kStreamed) f[x][h] = in.values(values, kKeys * key_wave, d + x);
+                else f[x][h] = In::values(values, h, d + x);
+            }
     };
     auto add = [&](const char* values) {
 #pragma unroll
@@ -934,26 +1034,33 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
     };
     if constexpr (kShared) {
         // Two sets of tiles in LDS: one barrier a tile.
+        constexpr int kSet = Lds::kTiles / 2;
         char* now = lds;
-        if (tile < end) in.store(now);
+        if constexpr (kStreamed) in.arrived();
+        else if (tile < end) in.store(now);
         __syncthreads();
         for (; tile < end; ++tile) {
-            if (tile + 1 < end) fetch(tile + 1);
+            char* const then = now == lds ? lds + kSet : lds;
+            if (tile + 1 < end) fetch(tile + 1, then);
             const int at = kKeys * key_wave;
-            const char* const values = now + (Sh::kRows + at) * Sh::TileT::kStride;
+            const char* const values = kStreamed ? now : now + (Sh::kRows + at) * Sh::TileT::kStride;
             i32x4 kf[2][kFrags];
 #pragma unroll
             for (int c = 0; c < kFrags; ++c)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) kf[u][c] = Sh::keys(now, at + 16 * u, c);
+                for (int u = 0; u < 2; ++u) {
+                    if constexpr (kStreamed) kf[u][c] = in.keys(now, at + 16 * u, c);
+                    else kf[u][c] = Sh::keys(now, at + 16 * u, c);
+                }
             keep_order();
             score([&](int u, int c) { return kf[u][c]; });
             ask(values, 0, vf[0]);
             keep_order();
             weigh(range[0], range[0].first_key(tile) + at);
             add(values);
-            now = now == lds ? lds + Sh::kBytes : lds;
-            if (tile + 1 < end) in.store(now);
+            now = then;
+            if constexpr (kStreamed) in.arrived();
+            else if (tile + 1 < end) in.store(now);
             __syncthreads();
         }
     } else {
@@ -961,7 +1068,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         for (; tile < end; tile += WAVES) {
             score([&](int u, int c) { return in.keys(u, c); });
             in.store_values(values);
-            if (tile + WAVES < end) fetch(tile + WAVES);
+            if (tile + WAVES < end) fetch(tile + WAVES, nullptr);
             lanes_exchange();
             ask(values, 0, vf[0]);
             if (kRanges == 2 && tile >= first_range) weigh(range[kRanges - 1], range[kRanges - 1].first_key(tile - first_range));

@@ -100,3 +100,24 @@ def test_scores_that_rise_and_fall(cuda_device, kind, bits):
     k = prefix[0].clone()
     k[:64] = -q[0, 0, 0] * 20  # about -160 for one row, anything for the others
     run(kind, q, (k, prefix[1]), own, None, bits)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("D", [8, 48, 64, 72, 80, 96, 104, 128])
+@pytest.mark.parametrize("P", [1281, 1312, 1344, 2111])
+def test_shared_rows_of_all_widths(cuda_device, kind, D, P):
+    """A start that many sequences' blocks read, inside a longer one: no numbers before it,
+    behind it and beside its rows, and in the keys that the window leaves out."""
+    q, prefix, own, _ = make(7, kind, 70, 1, P, 5, 4, 2, D)
+    wide = [torch.full((P + 70, 2, D + 16), math.nan, dtype=t.dtype, device="cuda") for t in prefix]
+    inside = [x[5:P + 5, :, :D] for x in wide]
+    for x, t in zip(inside, prefix):
+        x.copy_(t)
+    lengths = torch.arange(70, device="cuda") % 6
+    for window, sinks in ((None, 0), (1290, 3)):
+        how = {} if window is None else dict(window=window, sinks=sinks)
+        want = want_of(q, prefix, own, lengths, 0, **how)
+        if window is not None:
+            for x in inside:
+                x[sinks:max(sinks, P - window - 3)] = math.nan
+        close(step(q, inside, own, lengths, 0, **how), want, LIMIT[kind])
