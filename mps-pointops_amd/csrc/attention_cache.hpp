@@ -18,6 +18,11 @@
 // products lose none of their bits.  Sixteen columns, not 32: a step of one token has H / G
 // rows a key head, mostly 16 or fewer, and the products and exponentials of the columns
 // that stay empty are work too.
+//
+// A long cache's keys are bound by HBM: 4 x 65536 tokens of 32 heads over 8 of 128 in 8 bits 73 us,
+// 6.0 TB/s; in 4 bits under float16 by instructions (32 x 8192: 47 us, 4.6 TB/s); the start's rows by
+// what is issued beside the products (64 sequences behind 65536 tokens: 455 to 470 T/s of the pairs,
+// matrix units 40 % busy); short ones by one block's latency (10 to 18 us).
 #pragma once
 
 #include <algorithm>

@@ -1,7 +1,7 @@
 // A cache in 8 or 4 bits: writing new tokens to it and reading it back.
 //
-// Both are bound by memory: 8 x 16384 tokens of 8 heads of 128, float16 to 8 bits and back, take 160
-// and 152 us, 5.1 and 5.4 TB/s of what they read and write (a large copy: 4.7).  Four
+// Both are bound by memory: 8 x 16384 tokens of 8 heads of 128, float16 to 8 bits and back, take 169
+// and 158 us, 4.8 and 5.1 TB/s of what they read and write (a large copy: 4.7).  Four
 // neighbouring lanes hold a group of 32 values, eight each (16 bytes of a 16-bit type),
 // and find its scale among themselves; neighbouring lanes are pieces of a row, then the
 // tokens behind it, so that codes are written and read in whole lines (rows of 64 bytes
