@@ -293,6 +293,22 @@ struct Stage {
 // weights up to 2^8 cost no precision, and outputs are rescaled seldom.
 constexpr float kSlack = 8.f;
 
+// Where a weight is the sum of two values of 16 bits, bfloat16 keeps 16 bits of any of
+// them, and float16, whose smallest step is 2^-24, loses those of the small ones: so there a row's
+// reference lies 12 below its maximum and the weights fill float16's range, up to 2^15.
+// Those down to 2^-24 of the row's largest keep 12 bits and more; all are off by at most
+// 2^-37 of it (one key with 99.8 % of 16384's weight and a value of zero: error of the result
+// 2e-2 by weights of up to 1).
+template <typename T>
+constexpr float kMostLog = __is_same(T, f16) ? 15.f : kSlack;
+// A row's reference by the largest of its scores, in units of log 2.  (At 2^20 and more
+// a difference of 12 may be rounded up, and steps of 1/8 leave no small weights but of other scores.)
+template <typename T>
+__device__ __forceinline__ float reference_of(float top) {
+    if constexpr (__is_same(T, f16)) return fabsf(top) < 0x1p20f ? top - 12.f : top;
+    else return top;
+}
+
 // Rows of an inner tile: 64, or 32 where a value has 32 bits (the same LDS).
 template <typename T>
 constexpr int kInner = sizeof(T) == 4 ? 32 : 64;

@@ -80,7 +80,9 @@ struct CacheArgs {
 
 constexpr int kStepWaves = 4, kStepThreads = kStepWaves * kWave;
 constexpr int kKeys = 32;  // of a wave at a time
-constexpr float kMostWeight = 256.f;  // the running maximum may lie 8 (in units of log 2) below the true one
+// The running maximum may lie 8 (in units of log 2; float16: 3) below the true one.
+template <typename C>
+constexpr float kMostWeight = static_cast<float>(1 << static_cast<int>(kMostLog<C>));
 constexpr size_t kMostLds = 160 * 1024;
 
 // Parts of a sum over keys: of a unit (a key head with a block of rows), `splits` of them,
@@ -972,8 +974,8 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                 for (int e = 0; e < 8; ++e) x[n][e] = exp2_fast(__builtin_fmaf(s[n][e / 4][e % 4], factor, -less));
             }
         };
-        // The weights by the maximum so far; where one of them has outgrown it (or there is none
-        // yet), by a new one.  So the scores' own maximum is seldom asked for.
+        // The weights by the maximum so far (its reference, in m); where one of them has outgrown
+        // it (or there is none yet), by a new one.  So the scores' own maximum is seldom asked for.
         form();
         bool rises = false;
 #pragma unroll
@@ -981,7 +983,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
             float most = x[n][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) most = fmaxf(most, x[n][e]);
-            rises |= most > kMostWeight || m[n] == -kInf;
+            rises |= most > kMostWeight<C> || m[n] == -kInf;
         }
         if (ballot(rises) != 0) {
 #pragma unroll
@@ -989,7 +991,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                 float top = s[n][0][0];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) top = fmaxf(top, s[n][e / 4][e % 4]);
-                const float next = fmaxf(m[n], quads_max(top) * factor);
+                const float next = fmaxf(m[n], reference_of<C>(quads_max(top) * factor));
                 const float keep = m[n] == next ? 1.f : exp2_fast(m[n] - next);
                 m[n] = next;
                 l[n] *= keep;
