@@ -12,7 +12,7 @@
 //
 // As the products wait for memory, 16-bit weights keep their bits: values are
 // multiplied by the rounded weights and by what the rounding left, so that outputs
-// carry the result's rounding alone (bfloat16, error against 64 bits over one
+// carry the result's rounding alone (float16's fill its range for it; bfloat16, error against 64 bits over one
 // rounding's: 1.35 -> 1.0; 4 x 65536 keys, 32 heads over 8 of 128, 166.8 -> 168.7 us,
 // 4 x 2048, 8 heads over 2 of 64, window 512, 12.1 -> 12.6).
 #include <algorithm>
@@ -154,8 +154,8 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
 #pragma unroll
         for (int x = 1; x < 16; ++x) top = fmaxf(top, s[x]);
         top = halves_max(top);
-        if (ballot(top > m + kSlack) != 0) {
-            const float next = fmaxf(m, top);
+        if (ballot(top - m > kMostLog<T>) != 0) {
+            const float next = fmaxf(m, reference_of<T>(top));
             const float keep = m == next ? 1.f : exp2_fast(m - next);
             m = next;
             l *= keep;

@@ -26,9 +26,8 @@ float16 and bfloat16 are rounded to the type before a matrix product takes them:
 ``window_attention``'s weights (output and gradients) and the gradients of its
 scores; its errors are about 1.4 times those of one rounding of the exact
 result, and float16's weights and score gradients below 6e-5 keep fewer bits
-(scale the loss).  ``window_attention_step`` keeps its weights' bits, and so do
-the steps over kept keys; ``prefix_attention_step`` over float16 tensors holds them to 2 ** -37
-of a row's largest weight.  Callers
+(scale the loss).  ``window_attention_step`` and the steps over kept keys keep
+their weights' bits (over float16 tensors to 2 ** -37 of a row's largest).  Callers
 who need more take float32, whose exponentials and inverse roots are the
 hardware's (errors of about 4e-7 and 3e-7 of a result's norm).
 """
