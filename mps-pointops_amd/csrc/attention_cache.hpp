@@ -402,10 +402,12 @@ struct Incoming {
 
 // ------------------------------------------------------------ careful rows
 // One query by a whole wave, key by key, for rows whose sums are not finite: there a
-// product with a masked key's infinity or NaN may have spread.  Lane l holds elements l
-// and l + 64.
+// product with a masked key's infinity or NaN may have spread, or their finite values have
+// passed 32 bits (the weights reach 2^8 and their number).  Lane l holds elements l and l + 64.
+// m lies kAbove (in units of log 2) above the maximum: the sums of 2^30 keys are finite as their values are.
 template <typename T, int FORM>
 struct CarefulKept {
+    static constexpr float kAbove = 30.f;
     float q0, q1, m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
     bool d0, d1;
     float scale_log2;
@@ -426,7 +428,7 @@ struct CarefulKept {
         const int lane = lane_id();
         const float s = wave_sum((d0 ? q0 * value(k, ks, lane) : 0.f) + (d1 ? q1 * value(k, ks, lane + kWave) : 0.f)) * scale_log2 + bias;
         if (s == -kInf) return;
-        const float top = fmaxf(m, s), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
+        const float top = fmaxf(m, s + kAbove), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
         m = top;
         l = l * keep + w;
         o0 = o0 * keep + (d0 ? w * value(v, vs, lane) : 0.f);
@@ -1170,14 +1172,15 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                             done = none ? c.l != c.l : c.settled(n0, n1);
                         }
             }
-            if (none) {
+            // The finite sums, brought to the careful ones' maximum.  (Where these ended early, all of
+            // them are not finite again.)
+            const float by = done ? 1.f : exp2_fast(lm - c.m);
+            if (none || !done) {
                 lm = c.m;
                 ll = c.l;
             }
-            // To the maximum of the products' sums.
-            const float by = none ? 1.f : exp2_fast(c.m - lm);
-            x0 = n0 ? c.o0 * by : x0;
-            x1 = n1 ? c.o1 * by : x1;
+            x0 = n0 ? c.o0 : x0 * by;
+            x1 = n1 ? c.o1 : x1 * by;
         }
         if (KIND == kBoth || part == nullptr) {
             const Row at_row = row_of(r0 + row);
