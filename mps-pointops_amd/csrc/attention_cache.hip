@@ -37,9 +37,21 @@ __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const Jo
     if (id >= a.rows) return;
     const int g = a.all.of_row(id), in_g = id - g * static_cast<int>(a.all.d);
     const int b = a.per.of_row(in_g), row = in_g - b * static_cast<int>(a.per.d), i = a.group.of_row(row);
-    RowSum sum;
-    sum.add(a.start.first(parts, g, in_g, width), static_cast<int64_t>(a.start.rows) * width, a.start.splits, a.D);
-    sum.add(a.own.first(parts + a.start.floats, b * a.G + g, row, width), static_cast<int64_t>(a.own.rows) * width, a.own.splits, a.D);
+    auto join = [&](RowSum sum) {
+        sum.add(a.start.first(parts, g, in_g, width), static_cast<int64_t>(a.start.rows) * width, a.start.splits, a.D);
+        sum.add(a.own.first(parts + a.start.floats, b * a.G + g, row, width), static_cast<int64_t>(a.own.rows) * width, a.own.splits, a.D);
+        sum.divide();
+        return sum;
+    };
+    RowSum sum = join({});
+    if (ballot(!finite(sum.x0) || !finite(sum.x1)) != 0) {
+        // Values near the largest, of which a mean is finite and a sum need not be.
+        RowSum low;
+        low.above = 30.f;
+        low = join(low);
+        sum.x0 = finite(sum.x0) ? sum.x0 : low.x0;
+        sum.x1 = finite(sum.x1) ? sum.x1 : low.x1;
+    }
     const int h = g * static_cast<int>(a.group.d) + row - i * static_cast<int>(a.group.d);
     sum.write(out + ((static_cast<int64_t>(b) * a.Q + i) * a.H + h) * a.D, a.D);
 }

@@ -610,9 +610,10 @@ struct Streamed {
 };
 
 // ------------------------------------------------------------- joining parts
-// A row's sum over keys, in a wave: lane l holds values l and l + 64.
+// A row's sum over keys, in a wave: lane l holds values l and l + 64.  All are 2^-above of
+// what they are by the maximum m.
 struct RowSum {
-    float m = -kInf, l = 0.f, x0 = 0.f, x1 = 0.f;
+    float m = -kInf, l = 0.f, x0 = 0.f, x1 = 0.f, above = 0.f;
 
     // Adds `count` parts, `step` floats from one to the next, in order.
     __device__ __forceinline__ void add(const float* first, int64_t step, int count, int D) {
@@ -642,7 +643,7 @@ struct RowSum {
             const int s = from + lane;
             float by = 0.f;
             if (s < count) {
-                by = exp2_fast(first[s * step] - less);
+                by = exp2_fast(first[s * step] - less - above);
                 sum = __builtin_fmaf(first[s * step + 1], by, sum);
             }
             const int some = min(kWave, count - from);
@@ -660,12 +661,17 @@ struct RowSum {
         }
         l = __builtin_fmaf(l, keep, wave_sum(sum));
     }
+    // The means.
+    __device__ __forceinline__ void divide() {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        x0 *= inv;
+        x1 *= inv;
+    }
     template <typename T>
     __device__ __forceinline__ void write(T* dst, int D) const {
         const int lane = lane_id();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (lane < D) dst[lane] = from_float<T>(x0 * inv);
-        if (lane + kWave < D) dst[lane + kWave] = from_float<T>(x1 * inv);
+        if (lane < D) dst[lane] = from_float<T>(x0);
+        if (lane + kWave < D) dst[lane + kWave] = from_float<T>(x1);
     }
 };
 
@@ -1184,7 +1190,8 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
         }
         if (KIND == kBoth || part == nullptr) {
             const Row at_row = row_of(r0 + row);
-            const RowSum all{lm, ll, x0, x1};
+            RowSum all{lm, ll, x0, x1};
+            all.divide();
             all.write(out + ((static_cast<int64_t>(at_row.b) * a.Q + at_row.i) * a.H + g * group + at_row.h) * a.D, a.D);
         } else {
             float* const dst = part + static_cast<int64_t>(row) * part_width(DP);

@@ -42,3 +42,26 @@ def test_large_values(cuda_device, kind, bits, B, Q, P, N, H, G, D, largest):
     got = step(q, kept(start, bits), b, lengths, bits)
     if not bits:
         assert torch.isnan(got[..., 0]).all() and torch.isfinite(got[..., 1:]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8, 4])
+@pytest.mark.parametrize("B,P,N,D", [(1, 6000, 300, 64), (2, 40, 5000, 128), (40, 3000, 20, 128), (4, 500, 40, 64)])
+def test_few_keys_of_large_values(cuda_device, kind, bits, B, P, N, D):
+    """Some keys of equal scores far above the others', with the same large value: each part's sum is
+    finite, and that of all parts is not."""
+    print(kind, bits, B, P, N, D, flush=True)
+    large = 1.5e38 if bits == 4 else 3e38  # (3e38 is 3.53 x 2^126, which 4 bits round to 2^128)
+    q, start, own, _ = make(22, kind, B, 1, P, N, 4, 2, D)
+    q[..., 0] = 8.0
+    for k, v in (start, own):
+        keys = k.shape[-3]
+        k[..., 0] = 0.0
+        some = k[..., ::max(1, keys // 5), :, :]
+        some.zero_()
+        some[..., 0] = 5.0 * D ** 0.5
+        v[..., ::max(1, keys // 5), :, 1::2] = large
+    got = step(q, kept(start, bits), kept(own, bits), None, bits)
+    want = want_of(q, start, own, None, bits)
+    close(got, want, LIMIT[kind])
+    close(got[..., ::2], want[..., ::2], LIMIT[kind])
