@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
         if (ll == 0.f) {
             x0 = x1 = 0.f;
         } else if (whole ? ballot(masks) != 0 : ballot(n0 || n1) != 0) {
-            CarefulRow<T> c(a, b, g, a.q.at<T>(b, hh) + ii * a.q.n);
+            CarefulRow<T> c(a, b, g, a.q.at<T>(b, hh) + ii * a.q.n, 30.f);
             const Seen sees = seen_by(a, shift + ii, len);
             bool done = false;
             for (int t = begin; t < end && !done; ++t)
@@ -252,14 +252,15 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
                         c.add(j, biased ? bias_at(shift + ii - j, row) : 0.f);
                         done = whole ? c.l != c.l : c.settled(n0, n1);
                     }
-            if (whole) {
+            // The finite sums, brought to the careful ones' maximum.  (Where these ended early, all of
+            // them are not finite again.)
+            const float by = done ? 1.f : exp2_fast(lm - c.m);
+            if (whole || !done) {
                 lm = c.m;
                 ll = c.l;
             }
-            // To the maximum of the products' sums.
-            const float by = whole ? 1.f : exp2_fast(c.m - lm);
-            x0 = n0 ? c.o0 * by : x0;
-            x1 = n1 ? c.o1 * by : x1;
+            x0 = n0 ? c.o0 : x0 * by;
+            x1 = n1 ? c.o1 : x1 * by;
         }
         if (splits == 1) {
             const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -296,40 +297,54 @@ __global__ __launch_bounds__(kThreads) void attention_step_join_kernel(const Arg
     for (int s = lane; s < splits; s += kWave) top = fmaxf(top, src[s * step]);
     top = wave_max(top);
     const float base = top == -kInf ? 0.f : top;
-    float sum = 0.f, x0 = 0.f, x1 = 0.f;
     const int c0 = min(lane, a.D - 1), c1 = min(lane + kWave, a.D - 1);
-    for (int first = 0; first < splits; first += kWave) {
-        // A lane's split: its factor; then the splits' rows one after another.
-        const int s = first + lane;
-        float by = 0.f;
-        if (s < splits) {
-            by = exp2_fast(src[s * step] - base);
-            sum = __builtin_fmaf(src[s * step + 1], by, sum);
-        }
-        const int count = min(kWave, splits - first);
-        const float* const rows = src + first * step + 2;
-        constexpr int kAtOnce = 8;
-        for (int i = 0; i < count; i += kAtOnce) {
-            float y0[kAtOnce], y1[kAtOnce];
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                const int64_t at = min(i + k, count - 1) * step;
-                y0[k] = rows[at + c0];
-                y1[k] = rows[at + c1];
+    // The splits' mean; all sums are 2^-above of what they are by the maximum.
+    auto mean = [&](float above, float& x0, float& x1) {
+        float sum = x0 = x1 = 0.f;
+        for (int first = 0; first < splits; first += kWave) {
+            // A lane's split: its factor; then the splits' rows one after another.
+            const int s = first + lane;
+            float by = 0.f;
+            if (s < splits) {
+                by = exp2_fast(src[s * step] - base - above);
+                sum = __builtin_fmaf(src[s * step + 1], by, sum);
             }
+            const int count = min(kWave, splits - first);
+            const float* const rows = src + first * step + 2;
+            constexpr int kAtOnce = 8;
+            for (int i = 0; i < count; i += kAtOnce) {
+                float y0[kAtOnce], y1[kAtOnce];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                const float f = i + k < count ? i2f(readlane(f2i(by), min(i + k, count - 1))) : 0.f;
-                x0 = __builtin_fmaf(y0[k], f, x0);
-                x1 = __builtin_fmaf(y1[k], f, x1);
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int64_t at = min(i + k, count - 1) * step;
+                    y0[k] = rows[at + c0];
+                    y1[k] = rows[at + c1];
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const float f = i + k < count ? i2f(readlane(f2i(by), min(i + k, count - 1))) : 0.f;
+                    x0 = __builtin_fmaf(y0[k], f, x0);
+                    x1 = __builtin_fmaf(y1[k], f, x1);
+                }
             }
         }
+        sum = wave_sum(sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        x0 *= inv;
+        x1 *= inv;
+    };
+    float x0, x1;
+    mean(0.f, x0, x1);
+    if (ballot(!finite(x0) || !finite(x1)) != 0) {
+        // Values near the largest, of which a mean is finite and a sum need not be.
+        float y0, y1;
+        mean(30.f, y0, y1);
+        x0 = finite(x0) ? x0 : y0;
+        x1 = finite(x1) ? x1 : y1;
     }
-    sum = wave_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* const dst = out + ((static_cast<int64_t>(b) * a.Q + row / group) * a.H + g * group + row % group) * a.D;
-    if (lane < a.D) dst[lane] = from_float<T>(x0 * inv);
-    if (lane + kWave < a.D) dst[lane + kWave] = from_float<T>(x1 * inv);
+    if (lane < a.D) dst[lane] = from_float<T>(x0);
+    if (lane + kWave < a.D) dst[lane + kWave] = from_float<T>(x1);
 }
 
 struct Plan {
