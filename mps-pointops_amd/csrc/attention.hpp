@@ -537,17 +537,17 @@ __device__ __forceinline__ bool odd_value(uint64_t odd, int r, int c) {
 // there a product with a masked key's infinity or NaN may have spread.  Only
 // keys that the row sees are added (one whose score is -inf, or whose bias is,
 // whatever it holds, has no weight and is left out).  Lane l holds elements l and
-// l + 64, of which it needs those that came out not finite (n0, n1).  m lies `above` (in
-// units of log 2) above the maximum: 30, and the sums of 2^30 keys are finite as their values are.
+// l + 64, of which it needs those that came out not finite (n0, n1).  m lies kAbove (in
+// units of log 2) above the maximum: the sums of 2^30 keys are finite as their values are.
 template <typename T>
 struct CarefulRow {
     const Args& a;
     const T *k, *v;
-    const float above;
+    static constexpr float kAbove = 30.f;
     float q0, q1, m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
     bool d0, d1;
 
-    __device__ __forceinline__ CarefulRow(const Args& args, int b, int g, const T* q, float above = 0.f) : a(args), above(above) {
+    __device__ __forceinline__ CarefulRow(const Args& args, int b, int g, const T* q) : a(args) {
         const int lane = lane_id();
         k = a.k.at<T>(b, g) + lane;
         v = a.v.at<T>(b, g) + lane;
@@ -561,12 +561,14 @@ struct CarefulRow {
         const float k0 = d0 ? to_float(k[j * a.k.n]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + kWave]) : 0.f;
         const float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2 + bias;
         if (s == -kInf) return;
-        const float top = fmaxf(m, s + above), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
+        const float top = fmaxf(m, s + kAbove), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
         m = top;
         l = l * keep + w;
         o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n]) : 0.f);
         o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + kWave]) : 0.f);
     }
+    // log2 of the sum of 2^score (the maximum first: beside 30 it would lose bits).
+    __device__ __forceinline__ float log_sum() const { return (m - kAbove) + log2f(l * exp2f(kAbove)); }
     // Whether all that is needed has come out not finite again.
     __device__ __forceinline__ bool settled(bool n0, bool n1) const {
         return ballot((n0 && finite(o0)) || (n1 && finite(o1))) == 0;

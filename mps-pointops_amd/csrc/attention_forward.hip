@@ -83,7 +83,7 @@ __device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, 
     const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
     if (n0) out[lane] = from_float<T>(row.o0 * inv);
     if (n1) out[lane + kWave] = from_float<T>(row.o1 * inv);
-    if (whole && lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
+    if (whole && lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.log_sum();
 }
 
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>

@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
         if (ll == 0.f) {
             x0 = x1 = 0.f;
         } else if (whole ? ballot(masks) != 0 : ballot(n0 || n1) != 0) {
-            CarefulRow<T> c(a, b, g, a.q.at<T>(b, hh) + ii * a.q.n, 30.f);
+            CarefulRow<T> c(a, b, g, a.q.at<T>(b, hh) + ii * a.q.n);
             const Seen sees = seen_by(a, shift + ii, len);
             bool done = false;
             for (int t = begin; t < end && !done; ++t)
