@@ -18,6 +18,7 @@ from pathlib import Path
 
 import torch
 from torch.autograd import forward_ad
+from torch.utils import _python_dispatch
 
 LIB_NAME = "libpointops_hip.so"
 LIB_PATH = Path(__file__).resolve().with_name(LIB_NAME)
@@ -224,6 +225,18 @@ def untraced() -> bool:
     dispatch modes, all of which see tensor operations only."""
     return (_interpreter() is None and forward_ad._current_level < 0 and _modes() == 0
             and not _is_tracing() and not _is_compiling())
+
+
+def recorded(*tensors: torch.Tensor) -> bool:
+    """Whether a call of these is traced, transformed or compiled, runs under a dispatch
+    mode that takes the tensors' memory away (others, which count or log operations, leave
+    it as it is), or has tangents."""
+    if untraced():
+        return False
+    return (_interpreter() is not None or _is_tracing() or _is_compiling()
+            or any(mode.is_infra_mode() for mode in _python_dispatch._get_current_dispatch_mode_stack())
+            or (forward_ad._current_level >= 0
+                and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t.is_floating_point())))
 
 
 def plain(*tensors: torch.Tensor) -> bool:

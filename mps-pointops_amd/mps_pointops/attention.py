@@ -432,8 +432,12 @@ def _place_args(places: Tensor | None) -> tuple[Tensor | None, int, int]:
     return places, places.data_ptr(), _PLACES[places.dtype]
 
 
-def _check_untraced(name: str) -> None:
-    if not _native.untraced():
+def _check_unrecorded(name: str, *args) -> None:
+    """Of a call with these tensors and pairs of them."""
+    if _native.untraced():
+        return
+    every = (t for arg in args for t in (arg if isinstance(arg, (tuple, list)) else (arg,)))
+    if _native.recorded(*(t for t in every if isinstance(t, Tensor))):
         raise RuntimeError(f"{name} works on kept memory: traces, transforms and forward-mode differentiation "
                            "do not see it")
 
@@ -449,7 +453,7 @@ def cache_write(cache: QuantizedCache, k: Tensor, v: Tensor, lengths: Tensor | N
     stay as they are.  k and v are float32, float16 or bfloat16 with any strides; the
     rounding to codes has no gradient.
     """
-    _check_untraced("cache_write")
+    _check_unrecorded("cache_write", k, v)
     _check_cache(cache)
     if not isinstance(k, Tensor) or not isinstance(v, Tensor):
         raise TypeError("k and v must be tensors")
@@ -493,7 +497,7 @@ def cache_read(cache: QuantizedCache, *, dtype: torch.dtype = torch.bfloat16) ->
     and bfloat16 hold every value exactly but those below their smallest normal
     numbers, float16 those from 2 ** -14 to 65504.
     """
-    _check_untraced("cache_read")
+    _check_unrecorded("cache_read")
     _check_cache(cache)
     if dtype not in _TYPES:
         raise TypeError("dtype must be float32, float16 or bfloat16")
@@ -583,7 +587,7 @@ def quantized_attention_step(q: Tensor, cache: QuantizedCache, lengths: Tensor |
     that the cache holds, without a further rounding of them, of the queries or of
     the weights.  ``q (B, Q, H, D)`` is float32, float16 or bfloat16.
     """
-    _check_untraced("quantized_attention_step")
+    _check_unrecorded("quantized_attention_step", q, bias)
     _check_query(q)
     _check_coded(q, cache, "cache", q.shape[0])
     edges = _check_step(q, cache.heads, cache.tokens, window, sinks, bias, max_distance, lengths)
@@ -607,7 +611,7 @@ def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = Non
     Where they are long, the start's keys are read once for all queries of the batch.
     Without gradients.
     """
-    _check_untraced("prefix_attention_step")
+    _check_unrecorded("prefix_attention_step", q, prefix, cache, bias)
     _check_query(q)
     if type(prefix) is QuantizedCache or type(cache) is QuantizedCache:
         if type(prefix) is not type(cache):
