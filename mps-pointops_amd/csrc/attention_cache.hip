@@ -173,9 +173,9 @@ CachePlan plan_of(const CacheArgs& a, int type, int form) {
     else p.shape = all > 32 && pairs ? kPairs : kTwo;
     const ShapeRows rows = kShapeRows[p.shape];
     auto cut = [&](Parts& parts, int each, int64_t rows, int64_t heads) {
-        parts.rows = each;
         while ((1 << parts.shift) < each) ++parts.shift;
         parts.blocks = static_cast<int>((rows + each - 1) / each);
+        parts.rows = static_cast<int>(std::min<int64_t>(each, rows));
         parts.units = heads * parts.blocks;
     };
     cut(p.own, rows.own(), per, heads);

@@ -90,12 +90,14 @@ constexpr size_t kMostLds = 160 * 1024;
 __host__ __device__ constexpr int part_width(int DP) { return DP + 4; }
 
 struct Parts {
-    int rows, shift, blocks, splits;  // of a block (2^shift), blocks of rows of a key head, parts of each (0: none)
+    // A part's rows (of a block's 2^shift those that there are, where it is the only one), blocks of
+    // rows of a key head, parts of each (0: none).
+    int rows, shift, blocks, splits;
     int64_t units;                    // key heads (the caches': of all sequences) by blocks of rows
     int64_t floats;
     __device__ __forceinline__ const float* first(const float* parts, int head, int row, int width) const {
         const int64_t unit = static_cast<int64_t>(head) * blocks + (row >> shift);
-        return parts + (unit * splits * rows + (row & (rows - 1))) * width;
+        return parts + (unit * splits * rows + (row & ((1 << shift) - 1))) * width;
     }
 };
 
@@ -1224,12 +1226,12 @@ __global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (F
         const uint32_t row_block = in / left, keys = 8 * some + in - row_block * left, g = keys / splits, split_at = keys - g * splits;
         const int64_t place = (static_cast<int64_t>(g) * plan.start.blocks + row_block) * splits + split_at;
         attention_part<T, FORM, DP, COLS, ROW_WAVES, kStepWaves, kStart>(
-            a, out, parts + place * kStartRows * part_width(DP), 0, static_cast<int>(g), static_cast<int>(row_block) * kStartRows,
+            a, out, parts + place * plan.start.rows * part_width(DP), 0, static_cast<int>(g), static_cast<int>(row_block) * kStartRows,
             static_cast<int>(split_at), plan.start.splits, cache_lds);
     } else {
         const uint32_t at = block - first, unit = at / plan.own.splits, bg = unit / plan.own.blocks, b = bg / a.G;
         attention_part<T, FORM, DP, OWN_COLS, 1, kStepWaves, kOwn>(
-            a, out, plan.joined ? parts + plan.start.floats + static_cast<int64_t>(at) * kOwnRows * part_width(DP) : nullptr,
+            a, out, plan.joined ? parts + plan.start.floats + static_cast<int64_t>(at) * plan.own.rows * part_width(DP) : nullptr,
             static_cast<int>(b), static_cast<int>(bg - b * a.G), static_cast<int>(unit - bg * plan.own.blocks) * kOwnRows,
             static_cast<int>(at - unit * plan.own.splits), plan.own.splits, cache_lds);
     }
