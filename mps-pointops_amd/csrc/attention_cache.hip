@@ -32,8 +32,8 @@ struct JoinArgs {
 // One wave a row: its parts, of the start's keys and of its own.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_cache_join_kernel(const JoinArgs a, const float* __restrict__ parts,
-                                                                        T* __restrict__ out) {
-    const int width = part_width(padded(a.D)), id = uniform(static_cast<int>(blockIdx.x * kWaves + threadIdx.x / kWave));  // (g, b, row)
+                                                                        T* __restrict__ out, uint32_t first_block) {
+    const int width = part_width(padded(a.D)), id = uniform(static_cast<int>((first_block + blockIdx.x) * kWaves + threadIdx.x / kWave));  // (g, b, row)
     if (id >= a.rows) return;
     const int g = a.all.of_row(id), in_g = id - g * static_cast<int>(a.all.d);
     const int b = a.per.of_row(in_g), row = in_g - b * static_cast<int>(a.per.d), i = a.group.of_row(row);
@@ -211,9 +211,10 @@ hipError_t cache_step(const CacheArgs& a, int type, int form, void* out, void* w
     if (err != hipSuccess || !plan.joined) return err;
     const int64_t rows = static_cast<int64_t>(a.B) * a.Q * a.H;  // (at most 2^30)
     const JoinArgs join = {Divisor::of(rows / a.G), a.per, a.group, static_cast<int>(rows), a.Q, a.H, a.G, a.D, plan.start, plan.own};
-    hipLaunchKernelGGL(attention_cache_join_kernel<T>, dim3(static_cast<uint32_t>((rows + kWaves - 1) / kWaves)),
-                       dim3(kThreads), 0, stream, join, static_cast<const float*>(parts), static_cast<T*>(out));
-    return hipGetLastError();
+    return in_launches(static_cast<uint32_t>((rows + kWaves - 1) / kWaves), [&](uint32_t first, uint32_t count) {
+        hipLaunchKernelGGL(attention_cache_join_kernel<T>, dim3(count), dim3(kThreads), 0, stream, join,
+                           static_cast<const float*>(parts), static_cast<T*>(out), first);
+    });
 }
 
 bool kept_aligned(const Kept& k, int D) {

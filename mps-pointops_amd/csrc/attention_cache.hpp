@@ -1213,11 +1213,11 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
 // Registers: two waves a SIMD, one for 32-bit values, whose products take four times the operands.
 template <typename T, int FORM, int DP, int COLS, int ROW_WAVES, int OWN_COLS>
 __global__ __launch_bounds__(kStepThreads, FORM == kAny || (sizeof(T) == 4 && (FORM < kFour || COLS * OWN_COLS > 1)) ? 1 : 2) void attention_cache_kernel(
-    const CacheArgs a, const CachePlan plan, T* __restrict__ out, float* __restrict__ parts) {
+    const CacheArgs a, const CachePlan plan, T* __restrict__ out, float* __restrict__ parts, uint32_t first_block) {
     extern __shared__ __attribute__((aligned(16))) char cache_lds[];
     constexpr int kStartRows = 16 * COLS * ROW_WAVES, kOwnRows = 16 * OWN_COLS;
     // (A launch has fewer than 2^31 blocks; divisions of 64 bits are a hundred instructions each.)
-    const uint32_t block = blockIdx.x, first = static_cast<uint32_t>(plan.start.units) * plan.start.splits;
+    const uint32_t block = first_block + blockIdx.x, first = static_cast<uint32_t>(plan.start.units) * plan.start.splits;
     if (block < first) {
         // The row blocks of the same keys are eight blocks apart, on one XCD (whose L2 then
         // holds the keys for all of them).
@@ -1244,10 +1244,11 @@ constexpr int direct_waves(int size, int form, int DP) { return size == 4 && for
 
 template <typename T, int FORM, int DP>
 __global__ __launch_bounds__(kWave * direct_waves(sizeof(T), FORM, DP), direct_waves(sizeof(T), FORM, DP) / 4) void attention_direct_kernel(
-    const CacheArgs a, T* __restrict__ out) {
+    const CacheArgs a, T* __restrict__ out, uint32_t first_block) {
+    const uint32_t block = first_block + blockIdx.x;
     extern __shared__ __attribute__((aligned(16))) char cache_lds[];
     attention_part<T, FORM, DP, 1, 1, direct_waves(sizeof(T), FORM, DP), kBoth>(
-        a, out, nullptr, static_cast<int>(blockIdx.x / a.G), static_cast<int>(blockIdx.x % a.G), 0, 0, 1, cache_lds);
+        a, out, nullptr, static_cast<int>(block / a.G), static_cast<int>(block % a.G), 0, 0, 1, cache_lds);
 }
 
 // Kernels, by the rows of a start's block and of a cache's.
@@ -1269,8 +1270,9 @@ hipError_t launch_cache_form(const CacheArgs& a, const CachePlan& plan, void* ou
                 const hipError_t err = allow_lds(kernel, allowed, kMostLds);
                 if (err != hipSuccess) return err;
             }
-            hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kWave * waves), lds, stream, a, rest...);
-            return hipGetLastError();
+            return in_launches(static_cast<uint32_t>(blocks), [&](uint32_t first, uint32_t count) {
+                hipLaunchKernelGGL(kernel, dim3(count), dim3(kWave * waves), lds, stream, a, rest..., first);
+            });
         };
         auto parted = [&](auto shape) {
             constexpr ShapeRows R = kShapeRows[decltype(shape)::value];

@@ -45,8 +45,8 @@ struct Piece {
 // A block's pieces: whole rows of one key head's tokens (of 96 values 21, four threads
 // are left over), so that no thread divides by more than a row's lanes.
 __host__ __device__ constexpr int rows_of(int D) { return kThreads / lanes_of(D); }
-__device__ __forceinline__ Piece piece_of(const CacheCall& c, int tokens, uint32_t blocks) {
-    const uint32_t chunk = blockIdx.x % blocks, unit = blockIdx.x / blocks, lanes = lanes_of(c.D);
+__device__ __forceinline__ Piece piece_of(const CacheCall& c, int tokens, uint32_t blocks, uint32_t first) {
+    const uint32_t block = first + blockIdx.x, chunk = block % blocks, unit = block / blocks, lanes = lanes_of(c.D);
     const uint32_t row = threadIdx.x * (65536 / lanes + 1) >> 16;  // of fewer than 256 threads, exactly
     Piece p;
     p.t = static_cast<int>(chunk * rows_of(c.D) + row);
@@ -95,8 +95,8 @@ __device__ __forceinline__ void put(T* to, const T* x) {
 }
 
 template <typename T, int BITS>
-__global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheCall c, uint32_t blocks) {
-    const Piece p = piece_of(c, c.T, blocks);
+__global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheCall c, uint32_t blocks, uint32_t first) {
+    const Piece p = piece_of(c, c.T, blocks, first);
     const Side& s = c.side[p.side];
     int64_t length = c.N;
     if (c.lengths != nullptr) length = min(max(value_at(c.lengths, c.length_bits, p.b), int64_t(0)), int64_t(c.N));
@@ -158,8 +158,8 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(const CacheCall c
 
 template <typename T, int BITS>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(const CacheCall c, T* __restrict__ k, T* __restrict__ v,
-                                                              uint32_t blocks) {
-    const Piece p = piece_of(c, c.N, blocks);
+                                                              uint32_t blocks, uint32_t first) {
+    const Piece p = piece_of(c, c.N, blocks, first);
     if (!p.any || p.at >= c.D) return;
     const Side& s = c.side[p.side];
     const int64_t at = p.b * c.cache_b + p.g * c.cache_h + p.t;
@@ -281,8 +281,9 @@ hipError_t pointops_cache_write(const pointops_cache* cache, const void* k, cons
     uint32_t each, all;
     if (!blocks_of(c, c.T, &each, &all)) return hipErrorInvalidValue;
     return with_type(type, cache->bits, [&](auto t, auto bits) {
-        hipLaunchKernelGGL((cache_write_kernel<decltype(t), decltype(bits)::value>), dim3(all), dim3(kThreads), 0, stream, c, each);
-        return hipGetLastError();
+        return in_launches(all, [&](uint32_t first, uint32_t count) {
+            hipLaunchKernelGGL((cache_write_kernel<decltype(t), decltype(bits)::value>), dim3(count), dim3(kThreads), 0, stream, c, each, first);
+        });
     });
 }
 
@@ -298,9 +299,10 @@ hipError_t pointops_cache_read(const pointops_cache* cache, void* k, void* v, in
     if (!blocks_of(c, c.N, &each, &all)) return hipErrorInvalidValue;
     return with_type(type, cache->bits, [&](auto t, auto bits) {
         using T = decltype(t);
-        hipLaunchKernelGGL((cache_read_kernel<T, decltype(bits)::value>), dim3(all), dim3(kThreads), 0, stream, c,
-                           static_cast<T*>(k), static_cast<T*>(v), each);
-        return hipGetLastError();
+        return in_launches(all, [&](uint32_t first, uint32_t count) {
+            hipLaunchKernelGGL((cache_read_kernel<T, decltype(bits)::value>), dim3(count), dim3(kThreads), 0, stream, c,
+                               static_cast<T*>(k), static_cast<T*>(v), each, first);
+        });
     });
 }
 

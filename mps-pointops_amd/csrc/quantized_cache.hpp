@@ -19,6 +19,8 @@
 // large for those groups and nothing is cut.
 #pragma once
 
+#include <algorithm>
+
 #include "attention.hpp"
 
 namespace pointops {
@@ -32,6 +34,19 @@ constexpr int kGroup = 32;      // values with a common scale
 constexpr int kNoNumber = 255;  // the scale of a group with an infinity or NaN
 
 __host__ __device__ constexpr int padded(int D) { return (D + kGroup - 1) / kGroup * kGroup; }
+
+// A launch holds fewer than 2^32 threads: more than 2^23 blocks are several launches, each of
+// `count` blocks from `first` on.
+template <typename F>
+hipError_t in_launches(uint32_t blocks, F launch) {
+    constexpr uint32_t kMost = 1 << 23;
+    for (uint32_t first = 0; first < blocks; first += kMost) {
+        launch(first, std::min(kMost, blocks - first));
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+}
 
 // Rows are read in pieces of up to 16 bytes, a row's 2 or 4 scales at once.
 inline bool codes_aligned(const void* codes, const void* scales, int D) {
