@@ -132,7 +132,10 @@ bool pieces(const void* p, int64_t b, int64_t n, int64_t h) {
 }
 bool pieces(const Kept& k) { return k.tokens == 0 || (pieces(k.k, k.kb, k.kn, k.kh) && pieces(k.v, k.vb, k.vn, k.vh)); }
 
-// Rows that 16-byte reads serve: a row's reads stay inside it, as D is a multiple of a piece.
+// Rows that 16-byte reads serve: a row's reads stay inside it, as D is a multiple of a piece.  Where one
+// tensor's are not, all of a call's are read value by value, by kernels of 32 rows a wave that do not
+// share a start's keys (64 behind 16384, bfloat16, width 124: 773 us, 128: 66; 20: 131, 24: 43; 8 behind
+// 1024, window 512, width 60: 27.5, 64: 8.0).
 int form_of(const pointops_cache_attention& in, CacheArgs* a) {
     const int64_t size = size_of(in.type);
     const bool whole = in.D * size % 16 == 0;
@@ -150,12 +153,19 @@ size_t pairs_lds(const CacheArgs& a, int type, int form) {
 }
 
 // Where what a sequence's rows see are so many tiles at most, and so many of all sequences (whose
-// blocks each read the start's keys), one launch of whole rows is shorter than parts and their join.
+// blocks each read the start's keys), one launch of whole rows: a call of parts waits for the host 4.5 us
+// longer, for its workspace and its join.  4 sequences, 32 heads over 8 of 128, by one launch and by
+// parts: over 8 bits and 16 tiles 10.6 and 14.1 us, 32 tiles 13.3 and 14.1, 40 tiles 14.6 and 14.3;
+// bfloat16 14.7 and 19.3, 17.4 and 19.2, 20.9 and 19.0.  Recorded in a graph, where the host does not
+// count, parts are shorter from about 20 tiles on (8 bits 10.5 and 10.9, 13.6 and 11.1, 14.5 and 11.1), and
+// over float32 tensors, whose tiles take three times as long, they are everywhere (24 and 18, 41 and
+// 19, 49 and 20).  64 sequences of 40 tiles in 8 bits (20480 of all key heads): 38 and 32.
 constexpr int kDirectTiles = 40, kDirectWork = 16384;
 
-// Parts that give every compute unit the two blocks that its registers hold (4 x 65536 tokens in
-// 8 bits: 98 us by 512 blocks, 104 by 1024 in two rounds), at least two tiles a wave; the start's and
-// the caches' as their work is to each other.  By the caches' sizes: the lengths are on the device, and
+// Parts that give every compute unit two blocks, at least two tiles a wave; the start's and
+// the caches' as their work is to each other.  Kernels over codes of 16-bit queries would hold three;
+// by 256, 512, 768 and 1024 blocks: 4 x 65536 tokens in 8 bits 88, 90, 92, 91 us, 32 x 8192 under float16
+// in 8 bits 90, 89, 103, 93, in 4 bits 64, 56, 55, 62; 64 behind 65536, bfloat16, 166, 133, 145, 146.  By the caches' sizes: the lengths are on the device, and
 // a call does not wait for it.
 CachePlan plan_of(const CacheArgs& a, int type, int form) {
     CachePlan p = {};

@@ -20,7 +20,8 @@
 // that stay empty are work too.
 //
 // A long cache's keys are bound by HBM: 4 x 65536 tokens of 32 heads over 8 of 128 in 8 bits 73 us,
-// 6.0 TB/s; in 4 bits under float16 by instructions (32 x 8192: 47 us, 4.6 TB/s); the start's rows by
+// 6.0 TB/s; in 4 bits under float16 by what two waves a SIMD issue between their waits (32 x 8192: 47
+// us, 4.6 TB/s; vector instructions 40 % of the time, LDS 39, matrix units 25); the start's rows by
 // what is issued beside the products (64 sequences behind 65536 tokens: 455 to 470 T/s of the pairs,
 // matrix units 40 % busy); short ones by one block's latency (10 to 18 us).
 #pragma once
@@ -109,7 +110,7 @@ struct CachePlan {
 
 // ------------------------------------------------------------ small pieces
 // acc += A B of 32 values of 16 bits, or step e of four of 16 values of 32 bits.  An instruction
-// waits for the one before it on the same registers: the callers go round several.
+// waits for the one before it on the same registers: the callers take two or four sums in turn.
 template <typename T>
 constexpr int kMmaSteps = sizeof(T) == 4 ? 4 : 1;
 template <typename T>
@@ -183,9 +184,9 @@ __device__ __forceinline__ void split(const float* x, i32x4 (&out)[N]) {
 }
 
 // Buffer loads of what is read once and in whole lines: it does not stay in the caches.
-// Of a wave's own values (all its loads at 64 x 2048 bfloat16 tokens, 8 heads of 128, kept: 120 us,
-// values alone past the caches 94, keys too, of whose lines a load takes the half, 121;
-// 4 x 65536 in 8 bits 110, 93, 95; 32 x 8192 in 4 bits 53, 52, 55).
+// Of a wave's own values (32 heads over 8 of 128, all loads kept: 64 x 2048 bfloat16 tokens 103 us,
+// values alone past the caches 82, keys too, of whose lines a load takes the half, 93;
+// 4 x 65536 in 8 bits 108, 90, 94; 32 x 8192 in 4 bits, float16, 55, 55, 60).
 constexpr int kOnce = 2;
 // An offset behind every buffer: reads there give zeros and touch nothing.
 constexpr uint32_t kNothing = 0x80000000u;
@@ -525,8 +526,10 @@ struct Shared {
 
 // The same for rows of 16 bits, which memory loads write to LDS themselves: 64 lanes' pieces of
 // 16 bytes one behind the other, so that rows have no room between them.  Each lane asks for the
-// piece that belongs there: within a row, piece p lies at p ^ turn(row), with which the row operands'
-// reads of 8 rows and the transposing reads of 4 rows and 2 pieces fall on all banks.  What lies
+// piece that belongs there: within a row, piece p lies at p ^ turn(row), with which 8 neighbouring
+// rows of a row operand's read lie in 8 different places of 128 bytes, and the 4 rows and 2 pieces of a
+// transposing read too.  (Rows of 256 bytes have 16 places, of which these are one half, and rows 8
+// apart share them: counters call half of LDS's time conflicts.)  What lies
 // behind a row's width is cleared once; loads past the descriptor's end bring zeros.
 // 64 sequences behind 65536 tokens of width 128, in turn: 167 us through registers, 146 to 151 so (LDS
 // instructions 15 to 6 % of the time, the matrix units 37 to 40 % busy); 32 behind 32768 of width
@@ -536,7 +539,7 @@ struct Streamed {
     static constexpr int kRows = kKeys * KW, kRowBytes = DP * 2, kPerRow = DP / 8, kBytes = 2 * kRows * kRowBytes;
     static constexpr int kLoads = kRows * kPerRow / kWave / WAVES;  // of a wave and side, 1 KB each
     static_assert(kRows * kPerRow % (kWave * WAVES) == 0);
-    // Rows of a multiple of 128 bytes have 8 pieces and more to change places among, others 4.
+    // Pieces change places among 8 where rows are a multiple of 128 bytes, among 4 in others.
     __device__ static __forceinline__ uint32_t turn(uint32_t row) {
         if constexpr (kPerRow % 8 == 0) return (row & 3) << 1 | (row >> 2 & 1);
         else return (row >> 1 & 1) << 1 | (row >> 2 & 1);

@@ -334,7 +334,8 @@ class QuantizedCache:
     fraction bits, exponents from -6 to 8, even steps of 2 ** -9 below) or 6 (4 bits:
     0, 0.5, 1, 1.5, 2, 3, 4, 6) times it.  Quotients are rounded to the nearest value,
     to even codes at ties: by at most 1/16 of a value in 8 bits, 1/4 in 4 (below the
-    smallest exponents by half a step).  A group with an infinity or NaN reads as NaN.
+    smallest exponents by half a step).  A group with an infinity or NaN reads as NaN, and
+    a magnitude whose nearest value is 2 ** 128 (from 1.75 * 2 ** 127 on in 4 bits, 1.9375 in 8) as an infinity.
 
     ``k_codes, v_codes (batch, heads, tokens, bytes)`` and ``k_scales, v_scales (batch,
     heads, tokens, groups)`` are uint8 and zeros (values of zero) at first; a row's
@@ -608,8 +609,10 @@ def prefix_attention_step(q: Tensor, prefix, cache, lengths: Tensor | None = Non
     first ``lengths (B,)`` hold tokens, the new ones' own among them: the cloud's
     positions are 0 .. P + lengths - 1, and ``q (B, Q, H, D)`` stands at the last Q.
     Or both are a ``QuantizedCache`` of the same bits, the prefix with a batch of one.
-    Where they are long, the start's keys are read once for all queries of the batch.
-    Without gradients.
+    Where they are long, the start's keys are read once for up to 64 queries of the batch
+    at a time.  Tensors are best aligned to 16 bytes, and the head width a multiple of 8 (float32:
+    of 4): of others, also if only one is, rows are read value by value, for up to 32 queries
+    at a time, and a call takes many times as long.  Without gradients.
     """
     _check_unrecorded("prefix_attention_step", q, prefix, cache, bias)
     _check_query(q)
