@@ -533,18 +533,55 @@ __device__ __forceinline__ bool odd_value(uint64_t odd, int r, int c) {
     return (mine >> (c / 32 * 16 + c % 32 / 8 * 4 + c % 4) & 1) != 0;
 }
 
+// A wave's sums over the keys of one query: lane l has elements l and l + 64, of which it needs
+// those that came out not finite (n0, n1).  p is o 2^-30, which is finite where the values of 2^30
+// keys are, also if o is not.  (Alone it would lose bits of values below 2^-96.)
+struct CarefulSum {
+    float m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f, p0 = 0.f, p1 = 0.f;
+
+    __device__ __forceinline__ void add(float s, float v0, float v1) {
+        const float top = fmaxf(m, s), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top), low = w * 0x1p-30f;
+        m = top;
+        l = l * keep + w;
+        o0 = o0 * keep + w * v0;
+        o1 = o1 * keep + w * v1;
+        p0 = p0 * keep + low * v0;
+        p1 = p1 * keep + low * v1;
+    }
+    // Whether all that is needed has met values that are no numbers.
+    __device__ __forceinline__ bool settled(bool n0, bool n1) const { return ballot((n0 && finite(p0)) || (n1 && finite(p1))) == 0; }
+    // The means.
+    __device__ __forceinline__ float mean(float o, float p) const {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        return finite(o) ? o * inv : p * (0x1p30f * inv);
+    }
+    // The sums x by a maximum `top`, with their weights' sum: those needed from here, by that maximum,
+    // or, where there is none or they pass 32 bits by it, all by one of these.
+    __device__ __forceinline__ void replace(bool none, bool n0, bool n1, float& x0, float& x1, float& top, float& sum) const {
+        const float up = exp2_fast(m - top), y0 = o0 * up, y1 = o1 * up;
+        const bool passed = ballot((n0 && !finite(y0) && finite(p0)) || (n1 && !finite(y1) && finite(p1))) != 0;
+        if (none || passed) {
+            const float to = passed ? m + 30.f : m, by = exp2_fast(m - to), from = by * 0x1p30f, down = exp2_fast(top - to);
+            x0 = n0 ? (passed ? p0 * from : o0) : x0 * down;
+            x1 = n1 ? (passed ? p1 * from : o1) : x1 * down;
+            top = to;
+            sum = l * by;
+        } else {
+            x0 = n0 ? y0 : x0;
+            x1 = n1 ? y1 : x1;
+        }
+    }
+};
+
 // One query by a whole wave, key by key, for rows whose result is not finite:
 // there a product with a masked key's infinity or NaN may have spread.  Only
 // keys that the row sees are added (one whose score is -inf, or whose bias is,
-// whatever it holds, has no weight and is left out).  Lane l holds elements l and
-// l + 64, of which it needs those that came out not finite (n0, n1).  m lies kAbove (in
-// units of log 2) above the maximum: the sums of 2^30 keys are finite as their values are.
+// whatever it holds, has no weight and is left out).
 template <typename T>
-struct CarefulRow {
+struct CarefulRow : CarefulSum {
     const Args& a;
     const T *k, *v;
-    static constexpr float kAbove = 30.f;
-    float q0, q1, m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
+    float q0, q1;
     bool d0, d1;
 
     __device__ __forceinline__ CarefulRow(const Args& args, int b, int g, const T* q) : a(args) {
@@ -561,17 +598,7 @@ struct CarefulRow {
         const float k0 = d0 ? to_float(k[j * a.k.n]) : 0.f, k1 = d1 ? to_float(k[j * a.k.n + kWave]) : 0.f;
         const float s = wave_sum((d0 ? q0 * k0 : 0.f) + (d1 ? q1 * k1 : 0.f)) * a.scale_log2 + bias;
         if (s == -kInf) return;
-        const float top = fmaxf(m, s + kAbove), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
-        m = top;
-        l = l * keep + w;
-        o0 = o0 * keep + (d0 ? w * to_float(v[j * a.v.n]) : 0.f);
-        o1 = o1 * keep + (d1 ? w * to_float(v[j * a.v.n + kWave]) : 0.f);
-    }
-    // log2 of the sum of 2^score (the maximum first: beside 30 it would lose bits).
-    __device__ __forceinline__ float log_sum() const { return (m - kAbove) + log2f(l * exp2f(kAbove)); }
-    // Whether all that is needed has come out not finite again.
-    __device__ __forceinline__ bool settled(bool n0, bool n1) const {
-        return ballot((n0 && finite(o0)) || (n1 && finite(o1))) == 0;
+        CarefulSum::add(s, d0 ? to_float(v[j * a.v.n]) : 0.f, d1 ? to_float(v[j * a.v.n + kWave]) : 0.f);
     }
 };
 

@@ -406,12 +406,10 @@ struct Incoming {
 // ------------------------------------------------------------ careful rows
 // One query by a whole wave, key by key, for rows whose sums are not finite: there a
 // product with a masked key's infinity or NaN may have spread, or their finite values have
-// passed 32 bits (the weights reach 2^8 and their number).  Lane l holds elements l and l + 64.
-// m lies kAbove (in units of log 2) above the maximum: the sums of 2^30 keys are finite as their values are.
+// passed 32 bits (the weights reach 2^8 and their number).
 template <typename T, int FORM>
-struct CarefulKept {
-    static constexpr float kAbove = 30.f;
-    float q0, q1, m = -kInf, l = 0.f, o0 = 0.f, o1 = 0.f;
+struct CarefulKept : CarefulSum {
+    float q0, q1;
     bool d0, d1;
     float scale_log2;
 
@@ -431,14 +429,7 @@ struct CarefulKept {
         const int lane = lane_id();
         const float s = wave_sum((d0 ? q0 * value(k, ks, lane) : 0.f) + (d1 ? q1 * value(k, ks, lane + kWave) : 0.f)) * scale_log2 + bias;
         if (s == -kInf) return;
-        const float top = fmaxf(m, s + kAbove), keep = m == -kInf ? 0.f : exp2_fast(m - top), w = exp2_fast(s - top);
-        m = top;
-        l = l * keep + w;
-        o0 = o0 * keep + (d0 ? w * value(v, vs, lane) : 0.f);
-        o1 = o1 * keep + (d1 ? w * value(v, vs, lane + kWave) : 0.f);
-    }
-    __device__ __forceinline__ bool settled(bool n0, bool n1) const {
-        return ballot((n0 && finite(o0)) || (n1 && finite(o1))) == 0;
+        CarefulSum::add(s, d0 ? value(v, vs, lane) : 0.f, d1 ? value(v, vs, lane + kWave) : 0.f);
     }
 };
 
@@ -1183,15 +1174,7 @@ __device__ __forceinline__ void attention_part(const CacheArgs& a, T* __restrict
                             done = none ? c.l != c.l : c.settled(n0, n1);
                         }
             }
-            // The finite sums, brought to the careful ones' maximum.  (Where these ended early, all of
-            // them are not finite again.)
-            const float by = done ? 1.f : exp2_fast(lm - c.m);
-            if (none || !done) {
-                lm = c.m;
-                ll = c.l;
-            }
-            x0 = n0 ? c.o0 : x0 * by;
-            x1 = n1 ? c.o1 : x1 * by;
+            c.replace(none, n0, n1, x0, x1, lm, ll);
         }
         if (KIND == kBoth || part == nullptr) {
             const Row at_row = row_of(r0 + row);

@@ -80,10 +80,9 @@ __device__ __forceinline__ void careful_row(const Args& a, int b, int h, int i, 
     bool done = false;
     for (int j = 0; j < seen.first && !done; ++j) done = settled(j);
     for (int j = max(seen.low, seen.first); j < seen.low + seen.count && !done; ++j) done = settled(j);
-    const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
-    if (n0) out[lane] = from_float<T>(row.o0 * inv);
-    if (n1) out[lane + kWave] = from_float<T>(row.o1 * inv);
-    if (whole && lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.log_sum();
+    if (n0) out[lane] = from_float<T>(row.mean(row.o0, row.p0));
+    if (n1) out[lane + kWave] = from_float<T>(row.mean(row.o1, row.p1));
+    if (whole && lane == 0 && lse != nullptr) *lse = row.l == 0.f ? kInf : row.m + log2f(row.l);
 }
 
 template <typename T, int DP, bool VEC, bool BIAS, int SPLIT>

@@ -252,15 +252,7 @@ __global__ __launch_bounds__(kWave * WAVES, sizeof(T) == 4 ? 1 : 2) void attenti
                         c.add(j, biased ? bias_at(shift + ii - j, row) : 0.f);
                         done = whole ? c.l != c.l : c.settled(n0, n1);
                     }
-            // The finite sums, brought to the careful ones' maximum.  (Where these ended early, all of
-            // them are not finite again.)
-            const float by = done ? 1.f : exp2_fast(lm - c.m);
-            if (whole || !done) {
-                lm = c.m;
-                ll = c.l;
-            }
-            x0 = n0 ? c.o0 : x0 * by;
-            x1 = n1 ? c.o1 : x1 * by;
+            c.replace(whole, n0, n1, x0, x1, lm, ll);
         }
         if (splits == 1) {
             const float inv = ll == 0.f ? 0.f : 1.f / ll;

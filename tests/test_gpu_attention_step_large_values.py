@@ -52,3 +52,21 @@ def test_few_keys_of_large_values(cuda_device, kind, B, Q, N, H, G, D):
     some[..., 0] = 5.0 * D ** 0.5
     v[:, ::max(1, N // 5), :, 1::3] = 3e38
     check(q, k, v, None, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("B,N,window", [(3, 400, 300), (2, 6000, 4000)])
+def test_columns_beside_those_formed_again(cuda_device, kind, B, N, window):
+    """A masked value that is no number has one column formed again: the others, near the type's smallest
+    numbers, keep their bits."""
+    from mps_pointops.attention import window_attention_step
+
+    q, k, v, _ = make(23, B, 1, N, 4, 2, 64, TYPES[kind])
+    v *= 1e-33
+    with torch.no_grad():
+        want = window_attention_step(q, k, v, window=window, sinks=1)
+        v[:, N - window - 3:N - window, :, 5] = float("nan")
+        got = window_attention_step(q, k, v, window=window, sinks=1)
+    some = [c for c in range(64) if c != 5]
+    assert torch.equal(got[..., some], want[..., some]) and torch.isfinite(got).all()
+    assert (got.double() - want.double()).norm() <= 2 * LIMIT[kind] * want.double().norm()

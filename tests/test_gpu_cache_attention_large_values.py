@@ -65,3 +65,24 @@ def test_few_keys_of_large_values(cuda_device, kind, bits, B, P, N, D):
     want = want_of(q, start, own, None, bits)
     close(got, want, LIMIT[kind])
     close(got[..., ::2], want[..., ::2], LIMIT[kind])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("B,P,N,window", [(3, 400, 60, 300), (2, 6000, 90, 4000), (40, 3000, 20, 2500)])
+def test_columns_beside_those_formed_again(cuda_device, kind, bits, B, P, N, window):
+    """A masked value that is no number has one column formed again: the others, near the type's smallest
+    numbers, keep their bits."""
+    q, start, own, _ = make(23, kind, B, 1, P, N, 4, 2, 64)
+    start[1].mul_(1e-33)
+    own[1].mul_(1e-33)
+    how = dict(window=window, sinks=1)
+    a, b = kept(start, bits), kept(own, bits)
+    want = step(q, a, b, None, bits, **how)
+    low = P + N - window
+    start[1][low - 3:low, :, 5] = float("nan")  # in the tile of the first keys that are seen
+    got = step(q, kept(start, bits), b, None, bits, **how)
+    some = [c for c in range(64) if c != 5] if not bits else list(range(32, 64))
+    assert torch.equal(got[..., some], want[..., some])
+    assert torch.isfinite(got).all()
+    assert (got.double() - want.double()).norm() <= 2 * LIMIT[kind] * want.double().norm()
