@@ -594,7 +594,8 @@ hipError_t pointops_attention_step(const pointops_attention *in, void *out, void
  * smallest x >= -127 with max |v| <= M X, held as the byte x + 127, and codes v / X
  * rounded to the nearest value of the type, to even codes at ties: bits = 8: E4M3
  * (M = 448), bits = 4: E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6; M = 6; value 2 i in the low
- * half of byte i).  A group with an infinity or NaN has the byte 255 and reads as NaN. */
+ * half of byte i).  A group with an infinity or NaN has the byte 255 and reads as NaN; a
+ * magnitude whose nearest value is 2^128 reads as an infinity. */
 typedef struct {
     void *k, *v;
     uint8_t *k_scales, *v_scales;

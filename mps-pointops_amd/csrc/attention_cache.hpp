@@ -46,7 +46,8 @@ struct Kept {
 };
 
 // Division of 0 .. 2^31 - 1 by a number of the call, as a product and a shift (a division
-// by what the compiler does not know is some thirty instructions, and a row asks for several):
+// by what the compiler does not know is some thirty instructions, and a row asks for several), as by
+// Granlund and Montgomery, "Division by invariant integers using multiplication" (1994):
 // n / d = (n m / 2^32 + n) / 2^s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1.
 struct Divisor {
     uint32_t d, m, s;
